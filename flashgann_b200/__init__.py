@@ -32,7 +32,7 @@ __all__ = [
     "QuantizationGraph", "FlashGANNError", "QueryStats", "lib", "load_fvecs", "load_ivecs", "compute_recall",
     "append_run_stats_to_csv", "infer_metric_from_dataset_path", "effective_sort_beam_size", "METRIC_L2",
     "METRIC_IP",
-    "search_multi",
+    "search_multi", "KVPlan", "kv_plan", "kv_append", "paged_attention", "retrieved_attention",
 ]
 
 
@@ -306,3 +306,16 @@ def append_run_stats_to_csv(filename: str, k: int, beam: int, runtime: float, la
 def infer_metric_from_dataset_path(path: str) -> int:
     """include/metric.hpp:13-28."""
     return int(lib().fg_infer_metric_from_path(os.fsencode(path)))
+
+
+# flashgann_b200.attention needs torch, which the search's host-buffer calls do not: loaded on first use
+_ATTENTION = ("KVPlan", "kv_append", "kv_plan", "paged_attention", "retrieved_attention")
+
+
+def __getattr__(name: str):
+    if name not in _ATTENTION:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import attention
+    for n in _ATTENTION:
+        globals()[n] = getattr(attention, n)
+    return globals()[name]

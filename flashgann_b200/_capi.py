@@ -21,6 +21,8 @@ FG_ERR_NO_DEVICE = 7
 FG_METRIC_L2 = 0
 FG_METRIC_IP = 1
 FG_ASYNC_SLOTS = 4
+FG_DTYPE_F16 = 0
+FG_DTYPE_BF16 = 1
 FG_GOAL_LATENCY = 0
 FG_GOAL_THROUGHPUT = 1
 FG_PLAN_KERNELS = {0: "cta", 1: "warp", 2: "staged", 3: "pair"}
@@ -46,11 +48,33 @@ class QueryStats(ctypes.Structure):
                 ("estimates", ctypes.c_uint32)]
 
 
+class KVCacheArgs(ctypes.Structure):
+    """fg_kv_cache"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("heads", ctypes.c_int32), ("dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """fg_attention"""
+    _fields_ = [("q", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("out", ctypes.c_void_p), ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64),
+                ("lse", ctypes.c_void_p), ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("query_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("ids", ctypes.c_void_p),
+                ("ids_token_stride", ctypes.c_int64), ("ids_head_stride", ctypes.c_int64),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("tokens", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("requests", ctypes.c_int32), ("table_width", ctypes.c_int32),
+                ("max_new", ctypes.c_int32), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+                ("ids_count", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
 # (name, restype, argtypes) for every entry point of include/flashgann.h
 _vp = ctypes.c_void_p
 _u64 = ctypes.c_uint64
 _i32 = ctypes.c_int32
 _u32 = ctypes.c_uint32
+_i64 = ctypes.c_int64
 _f64 = ctypes.c_double
 _cs = ctypes.c_char_p
 SIGNATURES = [
@@ -73,6 +97,15 @@ SIGNATURES = [
     ("fg_query_prepare_device", ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     ("fg_beam_merge_device", ctypes.c_int, [_vp, _vp, _i32, _i32, _i32, _i32, _vp]),
     ("fg_shard_merge_device", ctypes.c_int, [_vp, _vp, ctypes.POINTER(_u32), _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
+    ("fg_kv_plan_device", ctypes.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _i64, _i32, _vp, _vp, _vp,
+                                         _vp, _vp, _vp, _vp]),
+    ("fg_kv_append_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32,
+                                           _vp]),
+    ("fg_attention_workspace_bytes", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs),
+                                                    ctypes.POINTER(_u64)]),
+    ("fg_paged_attention_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs), _vp]),
+    ("fg_retrieved_attention_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs),
+                                                     _vp]),
     ("fg_effective_sort_beam_size", _u32, [_u32]),
     ("fg_entry_point_centroid", _u32, [_vp, _u64, _u64, _u64, _i32]),
     ("fg_compute_recall", ctypes.c_float, [_vp, _vp, _u64, _i32, _i32]),

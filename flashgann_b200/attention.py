@@ -1,0 +1,247 @@
+"""A paged key/value cache and attention over it, for decoders that find the
+keys of a long context with this package's search.
+
+The loop of one step: ``kv_plan`` gives each request pages and each new token
+a slot, ``kv_append`` writes the new keys and values there, and then either
+``paged_attention`` (all of the context, or a sliding window and the first
+tokens) or ``retrieved_attention`` (window, first tokens and the ids that a
+search returned for each query head) reads them.  All four take torch CUDA
+tensors, run in libflashgann.so (include/flashgann.h has the exact rules) on
+``stream`` (default: torch's current stream) and wait for nothing.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _capi
+from ._capi import FG_ERR_ARG, FG_OK, AttentionArgs, FlashGANNError, KVCacheArgs, lib
+
+_DTYPES = {torch.float16: _capi.FG_DTYPE_F16, torch.bfloat16: _capi.FG_DTYPE_BF16}
+
+
+class KVPlan(NamedTuple):
+    """What kv_plan returns; R requests, T token rows."""
+    query_start: torch.Tensor  # int32 [R + 1]: first row of each request in the step's token tensors
+    kv_len: torch.Tensor       # int32 [R]: tokens after the step (0: refused)
+    position: torch.Tensor     # int32 [T]: position in the request (-1: no token, or refused)
+    slot: torch.Tensor         # int64 [T]: page * page_size + row, for kv_append (-1 likewise)
+    free_head: torch.Tensor    # int32 [1]: first free page that was not taken
+    refused: torch.Tensor      # int32 [R]: 1 where the pages did not suffice
+
+
+def _fail(message: str):
+    raise FlashGANNError(FG_ERR_ARG, message)
+
+
+def _raise(rc: int, what: str):
+    L = lib()
+    raise FlashGANNError(rc, f"{what}: {L.fg_status_string(rc).decode()} ({L.fg_last_error().decode()})")
+
+
+class _On:
+    """The device and stream of one call.  Output and scratch tensors made
+    inside belong to that stream; inputs that live on another one are marked
+    as in use there, so that the caller may drop them right after the call."""
+
+    __slots__ = ("device", "handle", "guard")
+
+    def __init__(self, like: torch.Tensor, stream):
+        if not like.is_cuda:
+            _fail("expected a CUDA tensor")
+        index = like.device.index
+        current = torch.cuda.current_stream(index)
+        self.guard = None
+        if stream is None or getattr(stream, "cuda_stream", stream) == current.cuda_stream:
+            self.handle = current.cuda_stream
+            if torch.cuda.current_device() != index:
+                self.guard = torch.cuda.device(index)
+        else:
+            handle = getattr(stream, "cuda_stream", stream) or 0
+            s = stream if isinstance(stream, torch.cuda.Stream) else (
+                torch.cuda.ExternalStream(handle, device=index) if handle else torch.cuda.default_stream(index))
+            self.handle = handle
+            self.guard = torch.cuda.stream(s)
+        self.device = like.device
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+    def uses(self, *tensors):
+        for t in tensors:
+            if t is None:
+                continue
+            if t.device != self.device:
+                _fail(f"a tensor is on {t.device}, not on {self.device}")
+            if self.guard is not None:
+                t.record_stream(torch.cuda.current_stream(self.device))
+
+
+def _ints(t: torch.Tensor, dims: int, name: str, dtype=torch.int32) -> torch.Tensor:
+    if t.dtype != dtype or t.dim() != dims:
+        _fail(f"{name} must be {dtype} with {dims} dimension(s), not {t.dtype} {tuple(t.shape)}")
+    return t if dims == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    """[tokens, heads, dim] with a contiguous last axis and 16-byte aligned rows (a copy where it is not)."""
+    if t.dim() != 3:
+        _fail(f"{name} must be [tokens, heads, dim], not {tuple(t.shape)}")
+    s = t.stride()
+    if (s[2] != 1 and t.shape[2] > 1) or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> KVCacheArgs:
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        _fail(f"caches must be [pages, page_size, heads, dim] alike, not {tuple(k_cache.shape)} and "
+              f"{tuple(v_cache.shape)}")
+    if k_cache.dtype not in _DTYPES or v_cache.dtype != k_cache.dtype:
+        _fail(f"caches must both be float16 or bfloat16, not {k_cache.dtype} and {v_cache.dtype}")
+    s = k_cache.stride()
+    if s != v_cache.stride() or s[3] != 1:
+        _fail(f"caches must have the same strides and a contiguous last axis, not {s} and {v_cache.stride()}")
+    pages, page_size, heads, dim = k_cache.shape
+    return KVCacheArgs(k_cache.data_ptr(), v_cache.data_ptr(), s[0], s[1], s[2], pages, page_size, heads, dim,
+                       _DTYPES[k_cache.dtype])
+
+
+def kv_plan(ctx_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, *,
+            tokens: int, page_size: int, free_head: Optional[torch.Tensor] = None, stream=None) -> KVPlan:
+    """Pages, slots and row offsets of one step, from lengths on the device
+    (fg_kv_plan_device).
+
+    ctx_len, new_len int32 [R]: tokens in the cache and new ones of each
+    request; block_table int32 [R, width], updated in place; free_pages int32
+    [F], used from ``free_head`` (int32 [1], default 0) on; tokens: rows of the
+    step's token tensors (at least the sum of new_len for all to be mapped)."""
+    with _On(ctx_len, stream) as on:
+        on.uses(ctx_len, new_len, block_table, free_pages, free_head)
+        ctx_len, new_len = _ints(ctx_len, 1, "ctx_len"), _ints(new_len, 1, "new_len")
+        free_pages = _ints(free_pages, 1, "free_pages")
+        if new_len.shape != ctx_len.shape:
+            _fail("ctx_len and new_len differ in length")
+        R = ctx_len.shape[0]
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != R or (
+                block_table.shape[1] > 1 and block_table.stride(1) != 1):
+            _fail(f"block_table must be int32 [{R}, width] with contiguous rows")
+        if free_head is not None and (free_head.dtype != torch.int32 or free_head.numel() != 1):
+            _fail("free_head must be int32 [1]")
+        heads = torch.empty(3 * R + 2 + max(tokens, 0), dtype=torch.int32, device=on.device)
+        slot = torch.empty(max(tokens, 0), dtype=torch.int64, device=on.device)
+        plan = KVPlan(heads[:R + 1], heads[R + 1:2 * R + 1], heads[3 * R + 2:], slot, heads[2 * R + 1:2 * R + 2],
+                      heads[2 * R + 2:3 * R + 2])
+        base = heads.data_ptr()
+        rc = lib().fg_kv_plan_device(ctx_len.data_ptr(), new_len.data_ptr(), R, free_pages.data_ptr(),
+                                     free_pages.shape[0], None if free_head is None else free_head.data_ptr(),
+                                     page_size, block_table.data_ptr(), block_table.shape[1], block_table.stride(0),
+                                     tokens, base, base + 4 * (R + 1), base + 4 * (3 * R + 2), slot.data_ptr(),
+                                     base + 4 * (2 * R + 1), base + 4 * (2 * R + 2), on.handle)
+        if rc != FG_OK:
+            _raise(rc, "fg_kv_plan_device")
+        return plan
+
+
+def kv_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, *,
+              stream=None) -> None:
+    """Writes rows k, v [T, heads, dim] to the slots (int64 [T], from kv_plan)
+    of the caches [pages, page_size, heads, dim]; negative slots are skipped
+    (fg_kv_append_device)."""
+    with _On(k_cache, stream) as on:
+        on.uses(k_cache, v_cache, k, v, slot)
+        c = _cache(k_cache, v_cache)
+        want = (slot.shape[0], c.heads, c.dim)
+        if k.shape != want or v.shape != want or k.dtype != k_cache.dtype or v.dtype != k_cache.dtype:
+            _fail(f"k and v must be {k_cache.dtype} {want}, not {k.dtype} {tuple(k.shape)} and {v.dtype} "
+                  f"{tuple(v.shape)}")
+        slot, k, v = _ints(slot, 1, "slot", torch.int64), _rows(k, "k"), _rows(v, "v")
+        rc = lib().fg_kv_append_device(c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                       v.stride(1), slot.data_ptr(), want[0], on.handle)
+        if rc != FG_OK:
+            _raise(rc, "fg_kv_append_device")
+
+
+def _attend(call: str, q, k_cache, v_cache, block_table, query_start, kv_len, max_new, ids, window, sinks, scale, out,
+            return_lse, stream):
+    with _On(q, stream) as on:
+        on.uses(q, k_cache, v_cache, block_table, query_start, kv_len, out, ids)
+        c = _cache(k_cache, v_cache)
+        q = _rows(q, "q")
+        T, heads, dim = q.shape
+        if q.dtype != k_cache.dtype or dim != c.dim:
+            _fail(f"q must be {k_cache.dtype} [tokens, heads, {c.dim}], not {q.dtype} {tuple(q.shape)}")
+        block_table = _ints(block_table, 2, "block_table")
+        query_start, kv_len = _ints(query_start, 1, "query_start"), _ints(kv_len, 1, "kv_len")
+        R = kv_len.shape[0]
+        if query_start.shape[0] != R + 1 or block_table.shape[0] != R:
+            _fail(f"{R} lengths need {R + 1} query_start entries and {R} table rows, not {query_start.shape[0]} and "
+                  f"{block_table.shape[0]}")
+        if out is None:
+            out = torch.empty((T, heads, dim), dtype=q.dtype, device=on.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+            _fail(f"out must be {q.dtype} {tuple(q.shape)} with a contiguous last axis")
+        lse = torch.empty((T, heads), dtype=torch.float32, device=on.device) if return_lse else None
+        a = AttentionArgs(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                          lse.data_ptr() if return_lse else None, block_table.data_ptr(), block_table.stride(0),
+                          query_start.data_ptr(), kv_len.data_ptr(), None, 0, 0, None, 0, T, heads, R,
+                          block_table.shape[1], max_new, -1 if window is None else window, sinks, 0,
+                          dim ** -0.5 if scale is None else scale)
+        if ids is not None:
+            if ids.dtype != torch.int32 or ids.dim() != 3 or ids.shape[:2] != q.shape[:2]:
+                _fail(f"ids must be int32 [{T}, {heads}, count], not {ids.dtype} {tuple(ids.shape)}")
+            if ids.stride(2) != 1 and ids.shape[2] > 1:
+                ids = ids.contiguous()
+            a.ids, a.ids_token_stride, a.ids_head_stride = ids.data_ptr(), ids.stride(0), ids.stride(1)
+            a.ids_count = ids.shape[2]
+        L = lib()
+        need = ctypes.c_uint64()
+        rc = L.fg_attention_workspace_bytes(c, a, need)
+        if rc == FG_OK:
+            work = torch.empty(need.value, dtype=torch.uint8, device=on.device)
+            a.workspace, a.workspace_bytes = work.data_ptr(), need.value
+            rc = getattr(L, call)(c, a, on.handle)
+        if rc != FG_OK:
+            _raise(rc, call)
+        return (out, lse) if return_lse else out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    query_start: torch.Tensor, kv_len: torch.Tensor, max_new: int, *, window: Optional[int] = None,
+                    sinks: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    return_lse: bool = False, stream=None):
+    """Causal attention of each request's new tokens over its cache
+    (fg_paged_attention_device).
+
+    q [T, heads, dim] (a request's rows are query_start[b] .. query_start[b+1],
+    its last ones the newest positions of kv_len[b]); caches [pages, page_size,
+    kv_heads, dim], any strides; heads a multiple of kv_heads.  max_new: most
+    new tokens of a request (picks the kernel).  window: how many newest keys
+    a token sees, itself included (None or -1: all); sinks: first tokens that
+    stay visible.  scale: default dim ** -0.5.  Returns out [T, heads, dim],
+    with return_lse also the rows' log-sum-exp float32 [T, heads]; a row that
+    sees nothing is 0 and -inf."""
+    return _attend("fg_paged_attention_device", q, k_cache, v_cache, block_table, query_start, kv_len, max_new, None,
+                   window, sinks, scale, out, return_lse, stream)
+
+
+def retrieved_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                        query_start: torch.Tensor, kv_len: torch.Tensor, ids: torch.Tensor, *, window: int,
+                        sinks: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                        return_lse: bool = False, stream=None):
+    """paged_attention over the window, the first tokens and retrieved keys
+    (fg_retrieved_attention_device): ids int32 [T, heads, count] are positions
+    of the request's context, in any order, as a search over its keys returns
+    them (uint32 ids as int32 bits; negative, repeated, already visible and
+    future ones count nothing)."""
+    return _attend("fg_retrieved_attention_device", q, k_cache, v_cache, block_table, query_start, kv_len, 1, ids,
+                   window, sinks, scale, out, return_lse, stream)

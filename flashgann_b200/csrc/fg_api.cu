@@ -808,6 +808,219 @@ int fg_shard_merge_device(const uint32_t* d_ids, const float* d_dists, const uin
     return e == cudaSuccess ? FG_OK : cuda_fail(e, "shard merge launch");
 }
 
+// ---- key/value cache and attention ----
+
+namespace {
+
+int check_cache(const fg_kv_cache* c) {
+    if (!c || !c->k || !c->v) return fail(FG_ERR_ARG, "null cache");
+    if (c->dtype != FG_DTYPE_F16 && c->dtype != FG_DTYPE_BF16) return fail(FG_ERR_ARG, "unknown cache dtype %d", c->dtype);
+    if (c->dim != 64 && c->dim != 96 && c->dim != 128)
+        return fail(FG_ERR_UNSUPPORTED, "head dim %d is not 64, 96 or 128", c->dim);
+    if (c->pages < 1 || c->heads < 1) return fail(FG_ERR_ARG, "bad cache shape pages=%d heads=%d", c->pages, c->heads);
+    if (c->page_size < 1 || (c->page_size & (c->page_size - 1)))
+        return fail(FG_ERR_UNSUPPORTED, "page size %d is not a power of two", c->page_size);
+    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
+        return fail(FG_ERR_ARG, "cache is not 16-byte aligned");
+    if ((c->page_stride | c->token_stride | c->head_stride) & 7)
+        return fail(FG_ERR_ARG, "cache strides are not multiples of 16 bytes");
+    if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0) return fail(FG_ERR_ARG, "negative cache stride");
+    return FG_OK;
+}
+
+int log2_of(int32_t x) {
+    int s = 0;
+    while ((1 << s) < x) ++s;
+    return s;
+}
+
+// Rows [tokens, heads, dim] given by a pointer and two strides.
+int check_rows(const void* p, int64_t token_stride, int64_t head_stride, const char* what) {
+    if (!p) return fail(FG_ERR_ARG, "null %s", what);
+    if (reinterpret_cast<uintptr_t>(p) & 15) return fail(FG_ERR_ARG, "%s is not 16-byte aligned", what);
+    if ((token_stride | head_stride) & 7) return fail(FG_ERR_ARG, "strides of %s are not multiples of 16 bytes", what);
+    if (token_stride < 0 || head_stride < 0) return fail(FG_ERR_ARG, "negative stride of %s", what);
+    return FG_OK;
+}
+
+int sm_count(int* sms) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+    return e == cudaSuccess ? FG_OK : fail(FG_ERR_NO_DEVICE, "no CUDA device available (%s)", cudaGetErrorString(e));
+}
+
+int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void* stream) {
+    int rc = check_cache(c);
+    if (rc) return rc;
+    if (!x) return fail(FG_ERR_ARG, "null arguments");
+    if (x->tokens < 0 || x->requests < 0 || x->table_width < 0 || x->max_new < 0)
+        return fail(FG_ERR_ARG, "bad attention shape tokens=%d requests=%d table_width=%d max_new=%d", x->tokens,
+                    x->requests, x->table_width, x->max_new);
+    if (x->heads < 1 || x->heads % c->heads)
+        return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", x->heads, c->heads);
+    if (x->heads / c->heads > 256) return fail(FG_ERR_UNSUPPORTED, "%d query heads for each kv head", x->heads / c->heads);
+    if (x->requests > fg::attention_max_requests())
+        return fail(FG_ERR_UNSUPPORTED, "%d requests, at most %d", x->requests, fg::attention_max_requests());
+    if (x->window < -1 || x->sinks < 0) return fail(FG_ERR_ARG, "bad mask window=%d sinks=%d", x->window, x->sinks);
+    if (!(std::fabs(x->scale) <= FLT_MAX)) return fail(FG_ERR_ARG, "scale is not finite");
+    if (retrieved) {
+        if (x->window < 0) return fail(FG_ERR_ARG, "retrieved attention needs a window >= 0");
+        if (x->ids_count < 0 || x->ids_token_stride < 0 || x->ids_head_stride < 0)
+            return fail(FG_ERR_ARG, "bad ids: count %d, or a negative stride", x->ids_count);
+        if (x->ids_count > 65536) return fail(FG_ERR_UNSUPPORTED, "%d ids for each row, at most 65536", x->ids_count);
+    }
+    if (x->tokens == 0 || x->requests == 0) return FG_OK;
+    if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, "q"))) return rc;
+    if ((rc = check_rows(x->out, x->out_token_stride, x->out_head_stride, "out"))) return rc;
+    if (!x->query_start || !x->kv_len || (!x->block_table && x->table_width > 0) || (retrieved && !x->ids && x->ids_count))
+        return fail(FG_ERR_ARG, "null buffer");
+    if (x->table_stride < 0) return fail(FG_ERR_ARG, "negative table stride");
+    if (!x->workspace || (reinterpret_cast<uintptr_t>(x->workspace) & 255))
+        return fail(FG_ERR_ARG, "workspace is null or not 256-byte aligned");
+    uint64_t need = 0;
+    if ((rc = fg_attention_workspace_bytes(c, x, &need))) return rc;
+    if (x->workspace_bytes < need)
+        return fail(FG_ERR_ARG, "workspace of %llu bytes, %llu needed", (unsigned long long)x->workspace_bytes,
+                    (unsigned long long)need);
+    fg::AttentionParams a;
+    a.k_cache = c->k;
+    a.v_cache = c->v;
+    a.page_stride = c->page_stride;
+    a.token_stride = c->token_stride;
+    a.head_stride = c->head_stride;
+    a.pages = c->pages;
+    a.page_size = c->page_size;
+    a.page_shift = log2_of(c->page_size);
+    a.dim = c->dim;
+    a.dtype = c->dtype;
+    a.q = x->q;
+    a.q_token_stride = x->q_token_stride;
+    a.q_head_stride = x->q_head_stride;
+    a.out = x->out;
+    a.out_token_stride = x->out_token_stride;
+    a.out_head_stride = x->out_head_stride;
+    a.lse = x->lse;
+    a.block_table = x->block_table;
+    a.table_stride = x->table_stride;
+    a.table_width = x->table_width;
+    a.query_start = x->query_start;
+    a.kv_len = x->kv_len;
+    a.requests = x->requests;
+    a.tokens = x->tokens;
+    a.heads = x->heads;
+    a.kv_heads = c->heads;
+    a.group = x->heads / c->heads;
+    a.window = x->window;
+    a.sinks = x->sinks;
+    a.scale_log2 = static_cast<float>(x->scale * 1.4426950408889634);
+    if (retrieved && x->ids_count > 0) {
+        a.ids = x->ids;
+        a.ids_count = x->ids_count;
+        a.ids_token_stride = x->ids_token_stride;
+        a.ids_head_stride = x->ids_head_stride;
+    }
+    a.workspace = x->workspace;
+    if ((rc = sm_count(&a.ctas))) return rc;
+    const cudaError_t e = fg::launch_attention_rows(a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FG_OK : cuda_fail(e, "attention launch");
+}
+
+}  // namespace
+
+int fg_kv_plan_device(const int32_t* d_ctx_len, const int32_t* d_new_len, int32_t requests,
+                      const int32_t* d_free_pages, int32_t free_count, const int32_t* d_free_head, int32_t page_size,
+                      int32_t* d_block_table, int32_t table_width, int64_t table_stride, int32_t tokens,
+                      int32_t* d_query_start, int32_t* d_kv_len, int32_t* d_position, int64_t* d_slot,
+                      int32_t* d_free_head_out, int32_t* d_refused, void* stream) {
+    g_err.clear();
+    if (requests < 1 || free_count < 0 || table_width < 0 || table_stride < 0 || tokens < 0)
+        return fail(FG_ERR_ARG, "bad plan shape requests=%d free_count=%d table_width=%d tokens=%d", requests, free_count,
+                    table_width, tokens);
+    if (requests > fg::kv_plan_max_requests())
+        return fail(FG_ERR_UNSUPPORTED, "%d requests, at most %d", requests, fg::kv_plan_max_requests());
+    if (page_size < 1 || (page_size & (page_size - 1)))
+        return fail(FG_ERR_UNSUPPORTED, "page size %d is not a power of two", page_size);
+    if (!d_ctx_len || !d_new_len || !d_query_start || !d_kv_len || !d_free_head_out || !d_refused ||
+        (free_count && !d_free_pages) || (table_width && !d_block_table) || (tokens && (!d_position || !d_slot)))
+        return fail(FG_ERR_ARG, "null buffer");
+    if (d_free_head == d_free_head_out) return fail(FG_ERR_ARG, "free_head and free_head_out are the same buffer");
+    fg::PlanArgs a;
+    a.ctx_len = d_ctx_len;
+    a.new_len = d_new_len;
+    a.free_pages = d_free_pages;
+    a.free_head = d_free_head;
+    a.block_table = d_block_table;
+    a.query_start = d_query_start;
+    a.kv_len = d_kv_len;
+    a.position = d_position;
+    a.slot = d_slot;
+    a.free_head_out = d_free_head_out;
+    a.refused = d_refused;
+    a.table_stride = table_stride;
+    a.requests = requests;
+    a.free_count = free_count;
+    a.page_shift = log2_of(page_size);
+    a.table_width = table_width;
+    a.tokens = tokens;
+    const cudaError_t e = fg::launch_kv_plan(a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FG_OK : cuda_fail(e, "plan launch");
+}
+
+int fg_kv_append_device(const fg_kv_cache* cache, const void* d_k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void* d_v, int64_t v_token_stride, int64_t v_head_stride, const int64_t* d_slot,
+                        int32_t tokens, void* stream) {
+    g_err.clear();
+    int rc = check_cache(cache);
+    if (rc) return rc;
+    if (tokens < 0) return fail(FG_ERR_ARG, "bad token count %d", tokens);
+    if (tokens == 0) return FG_OK;
+    if ((rc = check_rows(d_k, k_token_stride, k_head_stride, "k"))) return rc;
+    if ((rc = check_rows(d_v, v_token_stride, v_head_stride, "v"))) return rc;
+    if (!d_slot) return fail(FG_ERR_ARG, "null slots");
+    fg::AppendArgs a;
+    a.k_cache = cache->k;
+    a.v_cache = cache->v;
+    a.k = d_k;
+    a.v = d_v;
+    a.slot = d_slot;
+    a.page_stride = cache->page_stride / 8;
+    a.token_stride = cache->token_stride / 8;
+    a.head_stride = cache->head_stride / 8;
+    a.k_token_stride = k_token_stride / 8;
+    a.k_head_stride = k_head_stride / 8;
+    a.v_token_stride = v_token_stride / 8;
+    a.v_head_stride = v_head_stride / 8;
+    a.pages = cache->pages;
+    a.page_shift = log2_of(cache->page_size);
+    a.heads = cache->heads;
+    a.pieces = cache->dim / 8;
+    a.tokens = tokens;
+    const cudaError_t e = fg::launch_kv_append(a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FG_OK : cuda_fail(e, "append launch");
+}
+
+int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* args, uint64_t* bytes) {
+    g_err.clear();
+    int rc = check_cache(cache);
+    if (rc) return rc;
+    if (!args || !bytes) return fail(FG_ERR_ARG, "null argument");
+    int sms = 0;
+    if ((rc = sm_count(&sms))) return rc;
+    *bytes = fg::attention_rows_workspace(sms, cache->dim);
+    return FG_OK;
+}
+
+int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {
+    g_err.clear();
+    return attention(cache, args, false, stream);
+}
+
+int fg_retrieved_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {
+    g_err.clear();
+    return attention(cache, args, true, stream);
+}
+
 uint32_t fg_effective_sort_beam_size(uint32_t beam) { return fg::effective_sort_beam(beam); }
 
 uint32_t fg_entry_point_centroid(const float* rows, uint64_t n, uint64_t dim, uint64_t row, int32_t metric) {

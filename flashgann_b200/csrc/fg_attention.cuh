@@ -1,0 +1,317 @@
+// fg_attention.cuh -- what the attention kernels share: their arguments, the
+// mask, the list of key chunks a tile of query rows has to visit, and the
+// split of all tiles' chunks over a fixed number of CTAs.
+//
+// Mathematics.  Query row (token i of a request, head h) stands at position
+// p = kv_len - new + i and sees the keys
+//     V(p) = { j : 0 <= j <= p, and (no window, or p - j < window, or j < sinks) }
+// plus, for the retrieved form, those of its head's ids that are in [0, p].
+// With s_j = scale * q.k_j it returns o = sum_j e^(s_j) v_j / sum_j e^(s_j)
+// and lse = log sum_j e^(s_j) over j in V(p); 0 and -inf where V(p) is empty.
+// All kernels walk the keys once with a running maximum m, sum l and
+// unnormalised o (base 2 exponents), so that two disjoint sets of keys join as
+//     m = max(m1, m2), l = l1 2^(m1-m) + l2 2^(m2-m), o likewise.
+//
+// Work split.  Tiles (kv head, request, row tile) differ in length by orders
+// of magnitude (one short decode beside a chunk over a long context), so the
+// unit of work is not the tile but `kUnitChunks` chunks of keys of one tile.
+// All units are numbered in tile order and CTA c of P takes the contiguous
+// range [c*W/P, (c+1)*W/P) of the W units: every CTA gets the same amount of
+// key traffic to within one unit whatever the lengths, and at most its first
+// and its last tile are shared with a neighbour.  Those go to the workspace as
+// partial (o, m, l), which attention_combine_kernel joins in unit order: no
+// atomics, no waiting between CTAs, and the same bits on every run.
+#pragma once
+
+#include <cfloat>
+#include <cstdint>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "fg_internal.h"
+
+namespace fg {
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Header of the workspace and one record per CTA: the tile its range starts in.
+struct alignas(16) TileRecord {
+    int64_t first, last;  // the tile's units [first, last) in the global numbering
+    int32_t head, request, tile, pad;
+};
+constexpr size_t kHeaderBytes = 256;  // int64 W, then padding
+
+__host__ __device__ inline size_t workspace_records_bytes(int ctas) {
+    return kHeaderBytes + ((static_cast<size_t>(ctas) * sizeof(TileRecord) + 255) & ~static_cast<size_t>(255));
+}
+// one partial: rows x dim sums, then rows maxima and rows sums
+__host__ __device__ inline size_t partial_floats(int rows, int dim) { return static_cast<size_t>(rows) * (dim + 2); }
+
+// One request as every kernel reads it, clamped to the buffers the launch was given.
+struct Request {
+    int start, rows, kv_len;  // first query token, new tokens, keys
+};
+
+__device__ __forceinline__ Request load_request(const AttentionParams& a, int b) {
+    Request r;
+    const int s = max(0, min(a.query_start[b], a.tokens)), e = max(0, min(a.query_start[b + 1], a.tokens));
+    r.start = s;
+    r.rows = max(0, e - s);
+    r.kv_len = max(0, a.kv_len[b]);
+    return r;
+}
+
+// The chunks of kChunk keys that one tile visits: those of the first tokens
+// that lie before the window, those of the window (from `base`, up to `hi`),
+// then the retrieved ones.
+struct TileKeys {
+    int lo, hi, base;            // window part: keys [lo, hi), chunks start at base = lo rounded down to 16
+    int sink_hi;                 // first-token part: keys [0, sink_hi)
+    int sink_chunks, near_chunks, id_chunks, chunks;
+    int units;
+};
+
+// Token range [i0, i1] of a tile and the row layout.  Without ids a tile is
+// kRows consecutive (token, head of the group) pairs of a request; with ids it
+// is one token and up to kRows heads of the group.
+template <int kRows, bool kIds>
+struct Tiles {
+    __device__ static __forceinline__ int count(const AttentionParams& a, const Request& r) {
+        if (kIds) return r.rows * ((a.group + kRows - 1) / kRows);
+        return static_cast<int>((static_cast<int64_t>(r.rows) * a.group + kRows - 1) / kRows);
+    }
+    __device__ static __forceinline__ void tokens(const AttentionParams& a, const Request& r, int t, int* i0, int* i1) {
+        if (kIds) {
+            *i0 = *i1 = t / ((a.group + kRows - 1) / kRows);
+        } else {
+            const int64_t first = static_cast<int64_t>(t) * kRows;
+            *i0 = static_cast<int>(first / a.group);
+            *i1 = min(r.rows - 1, static_cast<int>((first + kRows - 1) / a.group));
+        }
+    }
+    // row -> (token of the request, head of the group); false past the tile's end
+    __device__ static __forceinline__ bool row(const AttentionParams& a, const Request& r, int t, int row, int* i, int* g) {
+        if (kIds) {
+            const int hg = (a.group + kRows - 1) / kRows;
+            *i = t / hg;
+            *g = (t % hg) * kRows + row;
+            return *g < a.group;
+        }
+        const int64_t R = static_cast<int64_t>(t) * kRows + row;
+        *i = static_cast<int>(R / a.group);
+        *g = static_cast<int>(R % a.group);
+        return *i < r.rows;
+    }
+};
+
+template <int kRows, bool kIds, int kChunk, int kUnitChunks>
+__device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Request& r, int t) {
+    TileKeys k;
+    int i0, i1;
+    Tiles<kRows, kIds>::tokens(a, r, t, &i0, &i1);
+    const int p0 = r.kv_len - r.rows + i0, p1 = r.kv_len - r.rows + i1;
+    const int64_t room = static_cast<int64_t>(a.table_width) * a.page_size;  // keys that the table can address
+    k.hi = p1 < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(p1) + 1, room));
+    k.lo = (a.window < 0 || p0 < a.window) ? 0 : min(p0 - a.window + 1, k.hi);
+    k.base = k.lo & ~15;
+    k.sink_hi = min(a.sinks, k.base);
+    k.sink_chunks = (k.sink_hi + kChunk - 1) / kChunk;
+    k.near_chunks = (k.hi - k.base + kChunk - 1) / kChunk;
+    k.id_chunks = 0;
+    if (kIds && k.lo > 0) {
+        const int hg = (a.group + kRows - 1) / kRows;
+        const int heads = min(kRows, a.group - (t % hg) * kRows);
+        k.id_chunks = heads * ((a.ids_count + kChunk - 1) / kChunk);
+    }
+    k.chunks = k.sink_chunks + k.near_chunks + k.id_chunks;
+    k.units = max(1, (k.chunks + kUnitChunks - 1) / kUnitChunks);  // a tile that sees nothing still writes its rows
+    return k;
+}
+
+template <int kRows, bool kIds, int kChunk, int kUnitChunks>
+__device__ __forceinline__ int request_units(const AttentionParams& a, const Request& r) {
+    const int n = Tiles<kRows, kIds>::count(a, r);
+    int u = 0;
+    for (int t = 0; t < n; ++t) u += tile_keys<kRows, kIds, kChunk, kUnitChunks>(a, r, t).units;
+    return u;
+}
+
+// Where a CTA's range begins, and the range.
+struct Place {
+    int64_t unit, end;   // this CTA's units [unit, end)
+    int64_t total;       // W
+    int ctas;            // CTAs with a non-empty range: min(P, W)
+    int head, request, tile, offset;  // the first unit: its tile and its place in it
+};
+
+// Called by all kThreads threads; scratch holds requests + 64 ints.
+template <int kRows, bool kIds, int kChunk, int kUnitChunks, int kThreads>
+__device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, int cta, int ctas) {
+    int* pre = scratch + 64;  // inclusive prefix of the requests' units
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kWarps = kThreads / 32;
+    int carry = 0;
+    for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
+        const int b = b0 + tid;
+        int u = 0;
+        if (b < a.requests) u = request_units<kRows, kIds, kChunk, kUnitChunks>(a, load_request(a, b));
+        int s = u;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xFFFFFFFFu, s, d);
+            if (lane >= d) s += v;
+        }
+        if (lane == 31) scratch[warp] = s;
+        __syncthreads();
+        int before = carry, sum = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            const int v = scratch[w];
+            if (w < warp) before += v;
+            sum += v;
+        }
+        if (b < a.requests) pre[b] = before + s;
+        carry += sum;
+        __syncthreads();
+    }
+    Place x;
+    const int64_t per_head = carry;
+    x.total = per_head * a.kv_heads;
+    x.ctas = static_cast<int>(min(static_cast<int64_t>(ctas), x.total));
+    if (cta >= x.ctas) {
+        x.unit = x.end = 0;
+        return x;
+    }
+    x.unit = x.total * cta / x.ctas;
+    x.end = x.total * (cta + 1) / x.ctas;
+    x.head = static_cast<int>(x.unit / per_head);
+    int rest = static_cast<int>(x.unit - x.head * per_head);
+    int lo = 0, hi = a.requests - 1;  // first request whose inclusive prefix exceeds rest
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] > rest) hi = mid;
+        else lo = mid + 1;
+    }
+    x.request = lo;
+    if (lo > 0) rest -= pre[lo - 1];
+    const Request r = load_request(a, lo);
+    const int tiles = Tiles<kRows, kIds>::count(a, r);
+    int t = 0;
+    for (; t + 1 < tiles; ++t) {
+        const int u = tile_keys<kRows, kIds, kChunk, kUnitChunks>(a, r, t).units;
+        if (rest < u) break;
+        rest -= u;
+    }
+    x.tile = t;
+    x.offset = rest;
+    return x;
+}
+
+// The next tile in the numbering after (head, request, tile); false after the last.
+template <int kRows, bool kIds>
+__device__ __forceinline__ bool next_tile(const AttentionParams& a, Request* r, int* head, int* request, int* tile) {
+    if (++*tile < Tiles<kRows, kIds>::count(a, *r)) return true;
+    *tile = 0;
+    do {
+        if (++*request == a.requests) {
+            *request = 0;
+            if (++*head == a.kv_heads) return false;
+        }
+        *r = load_request(a, *request);
+    } while (r->rows == 0);
+    return true;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+struct Half2;
+template <>
+struct Half2<__half> {
+    static constexpr uint32_t kExpMask = 0x7C00u;
+    __device__ static __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    __device__ static __forceinline__ float low(uint32_t v) { return __low2float(*reinterpret_cast<const __half2*>(&v)); }
+    __device__ static __forceinline__ float high(uint32_t v) { return __high2float(*reinterpret_cast<const __half2*>(&v)); }
+};
+template <>
+struct Half2<__nv_bfloat16> {
+    static constexpr uint32_t kExpMask = 0x7F80u;
+    __device__ static __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    __device__ static __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
+    __device__ static __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+};
+
+// Joins the partials of every tile that two or more CTAs of the main kernel
+// shared.  CTA c handles the tile that main CTA c's range starts inside of,
+// if c is the first such CTA.  Bandwidth-bound and tiny: at most 2 partials
+// per main CTA; launched as a dependent of the main kernel so that its start
+// overlaps the main kernel's tail.
+template <typename T, int kRows, int kDim, bool kIds>
+__global__ void __launch_bounds__(128) attention_combine_kernel(const AttentionParams a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const char* ws = static_cast<const char*>(a.workspace);
+    const int64_t total = *reinterpret_cast<const int64_t*>(ws);
+    const int ctas = static_cast<int>(min(static_cast<int64_t>(a.ctas), total));
+    const int c = blockIdx.x / a.combine_split + 1, part = blockIdx.x % a.combine_split;
+    if (c >= ctas) return;
+    const TileRecord rec = reinterpret_cast<const TileRecord*>(ws + kHeaderBytes)[c];
+    const int64_t begin = total * c / ctas, before = total * (c - 1) / ctas;
+    if (begin == rec.first || before > rec.first) return;
+    const float* partials = reinterpret_cast<const float*>(ws + workspace_records_bytes(a.ctas));
+    const size_t psize = partial_floats(kRows, kDim);
+    const float* p0 = partials + (2 * static_cast<size_t>(c - 1) + (before == rec.first ? 0 : 1)) * psize;
+    int last = c;
+    while (last + 1 < ctas && total * (last + 1) / ctas < rec.last) ++last;
+    const Request r = load_request(a, rec.request);
+    // each warp joins whole rows: lane owns 4-float pieces of the row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per = (kRows + a.combine_split - 1) / a.combine_split;
+    for (int row = part * per + warp; row < min(kRows, (part + 1) * per); row += 4) {
+        int i, g;
+        if (!Tiles<kRows, kIds>::row(a, r, rec.tile, row, &i, &g)) continue;
+        float m = p0[kRows * kDim + row], l = p0[kRows * kDim + kRows + row];
+        const int d = lane * 4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (d < kDim) o = *reinterpret_cast<const float4*>(p0 + row * kDim + d);
+        for (int x = c; x <= last; ++x) {
+            const float* p = partials + 2 * static_cast<size_t>(x) * psize;
+            const float m2 = p[kRows * kDim + row], l2 = p[kRows * kDim + kRows + row];
+            const float mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
+            const float s1 = exp2_fast(m - ref), s2 = exp2_fast(m2 - ref);
+            l = l * s1 + l2 * s2;
+            m = mn;
+            if (d < kDim) {
+                const float4 q = *reinterpret_cast<const float4*>(p + row * kDim + d);
+                o.x = o.x * s1 + q.x * s2;
+                o.y = o.y * s1 + q.y * s2;
+                o.z = o.z * s1 + q.z * s2;
+                o.w = o.w * s1 + q.w * s2;
+            }
+        }
+        const float inv = l == 0.f ? 1.f : 1.f / l;
+        const int64_t token = r.start + i;
+        const int head = rec.head * a.group + g;
+        if (d < kDim) {
+            T* out = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride + d;
+            *reinterpret_cast<uint2*>(out) =
+                make_uint2(Half2<T>::pack(o.x * inv, o.y * inv), Half2<T>::pack(o.z * inv, o.w * inv));
+        }
+        if (lane == 0 && a.lse) a.lse[token * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+    }
+}
+
+}  // namespace attn
+}  // namespace fg

@@ -1,0 +1,539 @@
+// fg_attention_rows.cu -- attention of few query rows over the paged cache:
+// decode steps, a few drafted tokens, and the retrieved form.
+//
+// A tile is 16 query rows of one kv head (the heads that share it, times the
+// request's tokens), the height of one m16n8k16 product.  With so few rows a
+// key costs 4*dim bytes of traffic and 16 * 4 * dim multiply-adds on the
+// matrix pipe, a quarter of what that pipe does in the time HBM needs for the
+// bytes: the kernel is bound by bandwidth, and everything serves keeping loads
+// in flight.
+//
+// Layout.  One CTA of 8 warps per SM.  A chunk is 16 keys; warp w of a CTA
+// takes chunks w, w+8, ... of the CTA's range and is on its own until the tile
+// ends: it looks the keys' pages up, copies their K and V rows to its own ring
+// of shared memory with 16-byte cp.async (kStages - 1 chunks ahead), and keeps
+// its own running maximum, sum and 16 x dim output in registers, so no barrier
+// sits between a load and its use.  Gathering by row costs nothing extra over
+// a tile copy here, and makes pages of any size, any strides, windows that
+// start inside a page and retrieved ids the same code.  At a tile's end the 8
+// warps join through shared memory.
+//
+// Retrieved ids are chunks like the others: 16 ids of one head, whose scores
+// count in that head's row alone.  The other rows' share of the product is
+// waste on a pipe that idles anyway.
+#include "fg_attention.cuh"
+
+namespace fg {
+namespace attn {
+namespace {
+
+constexpr int kRows = 16;
+constexpr int kChunk = 16;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+
+template <int kDim>
+struct Smem {
+    static constexpr int kPitch = kDim * 2 + 16;  // odd multiple of 16 bytes: ldmatrix reads 8 rows without conflicts
+    static constexpr int kTile = kChunk * kPitch;
+    static constexpr int kStages = 3;
+    static constexpr int kRing = kStages * 2 * kTile;  // K and V of each stage
+    static constexpr int kWarpBytes = kRing;
+    static constexpr int kBytes = kWarps * kWarpBytes;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+    const int n = ok ? 16 : 0;  // 0: the destination is filled with zeros and nothing is read
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The element offset of key j's row in the cache (either half), or -1 where
+// the table has no page for it.
+__device__ __forceinline__ int64_t key_offset(const AttentionParams& a, const int32_t* table, int j, int64_t head_off) {
+    const int page = j >> a.page_shift;
+    if (page >= a.table_width) return -1;
+    const int id = __ldg(table + page);
+    if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.pages)) return -1;
+    return id * a.page_stride + (j & (a.page_size - 1)) * a.token_stride + head_off;
+}
+
+// One chunk in flight.
+struct Chunk {
+    int key;        // first key (contiguous chunks)
+    int row;        // row that alone sees it (retrieved ids), or -1
+    uint32_t ok;    // bit i: key i is loaded and may be visible
+};
+
+template <typename T, int kDim, bool kIds>
+struct Warp {
+    using S = Smem<kDim>;
+    static constexpr int kPieces = kDim / 8;              // 16-byte pieces of a row
+    static constexpr int kCopies = kChunk * kPieces / 32;  // per lane and operand
+
+    const AttentionParams& a;
+    const int lane;
+    const uint32_t ring;
+    // the tile
+    Request req;
+    TileKeys keys;
+    const int32_t* table;
+    int64_t head_off;
+    int p0, p1;        // positions of the tile's first and last row
+    int prow[2];       // positions of this lane's two rows (-1: no row)
+    const int32_t* ids;  // retrieved ids of the tile's first row
+    // running state
+    uint32_t q[kDim / 16][4];
+    float o[kDim / 8][4];
+    float m[2], l[2];
+
+    __device__ __forceinline__ Warp(const AttentionParams& args, uint32_t ring_addr)
+        : a(args), lane(threadIdx.x & 31), ring(ring_addr) {}
+
+    __device__ __forceinline__ void begin(int head, int request, int tile) {
+        table = a.block_table + request * a.table_stride;
+        head_off = head * a.head_stride;
+        int i0, i1;
+        Tiles<kRows, kIds>::tokens(a, req, tile, &i0, &i1);
+        p0 = req.kv_len - req.rows + i0;
+        p1 = req.kv_len - req.rows + i1;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            int i, g;
+            const bool ok = Tiles<kRows, kIds>::row(a, req, tile, (lane >> 2) + 8 * x, &i, &g);
+            prow[x] = ok ? req.kv_len - req.rows + i : -1;
+            const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(req.start + i) * a.q_token_stride +
+                           static_cast<int64_t>(head * a.group + g) * a.q_head_stride + (lane & 3) * 2;
+#pragma unroll
+            for (int k = 0; k < kDim / 16; ++k) {
+                q[k][x] = ok ? *reinterpret_cast<const uint32_t*>(src + k * 16) : 0u;
+                q[k][x + 2] = ok ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8) : 0u;
+            }
+        }
+        if (kIds) {
+            int i, g;
+            Tiles<kRows, kIds>::row(a, req, tile, 0, &i, &g);
+            ids = a.ids + static_cast<int64_t>(req.start + i) * a.ids_token_stride +
+                  static_cast<int64_t>(head * a.group + g) * a.ids_head_stride;
+        }
+#pragma unroll
+        for (int n = 0; n < kDim / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+    }
+
+    // Looks chunk c's keys up and starts its copies into stage s.
+    __device__ __forceinline__ Chunk load(int c, int s) {
+        Chunk ch;
+        ch.row = -1;
+        ch.key = 0;
+        const int x = lane & 15;
+        int64_t off = -1;
+        if (c < keys.sink_chunks) {
+            ch.key = c * kChunk;
+            if (ch.key + x < keys.sink_hi) off = key_offset(a, table, ch.key + x, head_off);
+        } else if (c < keys.sink_chunks + keys.near_chunks) {
+            ch.key = keys.base + (c - keys.sink_chunks) * kChunk;
+            const int j = ch.key + x;
+            if (j < keys.hi && (j >= keys.lo || j < a.sinks)) off = key_offset(a, table, j, head_off);
+        } else if (kIds) {
+            const int per = (a.ids_count + kChunk - 1) / kChunk;
+            const int at = c - keys.sink_chunks - keys.near_chunks;
+            ch.row = at / per;
+            const int n = (at % per) * kChunk + x;
+            const int32_t* list = ids + ch.row * a.ids_head_stride;
+            const int id = n < a.ids_count ? __ldg(list + n) : -1;
+            // visible by the mask already (window, first tokens), beyond the row's position, or an empty place
+            bool fresh = id >= a.sinks && id <= p0 && p0 - id >= a.window && id >= 0;
+            // an id that stands earlier in the list counts there
+            const int stop = (at % per) * kChunk + kChunk;
+            for (int e0 = 0; e0 < stop; e0 += 32) {
+                const int e = e0 + lane;
+                const int other = e < a.ids_count ? __ldg(list + e) : -1;
+#pragma unroll
+                for (int y = 0; y < kChunk; ++y) {
+                    const int idy = __shfl_sync(0xFFFFFFFFu, id, y);
+                    const int ny = (at % per) * kChunk + y;
+                    const bool hit = __any_sync(0xFFFFFFFFu, other == idy && e < ny);
+                    if (x == y && hit) fresh = false;
+                }
+            }
+            if (fresh) off = key_offset(a, table, id, head_off);
+        }
+        ch.ok = __ballot_sync(0xFFFFFFFFu, off >= 0) & 0xFFFFu;
+        const uint32_t dst = ring + s * 2 * S::kTile;
+        const T* kc = static_cast<const T*>(a.k_cache);
+        const T* vc = static_cast<const T*>(a.v_cache);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int idx = i * 32 + lane, r = idx / kPieces, p = idx % kPieces;
+            const int64_t ro = __shfl_sync(0xFFFFFFFFu, off, r);
+            const bool ok = ro >= 0;
+            const int64_t from = ok ? ro + p * 8 : 0;
+            const uint32_t to = dst + r * S::kPitch + p * 16;
+            copy16(to, kc + from, ok);
+            copy16(to + S::kTile, vc + from, ok);
+        }
+        return ch;
+    }
+
+    __device__ __forceinline__ bool sees(const Chunk& ch, int x, int col) const {
+        if (!((ch.ok >> col) & 1u)) return false;
+        if (kIds && ch.row >= 0) return (lane >> 2) + 8 * x == ch.row;
+        const int j = ch.key + col, p = prow[x];
+        return j <= p && (a.window < 0 || p - j < a.window || j < a.sinks);
+    }
+
+    // V rows that some rows of the tile see and others do not: 0 * inf and
+    // 0 * NaN must not reach the ones that do not.  Each lane checks and clears
+    // the pieces that it copied itself.
+    __device__ __forceinline__ bool clear_nonfinite(int s) {
+        const uint32_t dst = ring + s * 2 * S::kTile + S::kTile;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int idx = i * 32 + lane, r = idx / kPieces, p = idx % kPieces;
+            const uint32_t at = dst + r * S::kPitch + p * 16;
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(at)
+                         : "memory");
+            bool here = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                constexpr uint32_t kE = Half2<T>::kExpMask;
+                if ((w[e] & kE) == kE) {
+                    w[e] &= 0xFFFF0000u;
+                    here = true;
+                }
+                if ((w[e] & (kE << 16)) == (kE << 16)) {
+                    w[e] &= 0x0000FFFFu;
+                    here = true;
+                }
+            }
+            if (here) {
+                bad = true;
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                             : "memory");
+            }
+        }
+        return __any_sync(0xFFFFFFFFu, bad);
+    }
+
+    // ... and the rows that do see them get them back.
+    __device__ __forceinline__ void add_nonfinite(const Chunk ch) {
+        const T* vc = static_cast<const T*>(a.v_cache);
+#pragma unroll 1
+        for (int col = 0; col < kChunk; ++col) {
+            if (!((ch.ok >> col) & 1u)) continue;
+            const bool see0 = sees(ch, 0, col), see1 = sees(ch, 1, col);
+            int j = ch.key + col;
+            if (kIds && ch.row >= 0) {
+                const int per = (a.ids_count + kChunk - 1) / kChunk;
+                j = __ldg(ids + ch.row * a.ids_head_stride + (id_chunk % per) * kChunk + col);
+            }
+            const T* src = vc + key_offset(a, table, j, head_off) + (lane & 3) * 2;
+#pragma unroll
+            for (int n = 0; n < kDim / 8; ++n) {
+                const uint32_t w = *reinterpret_cast<const uint32_t*>(src + n * 8);
+                const float v0 = Half2<T>::low(w), v1 = Half2<T>::high(w);
+                if (!isfinite(v0)) {
+                    if (see0) o[n][0] += v0;
+                    if (see1) o[n][2] += v0;
+                }
+                if (!isfinite(v1)) {
+                    if (see0) o[n][1] += v1;
+                    if (see1) o[n][3] += v1;
+                }
+            }
+        }
+    }
+    int id_chunk;  // number among the retrieved chunks of the chunk in work
+
+    __device__ __forceinline__ void compute(const Chunk& ch, int s) {
+        const uint32_t kt = ring + s * 2 * S::kTile, vt = kt + S::kTile;
+        float sc[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+        // keys (lane & 7) + 8 * (lane >= 16), k offset 8 * ((lane >> 3) & 1)
+        const uint32_t kaddr = kt + ((lane & 7) + ((lane >> 4) << 3)) * S::kPitch + ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int k = 0; k < kDim / 16; ++k) {
+            uint32_t b[4];
+            ldmatrix4(kaddr + k * 32, b);
+            mma<T>(sc[0], q[k], b[0], b[1]);
+            mma<T>(sc[1], q[k], b[2], b[3]);
+        }
+        const bool whole = ch.ok == 0xFFFFu && ch.row < 0 && ch.key + kChunk - 1 <= p0 &&
+                           (a.window < 0 || p1 - ch.key < a.window || ch.key + kChunk - 1 < a.sinks);
+        bool poison = false;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[n][e] *= a.scale_log2;
+        if (!whole) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (!sees(ch, e >> 1, n * 8 + (lane & 3) * 2 + (e & 1))) sc[n][e] = -INFINITY;
+            if (p0 != p1 || ch.row >= 0) poison = clear_nonfinite(s);
+            __syncwarp();
+        }
+        uint32_t pa[4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            float mx = fmaxf(fmaxf(sc[0][2 * x], sc[0][2 * x + 1]), fmaxf(sc[1][2 * x], sc[1][2 * x + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+            const float mn = fmaxf(m[x], mx), ref = mn == -INFINITY ? 0.f : mn;
+            if (__any_sync(0xFFFFFFFFu, mn > m[x])) {
+                const float f = exp2_fast(m[x] - ref);
+                l[x] *= f;
+#pragma unroll
+                for (int n = 0; n < kDim / 8; ++n) {
+                    o[n][2 * x] *= f;
+                    o[n][2 * x + 1] *= f;
+                }
+                m[x] = mn;
+            }
+            float e0 = exp2_fast(sc[0][2 * x] - ref), e1 = exp2_fast(sc[0][2 * x + 1] - ref);
+            float e2 = exp2_fast(sc[1][2 * x] - ref), e3 = exp2_fast(sc[1][2 * x + 1] - ref);
+            l[x] += (e0 + e1) + (e2 + e3);  // this lane's columns; joined over the 4 lanes of a row at the end
+            // weights go to the product in the cache's 16-bit type, as the matrix pipe takes them: at most 1, relative
+            // rounding 2^-8 (bf16) or 2^-11, in size that of the result's own rounding; the sum l keeps 32 bits
+            pa[x] = Half2<T>::pack(e0, e1);
+            pa[x + 2] = Half2<T>::pack(e2, e3);
+        }
+        // keys (lane & 15), dims 8 * (lane >= 16)
+        const uint32_t vaddr = vt + (lane & 15) * S::kPitch + (lane >> 4) * 16;
+#pragma unroll
+        for (int n = 0; n < kDim / 16; ++n) {
+            uint32_t b[4];
+            ldmatrix4_trans(vaddr + n * 32, b);
+            mma<T>(o[2 * n], pa, b[0], b[1]);
+            mma<T>(o[2 * n + 1], pa, b[2], b[3]);
+        }
+        if (poison) add_nonfinite(ch);
+    }
+};
+
+template <typename T, int kDim, bool kIds>
+__global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const AttentionParams a) {
+    using S = Smem<kDim>;
+    extern __shared__ __align__(128) char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    char* ws = static_cast<char*>(a.workspace);
+
+    const Place pl = locate<kRows, kIds, kChunk, kWarps, kThreads>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
+    __syncthreads();  // the rings overlay the scan
+    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
+    if (pl.unit >= pl.end) return;
+
+    Warp<T, kDim, kIds> w(a, smem_addr(smem) + warp * S::kWarpBytes);
+    int head = pl.head, request = pl.request, tile = pl.tile;
+    int64_t unit = pl.unit, tile_first = pl.unit - pl.offset;
+    w.req = load_request(a, request);
+    w.keys = tile_keys<kRows, kIds, kChunk, kWarps>(a, w.req, tile);
+    if (threadIdx.x == 0) {
+        TileRecord rec;
+        rec.first = tile_first;
+        rec.last = tile_first + w.keys.units;
+        rec.head = head;
+        rec.request = request;
+        rec.tile = tile;
+        rec.pad = 0;
+        reinterpret_cast<TileRecord*>(ws + kHeaderBytes)[blockIdx.x] = rec;
+    }
+    bool first_segment = true;
+    while (true) {
+        const int64_t tile_last = tile_first + w.keys.units;
+        const int u0 = static_cast<int>(unit - tile_first);
+        const int u1 = static_cast<int>(min(tile_last, pl.end) - tile_first);
+        const int c1 = min(u1 * kWarps, w.keys.chunks);
+        w.begin(head, request, tile);
+        // the chunks in flight: a shift register of kStages - 1 descriptors
+        Chunk flight[S::kStages - 1];
+        int c = u0 * kWarps + warp;
+#pragma unroll
+        for (int s = 0; s < S::kStages - 1; ++s) {
+            if (c + s * kWarps < c1) flight[s] = w.load(c + s * kWarps, s);
+            copy_commit();
+        }
+        int stage = 0;
+        for (; c < c1; c += kWarps) {
+            copy_wait<S::kStages - 2>();
+            __syncwarp();
+            const Chunk now = flight[0];
+#pragma unroll
+            for (int s = 0; s + 1 < S::kStages - 1; ++s) flight[s] = flight[s + 1];
+            const int ahead = c + (S::kStages - 1) * kWarps;
+            int next = stage + S::kStages - 1;
+            if (next >= S::kStages) next -= S::kStages;
+            if (ahead < c1) flight[S::kStages - 2] = w.load(ahead, next);
+            copy_commit();
+            w.id_chunk = c - w.keys.sink_chunks - w.keys.near_chunks;
+            w.compute(now, stage);
+            if (++stage == S::kStages) stage = 0;
+            __syncwarp();
+        }
+        copy_wait<0>();
+
+        // join the 8 warps: rows of (m, l) and sums, over the rings
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            w.l[x] += __shfl_xor_sync(0xFFFFFFFFu, w.l[x], 1);
+            w.l[x] += __shfl_xor_sync(0xFFFFFFFFu, w.l[x], 2);
+        }
+        __syncthreads();
+        constexpr int kSumPitch = kDim + 4;
+        float* sums = reinterpret_cast<float*>(smem);                       // [warp][row][kSumPitch]
+        float* stat = sums + kWarps * kRows * kSumPitch;                    // [warp][row][2]
+        static_assert((kWarps * kRows * (kSumPitch + 2)) * 4 <= S::kBytes, "the join fits the rings");
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int row = (lane >> 2) + 8 * x;
+            float* dst = sums + (warp * kRows + row) * kSumPitch + (lane & 3) * 2;
+#pragma unroll
+            for (int n = 0; n < kDim / 8; ++n)
+                *reinterpret_cast<float2*>(dst + n * 8) = make_float2(w.o[n][2 * x], w.o[n][2 * x + 1]);
+            if ((lane & 3) == 0) {
+                stat[(warp * kRows + row) * 2] = w.m[x];
+                stat[(warp * kRows + row) * 2 + 1] = w.l[x];
+            }
+        }
+        __syncthreads();
+        const bool whole_tile = u0 == 0 && u1 == w.keys.units;
+        float* part = nullptr;
+        if (!whole_tile) {
+            const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first_segment ? 0 : 1);
+            part = reinterpret_cast<float*>(ws + workspace_records_bytes(a.ctas)) + slot * partial_floats(kRows, kDim);
+        }
+        for (int idx = threadIdx.x; idx < kRows * (kDim / 4); idx += kThreads) {
+            const int row = idx / (kDim / 4), d = (idx % (kDim / 4)) * 4;
+            float mm = -INFINITY;
+#pragma unroll
+            for (int y = 0; y < kWarps; ++y) mm = fmaxf(mm, stat[(y * kRows + row) * 2]);
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            float ll = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int y = 0; y < kWarps; ++y) {
+                const float f = exp2_fast(stat[(y * kRows + row) * 2] - ref);
+                ll += stat[(y * kRows + row) * 2 + 1] * f;
+                const float4 v = *reinterpret_cast<const float4*>(sums + (y * kRows + row) * kSumPitch + d);
+                acc.x += v.x * f;
+                acc.y += v.y * f;
+                acc.z += v.z * f;
+                acc.w += v.w * f;
+            }
+            if (whole_tile) {
+                int i, g;
+                if (Tiles<kRows, kIds>::row(a, w.req, tile, row, &i, &g)) {
+                    const float inv = ll == 0.f ? 1.f : 1.f / ll;
+                    const int64_t token = w.req.start + i;
+                    const int h = head * a.group + g;
+                    T* out = static_cast<T*>(a.out) + token * a.out_token_stride + h * a.out_head_stride + d;
+                    *reinterpret_cast<uint2*>(out) = make_uint2(Half2<T>::pack(acc.x * inv, acc.y * inv),
+                                                                Half2<T>::pack(acc.z * inv, acc.w * inv));
+                    if (d == 0 && a.lse) a.lse[token * a.heads + h] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * kLn2;
+                }
+            } else {
+                *reinterpret_cast<float4*>(part + row * kDim + d) = acc;
+                if (d == 0) {
+                    part[kRows * kDim + row] = mm;
+                    part[kRows * kDim + kRows + row] = ll;
+                }
+            }
+        }
+        unit = tile_first + u1;
+        if (unit >= pl.end) break;
+        tile_first = tile_last;
+        if (!next_tile<kRows, kIds>(a, &w.req, &head, &request, &tile)) break;
+        w.keys = tile_keys<kRows, kIds, kChunk, kWarps>(a, w.req, tile);
+        first_segment = false;
+        __syncthreads();  // the join's reads end before the next tile's copies
+    }
+}
+
+template <typename T, int kDim, bool kIds>
+cudaError_t launch(AttentionParams a, cudaStream_t stream) {
+    constexpr int bytes = Smem<kDim>::kBytes;
+    cudaError_t e = cudaFuncSetAttribute(attention_rows_kernel<T, kDim, kIds>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    attention_rows_kernel<T, kDim, kIds><<<a.ctas, kThreads, bytes, stream>>>(a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    a.combine_split = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(max(1, a.ctas - 1)));
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_combine_kernel<T, kRows, kDim, kIds>, a);
+}
+
+template <typename T, int kDim>
+cudaError_t by_ids(const AttentionParams& a, cudaStream_t s) {
+    return a.ids ? launch<T, kDim, true>(a, s) : launch<T, kDim, false>(a, s);
+}
+template <typename T>
+cudaError_t by_dim(const AttentionParams& a, cudaStream_t s) {
+    switch (a.dim) {
+        case 64: return by_ids<T, 64>(a, s);
+        case 96: return by_ids<T, 96>(a, s);
+        default: return by_ids<T, 128>(a, s);
+    }
+}
+
+}  // namespace
+}  // namespace attn
+
+size_t attention_rows_workspace(int ctas, int dim) {
+    return attn::workspace_records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * attn::partial_floats(attn::kRows, dim) * sizeof(float);
+}
+int attention_max_requests() { return 16384; }
+
+cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream) {
+    return a.dtype == FG_DTYPE_BF16 ? attn::by_dim<__nv_bfloat16>(a, stream) : attn::by_dim<__half>(a, stream);
+}
+
+}  // namespace fg

@@ -78,6 +78,69 @@ int shard_merge_max_shards();
 cudaError_t launch_shard_merge(const uint32_t* ids, const float* dists, const uint32_t* offsets, int shards, int nq,
                                int k, int K, uint32_t* out_ids, float* out_dists, cudaStream_t stream);
 
+// ---- key/value cache and attention (fg_kv.cu, fg_attention_rows.cu, fg_attention_tiles.cu) ----
+
+struct PlanArgs {
+    const int32_t* ctx_len = nullptr;
+    const int32_t* new_len = nullptr;
+    const int32_t* free_pages = nullptr;
+    const int32_t* free_head = nullptr;  // optional
+    int32_t* block_table = nullptr;
+    int32_t* query_start = nullptr;
+    int32_t* kv_len = nullptr;
+    int32_t* position = nullptr;
+    int64_t* slot = nullptr;
+    int32_t* free_head_out = nullptr;
+    int32_t* refused = nullptr;
+    int64_t table_stride = 0;
+    int requests = 0, free_count = 0, page_shift = 0, table_width = 0, tokens = 0;
+};
+int kv_plan_max_requests();
+cudaError_t launch_kv_plan(const PlanArgs& a, cudaStream_t stream);
+
+struct AppendArgs {
+    void* k_cache = nullptr;
+    void* v_cache = nullptr;
+    const void* k = nullptr;
+    const void* v = nullptr;
+    const int64_t* slot = nullptr;
+    int64_t page_stride = 0, token_stride = 0, head_stride = 0;  // of the cache, in 16-byte pieces
+    int64_t k_token_stride = 0, k_head_stride = 0, v_token_stride = 0, v_head_stride = 0;  // in 16-byte pieces
+    int pages = 0, page_shift = 0, heads = 0, pieces = 0;  // pieces: 16-byte pieces of a row
+    int tokens = 0;
+};
+cudaError_t launch_kv_append(const AppendArgs& a, cudaStream_t stream);
+
+struct AttentionParams {
+    const void* k_cache = nullptr;
+    const void* v_cache = nullptr;
+    int64_t page_stride = 0, token_stride = 0, head_stride = 0;  // elements
+    int pages = 0, page_size = 0, page_shift = 0;
+    int dim = 0, dtype = 0;
+    const void* q = nullptr;
+    int64_t q_token_stride = 0, q_head_stride = 0;
+    void* out = nullptr;
+    int64_t out_token_stride = 0, out_head_stride = 0;
+    float* lse = nullptr;  // [tokens, heads], optional
+    const int32_t* block_table = nullptr;
+    int64_t table_stride = 0;
+    int table_width = 0;
+    const int32_t* query_start = nullptr;
+    const int32_t* kv_len = nullptr;
+    int requests = 0, tokens = 0, heads = 0, kv_heads = 0, group = 0;
+    int window = -1, sinks = 0;
+    float scale_log2 = 0.f;  // scale * log2(e): all exponents are base 2
+    const int32_t* ids = nullptr;
+    int ids_count = 0;
+    int64_t ids_token_stride = 0, ids_head_stride = 0;
+    void* workspace = nullptr;
+    int ctas = 0;           // CTAs that share the work
+    int combine_split = 1;  // CTAs that join one tile's partials
+};
+int attention_max_requests();
+size_t attention_rows_workspace(int ctas, int dim);
+cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream);
+
 // Host restatements shared with the CLI and the API.
 uint32_t effective_sort_beam(uint32_t beam);
 uint32_t candidate_buffer_size(int degree);

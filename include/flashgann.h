@@ -241,6 +241,115 @@ int fg_beam_merge_device(uint32_t* d_idx, float* d_dist, int32_t ncase, int32_t 
 int fg_shard_merge_device(const uint32_t* d_ids, const float* d_dists, const uint32_t* shard_offsets, int32_t shards,
                           int32_t nq, int32_t k, int32_t K, uint32_t* d_out_ids, float* d_out_dists, void* stream);
 
+/* ---- key/value cache and attention over it ----
+ *
+ * What a decoder needs next to a search over its keys (metric
+ * FG_METRIC_IP: the base is the keys of one kv head, a query is a query
+ * vector, the ids are positions of the context): a paged cache that the
+ * positions address, and attention over the first tokens, a sliding window
+ * and the retrieved ids.  No counterpart in the reference, which ends at the
+ * ids.
+ *
+ * All calls run on the calling thread's current device and are asynchronous
+ * on `stream` (a cudaStream_t, NULL = default stream); they allocate nothing,
+ * keep nothing and may be captured in a CUDA graph.  Buffers are device
+ * memory and must not overlap.  Lengths, tables, slots and ids are read on
+ * the device: values that address nothing (negative or too large pages,
+ * slots, ids) are skipped, never followed. */
+
+/* Element types of queries, caches and outputs. */
+#define FG_DTYPE_F16 0
+#define FG_DTYPE_BF16 1
+
+/* A paged cache: position j of a request lies in page block_table[j /
+ * page_size], row j % page_size.  Row (page, t, head) of K starts at element
+ * page * page_stride + t * token_stride + head * head_stride of k, and of V
+ * likewise of v: any order of the axes, and slices of a larger buffer.
+ * k, v and the strides in bytes must be multiples of 16; page_size a power of
+ * two; dim 64, 96 or 128, contiguous. */
+typedef struct fg_kv_cache {
+    void* k;
+    void* v;
+    int64_t page_stride, token_stride, head_stride; /* elements */
+    int32_t pages, page_size, heads, dim, dtype;
+} fg_kv_cache;
+
+/* The plan of one step for a batch of requests: request b has d_ctx_len[b]
+ * tokens in the cache and gets d_new_len[b] more (negative: 0).
+ * d_block_table [requests, table_width] (rows table_stride elements apart)
+ * holds the pages of the first and receives those of the rest, taken in
+ * request order from d_free_pages[free_count], starting at *d_free_head (NULL:
+ * 0).  Outputs: d_query_start[requests+1], the first row of each request in
+ * the step's token tensors; d_kv_len[requests] = ctx + new; for each token
+ * row d_position[tokens] and d_slot[tokens] (page * page_size + row), -1 past
+ * the last request's; d_free_head_out[1], the first page not taken (not
+ * d_free_head itself, which other CTAs may still be reading);
+ * d_refused[requests], 1 for a request that got nothing because its length
+ * passes the table's width, or because it needs pages that are no longer
+ * there after the requests before it (one that needs none goes on): its kv_len
+ * is 0, its positions and slots -1, its table row as it was.
+ * At most 8192 requests. */
+int fg_kv_plan_device(const int32_t* d_ctx_len, const int32_t* d_new_len, int32_t requests,
+                      const int32_t* d_free_pages, int32_t free_count, const int32_t* d_free_head, int32_t page_size,
+                      int32_t* d_block_table, int32_t table_width, int64_t table_stride, int32_t tokens,
+                      int32_t* d_query_start, int32_t* d_kv_len, int32_t* d_position, int64_t* d_slot,
+                      int32_t* d_free_head_out, int32_t* d_refused, void* stream);
+
+/* Writes the new tokens' rows to the cache: row t of d_k and d_v [tokens,
+ * heads, dim] (token and head strides in elements, multiples of 16 bytes) to
+ * slot d_slot[t]; slots below 0 or past the cache are skipped.  Slots of one
+ * call must differ. */
+int fg_kv_append_device(const fg_kv_cache* cache, const void* d_k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void* d_v, int64_t v_token_stride, int64_t v_head_stride, const int64_t* d_slot,
+                        int32_t tokens, void* stream);
+
+/* Arguments of the attention calls. */
+typedef struct fg_attention {
+    const void* q;                              /* [tokens, heads, dim] of the cache's dtype */
+    int64_t q_token_stride, q_head_stride;      /* elements, multiples of 16 bytes */
+    void* out;                                  /* [tokens, heads, dim] */
+    int64_t out_token_stride, out_head_stride;
+    float* lse;                                 /* [tokens, heads], natural log; NULL: not written */
+    const int32_t* block_table;                 /* [requests, table_width] */
+    int64_t table_stride;
+    const int32_t* query_start;                 /* [requests + 1] */
+    const int32_t* kv_len;                      /* [requests], new tokens included */
+    const int32_t* ids;                         /* fg_retrieved_attention_device: [tokens, heads, ids_count] */
+    int64_t ids_token_stride, ids_head_stride;
+    void* workspace;                            /* fg_attention_workspace_bytes, 256-byte aligned; contents do not matter */
+    uint64_t workspace_bytes;
+    int32_t tokens, heads, requests, table_width;
+    int32_t max_new;                            /* most new tokens of a request: picks the kernel, not the result */
+    int32_t window;                             /* -1: none */
+    int32_t sinks;
+    int32_t ids_count;
+    float scale;
+} fg_attention;
+
+/* Bytes of workspace that an attention call needs on the current device
+ * (partial results of rows whose keys are split over CTAs). */
+int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* args, uint64_t* bytes);
+
+/* Causal attention of a batch's new tokens over the cache.  Token i of
+ * request b (row query_start[b] + i) stands at p = kv_len[b] - new_b + i and
+ * sees the keys 0 <= j <= p, with a window >= 0 those with p - j < window or
+ * j < sinks; query head h reads kv head h / (heads / cache->heads).  out =
+ * softmax(scale * q.k) v over the visible keys, lse = log of the sum of
+ * exponentials; a row that sees nothing (or only scores of -inf) gets 0 and
+ * -inf.  K and V of keys that a row does not see do not touch it, whatever
+ * they hold.  Sums are kept in 32 bits; the weights of the second product are
+ * rounded to the cache's type.  Results are the same on every run.  Rows past
+ * query_start[requests] are not written.  At most 16384 requests, heads /
+ * cache->heads <= 256. */
+int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream);
+
+/* The same with retrieved keys: row (token, head) also sees the positions in
+ * ids[token, head, :] that are in [0, p].  The visible keys are a set: an id
+ * that repeats, or that the window or the first tokens hold already, counts
+ * once; ids outside [0, p] (such as the search's padding, 0xFFFFFFFF) count
+ * nothing.  Needs a window >= 0. */
+int fg_retrieved_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream);
+
 /* ---- host helpers of the reference CLI ---- */
 
 /* include/utils.cuh:119-127 */
