@@ -15,7 +15,7 @@ LIB     := flashgann_b200/libflashgann.so
 BIN_DIR := bin
 
 KERNEL_SRC := $(CSRC)/fg_search.cu $(CSRC)/fg_search_warp.cu $(CSRC)/fg_shard_merge.cu $(CSRC)/fg_kv.cu \
-              $(CSRC)/fg_attention_rows.cu $(CSRC)/fg_api.cu
+              $(CSRC)/fg_attention_rows.cu $(CSRC)/fg_attention_tiles.cu $(CSRC)/fg_api.cu
 HEADERS    := $(CSRC)/fg_config.h $(CSRC)/fg_internal.h $(CSRC)/fg_device.cuh include/flashgann.h
 ATTN_HEADERS := $(CSRC)/fg_attention.cuh
 OBJ_DIR    := flashgann_b200/_build
@@ -33,7 +33,7 @@ $(OBJ_DIR)/%.o: $(CSRC)/%.cu $(HEADERS) | $(OBJ_DIR)
 $(OBJ_DIR):
 	mkdir -p $(OBJ_DIR)
 
-$(OBJ_DIR)/fg_attention_rows.o: $(ATTN_HEADERS)
+$(OBJ_DIR)/fg_attention_rows.o $(OBJ_DIR)/fg_attention_tiles.o: $(ATTN_HEADERS)
 
 $(LIB): $(OBJS)
 	$(NVCC) $(GENCODE) -shared -o $@ $(OBJS)

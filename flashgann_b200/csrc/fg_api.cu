@@ -850,6 +850,15 @@ int sm_count(int* sms) {
     return e == cudaSuccess ? FG_OK : fail(FG_ERR_NO_DEVICE, "no CUDA device available (%s)", cudaGetErrorString(e));
 }
 
+// Which kernel takes a call: requests of up to 16 rows for each kv head (new
+// tokens x heads of the group) fill one tile of the rows kernel; above that it
+// would read the keys once for each 16 rows, and the tiles kernel takes them
+// 256 at a time.  That one folds the scale into its maxima, so it needs a
+// positive one.
+bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
+    return !retrieved && x->scale > 0.f && static_cast<int64_t>(x->max_new) * (x->heads / c->heads) > 16;
+}
+
 int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void* stream) {
     int rc = check_cache(c);
     if (rc) return rc;
@@ -922,7 +931,8 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     }
     a.workspace = x->workspace;
     if ((rc = sm_count(&a.ctas))) return rc;
-    const cudaError_t e = fg::launch_attention_rows(a, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = takes_tiles(c, x, retrieved) ? fg::launch_attention_tiles(a, static_cast<cudaStream_t>(stream))
+                                                       : fg::launch_attention_rows(a, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? FG_OK : cuda_fail(e, "attention launch");
 }
 
@@ -1007,7 +1017,10 @@ int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* a
     if (!args || !bytes) return fail(FG_ERR_ARG, "null argument");
     int sms = 0;
     if ((rc = sm_count(&sms))) return rc;
-    *bytes = fg::attention_rows_workspace(sms, cache->dim);
+    if (args->heads < 1 || args->heads % cache->heads)
+        return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", args->heads, cache->heads);
+    *bytes = takes_tiles(cache, args, args->ids != nullptr) ? fg::attention_tiles_workspace(sms, cache->dim)
+                                                            : fg::attention_rows_workspace(sms, cache->dim);
     return FG_OK;
 }
 

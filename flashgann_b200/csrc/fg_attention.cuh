@@ -236,6 +236,7 @@ struct Half2;
 template <>
 struct Half2<__half> {
     static constexpr uint32_t kExpMask = 0x7C00u;
+    static constexpr uint32_t kFormat = 0;  // as an operand of tcgen05.mma
     __device__ static __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -246,6 +247,7 @@ struct Half2<__half> {
 template <>
 struct Half2<__nv_bfloat16> {
     static constexpr uint32_t kExpMask = 0x7F80u;
+    static constexpr uint32_t kFormat = 1;
     __device__ static __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);

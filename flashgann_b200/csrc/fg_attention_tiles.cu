@@ -1,0 +1,734 @@
+// fg_attention_tiles.cu -- attention of many query rows over the paged cache:
+// prompts' chunks, and decodes that share a call with them.
+//
+// A tile is 256 query rows of one kv head (tokens x heads of the group), two
+// halves of 128; a block is 128 keys.  For each block and half the tensor
+// cores compute S = Q K^T into TMEM (tcgen05.mma, 128 x 128 x dim), the half's
+// warpgroup turns S into weights P = 2^(scale S - m) in place, one row to a
+// thread, and the tensor cores add P V to the output in TMEM with P as their
+// TMEM operand.  TMEM holds exactly S/P and O of both halves: 4 x 128 columns.
+//
+// Warp roles (16 warps, one CTA per SM):
+//   0-3, 4-7   softmax of half 0 and 1 (192 registers a thread)
+//   8-11       loads: 16-byte cp.async of whole key rows, gathered by page, into
+//              a ring of K and V tiles in the 128-byte swizzled layout that
+//              tcgen05 reads; zeros for rows that do not exist
+//   12         issues the products
+// The two halves run in antiphase: while half 0's weights are computed the
+// tensor cores work on half 1.
+//
+// What bounds it: per block and half 4 * 128 * 128 * dim operations, 1024
+// cycles of the tensor pipe at dim 128, and 128 * 128 exponentials, 1024
+// cycles of the SM's special-function units: both pipes are needed for the
+// whole time, see exp2_mixed.
+//
+// The running maximum that the weights are relative to is raised only when it
+// grows by more than 2^8: then O and the sum are scaled, which costs a round
+// trip of O through registers.  Weights up to 2^8 keep their relative
+// precision in both 16-bit types, and the 32-bit sums have room.
+//
+// Every wait is bounded: one that runs out marks the CTA, all roles leave
+// their loops, and the rows of the tiles in work get NaN.
+#include "fg_attention.cuh"
+
+namespace fg {
+namespace attn {
+namespace {
+
+constexpr int kRows = 256;
+constexpr int kHalf = 128;
+constexpr int kBlock = 128;  // keys
+constexpr int kThreads = 512;
+constexpr int kSlots = 4;    // K and V tiles in the ring
+constexpr float kRaise = 8.f;
+
+template <int kDim>
+struct Smem {
+    static constexpr int kPanels = (kDim + 63) / 64;      // 64 columns (128 bytes) each
+    static constexpr int kPanelRows = kBlock * 128;       // bytes of a panel of a K or V tile
+    static constexpr int kTile = kPanels * kPanelRows;
+    static constexpr int kQPanel = kRows * 128;
+    static constexpr int kQ = kPanels * kQPanel;
+    static constexpr int kRing = kSlots * kTile;
+    static constexpr int kBytes = kQ + kRing + 1024;      // + 1024: the tiles start on 1024 bytes
+};
+
+struct Shared {
+    uint64_t full[kSlots], empty[kSlots];
+    uint64_t q_full, q_empty;
+    uint64_t s_full[2], p_full[2], pv_done[2];
+    uint64_t drain;
+    uint32_t tmem;
+    int stalled;            // a wait ran out
+    int missing[4];         // 1 + number of the block with a key in range that has no page
+    int nonfinite[kSlots];  // 1 + number of the ring item whose V tile infinities or NaN were taken out of
+    uint8_t ok[4][kBlock];  // of block n % 4: key has a page
+    int scratch[64];
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void bar_init(uint64_t* b, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* b, int parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(b)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// false: the wait ran out, here or in another warp
+__device__ __forceinline__ bool bar_wait(uint64_t* b, int parity, Shared* sh) {
+    for (int i = 0; i < (1 << 22); ++i) {
+        if (bar_try(b, parity)) return true;
+        if ((i & 1023) == 1023 && *reinterpret_cast<volatile int*>(&sh->stalled)) return false;
+    }
+    *reinterpret_cast<volatile int*>(&sh->stalled) = 1;
+    return false;
+}
+
+// ---- tcgen05 ----
+
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes, one row to a thread
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float* r) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* u) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(
+            u[0]),
+        "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+        "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]),
+        "r"(u[20]), "r"(u[21]), "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]),
+        "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand descriptor, 128-byte swizzle: start address, strides in
+// 16-byte units.  K-major (Q, K): groups of 8 rows 1024 bytes apart.  MN-major
+// (V): 64-column panels `panel` bytes apart, groups of 8 keys 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t panel) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>((panel >> 4) & 0x3FFF) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+template <typename T>
+__host__ __device__ constexpr uint32_t instruction(int n, bool b_mn_major) {
+    const uint32_t f = Half2<T>::kFormat;
+    return (1u << 4) | (f << 7) | (f << 10) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(kHalf >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+// arrives on b when all products issued so far are done
+__device__ __forceinline__ void mma_commit(uint64_t* b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+
+// TMEM columns
+__device__ __forceinline__ constexpr uint32_t score_column(int half) { return half * 128; }
+__device__ __forceinline__ constexpr uint32_t output_column(int half) { return 256 + half * 128; }
+
+// ---- the walk over a CTA's range, the same in every role ----
+
+struct Walk {
+    const AttentionParams& a;
+    Request req;
+    TileKeys keys;
+    int head, request, tile;
+    int64_t unit, end, first;  // units left [unit, end); the tile's first unit
+    int u0, u1;                // blocks of the tile in this segment
+    int p0, p1;                // positions of the tile's first and last row
+    int rows;                  // rows in the tile
+    bool whole, opening;       // the segment is the whole tile; it is the CTA's first
+
+    __device__ __forceinline__ Walk(const AttentionParams& args, const Place& pl)
+        : a(args), head(pl.head), request(pl.request), tile(pl.tile), unit(pl.unit), end(pl.end), first(pl.unit - pl.offset),
+          opening(true) {
+        req = load_request(a, request);
+        set();
+    }
+    __device__ __forceinline__ void set() {
+        keys = tile_keys<kRows, false, kBlock, 1>(a, req, tile);
+        int i0, i1;
+        Tiles<kRows, false>::tokens(a, req, tile, &i0, &i1);
+        p0 = req.kv_len - req.rows + i0;
+        p1 = req.kv_len - req.rows + i1;
+        rows = static_cast<int>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(req.rows) * a.group - static_cast<int64_t>(tile) * kRows));
+        const int64_t last = first + keys.units;
+        u0 = static_cast<int>(unit - first);
+        u1 = static_cast<int>(min(last, end) - first);
+        whole = u0 == 0 && u1 == keys.units;
+    }
+    __device__ __forceinline__ bool next() {
+        unit = first + u1;
+        if (unit >= end) return false;
+        first += keys.units;
+        if (!next_tile<kRows, false>(a, &req, &head, &request, &tile)) return false;
+        opening = false;
+        set();
+        return true;
+    }
+    // first key of block u; `limit`: keys from it on are not loaded
+    __device__ __forceinline__ int block(int u, int* limit) const {
+        if (u < keys.sink_chunks) {
+            *limit = keys.sink_hi;
+            return u * kBlock;
+        }
+        *limit = keys.hi;
+        return keys.base + (u - keys.sink_chunks) * kBlock;
+    }
+    // every row between positions a and b sees all keys of the block at j0
+    __device__ __forceinline__ bool all_see(int j0, int from, int to) const {
+        return j0 + kBlock - 1 <= from && (a.window < 0 || to - j0 < a.window || j0 + kBlock - 1 < a.sinks);
+    }
+};
+
+// ---- loads ----
+
+template <typename T, int kDim>
+struct Loader {
+    using S = Smem<kDim>;
+    static constexpr int kPieces = kDim / 8;
+    const AttentionParams& a;
+    Shared* sh;
+    const uint32_t q, ring;
+    const int tid, lane, warp;  // within the 4 load warps
+    // items whose copies are under way: -1 Q, else 2 * number in the ring + (V tile that must be checked)
+    int pending[2];
+    int waiting = 0;
+
+    __device__ __forceinline__ Loader(const AttentionParams& args, Shared* s, uint32_t q_addr, uint32_t ring_addr)
+        : a(args), sh(s), q(q_addr), ring(ring_addr), tid(threadIdx.x & 127), lane(threadIdx.x & 31),
+          warp((threadIdx.x & 127) >> 5) {}
+
+    __device__ __forceinline__ void finish(int item) {
+        if (item >= 0 && (item & 1)) clear_nonfinite(item >> 1);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        bar_arrive(item < 0 ? &sh->q_full : &sh->full[(item >> 1) % kSlots]);
+    }
+    __device__ __forceinline__ void push(int item) {
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (waiting == 2) {
+            asm volatile("cp.async.wait_group 2;" ::: "memory");
+            finish(pending[0]);
+            pending[0] = pending[1];
+            pending[1] = item;
+        } else {
+            if (waiting == 0) pending[0] = item;
+            else pending[1] = item;
+            ++waiting;
+        }
+    }
+    __device__ __forceinline__ void flush() {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (waiting > 0) finish(pending[0]);
+        if (waiting > 1) finish(pending[1]);
+        waiting = 0;
+    }
+    // before a wait that can only end when the items under way are announced
+    __device__ __forceinline__ bool acquire(uint64_t* b, int parity) {
+        if (bar_try(b, parity)) return true;
+        flush();
+        return bar_wait(b, parity, sh);
+    }
+
+    __device__ __forceinline__ void copy(uint32_t dst, const void* src, bool ok) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+    }
+
+    __device__ __forceinline__ void load_q(const Walk& w) {
+        const int p = tid & 15;
+        if (p < kPieces) {
+            const T* base = static_cast<const T*>(a.q) + p * 8;
+            for (int r = tid >> 4; r < kRows; r += 8) {
+                int i, g;
+                const bool ok = Tiles<kRows, false>::row(a, w.req, w.tile, r, &i, &g);
+                const T* src = ok ? base + static_cast<int64_t>(w.req.start + i) * a.q_token_stride +
+                                        static_cast<int64_t>(w.head * a.group + g) * a.q_head_stride
+                                  : base;
+                copy(q + (p >> 3) * S::kQPanel + r * 128 + (((p & 7) ^ (r & 7)) << 4), src, ok);
+            }
+        }
+        push(-1);
+    }
+
+    // K and V rows of block n (n: number of the block in this CTA)
+    __device__ __forceinline__ bool load_block(const Walk& w, int u, int n) {
+        int limit;
+        const int j0 = w.block(u, &limit);
+        // each lane looks one row up: rows 8 i + 2 warp + h of this warp, lane = 2 i + h
+        const int row = (lane >> 1) * 8 + warp * 2 + (lane & 1);
+        const int j = j0 + row;
+        const bool want = j < limit && (j >= w.keys.lo || j < a.sinks);
+        int64_t off = -1;
+        if (want) {
+            const int page = j >> a.page_shift;  // j < hi: within the table
+            const int id = __ldg(a.block_table + w.request * a.table_stride + page);
+            if (static_cast<uint32_t>(id) < static_cast<uint32_t>(a.pages))
+                off = id * a.page_stride + (j & (a.page_size - 1)) * a.token_stride + w.head * a.head_stride;
+        }
+        const bool lost = __any_sync(0xFFFFFFFFu, want && off < 0);
+        const bool check = w.p0 != w.p1 && !w.all_see(j0, w.p0, w.p1);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {  // K, then V
+            const int f = 2 * n + half, slot = f % kSlots;
+            if (!acquire(&sh->empty[slot], ((f / kSlots) & 1) ^ 1)) return false;
+            if (half == 0) {
+                sh->ok[n & 3][row] = off >= 0;
+                if (lost && lane == 0) sh->missing[n & 3] = 1 + n;
+            }
+            const T* base = static_cast<const T*>(half == 0 ? a.k_cache : a.v_cache);
+            const uint32_t dst = ring + slot * S::kTile;
+            const int p = tid & 15, h = (tid >> 4) & 1;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int64_t from = __shfl_sync(0xFFFFFFFFu, off, 2 * i + h);
+                const int r = 8 * i + 2 * warp + h;
+                if (p < kPieces)
+                    copy(dst + (p >> 3) * S::kPanelRows + r * 128 + (((p & 7) ^ (r & 7)) << 4),
+                         base + (from >= 0 ? from + p * 8 : 0), from >= 0);
+            }
+            push(2 * f + (half == 1 && check));
+        }
+        return true;
+    }
+
+    // A V tile that some rows see and others do not: 0 * inf and 0 * NaN must not
+    // reach the ones that do not.  Each thread clears the pieces that it copied;
+    // the softmax warps give the values back to the rows that see them.
+    __device__ __forceinline__ void clear_nonfinite(int f) {
+        const uint32_t base = ring + (f % kSlots) * S::kTile;
+        const int p = tid & 15, h = (tid >> 4) & 1;
+        bool bad = false;
+        if (p < kPieces) {
+#pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+                const int r = 8 * i + 2 * warp + h;
+                const uint32_t at = base + (p >> 3) * S::kPanelRows + r * 128 + (((p & 7) ^ (r & 7)) << 4);
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                             : "r"(at)
+                             : "memory");
+                bool here = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    constexpr uint32_t kE = Half2<T>::kExpMask;
+                    if ((w[e] & kE) == kE) {
+                        w[e] &= 0xFFFF0000u;
+                        here = true;
+                    }
+                    if ((w[e] & (kE << 16)) == (kE << 16)) {
+                        w[e] &= 0x0000FFFFu;
+                        here = true;
+                    }
+                }
+                if (here) {
+                    bad = true;
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                                 "r"(w[3])
+                                 : "memory");
+                }
+            }
+        }
+        if (bad) sh->nonfinite[f % kSlots] = 1 + f;
+    }
+};
+
+// ---- weights ----
+
+template <typename T, int kDim>
+struct Softmax {
+    const AttentionParams& a;
+    Shared* sh;
+    const int half;       // 0, 1
+    const uint32_t lane0; // this warp's first TMEM lane, in address form
+    const int row;        // of the tile
+    float m, l;           // base of the weights, their sum
+    int done = 0;         // blocks of this half so far, over all tiles
+
+    __device__ __forceinline__ Softmax(const AttentionParams& args, Shared* s, uint32_t tmem)
+        : a(args), sh(s), half(threadIdx.x >> 7), lane0(tmem + (((threadIdx.x >> 5) & 3) << 21)), row(threadIdx.x & 255) {}
+
+    // block u of the walk's tile, number n in the CTA; false: stalled
+    __device__ __forceinline__ bool block(const Walk& w, int u, int n, bool first, int p, int from, int to) {
+        int limit;
+        const int j0 = w.block(u, &limit);
+        if (!bar_wait(&sh->s_full[half], done & 1, sh)) return false;
+        tmem_fence_after();
+        float s[kBlock];
+#pragma unroll
+        for (int c = 0; c < kBlock; c += 32) tmem_load32(lane0 + score_column(half) + c, s + c);
+        tmem_load_wait();
+        const bool lost = sh->missing[n & 3] == 1 + n;
+        bool poison = false;
+        if (lost || !w.all_see(j0, from, to)) {
+            // visible: c <= last and (c >= near or c < sink)
+            const int last = min(p - j0, limit - 1 - j0);
+            const int near = (a.window < 0 || p < a.window) ? 0 : p - a.window + 1 - j0;
+            const int sink = a.sinks - j0;
+#pragma unroll
+            for (int c = 0; c < kBlock; ++c)
+                if (!(c <= last && (c >= near || c < sink))) s[c] = -INFINITY;
+            if (lost) {
+#pragma unroll
+                for (int c = 0; c < kBlock; ++c)
+                    if (!sh->ok[n & 3][c]) s[c] = -INFINITY;
+            }
+        }
+        if (w.p0 != w.p1 && !w.all_see(j0, w.p0, w.p1)) {  // the V tile was checked
+            const int f = 2 * n + 1;
+            if (!bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh)) return false;
+            poison = sh->nonfinite[f % kSlots] == 1 + f;
+        }
+        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < kBlock; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+        if (first) {
+            m = mx;
+            l = 0.f;
+        } else if (__any_sync(0xFFFFFFFFu, mx > m + kRaise || (m == -INFINITY && mx > m))) {
+            // raise the base: wait for the products that write O, scale it
+            if (!bar_wait(&sh->pv_done[half], (done - 1) & 1, sh)) return false;
+            tmem_fence_after();
+            const float mn = fmaxf(m, mx);
+            const float f = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll 1
+            for (int d = 0; d < kDim; d += 32) {
+                float o[32];
+                tmem_load32(lane0 + output_column(half) + d, o);
+                tmem_load_wait();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) o[x] *= f;
+                tmem_store32(lane0 + output_column(half) + d, reinterpret_cast<const uint32_t*>(o));
+            }
+        }
+        const float base = m == -INFINITY ? 0.f : -m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c0 = 0; c0 < kBlock; c0 += 64) {
+            uint32_t pk[32];
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+                const float e0 = exp2_fast(fmaf(s[c0 + c], a.scale_log2, base));
+                const float e1 = exp2_fast(fmaf(s[c0 + c + 1], a.scale_log2, base));
+                sum[c & 2] += e0;
+                sum[(c & 2) + 1] += e1;
+                // weights go to the product in the cache's 16-bit type, as the tensor cores take them; the sum keeps 32 bits
+                pk[c / 2] = Half2<T>::pack(e0, e1);
+            }
+            tmem_store32(lane0 + score_column(half) + c0 / 2, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_store_wait();
+        tmem_fence_before();
+        bar_arrive(&sh->p_full[half]);
+        ++done;
+        if (poison) {
+            if (!bar_wait(&sh->pv_done[half], (done - 1) & 1, sh)) return false;
+            tmem_fence_after();
+            add_nonfinite(w, u, n, p);
+            tmem_store_wait();
+            tmem_fence_before();
+        }
+        return true;
+    }
+
+    // Infinities and NaN that the loader took out of V, for the rows that see them.
+    __device__ __forceinline__ void add_nonfinite(const Walk& w, int u, int n, int p) {
+        int limit;
+        const int j0 = w.block(u, &limit);
+        const int32_t* table = a.block_table + w.request * a.table_stride;
+#pragma unroll 1
+        for (int d = 0; d < kDim; d += 32) {
+            float o[32];
+            tmem_load32(lane0 + output_column(half) + d, o);
+            tmem_load_wait();
+#pragma unroll 1
+            for (int c = 0; c < kBlock; ++c) {
+                const int j = j0 + c;
+                if (j >= limit || j > p || !(a.window < 0 || p - j < a.window || j < a.sinks)) continue;
+                const int id = __ldg(table + (j >> a.page_shift));
+                if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.pages)) continue;
+                const T* v = static_cast<const T*>(a.v_cache) + id * a.page_stride + (j & (a.page_size - 1)) * a.token_stride +
+                             w.head * a.head_stride + d;
+#pragma unroll
+                for (int x = 0; x < 32; x += 2) {
+                    const uint32_t word = *reinterpret_cast<const uint32_t*>(v + x);
+                    const float v0 = Half2<T>::low(word), v1 = Half2<T>::high(word);
+                    if (!isfinite(v0)) o[x] += v0;
+                    if (!isfinite(v1)) o[x + 1] += v1;
+                }
+            }
+            tmem_store32(lane0 + output_column(half) + d, reinterpret_cast<const uint32_t*>(o));
+        }
+    }
+
+    // The segment's end: this thread's row of O to the output or, for part of a tile, to the workspace.
+    __device__ __forceinline__ bool store(const Walk& w, bool ok) {
+        if (ok) ok = bar_wait(&sh->pv_done[half], (done - 1) & 1, sh);
+        tmem_fence_after();
+        int i = 0, g = 0;
+        const bool valid = Tiles<kRows, false>::row(a, w.req, w.tile, row, &i, &g);
+        const int64_t token = w.req.start + i;
+        const int head = w.head * a.group + g;
+        char* ws = static_cast<char*>(a.workspace);
+        float* part = reinterpret_cast<float*>(ws + workspace_records_bytes(a.ctas)) +
+                      (2 * static_cast<size_t>(blockIdx.x) + (w.opening ? 0 : 1)) * partial_floats(kRows, kDim);
+        const float inv = !ok ? NAN : l == 0.f ? 1.f : 1.f / l;
+        T* out = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride;
+#pragma unroll 1
+        for (int d = 0; d < kDim; d += 32) {
+            float o[32];
+            tmem_load32(lane0 + output_column(half) + d, o);
+            tmem_load_wait();
+            if (!valid) continue;
+            if (w.whole) {
+#pragma unroll
+                for (int x = 0; x < 32; x += 8)
+                    *reinterpret_cast<uint4*>(out + d + x) =
+                        make_uint4(Half2<T>::pack(o[x] * inv, o[x + 1] * inv), Half2<T>::pack(o[x + 2] * inv, o[x + 3] * inv),
+                                   Half2<T>::pack(o[x + 4] * inv, o[x + 5] * inv), Half2<T>::pack(o[x + 6] * inv, o[x + 7] * inv));
+            } else {
+#pragma unroll
+                for (int x = 0; x < 32; x += 4)
+                    *reinterpret_cast<float4*>(part + row * kDim + d + x) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+            }
+        }
+        if (valid && w.whole) {
+            if (a.lse) a.lse[token * a.heads + head] = !ok ? NAN : l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        } else if (valid) {
+            part[kRows * kDim + row] = ok ? m : NAN;
+            part[kRows * kDim + kRows + row] = ok ? l : NAN;
+        }
+        tmem_fence_before();
+        return ok;
+    }
+};
+
+template <typename T, int kDim>
+__global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const AttentionParams a) {
+    using S = Smem<kDim>;
+    extern __shared__ char dynamic[];
+    __shared__ Shared shared;
+    Shared* sh = &shared;
+    const uint32_t raw = smem_addr(dynamic);
+    const uint32_t q = (raw + 1023) & ~1023u, ring = q + S::kQ;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    char* ws = static_cast<char*>(a.workspace);
+
+    const Place pl = locate<kRows, false, kBlock, 1, kThreads>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
+    if (pl.unit >= pl.end) return;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kSlots; ++i) {
+            bar_init(&sh->full[i], 128);
+            bar_init(&sh->empty[i], 1);
+            sh->nonfinite[i] = 0;
+        }
+        bar_init(&sh->q_full, 128);
+        bar_init(&sh->q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&sh->s_full[i], 1);
+            bar_init(&sh->p_full[i], 128);
+            bar_init(&sh->pv_done[i], 1);
+        }
+        bar_init(&sh->drain, 1);
+        for (int i = 0; i < 4; ++i) sh->missing[i] = 0;
+        sh->stalled = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = sh->tmem;
+    Walk w(a, pl);
+    if (threadIdx.x == 0) {
+        TileRecord rec;
+        rec.first = w.first;
+        rec.last = w.first + w.keys.units;
+        rec.head = w.head;
+        rec.request = w.request;
+        rec.tile = w.tile;
+        rec.pad = 0;
+        reinterpret_cast<TileRecord*>(ws + kHeaderBytes)[blockIdx.x] = rec;
+    }
+
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        Softmax<T, kDim> sm(a, sh, tmem);
+        int n = 0;
+        bool ok = true;
+        do {
+            if (sm.half * kHalf >= w.rows) {  // nothing in this half
+                n += w.u1 - w.u0;
+                continue;
+            }
+            int i = 0, g = 0;
+            const bool valid = Tiles<kRows, false>::row(a, w.req, w.tile, sm.row, &i, &g);
+            const int p = valid ? w.req.kv_len - w.req.rows + i : -1;
+            // positions of the half's first and last row
+            const int64_t r0 = static_cast<int64_t>(w.tile) * kRows + sm.half * kHalf;
+            const int from = w.req.kv_len - w.req.rows + static_cast<int>(r0 / a.group);
+            const int to = w.req.kv_len - w.req.rows + min(w.req.rows - 1, static_cast<int>((r0 + kHalf - 1) / a.group));
+            for (int u = w.u0; ok && u < w.u1; ++u, ++n) ok = sm.block(w, u, n, u == w.u0, p, from, to);
+            ok = sm.store(w, ok);
+        } while (w.next() && ok);
+    } else if (warp < 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        Loader<T, kDim> ld(a, sh, q, ring);
+        int n = 0, segment = 0;
+        bool ok = true;
+        do {
+            ok = ld.acquire(&sh->q_empty, (segment & 1) ^ 1);
+            if (ok) ld.load_q(w);
+            for (int u = w.u0; ok && u < w.u1; ++u, ++n) ok = ld.load_block(w, u, n);
+            ++segment;
+        } while (ok && w.next());
+        ld.flush();
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 12 && lane == 0) {
+            constexpr uint32_t kQk = instruction<T>(kBlock, false), kPv = instruction<T>(kDim, true);
+            const auto scores = [&](int half, int slot) {
+                const uint32_t qa = q + half * (kHalf * 128), kb = ring + slot * S::kTile;
+#pragma unroll
+                for (int k = 0; k < kDim / 16; ++k)
+                    mma_smem(tmem + score_column(half), operand(qa + (k >> 2) * S::kQPanel + (k & 3) * 32, 16),
+                             operand(kb + (k >> 2) * S::kPanelRows + (k & 3) * 32, 16), kQk, k > 0);
+                mma_commit(&sh->s_full[half]);
+            };
+            const auto output = [&](int half, int slot, bool add) {
+                const uint32_t vb = ring + slot * S::kTile;
+#pragma unroll
+                for (int k = 0; k < kBlock / 16; ++k)
+                    mma_tmem(tmem + output_column(half), tmem + score_column(half) + k * 8, operand(vb + k * 2048, S::kPanelRows), kPv, add || k > 0);
+                mma_commit(&sh->pv_done[half]);
+            };
+            const auto filled = [&](int f) { return bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh); };
+            int n = 0, segment = 0, done[2] = {0, 0};
+            bool ok = true;
+            do {
+                const int halves = w.rows > kHalf ? 2 : 1, blocks = w.u1 - w.u0;
+                ok = bar_wait(&sh->q_full, segment & 1, sh) && filled(2 * n);
+                if (!ok) break;
+                for (int h = 0; h < halves; ++h) scores(h, (2 * n) % kSlots);
+                mma_commit(&sh->empty[(2 * n) % kSlots]);
+                if (blocks == 1) mma_commit(&sh->q_empty);
+                for (int b = 0; b < blocks && ok; ++b, ++n) {
+                    const bool more = b + 1 < blocks;
+                    ok = filled(2 * n + 1) && (!more || filled(2 * n + 2));
+                    for (int h = 0; h < halves && ok; ++h) {
+                        ok = bar_wait(&sh->p_full[h], done[h] & 1, sh);
+                        if (!ok) break;
+                        ++done[h];
+                        tmem_fence_after();
+                        output(h, (2 * n + 1) % kSlots, b > 0);
+                        if (more) scores(h, (2 * n + 2) % kSlots);
+                    }
+                    if (!ok) break;
+                    mma_commit(&sh->empty[(2 * n + 1) % kSlots]);
+                    if (more) {
+                        mma_commit(&sh->empty[(2 * n + 2) % kSlots]);
+                        if (b + 2 == blocks) mma_commit(&sh->q_empty);
+                    }
+                }
+                ++segment;
+            } while (ok && w.next());
+            // all products end before the block does, also after a stall
+            mma_commit(&sh->drain);
+            for (int i = 0; i < (1 << 22) && !bar_try(&sh->drain, 0); ++i) {
+            }
+        }
+        __syncwarp();
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <typename T, int kDim>
+cudaError_t launch(AttentionParams a, cudaStream_t stream) {
+    constexpr int bytes = Smem<kDim>::kBytes;
+    cudaError_t e = cudaFuncSetAttribute(attention_tiles_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    attention_tiles_kernel<T, kDim><<<a.ctas, kThreads, bytes, stream>>>(a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    a.combine_split = 8;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(max(1, (a.ctas - 1) * a.combine_split)));
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_combine_kernel<T, kRows, kDim, false>, a);
+}
+
+template <typename T>
+cudaError_t by_dim(const AttentionParams& a, cudaStream_t s) {
+    switch (a.dim) {
+        case 64: return launch<T, 64>(a, s);
+        case 96: return launch<T, 96>(a, s);
+        default: return launch<T, 128>(a, s);
+    }
+}
+
+}  // namespace
+}  // namespace attn
+
+size_t attention_tiles_workspace(int ctas, int dim) {
+    return attn::workspace_records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * attn::partial_floats(attn::kRows, dim) * sizeof(float);
+}
+
+cudaError_t launch_attention_tiles(const AttentionParams& a, cudaStream_t stream) {
+    return a.dtype == FG_DTYPE_BF16 ? attn::by_dim<__nv_bfloat16>(a, stream) : attn::by_dim<__half>(a, stream);
+}
+
+}  // namespace fg

@@ -140,6 +140,8 @@ struct AttentionParams {
 int attention_max_requests();
 size_t attention_rows_workspace(int ctas, int dim);
 cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream);
+size_t attention_tiles_workspace(int ctas, int dim);
+cudaError_t launch_attention_tiles(const AttentionParams& a, cudaStream_t stream);
 
 // Host restatements shared with the CLI and the API.
 uint32_t effective_sort_beam(uint32_t beam);
