@@ -854,9 +854,10 @@ int sm_count(int* sms) {
 // tokens x heads of the group) fill one tile of the rows kernel; above that it
 // would read the keys once for each 16 rows, and the tiles kernel takes them
 // 256 at a time.  That one folds the scale into its maxima, so it needs a
-// positive one.
+// positive one, and its copies are whole groups of 8 rows of a page.
 bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
-    return !retrieved && x->scale > 0.f && static_cast<int64_t>(x->max_new) * (x->heads / c->heads) > 16;
+    return !retrieved && x->scale > 0.f && c->page_size >= 8 &&
+           static_cast<int64_t>(x->max_new) * (x->heads / c->heads) > 16;
 }
 
 int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void* stream) {

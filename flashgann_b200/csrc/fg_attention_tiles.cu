@@ -10,10 +10,13 @@
 //
 // Warp roles (16 warps, one CTA per SM):
 //   0-3, 4-7   softmax of half 0 and 1 (192 registers a thread)
-//   8-11       loads: 16-byte cp.async of whole key rows, gathered by page, into
-//              a ring of K and V tiles in the 128-byte swizzled layout that
-//              tcgen05 reads; zeros for rows that do not exist
+//   8-11       copy the query rows in (16-byte cp.async), and look through the V
+//              tiles that not all rows see whole, see clear_masked
 //   12         issues the products
+//   13         loads K and V with TMA, one copy for each page (or 16 rows of it)
+//              and 64 columns, into a ring of tiles in the 128-byte swizzled
+//              layout that tcgen05 reads; a page that is not there is a
+//              coordinate out of range, which TMA fills with zeros
 // The two halves run in antiphase: while half 0's weights are computed the
 // tensor cores work on half 1.
 //
@@ -29,6 +32,8 @@
 //
 // Every wait is bounded: one that runs out marks the CTA, all roles leave
 // their loops, and the rows of the tiles in work get NaN.
+#include <cuda.h>
+
 #include "fg_attention.cuh"
 
 namespace fg {
@@ -39,7 +44,7 @@ constexpr int kRows = 256;
 constexpr int kHalf = 128;
 constexpr int kBlock = 128;  // keys
 constexpr int kThreads = 512;
-constexpr int kSlots = 4;    // K and V tiles in the ring
+constexpr int kSlots = 5;    // K and V tiles in the ring: two blocks and a half
 constexpr float kRaise = 8.f;
 
 template <int kDim>
@@ -54,15 +59,15 @@ struct Smem {
 };
 
 struct Shared {
-    uint64_t full[kSlots], empty[kSlots];
+    uint64_t full[kSlots], clean[kSlots], empty[kSlots];
     uint64_t q_full, q_empty;
     uint64_t s_full[2], p_full[2], pv_done[2];
     uint64_t drain;
     uint32_t tmem;
     int stalled;            // a wait ran out
-    int missing[4];         // 1 + number of the block with a key in range that has no page
+    int missing[4];         // 1 + number of the block that has keys in range without a page
+    uint32_t boxes[4];      // of block n % 4: bit i, copy i found its page
     int nonfinite[kSlots];  // 1 + number of the ring item whose V tile infinities or NaN were taken out of
-    uint8_t ok[4][kBlock];  // of block n % 4: key has a page
     int scratch[64];
 };
 
@@ -84,6 +89,9 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, int parity) {
         : "r"(smem_addr(b)), "r"(parity)
         : "memory");
     return ok != 0;
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
 }
 // false: the wait ran out, here or in another warp
 __device__ __forceinline__ bool bar_wait(uint64_t* b, int parity, Shared* sh) {
@@ -213,6 +221,11 @@ struct Walk {
         *limit = keys.hi;
         return keys.base + (u - keys.sink_chunks) * kBlock;
     }
+    // whether block u's V tile is looked through before it is used
+    __device__ __forceinline__ bool checked(int u) const {
+        int limit;
+        return !all_see(block(u, &limit), p0, p1);
+    }
     // every row between positions a and b sees all keys of the block at j0
     __device__ __forceinline__ bool all_see(int j0, int from, int to) const {
         return j0 + kBlock - 1 <= from && (a.window < 0 || to - j0 < a.window || j0 + kBlock - 1 < a.sinks);
@@ -221,56 +234,75 @@ struct Walk {
 
 // ---- loads ----
 
-template <typename T, int kDim>
+// Copies a box of the cache: 64 columns (from x on) of consecutive rows of one page and head.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int row, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(map), "r"(smem_addr(bar)), "r"(x), "r"(row), "r"(head), "r"(page)
+        : "memory");
+}
+
+// The TMA warp: K, then V of every block.
+template <int kDim>
 struct Loader {
+    using S = Smem<kDim>;
+    const AttentionParams& a;
+    Shared* sh;
+    const uint32_t ring;
+    const int lane, box_shift;
+    const int box, panel;  // this lane's copy
+
+    __device__ __forceinline__ Loader(const AttentionParams& args, Shared* s, uint32_t ring_addr, int shift)
+        : a(args), sh(s), ring(ring_addr), lane(threadIdx.x & 31), box_shift(shift), box((threadIdx.x & 31) / S::kPanels),
+          panel((threadIdx.x & 31) % S::kPanels) {}
+
+    // the page of this lane's copy in the block at j0, `pages` (out of range) where there is none
+    __device__ __forceinline__ int page(const Walk& w, int j0, int limit) const {
+        const int j = j0 + (box << box_shift);
+        if ((box << box_shift) >= kBlock || j >= limit) return a.pages;
+        const int id = __ldg(a.block_table + w.request * a.table_stride + (j >> a.page_shift));  // j < hi: in the table
+        return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.pages) ? id : a.pages;
+    }
+
+    __device__ __forceinline__ bool block(const Walk& w, int j0, int limit, int pg, int n, const CUtensorMap* k_map, const CUtensorMap* v_map) {
+        const int j = j0 + (box << box_shift);
+        const bool mine = (box << box_shift) < kBlock;
+        const uint32_t found = __ballot_sync(0xFFFFFFFFu, mine && pg < a.pages);
+        const uint32_t wanted = __ballot_sync(0xFFFFFFFFu, mine && j < limit);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int f = 2 * n + half, slot = f % kSlots;
+            if (!bar_wait(&sh->empty[slot], ((f / kSlots) & 1) ^ 1, sh)) return false;
+            if (lane == 0) {
+                if (half == 0 && found != wanted) {
+                    uint32_t bits = 0;
+                    for (int b = 0; b < 32 / S::kPanels; ++b) bits |= ((found >> (b * S::kPanels)) & 1u) << b;
+                    sh->boxes[n & 3] = bits;
+                    sh->missing[n & 3] = 1 + n;
+                }
+                bar_expect(&sh->full[slot], S::kTile);
+            }
+            __syncwarp();
+            if (mine)
+                load_box(ring + slot * S::kTile + panel * S::kPanelRows + (box << box_shift) * 128, half == 0 ? k_map : v_map,
+                         &sh->full[slot], panel * 64, j & (a.page_size - 1), w.head, pg);
+        }
+        return true;
+    }
+};
+
+// Warps 8-11.
+template <typename T, int kDim>
+struct Helper {
     using S = Smem<kDim>;
     static constexpr int kPieces = kDim / 8;
     const AttentionParams& a;
     Shared* sh;
     const uint32_t q, ring;
-    const int tid, lane, warp;  // within the 4 load warps
-    // items whose copies are under way: -1 Q, else 2 * number in the ring + (V tile that must be checked)
-    int pending[2];
-    int waiting = 0;
+    const int tid;  // 0 .. 127
 
-    __device__ __forceinline__ Loader(const AttentionParams& args, Shared* s, uint32_t q_addr, uint32_t ring_addr)
-        : a(args), sh(s), q(q_addr), ring(ring_addr), tid(threadIdx.x & 127), lane(threadIdx.x & 31),
-          warp((threadIdx.x & 127) >> 5) {}
-
-    __device__ __forceinline__ void finish(int item) {
-        if (item >= 0 && (item & 1)) clear_nonfinite(item >> 1);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        bar_arrive(item < 0 ? &sh->q_full : &sh->full[(item >> 1) % kSlots]);
-    }
-    __device__ __forceinline__ void push(int item) {
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (waiting == 2) {
-            asm volatile("cp.async.wait_group 2;" ::: "memory");
-            finish(pending[0]);
-            pending[0] = pending[1];
-            pending[1] = item;
-        } else {
-            if (waiting == 0) pending[0] = item;
-            else pending[1] = item;
-            ++waiting;
-        }
-    }
-    __device__ __forceinline__ void flush() {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (waiting > 0) finish(pending[0]);
-        if (waiting > 1) finish(pending[1]);
-        waiting = 0;
-    }
-    // before a wait that can only end when the items under way are announced
-    __device__ __forceinline__ bool acquire(uint64_t* b, int parity) {
-        if (bar_try(b, parity)) return true;
-        flush();
-        return bar_wait(b, parity, sh);
-    }
-
-    __device__ __forceinline__ void copy(uint32_t dst, const void* src, bool ok) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-    }
+    __device__ __forceinline__ Helper(const AttentionParams& args, Shared* s, uint32_t q_addr, uint32_t ring_addr)
+        : a(args), sh(s), q(q_addr), ring(ring_addr), tid(threadIdx.x & 127) {}
 
     __device__ __forceinline__ void load_q(const Walk& w) {
         const int p = tid & 15;
@@ -282,92 +314,66 @@ struct Loader {
                 const T* src = ok ? base + static_cast<int64_t>(w.req.start + i) * a.q_token_stride +
                                         static_cast<int64_t>(w.head * a.group + g) * a.q_head_stride
                                   : base;
-                copy(q + (p >> 3) * S::kQPanel + r * 128 + (((p & 7) ^ (r & 7)) << 4), src, ok);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                 q + (p >> 3) * S::kQPanel + r * 128 + (((p & 7) ^ (r & 7)) << 4)),
+                             "l"(src), "r"(ok ? 16 : 0)
+                             : "memory");
             }
         }
-        push(-1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if ((tid & 31) == 0) bar_arrive(&sh->q_full);
     }
 
-    // K and V rows of block n (n: number of the block in this CTA)
-    __device__ __forceinline__ bool load_block(const Walk& w, int u, int n) {
-        int limit;
-        const int j0 = w.block(u, &limit);
-        // each lane looks one row up: rows 8 i + 2 warp + h of this warp, lane = 2 i + h
-        const int row = (lane >> 1) * 8 + warp * 2 + (lane & 1);
-        const int j = j0 + row;
-        const bool want = j < limit && (j >= w.keys.lo || j < a.sinks);
-        int64_t off = -1;
-        if (want) {
-            const int page = j >> a.page_shift;  // j < hi: within the table
-            const int id = __ldg(a.block_table + w.request * a.table_stride + page);
-            if (static_cast<uint32_t>(id) < static_cast<uint32_t>(a.pages))
-                off = id * a.page_stride + (j & (a.page_size - 1)) * a.token_stride + w.head * a.head_stride;
-        }
-        const bool lost = __any_sync(0xFFFFFFFFu, want && off < 0);
-        const bool check = w.p0 != w.p1 && !w.all_see(j0, w.p0, w.p1);
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {  // K, then V
-            const int f = 2 * n + half, slot = f % kSlots;
-            if (!acquire(&sh->empty[slot], ((f / kSlots) & 1) ^ 1)) return false;
-            if (half == 0) {
-                sh->ok[n & 3][row] = off >= 0;
-                if (lost && lane == 0) sh->missing[n & 3] = 1 + n;
-            }
-            const T* base = static_cast<const T*>(half == 0 ? a.k_cache : a.v_cache);
-            const uint32_t dst = ring + slot * S::kTile;
-            const int p = tid & 15, h = (tid >> 4) & 1;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int64_t from = __shfl_sync(0xFFFFFFFFu, off, 2 * i + h);
-                const int r = 8 * i + 2 * warp + h;
-                if (p < kPieces)
-                    copy(dst + (p >> 3) * S::kPanelRows + r * 128 + (((p & 7) ^ (r & 7)) << 4),
-                         base + (from >= 0 ? from + p * 8 : 0), from >= 0);
-            }
-            push(2 * f + (half == 1 && check));
-        }
-        return true;
-    }
-
-    // A V tile that some rows see and others do not: 0 * inf and 0 * NaN must not
-    // reach the ones that do not.  Each thread clears the pieces that it copied;
-    // the softmax warps give the values back to the rows that see them.
-    __device__ __forceinline__ void clear_nonfinite(int f) {
-        const uint32_t base = ring + (f % kSlots) * S::kTile;
-        const int p = tid & 15, h = (tid >> 4) & 1;
+    // A V tile that not all rows see whole: 0 * inf and 0 * NaN must not reach
+    // the rows that do not see the key.  Infinities and NaN are
+    // taken out; the softmax warps give those of keys in range back to the rows
+    // that see them.  j0: the tile's first key, f: its number
+    // in the ring.
+    __device__ __forceinline__ bool clear_masked(const Walk& w, int j0, int limit, int f) {
+        const int slot = f % kSlots;
+        if (!bar_wait(&sh->full[slot], (f / kSlots) & 1, sh)) return false;
+        const uint32_t base = ring + slot * S::kTile;
+        const int p = tid & 15;
         bool bad = false;
         if (p < kPieces) {
 #pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-                const int r = 8 * i + 2 * warp + h;
+            for (int r = tid >> 4; r < kBlock; r += 8) {
+                const int j = j0 + r;
+                const bool seen = j < limit && (j >= w.keys.lo || j < a.sinks);
                 const uint32_t at = base + (p >> 3) * S::kPanelRows + r * 128 + (((p & 7) ^ (r & 7)) << 4);
-                uint32_t w[4];
+                uint32_t v[4];
                 asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                             : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                              : "r"(at)
                              : "memory");
                 bool here = false;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     constexpr uint32_t kE = Half2<T>::kExpMask;
-                    if ((w[e] & kE) == kE) {
-                        w[e] &= 0xFFFF0000u;
+                    if ((v[e] & kE) == kE) {
+                        v[e] &= 0xFFFF0000u;
                         here = true;
                     }
-                    if ((w[e] & (kE << 16)) == (kE << 16)) {
-                        w[e] &= 0x0000FFFFu;
+                    if ((v[e] & (kE << 16)) == (kE << 16)) {
+                        v[e] &= 0x0000FFFFu;
                         here = true;
                     }
                 }
                 if (here) {
-                    bad = true;
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                                 "r"(w[3])
+                    bad |= seen;
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                                  : "memory");
                 }
             }
         }
-        if (bad) sh->nonfinite[f % kSlots] = 1 + f;
+        if (bad) sh->nonfinite[slot] = 1 + f;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if ((tid & 31) == 0) bar_arrive(&sh->clean[slot]);
+        return true;
     }
 };
 
@@ -382,9 +388,18 @@ struct Softmax {
     const int row;        // of the tile
     float m, l;           // base of the weights, their sum
     int done = 0;         // blocks of this half so far, over all tiles
+    const int box_shift;
+    uint32_t cleans = 0;  // bit s: parity of the number of checked V tiles that slot s has had
 
-    __device__ __forceinline__ Softmax(const AttentionParams& args, Shared* s, uint32_t tmem)
-        : a(args), sh(s), half(threadIdx.x >> 7), lane0(tmem + (((threadIdx.x >> 5) & 3) << 21)), row(threadIdx.x & 255) {}
+    __device__ __forceinline__ Softmax(const AttentionParams& args, Shared* s, uint32_t tmem, int shift)
+        : a(args), sh(s), half(threadIdx.x >> 7), lane0(tmem + (((threadIdx.x >> 5) & 3) << 21)), row(threadIdx.x & 255),
+          box_shift(shift) {}
+
+    // the blocks of a tile that has no rows in this half
+    __device__ __forceinline__ void skip(const Walk& w, int n) {
+        for (int u = w.u0; u < w.u1; ++u, ++n)
+            if (w.checked(u)) cleans ^= 1u << ((2 * n + 1) % kSlots);
+    }
 
     // block u of the walk's tile, number n in the CTA; false: stalled
     __device__ __forceinline__ bool block(const Walk& w, int u, int n, bool first, int p, int from, int to) {
@@ -407,14 +422,16 @@ struct Softmax {
             for (int c = 0; c < kBlock; ++c)
                 if (!(c <= last && (c >= near || c < sink))) s[c] = -INFINITY;
             if (lost) {
+                const uint32_t found = sh->boxes[n & 3];
 #pragma unroll
                 for (int c = 0; c < kBlock; ++c)
-                    if (!sh->ok[n & 3][c]) s[c] = -INFINITY;
+                    if (!((found >> (c >> box_shift)) & 1u)) s[c] = -INFINITY;
             }
         }
-        if (w.p0 != w.p1 && !w.all_see(j0, w.p0, w.p1)) {  // the V tile was checked
+        if (w.checked(u)) {
             const int f = 2 * n + 1;
-            if (!bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh)) return false;
+            if (!bar_wait(&sh->clean[f % kSlots], (cleans >> (f % kSlots)) & 1, sh)) return false;
+            cleans ^= 1u << (f % kSlots);
             poison = sh->nonfinite[f % kSlots] == 1 + f;
         }
         float top[4] = {s[0], s[1], s[2], s[3]};
@@ -461,7 +478,8 @@ struct Softmax {
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tmem_store_wait();
         tmem_fence_before();
-        bar_arrive(&sh->p_full[half]);
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) bar_arrive(&sh->p_full[half]);
         ++done;
         if (poison) {
             if (!bar_wait(&sh->pv_done[half], (done - 1) & 1, sh)) return false;
@@ -546,7 +564,9 @@ struct Softmax {
 };
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const AttentionParams a) {
+__global__ void __launch_bounds__(kThreads, 1)
+attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                       const int box_shift) {
     using S = Smem<kDim>;
     extern __shared__ char dynamic[];
     __shared__ Shared shared;
@@ -561,15 +581,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const Atte
     if (pl.unit >= pl.end) return;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) {
-            bar_init(&sh->full[i], 128);
+            bar_init(&sh->full[i], 1);
+            bar_init(&sh->clean[i], 4);
             bar_init(&sh->empty[i], 1);
             sh->nonfinite[i] = 0;
         }
-        bar_init(&sh->q_full, 128);
+        bar_init(&sh->q_full, 4);
         bar_init(&sh->q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             bar_init(&sh->s_full[i], 1);
-            bar_init(&sh->p_full[i], 128);
+            bar_init(&sh->p_full[i], 4);
             bar_init(&sh->pv_done[i], 1);
         }
         bar_init(&sh->drain, 1);
@@ -599,11 +620,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const Atte
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-        Softmax<T, kDim> sm(a, sh, tmem);
+        Softmax<T, kDim> sm(a, sh, tmem, box_shift);
         int n = 0;
         bool ok = true;
         do {
             if (sm.half * kHalf >= w.rows) {  // nothing in this half
+                sm.skip(w, n);
                 n += w.u1 - w.u0;
                 continue;
             }
@@ -619,16 +641,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const Atte
         } while (w.next() && ok);
     } else if (warp < 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        Loader<T, kDim> ld(a, sh, q, ring);
+        Helper<T, kDim> hp(a, sh, q, ring);
         int n = 0, segment = 0;
         bool ok = true;
         do {
-            ok = ld.acquire(&sh->q_empty, (segment & 1) ^ 1);
-            if (ok) ld.load_q(w);
-            for (int u = w.u0; ok && u < w.u1; ++u, ++n) ok = ld.load_block(w, u, n);
+            ok = bar_wait(&sh->q_empty, (segment & 1) ^ 1, sh);
+            if (!ok) break;
+            hp.load_q(w);
+            for (int u = w.u0; ok && u < w.u1; ++u, ++n) {
+                if (!w.checked(u)) continue;
+                int limit;
+                const int j0 = w.block(u, &limit);
+                ok = hp.clear_masked(w, j0, limit, 2 * n + 1);
+            }
             ++segment;
         } while (ok && w.next());
-        ld.flush();
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == 12 && lane == 0) {
@@ -649,6 +676,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const Atte
                 mma_commit(&sh->pv_done[half]);
             };
             const auto filled = [&](int f) { return bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh); };
+            uint32_t cleans = 0;
+            const auto value_ready = [&](int f, bool checked) {
+                const int slot = f % kSlots;
+                if (!checked) return filled(f);
+                const int parity = (cleans >> slot) & 1;
+                cleans ^= 1u << slot;
+                return bar_wait(&sh->clean[slot], parity, sh);
+            };
             int n = 0, segment = 0, done[2] = {0, 0};
             bool ok = true;
             do {
@@ -660,14 +695,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const Atte
                 if (blocks == 1) mma_commit(&sh->q_empty);
                 for (int b = 0; b < blocks && ok; ++b, ++n) {
                     const bool more = b + 1 < blocks;
-                    ok = filled(2 * n + 1) && (!more || filled(2 * n + 2));
+                    ok = value_ready(2 * n + 1, w.checked(w.u0 + b));
                     for (int h = 0; h < halves && ok; ++h) {
                         ok = bar_wait(&sh->p_full[h], done[h] & 1, sh);
                         if (!ok) break;
                         ++done[h];
                         tmem_fence_after();
                         output(h, (2 * n + 1) % kSlots, b > 0);
-                        if (more) scores(h, (2 * n + 2) % kSlots);
+                        if (!more) continue;
+                        if (h == 0) ok = filled(2 * n + 2);
+                        if (ok) scores(h, (2 * n + 2) % kSlots);
                     }
                     if (!ok) break;
                     mma_commit(&sh->empty[(2 * n + 1) % kSlots]);
@@ -682,6 +719,31 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const Atte
             mma_commit(&sh->drain);
             for (int i = 0; i < (1 << 22) && !bar_try(&sh->drain, 0); ++i) {
             }
+        } else if (warp == 13) {
+            Loader<kDim> ld(a, sh, ring, box_shift);
+            int n = 0;
+            bool ok = true;
+            do {
+                int limit, j0 = w.block(w.u0, &limit);
+                int pg = ld.page(w, j0, limit);
+                for (int u = w.u0; ok && u < w.u1; ++u, ++n) {
+                    int next_limit = 0, next_j0 = 0, next_pg = 0;
+                    if (u + 1 < w.u1) {  // looked up one block ahead
+                        next_j0 = w.block(u + 1, &next_limit);
+                        next_pg = ld.page(w, next_j0, next_limit);
+                    }
+                    ok = ld.block(w, j0, limit, pg, n, &k_map, &v_map);
+                    j0 = next_j0;
+                    limit = next_limit;
+                    pg = next_pg;
+                }
+            } while (ok && w.next());
+            // copies under way end before the block does, also after a stall
+            if (!ok) {
+                for (int f = max(0, 2 * n - kSlots); f < 2 * n + 2; ++f)
+                    for (int i = 0; i < (1 << 16) && !bar_try(&sh->full[f % kSlots], (f / kSlots) & 1); ++i) {
+                    }
+            }
         }
         __syncwarp();
     }
@@ -691,12 +753,48 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tiles_kernel(const Atte
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode find_encode() {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+        return nullptr;
+    return reinterpret_cast<Encode>(f);
+}
+
+// The cache as [page][head][row][dim]; boxes of 64 columns and 2^box_shift rows.
+bool encode(CUtensorMap* map, const AttentionParams& a, const void* cache, int box_shift) {
+    static const Encode f = find_encode();
+    if (!f) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.page_size),
+                                static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};
+    // the stride of an axis of one entry is never used, whatever it says
+    const int64_t row = a.page_size > 1 ? a.token_stride : a.dim;
+    const int64_t head = a.kv_heads > 1 ? a.head_stride : a.dim;
+    const int64_t page = a.pages > 1 ? a.page_stride : a.dim;
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(row) * 2, static_cast<cuuint64_t>(head) * 2,
+                                   static_cast<cuuint64_t>(page) * 2};
+    const cuuint32_t box[4] = {64, 1u << box_shift, 1, 1}, step[4] = {1, 1, 1, 1};
+    return f(map, a.dtype == FG_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+             const_cast<void*>(cache), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int kDim>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = Smem<kDim>::kBytes;
     cudaError_t e = cudaFuncSetAttribute(attention_tiles_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
-    attention_tiles_kernel<T, kDim><<<a.ctas, kThreads, bytes, stream>>>(a);
+    // blocks start at multiples of 16 keys, so a box of up to 16 rows never leaves its page; without a window they start
+    // at multiples of 128, and a box is as much of a page as a block takes
+    const int box_shift = min(a.page_shift, a.window < 0 ? 7 : 4);
+    CUtensorMap k_map, v_map;
+    if (!encode(&k_map, a, a.k_cache, box_shift) || !encode(&v_map, a, a.v_cache, box_shift)) return cudaErrorInvalidValue;
+    attention_tiles_kernel<T, kDim><<<a.ctas, kThreads, bytes, stream>>>(a, k_map, v_map, box_shift);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     a.combine_split = 8;
     cudaLaunchConfig_t cfg = {};
