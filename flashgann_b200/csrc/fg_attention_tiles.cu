@@ -46,6 +46,7 @@ constexpr int kBlock = 128;  // keys
 constexpr int kThreads = 512;
 constexpr int kSlots = 5;    // K and V tiles in the ring: two blocks and a half
 constexpr float kRaise = 8.f;
+constexpr int kPolyPairs = 3;  // of 8 pairs of weights, see exp2_poly
 
 template <int kDim>
 struct Smem {
@@ -61,7 +62,7 @@ struct Smem {
 struct Shared {
     uint64_t full[kSlots], clean[kSlots], empty[kSlots];
     uint64_t q_full, q_empty;
-    uint64_t s_full[2], p_full[2], pv_done[2];
+    uint64_t s_full[2], p_full[2][2], pv_done[2];  // p_full: of each half, the weights of keys 0-63 and 64-127
     uint64_t drain;
     uint32_t tmem;
     int stalled;            // a wait ran out
@@ -131,16 +132,31 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* u) {
         "r"(u[29]), "r"(u[30]), "r"(u[31]), "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float* r) {
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* u) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(u[0]),
+        "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+        "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(addr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Shared-memory operand descriptor, 128-byte swizzle: start address, strides in
-// 16-byte units.  K-major (Q, K): groups of 8 rows 1024 bytes apart.  MN-major
-// (V): 64-column panels `panel` bytes apart, groups of 8 keys 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t panel) {
-    return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (static_cast<uint64_t>((panel >> 4) & 0x3FFF) << 16) |
-           (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+// Shared-memory operand descriptor, 128-byte swizzle: start address and strides
+// in 16-byte units.  K-major (Q, K): groups of 8 rows 1024 bytes apart.
+// MN-major (V): 64-column panels `panel` bytes apart, groups of 8 keys 1024
+// bytes apart.  The upper word is the same for all; advancing the start address
+// adds to the lower.
+constexpr uint32_t kOperandHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t operand_low(uint32_t addr, uint32_t panel) { return (addr >> 4) | ((panel >> 4) << 16); }
 
 template <typename T>
 __host__ __device__ constexpr uint32_t instruction(int n, bool b_mn_major) {
@@ -149,20 +165,27 @@ __host__ __device__ constexpr uint32_t instruction(int n, bool b_mn_major) {
            (static_cast<uint32_t>(kHalf >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_smem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(kOperandHigh)
         : "memory");
 }
-__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(kOperandHigh)
         : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
+// a value that all lanes share, in a form that the compiler knows to be shared
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xFFFFFFFFu, x, 0); }
 // arrives on b when all products issued so far are done
 __device__ __forceinline__ void mma_commit(uint64_t* b) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
@@ -379,12 +402,62 @@ struct Helper {
 
 // ---- weights ----
 
+struct Pair {
+    float x, y;
+};
+__device__ __forceinline__ uint64_t bits(Pair v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ Pair pair(uint64_t r) {
+    Pair v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+    return v;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return pair(r);
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return pair(r);
+}
+// NaN if any is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x for x in [-inf, 2^21], without the special-function units: x = n + f with
+// n the nearest integer (left in the low bits by adding 1.5 * 2^23), 2^f by the
+// polynomial of degree 4 with the least relative error on [-1/2, 1/2] (2.6e-6,
+// from a Remez exchange), n added to its exponent.  Below 2^-126 the result is
+// about 2^-126.  NaN is not kept.
+__device__ __forceinline__ Pair exp2_poly(Pair x) {
+    constexpr float kShift = 12582912.f;
+    x.x = fmaxf(x.x, -126.f);
+    x.y = fmaxf(x.y, -126.f);
+    const Pair t = add2(x, Pair{kShift, kShift});
+    const Pair n = add2(t, Pair{-kShift, -kShift});
+    const Pair f = fma2(n, Pair{-1.f, -1.f}, x);
+    Pair y = fma2(f, Pair{0.00957010221f, 0.00957010221f}, Pair{0.0559178591f, 0.0559178591f});
+    y = fma2(y, f, Pair{0.240247443f, 0.240247443f});
+    y = fma2(y, f, Pair{0.693121791f, 0.693121791f});
+    y = fma2(y, f, Pair{0.999999285f, 0.999999285f});
+    return Pair{__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
+                __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23))};
+}
+
 template <typename T, int kDim>
 struct Softmax {
     const AttentionParams& a;
     Shared* sh;
     const int half;       // 0, 1
-    const uint32_t lane0; // this warp's first TMEM lane, in address form
+    const uint32_t score, output;  // TMEM addresses of this warp's lanes
     const int row;        // of the tile
     float m, l;           // base of the weights, their sum
     int done = 0;         // blocks of this half so far, over all tiles
@@ -392,13 +465,45 @@ struct Softmax {
     uint32_t cleans = 0;  // bit s: parity of the number of checked V tiles that slot s has had
 
     __device__ __forceinline__ Softmax(const AttentionParams& args, Shared* s, uint32_t tmem, int shift)
-        : a(args), sh(s), half(threadIdx.x >> 7), lane0(tmem + (((threadIdx.x >> 5) & 3) << 21)), row(threadIdx.x & 255),
+        : a(args), sh(s), half(threadIdx.x >> 7), score(tmem + (((threadIdx.x >> 5) & 3) << 21) + score_column(threadIdx.x >> 7)),
+          output(tmem + (((threadIdx.x >> 5) & 3) << 21) + output_column(threadIdx.x >> 7)), row(threadIdx.x & 255),
           box_shift(shift) {}
 
     // the blocks of a tile that has no rows in this half
     __device__ __forceinline__ void skip(const Walk& w, int n) {
         for (int u = w.u0; u < w.u1; ++u, ++n)
             if (w.checked(u)) cleans ^= 1u << ((2 * n + 1) % kSlots);
+    }
+
+    // Weights of the block from its scores.  kMixed: three pairs in eight by
+    // exp2_poly, the others by the special-function units, so that neither those
+    // nor the issue slots bound the block alone; only where no score is masked
+    // and the base is finite.
+    template <bool kMixed>
+    __device__ __forceinline__ void weights(const float (&s)[kBlock], float base) {
+        const Pair scale{a.scale_log2, a.scale_log2}, shift{base, base};
+        Pair sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+        for (int c0 = 0; c0 < kBlock; c0 += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+                const Pair x = fma2(Pair{s[c0 + c], s[c0 + c + 1]}, scale, shift);
+                const Pair e = kMixed && ((c / 2) & 7) < kPolyPairs ? exp2_poly(x) : Pair{exp2_fast(x.x), exp2_fast(x.y)};
+                sum[(c / 2) & 1] = add2(sum[(c / 2) & 1], e);
+                // weights go to the product in the cache's 16-bit type, as the tensor cores take them; the sum keeps 32 bits
+                pk[c / 2] = Half2<T>::pack(e.x, e.y);
+            }
+            tmem_store16(score + c0 / 2, pk);
+            if (c0 == 32 || c0 == 96) {  // the products of the first 64 keys need not wait for the others
+                tmem_store_wait();
+                tmem_fence_before();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) bar_arrive(&sh->p_full[half][c0 / 64]);
+            }
+        }
+        const Pair all = add2(sum[0], sum[1]);
+        l += all.x + all.y;
     }
 
     // block u of the walk's tile, number n in the CTA; false: stalled
@@ -409,11 +514,12 @@ struct Softmax {
         tmem_fence_after();
         float s[kBlock];
 #pragma unroll
-        for (int c = 0; c < kBlock; c += 32) tmem_load32(lane0 + score_column(half) + c, s + c);
-        tmem_load_wait();
+        for (int c = 0; c < kBlock; c += 32) tmem_load32(score + c, s + c);
         const bool lost = sh->missing[n & 3] == 1 + n;
+        const bool whole = !lost && w.all_see(j0, from, to);
         bool poison = false;
-        if (lost || !w.all_see(j0, from, to)) {
+        tmem_load_wait();
+        if (!whole) {
             // visible: c <= last and (c >= near or c < sink)
             const int last = min(p - j0, limit - 1 - j0);
             const int near = (a.window < 0 || p < a.window) ? 0 : p - a.window + 1 - j0;
@@ -436,50 +542,37 @@ struct Softmax {
         }
         float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 4; c < kBlock; ++c) top[c & 3] = fmaxf(top[c & 3], s[c]);
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+        for (int c = 4; c < kBlock - 4; c += 8)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) top[x] = max3(top[x], s[c + 2 * x], s[c + 2 * x + 1]);
+        top[0] = max3(top[0], s[kBlock - 4], s[kBlock - 3]);
+        top[1] = max3(top[1], s[kBlock - 2], s[kBlock - 1]);
+        const float mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
         if (first) {
             m = mx;
             l = 0.f;
-        } else if (__any_sync(0xFFFFFFFFu, mx > m + kRaise || (m == -INFINITY && mx > m))) {
+        } else if (__any_sync(0xFFFFFFFFu, !(mx <= m + kRaise))) {  // also where mx is NaN: so becomes the row
             // raise the base: wait for the products that write O, scale it
             if (!bar_wait(&sh->pv_done[half], (done - 1) & 1, sh)) return false;
             tmem_fence_after();
-            const float mn = fmaxf(m, mx);
+            const float mn = max3(m, mx, mx);
             const float f = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
             m = mn;
             l *= f;
 #pragma unroll 1
-            for (int d = 0; d < kDim; d += 32) {
-                float o[32];
-                tmem_load32(lane0 + output_column(half) + d, o);
+            for (int d = 0; d < kDim; d += 16) {
+                float o[16];
+                tmem_load16(output + d, o);
                 tmem_load_wait();
 #pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] *= f;
-                tmem_store32(lane0 + output_column(half) + d, reinterpret_cast<const uint32_t*>(o));
+                for (int x = 0; x < 16; ++x) o[x] *= f;
+                tmem_store16(output + d, reinterpret_cast<const uint32_t*>(o));
             }
         }
-        const float base = m == -INFINITY ? 0.f : -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c0 = 0; c0 < kBlock; c0 += 64) {
-            uint32_t pk[32];
-#pragma unroll
-            for (int c = 0; c < 64; c += 2) {
-                const float e0 = exp2_fast(fmaf(s[c0 + c], a.scale_log2, base));
-                const float e1 = exp2_fast(fmaf(s[c0 + c + 1], a.scale_log2, base));
-                sum[c & 2] += e0;
-                sum[(c & 2) + 1] += e1;
-                // weights go to the product in the cache's 16-bit type, as the tensor cores take them; the sum keeps 32 bits
-                pk[c / 2] = Half2<T>::pack(e0, e1);
-            }
-            tmem_store32(lane0 + score_column(half) + c0 / 2, pk);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_store_wait();
-        tmem_fence_before();
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) bar_arrive(&sh->p_full[half]);
+        // a row without a visible key yet has no base; one with a score of +inf is NaN, as inf - inf
+        const float base = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m;
+        if (whole && !__any_sync(0xFFFFFFFFu, m == -INFINITY)) weights<true>(s, base);
+        else weights<false>(s, base);
         ++done;
         if (poison) {
             if (!bar_wait(&sh->pv_done[half], (done - 1) & 1, sh)) return false;
@@ -499,7 +592,7 @@ struct Softmax {
 #pragma unroll 1
         for (int d = 0; d < kDim; d += 32) {
             float o[32];
-            tmem_load32(lane0 + output_column(half) + d, o);
+            tmem_load32(output + d, o);
             tmem_load_wait();
 #pragma unroll 1
             for (int c = 0; c < kBlock; ++c) {
@@ -517,7 +610,7 @@ struct Softmax {
                     if (!isfinite(v1)) o[x + 1] += v1;
                 }
             }
-            tmem_store32(lane0 + output_column(half) + d, reinterpret_cast<const uint32_t*>(o));
+            tmem_store32(output + d, reinterpret_cast<const uint32_t*>(o));
         }
     }
 
@@ -537,7 +630,7 @@ struct Softmax {
 #pragma unroll 1
         for (int d = 0; d < kDim; d += 32) {
             float o[32];
-            tmem_load32(lane0 + output_column(half) + d, o);
+            tmem_load32(output + d, o);
             tmem_load_wait();
             if (!valid) continue;
             if (w.whole) {
@@ -590,7 +683,8 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
         bar_init(&sh->q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             bar_init(&sh->s_full[i], 1);
-            bar_init(&sh->p_full[i], 4);
+            bar_init(&sh->p_full[i][0], 4);
+            bar_init(&sh->p_full[i][1], 4);
             bar_init(&sh->pv_done[i], 1);
         }
         bar_init(&sh->drain, 1);
@@ -658,22 +752,34 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
         } while (ok && w.next());
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-        if (warp == 12 && lane == 0) {
+        if (warp == 12) {
+            // all lanes walk along, so that addresses stay in uniform registers; one issues
+            const bool lead = elect_one();
             constexpr uint32_t kQk = instruction<T>(kBlock, false), kPv = instruction<T>(kDim, true);
-            const auto scores = [&](int half, int slot) {
-                const uint32_t qa = q + half * (kHalf * 128), kb = ring + slot * S::kTile;
-#pragma unroll
-                for (int k = 0; k < kDim / 16; ++k)
-                    mma_smem(tmem + score_column(half), operand(qa + (k >> 2) * S::kQPanel + (k & 3) * 32, 16),
-                             operand(kb + (k >> 2) * S::kPanelRows + (k & 3) * 32, 16), kQk, k > 0);
-                mma_commit(&sh->s_full[half]);
+            const uint32_t tm = uniform(tmem), q_low = uniform(operand_low(q, 16)), k_low = uniform(operand_low(ring, 16)),
+                           v_low = uniform(operand_low(ring, S::kPanelRows));
+            const auto commit = [&](uint64_t* b) {
+                if (lead) mma_commit(b);
             };
-            const auto output = [&](int half, int slot, bool add) {
-                const uint32_t vb = ring + slot * S::kTile;
+            const auto scores = [&](int half, uint32_t slot) {
+                const uint32_t qa = q_low + half * (kHalf * 128 / 16), kb = k_low + slot * (S::kTile / 16);
+                if (lead) {
 #pragma unroll
-                for (int k = 0; k < kBlock / 16; ++k)
-                    mma_tmem(tmem + output_column(half), tmem + score_column(half) + k * 8, operand(vb + k * 2048, S::kPanelRows), kPv, add || k > 0);
-                mma_commit(&sh->pv_done[half]);
+                    for (int k = 0; k < kDim / 16; ++k)
+                        mma_smem(tm + score_column(half), qa + ((k >> 2) * S::kQPanel + (k & 3) * 32) / 16,
+                                 kb + ((k >> 2) * S::kPanelRows + (k & 3) * 32) / 16, kQk, k > 0);
+                    mma_commit(&sh->s_full[half]);
+                }
+            };
+            // keys 64 part .. 64 part + 63
+            const auto output = [&](int half, uint32_t slot, int part, bool add) {
+                const uint32_t vb = v_low + slot * (S::kTile / 16);
+                if (lead) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_tmem(tm + output_column(half), tm + score_column(half) + (part * 4 + k) * 8, vb + (part * 4 + k) * (2048 / 16),
+                                 kPv, add || k > 0);
+                }
             };
             const auto filled = [&](int f) { return bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh); };
             uint32_t cleans = 0;
@@ -690,33 +796,43 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                 const int halves = w.rows > kHalf ? 2 : 1, blocks = w.u1 - w.u0;
                 ok = bar_wait(&sh->q_full, segment & 1, sh) && filled(2 * n);
                 if (!ok) break;
-                for (int h = 0; h < halves; ++h) scores(h, (2 * n) % kSlots);
-                mma_commit(&sh->empty[(2 * n) % kSlots]);
-                if (blocks == 1) mma_commit(&sh->q_empty);
+                const uint32_t first = uniform((2 * n) % kSlots);
+                scores(0, first);
+                if (halves == 2) scores(1, first);
+                commit(&sh->empty[first]);
+                if (blocks == 1) commit(&sh->q_empty);
                 for (int b = 0; b < blocks && ok; ++b, ++n) {
                     const bool more = b + 1 < blocks;
+                    const uint32_t v_slot = uniform((2 * n + 1) % kSlots), k_slot = uniform((2 * n + 2) % kSlots);
                     ok = value_ready(2 * n + 1, w.checked(w.u0 + b));
-                    for (int h = 0; h < halves && ok; ++h) {
-                        ok = bar_wait(&sh->p_full[h], done[h] & 1, sh);
-                        if (!ok) break;
-                        ++done[h];
+                    const auto turn = [&](int h) {
+                        ok = ok && bar_wait(&sh->p_full[h][0], done[h] & 1, sh);
+                        if (!ok) return;
                         tmem_fence_after();
-                        output(h, (2 * n + 1) % kSlots, b > 0);
-                        if (!more) continue;
+                        output(h, v_slot, 0, b > 0);
+                        ok = bar_wait(&sh->p_full[h][1], done[h] & 1, sh);
+                        if (!ok) return;
+                        tmem_fence_after();
+                        output(h, v_slot, 1, true);
+                        commit(&sh->pv_done[h]);
+                        ++done[h];
+                        if (!more) return;
                         if (h == 0) ok = filled(2 * n + 2);
-                        if (ok) scores(h, (2 * n + 2) % kSlots);
-                    }
+                        if (ok) scores(h, k_slot);
+                    };
+                    turn(0);
+                    if (halves == 2) turn(1);
                     if (!ok) break;
-                    mma_commit(&sh->empty[(2 * n + 1) % kSlots]);
+                    commit(&sh->empty[v_slot]);
                     if (more) {
-                        mma_commit(&sh->empty[(2 * n + 2) % kSlots]);
-                        if (b + 2 == blocks) mma_commit(&sh->q_empty);
+                        commit(&sh->empty[k_slot]);
+                        if (b + 2 == blocks) commit(&sh->q_empty);
                     }
                 }
                 ++segment;
             } while (ok && w.next());
             // all products end before the block does, also after a stall
-            mma_commit(&sh->drain);
+            commit(&sh->drain);
             for (int i = 0; i < (1 << 22) && !bar_try(&sh->drain, 0); ++i) {
             }
         } else if (warp == 13) {
