@@ -870,6 +870,8 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     if (x->heads < 1 || x->heads % c->heads)
         return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", x->heads, c->heads);
     if (x->heads / c->heads > 256) return fail(FG_ERR_UNSUPPORTED, "%d query heads for each kv head", x->heads / c->heads);
+    if (static_cast<int64_t>(x->tokens) * (x->heads / c->heads) > INT32_MAX - 512)
+        return fail(FG_ERR_UNSUPPORTED, "%d tokens of %d heads for each kv head", x->tokens, x->heads / c->heads);
     if (x->requests > fg::attention_max_requests())
         return fail(FG_ERR_UNSUPPORTED, "%d requests, at most %d", x->requests, fg::attention_max_requests());
     if (x->window < -1 || x->sinks < 0) return fail(FG_ERR_ARG, "bad mask window=%d sinks=%d", x->window, x->sinks);
@@ -921,6 +923,9 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     a.heads = x->heads;
     a.kv_heads = c->heads;
     a.group = x->heads / c->heads;
+    const int up = log2_of(a.group);  // 2^(31 + up) / group, rounded up, fits 32 bits and is exact for 31-bit dividends
+    a.group_shift = 31 + up;
+    a.group_mul = static_cast<uint32_t>(((1ull << a.group_shift) + a.group - 1) / a.group);
     a.window = x->window;
     a.sinks = x->sinks;
     a.scale_log2 = static_cast<float>(x->scale * 1.4426950408889634);

@@ -75,35 +75,40 @@ struct TileKeys {
     int units;
 };
 
+// n / group for 0 <= n < 2^31 (the host sees to it): 64-bit divisions of every
+// row's number cost more than the copy of the row.
+__device__ __forceinline__ int div_group(const AttentionParams& a, int n) {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * a.group_mul) >> a.group_shift);
+}
+
 // Token range [i0, i1] of a tile and the row layout.  Without ids a tile is
 // kRows consecutive (token, head of the group) pairs of a request; with ids it
 // is one token and up to kRows heads of the group.
 template <int kRows, bool kIds>
 struct Tiles {
+    __device__ static __forceinline__ int parts(const AttentionParams& a) { return (a.group + kRows - 1) / kRows; }
     __device__ static __forceinline__ int count(const AttentionParams& a, const Request& r) {
-        if (kIds) return r.rows * ((a.group + kRows - 1) / kRows);
-        return static_cast<int>((static_cast<int64_t>(r.rows) * a.group + kRows - 1) / kRows);
+        return kIds ? r.rows * parts(a) : (r.rows * a.group + kRows - 1) / kRows;
     }
     __device__ static __forceinline__ void tokens(const AttentionParams& a, const Request& r, int t, int* i0, int* i1) {
         if (kIds) {
-            *i0 = *i1 = t / ((a.group + kRows - 1) / kRows);
+            *i0 = *i1 = t / parts(a);
         } else {
-            const int64_t first = static_cast<int64_t>(t) * kRows;
-            *i0 = static_cast<int>(first / a.group);
-            *i1 = min(r.rows - 1, static_cast<int>((first + kRows - 1) / a.group));
+            *i0 = div_group(a, t * kRows);
+            *i1 = min(r.rows - 1, div_group(a, t * kRows + kRows - 1));
         }
     }
     // row -> (token of the request, head of the group); false past the tile's end
     __device__ static __forceinline__ bool row(const AttentionParams& a, const Request& r, int t, int row, int* i, int* g) {
         if (kIds) {
-            const int hg = (a.group + kRows - 1) / kRows;
+            const int hg = parts(a);
             *i = t / hg;
-            *g = (t % hg) * kRows + row;
+            *g = (t - *i * hg) * kRows + row;
             return *g < a.group;
         }
-        const int64_t R = static_cast<int64_t>(t) * kRows + row;
-        *i = static_cast<int>(R / a.group);
-        *g = static_cast<int>(R % a.group);
+        const int R = t * kRows + row;
+        *i = div_group(a, R);
+        *g = R - *i * a.group;
         return *i < r.rows;
     }
 };
@@ -132,14 +137,6 @@ __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Re
     return k;
 }
 
-template <int kRows, bool kIds, int kChunk, int kUnitChunks>
-__device__ __forceinline__ int request_units(const AttentionParams& a, const Request& r) {
-    const int n = Tiles<kRows, kIds>::count(a, r);
-    int u = 0;
-    for (int t = 0; t < n; ++t) u += tile_keys<kRows, kIds, kChunk, kUnitChunks>(a, r, t).units;
-    return u;
-}
-
 // Where a CTA's range begins, and the range.
 struct Place {
     int64_t unit, end;   // this CTA's units [unit, end)
@@ -148,18 +145,23 @@ struct Place {
     int head, request, tile, offset;  // the first unit: its tile and its place in it
 };
 
-// Called by all kThreads threads; scratch holds requests + 64 ints.
-template <int kRows, bool kIds, int kChunk, int kUnitChunks, int kThreads>
+// Called by all kThreads threads; scratch holds requests + 64 ints.  kLanes
+// threads count the tiles of a request: 1 where requests are short, 8 where
+// they have many tiles.
+template <int kRows, bool kIds, int kChunk, int kUnitChunks, int kThreads, int kLanes>
 __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, int cta, int ctas) {
     int* pre = scratch + 64;  // inclusive prefix of the requests' units
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kWarps = kThreads / 32;
     int carry = 0;
-    for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
-        const int b = b0 + tid;
-        int u = 0;
-        if (b < a.requests) u = request_units<kRows, kIds, kChunk, kUnitChunks>(a, load_request(a, b));
-        int s = u;
+    for (int b0 = 0; b0 < a.requests; b0 += kThreads / kLanes) {
+        const int b = b0 + tid / kLanes;
+        int s = 0;
+        if (b < a.requests) {
+            const Request r = load_request(a, b);
+            const int n = Tiles<kRows, kIds>::count(a, r);
+            for (int t = tid % kLanes; t < n; t += kLanes) s += tile_keys<kRows, kIds, kChunk, kUnitChunks>(a, r, t).units;
+        }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int v = __shfl_up_sync(0xFFFFFFFFu, s, d);
@@ -173,7 +175,7 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
             if (w < warp) before += v;
             sum += v;
         }
-        if (b < a.requests) pre[b] = before + s;
+        if (b < a.requests && tid % kLanes == kLanes - 1) pre[b] = before + s;
         carry += sum;
         __syncthreads();
     }
@@ -198,12 +200,27 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
     x.request = lo;
     if (lo > 0) rest -= pre[lo - 1];
     const Request r = load_request(a, lo);
+    // the tile that holds unit `rest` of the request, 32 tiles at a time, in every warp
     const int tiles = Tiles<kRows, kIds>::count(a, r);
     int t = 0;
-    for (; t + 1 < tiles; ++t) {
-        const int u = tile_keys<kRows, kIds, kChunk, kUnitChunks>(a, r, t).units;
-        if (rest < u) break;
-        rest -= u;
+    for (int t0 = 0; t0 < tiles; t0 += 32) {
+        const int mine = t0 + lane;
+        const int u = mine < tiles ? tile_keys<kRows, kIds, kChunk, kUnitChunks>(a, r, mine).units : 0;
+        int s = u;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xFFFFFFFFu, s, d);
+            if (lane >= d) s += v;
+        }
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, s > rest);
+        if (past) {
+            const int first = __ffs(past) - 1;
+            t = t0 + first;
+            rest -= __shfl_sync(0xFFFFFFFFu, s - u, first);
+            break;
+        }
+        t = min(t0 + 32, tiles) - 1;
+        rest -= __shfl_sync(0xFFFFFFFFu, s, 31);
     }
     x.tile = t;
     x.offset = rest;

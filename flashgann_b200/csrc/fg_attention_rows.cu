@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     char* ws = static_cast<char*>(a.workspace);
 
-    const Place pl = locate<kRows, kIds, kChunk, kWarps, kThreads>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, kIds, kChunk, kWarps, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
     __syncthreads();  // the rings overlay the scan
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
     if (pl.unit >= pl.end) return;

@@ -60,7 +60,8 @@ struct Smem {
 };
 
 struct Shared {
-    uint64_t full[kSlots], clean[kSlots], empty[kSlots];
+    uint64_t full[kSlots], empty[kSlots];
+    uint64_t raw[kSlots];   // a V tile that is to be looked through has arrived; `full` follows when that is done
     uint64_t q_full, q_empty;
     uint64_t s_full[2], p_full[2][2], pv_done[2];  // p_full: of each half, the weights of keys 0-63 and 64-127
     uint64_t drain;
@@ -79,6 +80,9 @@ __device__ __forceinline__ void bar_init(uint64_t* b, int count) {
 }
 __device__ __forceinline__ void bar_arrive(uint64_t* b) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ void bar_arrive3(uint64_t* b) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], 3;" ::"r"(smem_addr(b)) : "memory");
 }
 __device__ __forceinline__ bool bar_try(uint64_t* b, int parity) {
     uint32_t ok;
@@ -220,7 +224,7 @@ struct Walk {
         Tiles<kRows, false>::tokens(a, req, tile, &i0, &i1);
         p0 = req.kv_len - req.rows + i0;
         p1 = req.kv_len - req.rows + i1;
-        rows = static_cast<int>(min(static_cast<int64_t>(kRows), static_cast<int64_t>(req.rows) * a.group - static_cast<int64_t>(tile) * kRows));
+        rows = min(kRows, req.rows * a.group - tile * kRows);
         const int64_t last = first + keys.units;
         u0 = static_cast<int>(unit - first);
         u1 = static_cast<int>(min(last, end) - first);
@@ -247,11 +251,12 @@ struct Walk {
     // whether block u's V tile is looked through before it is used
     __device__ __forceinline__ bool checked(int u) const {
         int limit;
-        return !all_see(block(u, &limit), p0, p1);
+        const int j0 = block(u, &limit);
+        return !all_see(j0, limit, p0, p1);
     }
-    // every row between positions a and b sees all keys of the block at j0
-    __device__ __forceinline__ bool all_see(int j0, int from, int to) const {
-        return j0 + kBlock - 1 <= from && (a.window < 0 || to - j0 < a.window || j0 + kBlock - 1 < a.sinks);
+    // every row between two positions sees all keys of the block at j0, and all are loaded
+    __device__ __forceinline__ bool all_see(int j0, int limit, int from, int to) const {
+        return j0 + kBlock <= limit && j0 + kBlock - 1 <= from && (a.window < 0 || to - j0 < a.window || j0 + kBlock - 1 < a.sinks);
     }
 };
 
@@ -287,7 +292,9 @@ struct Loader {
         return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.pages) ? id : a.pages;
     }
 
-    __device__ __forceinline__ bool block(const Walk& w, int j0, int limit, int pg, int n, const CUtensorMap* k_map, const CUtensorMap* v_map) {
+    __device__ __forceinline__ bool block(const Walk& w, int u, int j0, int limit, int pg, int n, const CUtensorMap* k_map,
+                                          const CUtensorMap* v_map) {
+        const bool checked = w.checked(u);
         const int j = j0 + (box << box_shift);
         const bool mine = (box << box_shift) < kBlock;
         const uint32_t found = __ballot_sync(0xFFFFFFFFu, mine && pg < a.pages);
@@ -303,12 +310,17 @@ struct Loader {
                     sh->boxes[n & 3] = bits;
                     sh->missing[n & 3] = 1 + n;
                 }
-                bar_expect(&sh->full[slot], S::kTile);
+                if (half == 1 && checked) {
+                    bar_expect(&sh->raw[slot], S::kTile);
+                } else {
+                    bar_arrive3(&sh->full[slot]);
+                    bar_expect(&sh->full[slot], S::kTile);
+                }
             }
             __syncwarp();
             if (mine)
                 load_box(ring + slot * S::kTile + panel * S::kPanelRows + (box << box_shift) * 128, half == 0 ? k_map : v_map,
-                         &sh->full[slot], panel * 64, j & (a.page_size - 1), w.head, pg);
+                         half == 1 && checked ? &sh->raw[slot] : &sh->full[slot], panel * 64, j & (a.page_size - 1), w.head, pg);
         }
         return true;
     }
@@ -322,7 +334,8 @@ struct Helper {
     const AttentionParams& a;
     Shared* sh;
     const uint32_t q, ring;
-    const int tid;  // 0 .. 127
+    const int tid;        // 0 .. 127
+    uint32_t looked = 0;  // bit s: parity of the number of tiles looked through in slot s
 
     __device__ __forceinline__ Helper(const AttentionParams& args, Shared* s, uint32_t q_addr, uint32_t ring_addr)
         : a(args), sh(s), q(q_addr), ring(ring_addr), tid(threadIdx.x & 127) {}
@@ -357,7 +370,8 @@ struct Helper {
     // in the ring.
     __device__ __forceinline__ bool clear_masked(const Walk& w, int j0, int limit, int f) {
         const int slot = f % kSlots;
-        if (!bar_wait(&sh->full[slot], (f / kSlots) & 1, sh)) return false;
+        if (!bar_wait(&sh->raw[slot], (looked >> slot) & 1, sh)) return false;
+        looked ^= 1u << slot;
         const uint32_t base = ring + slot * S::kTile;
         const int p = tid & 15;
         bool bad = false;
@@ -372,17 +386,20 @@ struct Helper {
                              : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                              : "r"(at)
                              : "memory");
+                // a half word whose exponent bits are all set is zero in x; the usual test for a zero among the two
+                constexpr uint32_t kE = Half2<T>::kExpMask | (Half2<T>::kExpMask << 16);
                 bool here = false;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    constexpr uint32_t kE = Half2<T>::kExpMask;
-                    if ((v[e] & kE) == kE) {
-                        v[e] &= 0xFFFF0000u;
-                        here = true;
-                    }
-                    if ((v[e] & (kE << 16)) == (kE << 16)) {
-                        v[e] &= 0x0000FFFFu;
-                        here = true;
+                    const uint32_t x = ~v[e] & kE;
+                    here |= ((x - 0x00010001u) & ~x & 0x80008000u) != 0;
+                }
+                if (here) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t x = ~v[e] & kE;
+                        if (!(x & 0xFFFFu)) v[e] &= 0xFFFF0000u;
+                        if (!(x >> 16)) v[e] &= 0x0000FFFFu;
                     }
                 }
                 if (here) {
@@ -395,7 +412,7 @@ struct Helper {
         if (bad) sh->nonfinite[slot] = 1 + f;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if ((tid & 31) == 0) bar_arrive(&sh->clean[slot]);
+        if ((tid & 31) == 0) bar_arrive(&sh->full[slot]);
         return true;
     }
 };
@@ -425,6 +442,8 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
     return pair(r);
 }
+// bits 0 .. n - 1
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 // NaN if any is
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -462,18 +481,11 @@ struct Softmax {
     float m, l;           // base of the weights, their sum
     int done = 0;         // blocks of this half so far, over all tiles
     const int box_shift;
-    uint32_t cleans = 0;  // bit s: parity of the number of checked V tiles that slot s has had
 
     __device__ __forceinline__ Softmax(const AttentionParams& args, Shared* s, uint32_t tmem, int shift)
         : a(args), sh(s), half(threadIdx.x >> 7), score(tmem + (((threadIdx.x >> 5) & 3) << 21) + score_column(threadIdx.x >> 7)),
           output(tmem + (((threadIdx.x >> 5) & 3) << 21) + output_column(threadIdx.x >> 7)), row(threadIdx.x & 255),
           box_shift(shift) {}
-
-    // the blocks of a tile that has no rows in this half
-    __device__ __forceinline__ void skip(const Walk& w, int n) {
-        for (int u = w.u0; u < w.u1; ++u, ++n)
-            if (w.checked(u)) cleans ^= 1u << ((2 * n + 1) % kSlots);
-    }
 
     // Weights of the block from its scores.  kMixed: three pairs in eight by
     // exp2_poly, the others by the special-function units, so that neither those
@@ -516,7 +528,7 @@ struct Softmax {
 #pragma unroll
         for (int c = 0; c < kBlock; c += 32) tmem_load32(score + c, s + c);
         const bool lost = sh->missing[n & 3] == 1 + n;
-        const bool whole = !lost && w.all_see(j0, from, to);
+        const bool whole = !lost && w.all_see(j0, limit, from, to);
         bool poison = false;
         tmem_load_wait();
         if (!whole) {
@@ -525,19 +537,22 @@ struct Softmax {
             const int near = (a.window < 0 || p < a.window) ? 0 : p - a.window + 1 - j0;
             const int sink = a.sinks - j0;
 #pragma unroll
-            for (int c = 0; c < kBlock; ++c)
-                if (!(c <= last && (c >= near || c < sink))) s[c] = -INFINITY;
-            if (lost) {
-                const uint32_t found = sh->boxes[n & 3];
+            for (int c0 = 0; c0 < kBlock; c0 += 32) {  // 32 columns at a time as bits
+                uint32_t see = below(last + 1 - c0) & (~below(near - c0) | below(sink - c0));
+                if (lost) {
+                    const uint32_t found = sh->boxes[n & 3];
+#pragma unroll 1
+                    for (int c = 0; c < 32; c += 8)  // a box is 8 keys or more
+                        if (!((found >> ((c0 + c) >> box_shift)) & 1u)) see &= ~(0xFFu << c);
+                }
 #pragma unroll
-                for (int c = 0; c < kBlock; ++c)
-                    if (!((found >> (c >> box_shift)) & 1u)) s[c] = -INFINITY;
+                for (int c = 0; c < 32; ++c)
+                    if (!((see >> c) & 1u)) s[c0 + c] = -INFINITY;
             }
         }
         if (w.checked(u)) {
             const int f = 2 * n + 1;
-            if (!bar_wait(&sh->clean[f % kSlots], (cleans >> (f % kSlots)) & 1, sh)) return false;
-            cleans ^= 1u << (f % kSlots);
+            if (!bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh)) return false;
             poison = sh->nonfinite[f % kSlots] == 1 + f;
         }
         float top[4] = {s[0], s[1], s[2], s[3]};
@@ -669,13 +684,13 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     char* ws = static_cast<char*>(a.workspace);
 
-    const Place pl = locate<kRows, false, kBlock, 1, kThreads>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, false, kBlock, 1, kThreads, 8>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
     if (pl.unit >= pl.end) return;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) {
-            bar_init(&sh->full[i], 1);
-            bar_init(&sh->clean[i], 4);
+            bar_init(&sh->full[i], 4);  // the four helper warps, or four times the loader
+            bar_init(&sh->raw[i], 1);
             bar_init(&sh->empty[i], 1);
             sh->nonfinite[i] = 0;
         }
@@ -719,7 +734,6 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
         bool ok = true;
         do {
             if (sm.half * kHalf >= w.rows) {  // nothing in this half
-                sm.skip(w, n);
                 n += w.u1 - w.u0;
                 continue;
             }
@@ -727,9 +741,9 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
             const bool valid = Tiles<kRows, false>::row(a, w.req, w.tile, sm.row, &i, &g);
             const int p = valid ? w.req.kv_len - w.req.rows + i : -1;
             // positions of the half's first and last row
-            const int64_t r0 = static_cast<int64_t>(w.tile) * kRows + sm.half * kHalf;
-            const int from = w.req.kv_len - w.req.rows + static_cast<int>(r0 / a.group);
-            const int to = w.req.kv_len - w.req.rows + min(w.req.rows - 1, static_cast<int>((r0 + kHalf - 1) / a.group));
+            const int r0 = w.tile * kRows + sm.half * kHalf;
+            const int from = w.req.kv_len - w.req.rows + div_group(a, r0);
+            const int to = w.req.kv_len - w.req.rows + min(w.req.rows - 1, div_group(a, r0 + kHalf - 1));
             for (int u = w.u0; ok && u < w.u1; ++u, ++n) ok = sm.block(w, u, n, u == w.u0, p, from, to);
             ok = sm.store(w, ok);
         } while (w.next() && ok);
@@ -782,14 +796,6 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                 }
             };
             const auto filled = [&](int f) { return bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh); };
-            uint32_t cleans = 0;
-            const auto value_ready = [&](int f, bool checked) {
-                const int slot = f % kSlots;
-                if (!checked) return filled(f);
-                const int parity = (cleans >> slot) & 1;
-                cleans ^= 1u << slot;
-                return bar_wait(&sh->clean[slot], parity, sh);
-            };
             int n = 0, segment = 0, done[2] = {0, 0};
             bool ok = true;
             do {
@@ -804,7 +810,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                 for (int b = 0; b < blocks && ok; ++b, ++n) {
                     const bool more = b + 1 < blocks;
                     const uint32_t v_slot = uniform((2 * n + 1) % kSlots), k_slot = uniform((2 * n + 2) % kSlots);
-                    ok = value_ready(2 * n + 1, w.checked(w.u0 + b));
+                    ok = filled(2 * n + 1);
                     const auto turn = [&](int h) {
                         ok = ok && bar_wait(&sh->p_full[h][0], done[h] & 1, sh);
                         if (!ok) return;
@@ -848,18 +854,15 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                         next_j0 = w.block(u + 1, &next_limit);
                         next_pg = ld.page(w, next_j0, next_limit);
                     }
-                    ok = ld.block(w, j0, limit, pg, n, &k_map, &v_map);
+                    ok = ld.block(w, u, j0, limit, pg, n, &k_map, &v_map);
                     j0 = next_j0;
                     limit = next_limit;
                     pg = next_pg;
                 }
             } while (ok && w.next());
-            // copies under way end before the block does, also after a stall
-            if (!ok) {
-                for (int f = max(0, 2 * n - kSlots); f < 2 * n + 2; ++f)
-                    for (int i = 0; i < (1 << 16) && !bar_try(&sh->full[f % kSlots], (f / kSlots) & 1); ++i) {
-                    }
-            }
+            // after a stall: time for the copies under way to end before the block does
+            if (!ok)
+                for (int i = 0; i < (1 << 14); ++i) bar_try(&sh->drain, 0);
         }
         __syncwarp();
     }

@@ -128,6 +128,8 @@ struct AttentionParams {
     const int32_t* query_start = nullptr;
     const int32_t* kv_len = nullptr;
     int requests = 0, tokens = 0, heads = 0, kv_heads = 0, group = 0;
+    uint32_t group_mul = 0;  // n / group = n * group_mul >> group_shift for n < 2^31
+    int group_shift = 0;
     int window = -1, sinks = 0;
     float scale_log2 = 0.f;  // scale * log2(e): all exponents are base 2
     const int32_t* ids = nullptr;

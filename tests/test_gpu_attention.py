@@ -168,7 +168,7 @@ SHAPES = [
     ([250, 3], [129, 128], 8, 2, 128, 16, "fp16", "phd"),
     ([513], [65], 16, 2, 64, 32, "bf16", "phd"),
 ]
-MASKS = [(-1, 0), (0, 0), (0, 3), (1, 0), (17, 4), (64, 100), (1000, 16)]
+MASKS = [(-1, 0), (0, 0), (0, 3), (1, 0), (17, 4), (64, 100), (100, 200), (5, 300), (1000, 16)]
 
 
 @pytest.mark.parametrize("mask", MASKS)
