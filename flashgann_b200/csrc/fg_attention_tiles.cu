@@ -46,7 +46,7 @@ constexpr int kBlock = 128;  // keys
 constexpr int kThreads = 512;
 constexpr int kSlots = 5;    // K and V tiles in the ring: two blocks and a half
 constexpr float kRaise = 8.f;
-constexpr int kPolyPairs = 3;  // of 8 pairs of weights, see exp2_poly
+constexpr int kPolyPairs = 1;  // of 8 pairs of weights, see exp2_poly
 
 template <int kDim>
 struct Smem {
@@ -98,14 +98,25 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, int parity) {
 __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
 }
-// false: the wait ran out, here or in another warp
+// false: the wait ran out
 __device__ __forceinline__ bool bar_wait(uint64_t* b, int parity, Shared* sh) {
-    for (int i = 0; i < (1 << 22); ++i) {
-        if (bar_try(b, parity)) return true;
-        if ((i & 1023) == 1023 && *reinterpret_cast<volatile int*>(&sh->stalled)) return false;
+    for (int i = 0; !bar_try(b, parity); ++i)
+        if (i == (1 << 22)) {
+            *reinterpret_cast<volatile int*>(&sh->stalled) = 1;
+            return false;
+        }
+    return true;
+}
+// for waits that nothing hurries: leaves the issue slots to the other warps
+__device__ __forceinline__ bool bar_wait_idle(uint64_t* b, int parity, Shared* sh) {
+    for (int i = 0; !bar_try(b, parity); ++i) {
+        if (i == (1 << 18)) {
+            *reinterpret_cast<volatile int*>(&sh->stalled) = 1;
+            return false;
+        }
+        __nanosleep(200);
     }
-    *reinterpret_cast<volatile int*>(&sh->stalled) = 1;
-    return false;
+    return true;
 }
 
 // ---- tcgen05 ----
@@ -201,6 +212,12 @@ __device__ __forceinline__ constexpr uint32_t output_column(int half) { return 2
 
 // ---- the walk over a CTA's range, the same in every role ----
 
+// Blocks [0, sinks) and [begin, end) of a tile.
+struct Span {
+    int sinks, begin, end;
+    __device__ __forceinline__ bool has(int u) const { return u < sinks || (u >= begin && u < end); }
+};
+
 struct Walk {
     const AttentionParams& a;
     Request req;
@@ -211,6 +228,7 @@ struct Walk {
     int p0, p1;                // positions of the tile's first and last row
     int rows;                  // rows in the tile
     bool whole, opening;       // the segment is the whole tile; it is the CTA's first
+    Span all;                  // blocks that all rows see; the V tiles of the others are looked through before their use
 
     __device__ __forceinline__ Walk(const AttentionParams& args, const Place& pl)
         : a(args), head(pl.head), request(pl.request), tile(pl.tile), unit(pl.unit), end(pl.end), first(pl.unit - pl.offset),
@@ -229,6 +247,7 @@ struct Walk {
         u0 = static_cast<int>(unit - first);
         u1 = static_cast<int>(min(last, end) - first);
         whole = u0 == 0 && u1 == keys.units;
+        all = seen(p0, p1);
     }
     __device__ __forceinline__ bool next() {
         unit = first + u1;
@@ -248,15 +267,15 @@ struct Walk {
         *limit = keys.hi;
         return keys.base + (u - keys.sink_chunks) * kBlock;
     }
-    // whether block u's V tile is looked through before it is used
-    __device__ __forceinline__ bool checked(int u) const {
-        int limit;
-        const int j0 = block(u, &limit);
-        return !all_see(j0, limit, p0, p1);
-    }
-    // every row between two positions sees all keys of the block at j0, and all are loaded
-    __device__ __forceinline__ bool all_see(int j0, int limit, int from, int to) const {
-        return j0 + kBlock <= limit && j0 + kBlock - 1 <= from && (a.window < 0 || to - j0 < a.window || j0 + kBlock - 1 < a.sinks);
+    // The blocks that every row between positions `from` and `to` sees whole.
+    __device__ __forceinline__ Span seen(int from, int to) const {
+        Span s;
+        s.sinks = keys.sink_hi / kBlock;
+        const int last = min(from, keys.hi - 1) - (kBlock - 1) - keys.base;  // blocks that start here or before end in time
+        const int near = a.window < 0 ? -1 : to - a.window - keys.base;      // blocks that start here or before are too far back
+        s.begin = keys.sink_chunks + (near < 0 ? 0 : near / kBlock + 1);
+        s.end = keys.sink_chunks + (last < 0 ? 0 : last / kBlock + 1);
+        return s;
     }
 };
 
@@ -294,7 +313,7 @@ struct Loader {
 
     __device__ __forceinline__ bool block(const Walk& w, int u, int j0, int limit, int pg, int n, const CUtensorMap* k_map,
                                           const CUtensorMap* v_map) {
-        const bool checked = w.checked(u);
+        const bool checked = !w.all.has(u);
         const int j = j0 + (box << box_shift);
         const bool mine = (box << box_shift) < kBlock;
         const uint32_t found = __ballot_sync(0xFFFFFFFFu, mine && pg < a.pages);
@@ -370,7 +389,7 @@ struct Helper {
     // in the ring.
     __device__ __forceinline__ bool clear_masked(const Walk& w, int j0, int limit, int f) {
         const int slot = f % kSlots;
-        if (!bar_wait(&sh->raw[slot], (looked >> slot) & 1, sh)) return false;
+        if (!bar_wait_idle(&sh->raw[slot], (looked >> slot) & 1, sh)) return false;
         looked ^= 1u << slot;
         const uint32_t base = ring + slot * S::kTile;
         const int p = tid & 15;
@@ -519,20 +538,20 @@ struct Softmax {
     }
 
     // block u of the walk's tile, number n in the CTA; false: stalled
-    __device__ __forceinline__ bool block(const Walk& w, int u, int n, bool first, int p, int from, int to) {
-        int limit;
-        const int j0 = w.block(u, &limit);
+    __device__ __forceinline__ bool block(const Walk& w, int u, int n, bool first, int p, const Span& mine) {
         if (!bar_wait(&sh->s_full[half], done & 1, sh)) return false;
         tmem_fence_after();
         float s[kBlock];
 #pragma unroll
         for (int c = 0; c < kBlock; c += 32) tmem_load32(score + c, s + c);
         const bool lost = sh->missing[n & 3] == 1 + n;
-        const bool whole = !lost && w.all_see(j0, limit, from, to);
+        const bool whole = !lost && mine.has(u);
         bool poison = false;
         tmem_load_wait();
         if (!whole) {
             // visible: c <= last and (c >= near or c < sink)
+            int limit;
+            const int j0 = w.block(u, &limit);
             const int last = min(p - j0, limit - 1 - j0);
             const int near = (a.window < 0 || p < a.window) ? 0 : p - a.window + 1 - j0;
             const int sink = a.sinks - j0;
@@ -550,7 +569,7 @@ struct Softmax {
                     if (!((see >> c) & 1u)) s[c0 + c] = -INFINITY;
             }
         }
-        if (w.checked(u)) {
+        if (!w.all.has(u)) {  // the V tile was looked through
             const int f = 2 * n + 1;
             if (!bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh)) return false;
             poison = sh->nonfinite[f % kSlots] == 1 + f;
@@ -744,7 +763,8 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
             const int r0 = w.tile * kRows + sm.half * kHalf;
             const int from = w.req.kv_len - w.req.rows + div_group(a, r0);
             const int to = w.req.kv_len - w.req.rows + min(w.req.rows - 1, div_group(a, r0 + kHalf - 1));
-            for (int u = w.u0; ok && u < w.u1; ++u, ++n) ok = sm.block(w, u, n, u == w.u0, p, from, to);
+            const Span mine = w.seen(from, to);
+            for (int u = w.u0; ok && u < w.u1; ++u, ++n) ok = sm.block(w, u, n, u == w.u0, p, mine);
             ok = sm.store(w, ok);
         } while (w.next() && ok);
     } else if (warp < 12) {
@@ -753,11 +773,11 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
         int n = 0, segment = 0;
         bool ok = true;
         do {
-            ok = bar_wait(&sh->q_empty, (segment & 1) ^ 1, sh);
+            ok = bar_wait_idle(&sh->q_empty, (segment & 1) ^ 1, sh);
             if (!ok) break;
             hp.load_q(w);
             for (int u = w.u0; ok && u < w.u1; ++u, ++n) {
-                if (!w.checked(u)) continue;
+                if (w.all.has(u)) continue;
                 int limit;
                 const int j0 = w.block(u, &limit);
                 ok = hp.clear_masked(w, j0, limit, 2 * n + 1);
@@ -795,43 +815,56 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                                  kPv, add || k > 0);
                 }
             };
-            const auto filled = [&](int f) { return bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh); };
-            int n = 0, segment = 0, done[2] = {0, 0};
+            struct Turn {  // place in the ring, and the parity of its use
+                uint32_t slot;
+                int parity;
+                __device__ __forceinline__ void advance() {
+                    if (++slot == kSlots) {
+                        slot = 0;
+                        parity ^= 1;
+                    }
+                }
+            } at{0, 0};  // the next tile to be used
+            const auto filled = [&](const Turn& t) { return bar_wait(&sh->full[t.slot], t.parity, sh); };
+            int segment = 0, done[2] = {0, 0};
             bool ok = true;
             do {
                 const int halves = w.rows > kHalf ? 2 : 1, blocks = w.u1 - w.u0;
-                ok = bar_wait(&sh->q_full, segment & 1, sh) && filled(2 * n);
+                ok = bar_wait(&sh->q_full, segment & 1, sh) && filled(at);
                 if (!ok) break;
-                const uint32_t first = uniform((2 * n) % kSlots);
-                scores(0, first);
-                if (halves == 2) scores(1, first);
-                commit(&sh->empty[first]);
+                scores(0, at.slot);
+                if (halves == 2) scores(1, at.slot);
+                commit(&sh->empty[at.slot]);
                 if (blocks == 1) commit(&sh->q_empty);
-                for (int b = 0; b < blocks && ok; ++b, ++n) {
+                at.advance();
+                for (int b = 0; b < blocks && ok; ++b) {
                     const bool more = b + 1 < blocks;
-                    const uint32_t v_slot = uniform((2 * n + 1) % kSlots), k_slot = uniform((2 * n + 2) % kSlots);
-                    ok = filled(2 * n + 1);
+                    const Turn v = at;
+                    at.advance();
+                    const Turn k = at;
+                    if (more) at.advance();
+                    ok = filled(v);
                     const auto turn = [&](int h) {
                         ok = ok && bar_wait(&sh->p_full[h][0], done[h] & 1, sh);
                         if (!ok) return;
                         tmem_fence_after();
-                        output(h, v_slot, 0, b > 0);
+                        output(h, v.slot, 0, b > 0);
                         ok = bar_wait(&sh->p_full[h][1], done[h] & 1, sh);
                         if (!ok) return;
                         tmem_fence_after();
-                        output(h, v_slot, 1, true);
+                        output(h, v.slot, 1, true);
                         commit(&sh->pv_done[h]);
                         ++done[h];
                         if (!more) return;
-                        if (h == 0) ok = filled(2 * n + 2);
-                        if (ok) scores(h, k_slot);
+                        if (h == 0) ok = filled(k);
+                        if (ok) scores(h, k.slot);
                     };
                     turn(0);
                     if (halves == 2) turn(1);
                     if (!ok) break;
-                    commit(&sh->empty[v_slot]);
+                    commit(&sh->empty[v.slot]);
                     if (more) {
-                        commit(&sh->empty[k_slot]);
+                        commit(&sh->empty[k.slot]);
                         if (b + 2 == blocks) commit(&sh->q_empty);
                     }
                 }
