@@ -9,7 +9,7 @@
 // TMEM operand.  TMEM holds exactly S/P and O of both halves: 4 x 128 columns.
 //
 // Warp roles (16 warps, one CTA per SM):
-//   0-3, 4-7   softmax of half 0 and 1 (192 registers a thread)
+//   0-3, 4-7   softmax of half 0 and 1 (200 registers a thread)
 //   8-11       copy the query rows in (16-byte cp.async), and look through the V
 //              tiles that not all rows see whole, see clear_masked
 //   12         issues the products
@@ -44,7 +44,7 @@ constexpr int kRows = 256;
 constexpr int kHalf = 128;
 constexpr int kBlock = 128;  // keys
 constexpr int kThreads = 512;
-constexpr int kSlots = 5;    // K and V tiles in the ring: two blocks and a half
+constexpr int kSlots = 5;    // see Loader::block; K and V tiles in the ring: two blocks and a half
 constexpr float kRaise = 8.f;
 constexpr int kPolyPairs = 1;  // of 8 pairs of weights, see exp2_poly
 
@@ -60,7 +60,8 @@ struct Smem {
 };
 
 struct Shared {
-    uint64_t full[kSlots], empty[kSlots];
+    uint64_t full[kSlots];
+    uint64_t used[4];       // of block n % 4: its V tile, the next block's K tile and, of a segment's first block, its K tile are free
     uint64_t raw[kSlots];   // a V tile that is to be looked through has arrived; `full` follows when that is done
     uint64_t q_full, q_empty;
     uint64_t s_full[2], p_full[2][2], pv_done[2];  // p_full: of each half, the weights of keys 0-63 and 64-127
@@ -114,7 +115,7 @@ __device__ __forceinline__ bool bar_wait_idle(uint64_t* b, int parity, Shared* s
             *reinterpret_cast<volatile int*>(&sh->stalled) = 1;
             return false;
         }
-        __nanosleep(200);
+        __nanosleep(50);
     }
     return true;
 }
@@ -311,8 +312,9 @@ struct Loader {
         return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.pages) ? id : a.pages;
     }
 
-    __device__ __forceinline__ bool block(const Walk& w, int u, int j0, int limit, int pg, int n, const CUtensorMap* k_map,
-                                          const CUtensorMap* v_map) {
+    // before: whether block n - 2 was the first of its segment
+    __device__ __forceinline__ bool block(const Walk& w, int u, int j0, int limit, int pg, int n, bool before,
+                                          const CUtensorMap* k_map, const CUtensorMap* v_map) {
         const bool checked = !w.all.has(u);
         const int j = j0 + (box << box_shift);
         const bool mine = (box << box_shift) < kBlock;
@@ -321,7 +323,9 @@ struct Loader {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int f = 2 * n + half, slot = f % kSlots;
-            if (!bar_wait(&sh->empty[slot], ((f / kSlots) & 1) ^ 1, sh)) return false;
+            // the slot's last content: V of block n - 3, then K of block n - 2
+            const int e = half == 1 && before ? n - 2 : n - 3;
+            if (e >= 0 && !bar_wait_idle(&sh->used[e & 3], (e >> 2) & 1, sh)) return false;
             if (lane == 0) {
                 if (half == 0 && found != wanted) {
                     uint32_t bits = 0;
@@ -499,6 +503,7 @@ struct Softmax {
     const int row;        // of the tile
     float m, l;           // base of the weights, their sum
     int done = 0;         // blocks of this half so far, over all tiles
+    int settled = 0;      // of them, those whose products pv_done tells of: a segment's last, and with a V tile looked through
     const int box_shift;
 
     __device__ __forceinline__ Softmax(const AttentionParams& args, Shared* s, uint32_t tmem, int shift)
@@ -506,16 +511,15 @@ struct Softmax {
           output(tmem + (((threadIdx.x >> 5) & 3) << 21) + output_column(threadIdx.x >> 7)), row(threadIdx.x & 255),
           box_shift(shift) {}
 
-    // Weights of the block from its scores.  kMixed: three pairs in eight by
-    // exp2_poly, the others by the special-function units, so that neither those
-    // nor the issue slots bound the block alone; only where no score is masked
-    // and the base is finite.
-    template <bool kMixed>
-    __device__ __forceinline__ void weights(const float (&s)[kBlock], float base) {
+    // The weights of 64 keys from key kFrom on from their scores, into place.
+    // kMixed: one pair in eight by exp2_poly, the others by the special-function
+    // units (measured: 0, 1, 2, 3, 4 in eight); only where no score is masked and
+    // the base is finite.
+    template <bool kMixed, int kFrom>
+    __device__ __forceinline__ void weights(const float (&s)[kBlock], float base, Pair (&sum)[2]) {
         const Pair scale{a.scale_log2, a.scale_log2}, shift{base, base};
-        Pair sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-        for (int c0 = 0; c0 < kBlock; c0 += 32) {
+        for (int c0 = kFrom; c0 < kFrom + 64; c0 += 32) {
             uint32_t pk[16];
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
@@ -526,26 +530,36 @@ struct Softmax {
                 pk[c / 2] = Half2<T>::pack(e.x, e.y);
             }
             tmem_store16(score + c0 / 2, pk);
-            if (c0 == 32 || c0 == 96) {  // the products of the first 64 keys need not wait for the others
-                tmem_store_wait();
-                tmem_fence_before();
-                __syncwarp();
-                if ((threadIdx.x & 31) == 0) bar_arrive(&sh->p_full[half][c0 / 64]);
-            }
         }
-        const Pair all = add2(sum[0], sum[1]);
-        l += all.x + all.y;
+    }
+    __device__ __forceinline__ float row_max(const float (&s)[kBlock]) {
+        float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int c = 4; c < kBlock - 4; c += 8)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) top[x] = max3(top[x], s[c + 2 * x], s[c + 2 * x + 1]);
+        top[0] = max3(top[0], s[kBlock - 4], s[kBlock - 3]);
+        top[1] = max3(top[1], s[kBlock - 2], s[kBlock - 1]);
+        return max3(max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
+    }
+    // the products of these 64 keys need not wait for the others
+    __device__ __forceinline__ void hand_over(int part) {
+        tmem_store_wait();
+        tmem_fence_before();
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) bar_arrive(&sh->p_full[half][part]);
     }
 
     // block u of the walk's tile, number n in the CTA; false: stalled
-    __device__ __forceinline__ bool block(const Walk& w, int u, int n, bool first, int p, const Span& mine) {
+    __device__ __forceinline__ bool block(const Walk& w, int u, int n, int p, const Span& mine) {
+        // the scores are there, and with them the products of the block before have reached O
         if (!bar_wait(&sh->s_full[half], done & 1, sh)) return false;
         tmem_fence_after();
         float s[kBlock];
 #pragma unroll
         for (int c = 0; c < kBlock; c += 32) tmem_load32(score + c, s + c);
         const bool lost = sh->missing[n & 3] == 1 + n;
-        const bool whole = !lost && mine.has(u);
+        const bool whole = !lost && mine.has(u), checked = !w.all.has(u);
         bool poison = false;
         tmem_load_wait();
         if (!whole) {
@@ -569,47 +583,45 @@ struct Softmax {
                     if (!((see >> c) & 1u)) s[c0 + c] = -INFINITY;
             }
         }
-        if (!w.all.has(u)) {  // the V tile was looked through
+        if (checked) {  // the V tile was looked through
             const int f = 2 * n + 1;
             if (!bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh)) return false;
             poison = sh->nonfinite[f % kSlots] == 1 + f;
         }
-        float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-        for (int c = 4; c < kBlock - 4; c += 8)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) top[x] = max3(top[x], s[c + 2 * x], s[c + 2 * x + 1]);
-        top[0] = max3(top[0], s[kBlock - 4], s[kBlock - 3]);
-        top[1] = max3(top[1], s[kBlock - 2], s[kBlock - 1]);
-        const float mx = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
-        if (first) {
-            m = mx;
-            l = 0.f;
-        } else if (__any_sync(0xFFFFFFFFu, !(mx <= m + kRaise))) {  // also where mx is NaN: so becomes the row
-            // raise the base: wait for the products that write O, scale it
-            if (!bar_wait(&sh->pv_done[half], (done - 1) & 1, sh)) return false;
-            tmem_fence_after();
+        const float mx = row_max(s);
+        if (__any_sync(0xFFFFFFFFu, !(mx <= m + kRaise))) {  // also where mx is NaN: so becomes the row
             const float mn = max3(m, mx, mx);
-            const float f = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
-            m = mn;
-            l *= f;
+            if (u != w.u0) {  // the segment's first products write O, all others add to it
+                const float f = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+                l *= f;
 #pragma unroll 1
-            for (int d = 0; d < kDim; d += 16) {
-                float o[16];
-                tmem_load16(output + d, o);
-                tmem_load_wait();
+                for (int d = 0; d < kDim; d += 16) {
+                    float o[16];
+                    tmem_load16(output + d, o);
+                    tmem_load_wait();
 #pragma unroll
-                for (int x = 0; x < 16; ++x) o[x] *= f;
-                tmem_store16(output + d, reinterpret_cast<const uint32_t*>(o));
+                    for (int x = 0; x < 16; ++x) o[x] *= f;
+                    tmem_store16(output + d, reinterpret_cast<const uint32_t*>(o));
+                }
             }
+            m = mn;
         }
         // a row without a visible key yet has no base; one with a score of +inf is NaN, as inf - inf
         const float base = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m;
-        if (whole && !__any_sync(0xFFFFFFFFu, m == -INFINITY)) weights<true>(s, base);
-        else weights<false>(s, base);
+        const bool mixed = whole && __all_sync(0xFFFFFFFFu, m != -INFINITY);
+        Pair sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+        if (mixed) weights<true, 0>(s, base, sum);
+        else weights<false, 0>(s, base, sum);
+        hand_over(0);
+        if (mixed) weights<true, 64>(s, base, sum);
+        else weights<false, 64>(s, base, sum);
+        hand_over(1);
+        const Pair both = add2(sum[0], sum[1]);
+        l += both.x + both.y;
         ++done;
+        if (checked || u + 1 == w.u1) ++settled;
         if (poison) {
-            if (!bar_wait(&sh->pv_done[half], (done - 1) & 1, sh)) return false;
+            if (!bar_wait(&sh->pv_done[half], (settled - 1) & 1, sh)) return false;
             tmem_fence_after();
             add_nonfinite(w, u, n, p);
             tmem_store_wait();
@@ -650,7 +662,7 @@ struct Softmax {
 
     // The segment's end: this thread's row of O to the output or, for part of a tile, to the workspace.
     __device__ __forceinline__ bool store(const Walk& w, bool ok) {
-        if (ok) ok = bar_wait(&sh->pv_done[half], (done - 1) & 1, sh);
+        if (ok) ok = bar_wait(&sh->pv_done[half], (settled - 1) & 1, sh);
         tmem_fence_after();
         int i = 0, g = 0;
         const bool valid = Tiles<kRows, false>::row(a, w.req, w.tile, row, &i, &g);
@@ -710,7 +722,6 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
         for (int i = 0; i < kSlots; ++i) {
             bar_init(&sh->full[i], 4);  // the four helper warps, or four times the loader
             bar_init(&sh->raw[i], 1);
-            bar_init(&sh->empty[i], 1);
             sh->nonfinite[i] = 0;
         }
         bar_init(&sh->q_full, 4);
@@ -722,7 +733,10 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
             bar_init(&sh->pv_done[i], 1);
         }
         bar_init(&sh->drain, 1);
-        for (int i = 0; i < 4; ++i) sh->missing[i] = 0;
+        for (int i = 0; i < 4; ++i) {
+            bar_init(&sh->used[i], 1);
+            sh->missing[i] = 0;
+        }
         sh->stalled = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -747,7 +761,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     }
 
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         Softmax<T, kDim> sm(a, sh, tmem, box_shift);
         int n = 0;
         bool ok = true;
@@ -764,11 +778,13 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
             const int from = w.req.kv_len - w.req.rows + div_group(a, r0);
             const int to = w.req.kv_len - w.req.rows + min(w.req.rows - 1, div_group(a, r0 + kHalf - 1));
             const Span mine = w.seen(from, to);
-            for (int u = w.u0; ok && u < w.u1; ++u, ++n) ok = sm.block(w, u, n, u == w.u0, p, mine);
+            sm.m = -INFINITY;
+            sm.l = 0.f;
+            for (int u = w.u0; ok && u < w.u1; ++u, ++n) ok = sm.block(w, u, n, p, mine);
             ok = sm.store(w, ok);
         } while (w.next() && ok);
     } else if (warp < 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         Helper<T, kDim> hp(a, sh, q, ring);
         int n = 0, segment = 0;
         bool ok = true;
@@ -785,7 +801,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
             ++segment;
         } while (ok && w.next());
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 12) {
             // all lanes walk along, so that addresses stay in uniform registers; one issues
             const bool lead = elect_one();
@@ -826,7 +842,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                 }
             } at{0, 0};  // the next tile to be used
             const auto filled = [&](const Turn& t) { return bar_wait(&sh->full[t.slot], t.parity, sh); };
-            int segment = 0, done[2] = {0, 0};
+            int n = 0, segment = 0, done[2] = {0, 0};
             bool ok = true;
             do {
                 const int halves = w.rows > kHalf ? 2 : 1, blocks = w.u1 - w.u0;
@@ -834,11 +850,10 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                 if (!ok) break;
                 scores(0, at.slot);
                 if (halves == 2) scores(1, at.slot);
-                commit(&sh->empty[at.slot]);
                 if (blocks == 1) commit(&sh->q_empty);
                 at.advance();
-                for (int b = 0; b < blocks && ok; ++b) {
-                    const bool more = b + 1 < blocks;
+                for (int b = 0; b < blocks; ++b, ++n) {
+                    const bool more = b + 1 < blocks, tell = !more || !w.all.has(w.u0 + b);
                     const Turn v = at;
                     at.advance();
                     const Turn k = at;
@@ -853,7 +868,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                         if (!ok) return;
                         tmem_fence_after();
                         output(h, v.slot, 1, true);
-                        commit(&sh->pv_done[h]);
+                        if (tell) commit(&sh->pv_done[h]);
                         ++done[h];
                         if (!more) return;
                         if (h == 0) ok = filled(k);
@@ -862,11 +877,8 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                     turn(0);
                     if (halves == 2) turn(1);
                     if (!ok) break;
-                    commit(&sh->empty[v.slot]);
-                    if (more) {
-                        commit(&sh->empty[k.slot]);
-                        if (b + 2 == blocks) commit(&sh->q_empty);
-                    }
+                    commit(&sh->used[n & 3]);
+                    if (b + 2 == blocks) commit(&sh->q_empty);
                 }
                 ++segment;
             } while (ok && w.next());
@@ -877,6 +889,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
         } else if (warp == 13) {
             Loader<kDim> ld(a, sh, ring, box_shift);
             int n = 0;
+            uint32_t firsts = 0;  // bit i: block n - 1 - i was the first of its segment
             bool ok = true;
             do {
                 int limit, j0 = w.block(w.u0, &limit);
@@ -887,7 +900,8 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                         next_j0 = w.block(u + 1, &next_limit);
                         next_pg = ld.page(w, next_j0, next_limit);
                     }
-                    ok = ld.block(w, u, j0, limit, pg, n, &k_map, &v_map);
+                    ok = ld.block(w, u, j0, limit, pg, n, (firsts >> 1) & 1, &k_map, &v_map);
+                    firsts = firsts << 1 | (u == w.u0);
                     j0 = next_j0;
                     limit = next_limit;
                     pg = next_pg;
