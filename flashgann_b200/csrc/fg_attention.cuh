@@ -69,7 +69,7 @@ __device__ __forceinline__ Request load_request(const AttentionParams& a, int b)
 // that lie before the window, those of the window (from `base`, up to `hi`),
 // then the retrieved ones.
 struct TileKeys {
-    int lo, hi, base;            // window part: keys [lo, hi), chunks start at base = lo rounded down to 16
+    int lo, hi, base;            // window part: keys [lo, hi), chunks start at base = lo rounded down to base_align
     int sink_hi;                 // first-token part: keys [0, sink_hi)
     int sink_chunks, near_chunks, id_chunks, chunks;
     int units;
@@ -81,18 +81,29 @@ __device__ __forceinline__ int div_group(const AttentionParams& a, int n) {
     return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * a.group_mul) >> a.group_shift);
 }
 
-// Token range [i0, i1] of a tile and the row layout.  Without ids a tile is
-// kRows consecutive (token, head of the group) pairs of a request; with ids it
-// is one token and up to kRows heads of the group.
-template <int kRows, bool kIds>
+// The query rows of a tile of one kv head.
+//   kPacked  kRows consecutive (token, head of the group) pairs of a request
+//   kTokens  the group's heads of as many tokens as fit kRows rows
+//   kToken   one token, kRows heads of the group (what each head retrieved is its own)
+enum Layout { kPacked, kTokens, kToken };
+
+template <int kRows, Layout kLayout>
 struct Tiles {
-    __device__ static __forceinline__ int parts(const AttentionParams& a) { return (a.group + kRows - 1) / kRows; }
+    // tokens of a tile, or tiles of a token
+    __device__ static __forceinline__ int per(const AttentionParams& a) {
+        return kLayout == kTokens ? div_group(a, kRows) : (a.group + kRows - 1) / kRows;
+    }
     __device__ static __forceinline__ int count(const AttentionParams& a, const Request& r) {
-        return kIds ? r.rows * parts(a) : (r.rows * a.group + kRows - 1) / kRows;
+        if (kLayout == kToken) return r.rows * per(a);
+        if (kLayout == kTokens) return (r.rows + per(a) - 1) / per(a);
+        return (r.rows * a.group + kRows - 1) / kRows;
     }
     __device__ static __forceinline__ void tokens(const AttentionParams& a, const Request& r, int t, int* i0, int* i1) {
-        if (kIds) {
-            *i0 = *i1 = t / parts(a);
+        if (kLayout == kToken) {
+            *i0 = *i1 = t / per(a);
+        } else if (kLayout == kTokens) {
+            *i0 = t * per(a);
+            *i1 = min(r.rows, *i0 + per(a)) - 1;
         } else {
             *i0 = div_group(a, t * kRows);
             *i1 = min(r.rows - 1, div_group(a, t * kRows + kRows - 1));
@@ -100,36 +111,36 @@ struct Tiles {
     }
     // row -> (token of the request, head of the group); false past the tile's end
     __device__ static __forceinline__ bool row(const AttentionParams& a, const Request& r, int t, int row, int* i, int* g) {
-        if (kIds) {
-            const int hg = parts(a);
-            *i = t / hg;
-            *g = (t - *i * hg) * kRows + row;
+        if (kLayout == kToken) {
+            const int n = per(a);
+            *i = t / n;
+            *g = (t - *i * n) * kRows + row;
             return *g < a.group;
         }
-        const int R = t * kRows + row;
-        *i = div_group(a, R);
-        *g = R - *i * a.group;
-        return *i < r.rows;
+        const int R = kLayout == kTokens ? row : t * kRows + row;
+        const int x = div_group(a, R);
+        *g = R - x * a.group;
+        *i = kLayout == kTokens ? t * per(a) + x : x;
+        return *i < r.rows && (kLayout == kPacked || x < per(a));
     }
 };
 
-template <int kRows, bool kIds, int kChunk, int kUnitChunks>
+template <int kRows, Layout kLayout, int kChunk, int kUnitChunks>
 __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Request& r, int t) {
     TileKeys k;
     int i0, i1;
-    Tiles<kRows, kIds>::tokens(a, r, t, &i0, &i1);
+    Tiles<kRows, kLayout>::tokens(a, r, t, &i0, &i1);
     const int p0 = r.kv_len - r.rows + i0, p1 = r.kv_len - r.rows + i1;
     const int64_t room = static_cast<int64_t>(a.table_width) * a.page_size;  // keys that the table can address
     k.hi = p1 < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(p1) + 1, room));
     k.lo = (a.window < 0 || p0 < a.window) ? 0 : min(p0 - a.window + 1, k.hi);
-    k.base = k.lo & ~15;
+    k.base = k.lo & -a.base_align;
     k.sink_hi = min(a.sinks, k.base);
     k.sink_chunks = (k.sink_hi + kChunk - 1) / kChunk;
     k.near_chunks = (k.hi - k.base + kChunk - 1) / kChunk;
     k.id_chunks = 0;
-    if (kIds && k.lo > 0) {
-        const int hg = (a.group + kRows - 1) / kRows;
-        const int heads = min(kRows, a.group - (t % hg) * kRows);
+    if (kLayout == kToken && a.ids_count > 0 && k.lo > 0) {
+        const int heads = min(kRows, a.group - (t % Tiles<kRows, kLayout>::per(a)) * kRows);
         k.id_chunks = heads * ((a.ids_count + kChunk - 1) / kChunk);
     }
     k.chunks = k.sink_chunks + k.near_chunks + k.id_chunks;
@@ -148,7 +159,7 @@ struct Place {
 // Called by all kThreads threads; scratch holds requests + 64 ints.  kLanes
 // threads count the tiles of a request: 1 where requests are short, 8 where
 // they have many tiles.
-template <int kRows, bool kIds, int kChunk, int kUnitChunks, int kThreads, int kLanes>
+template <int kRows, Layout kLayout, int kChunk, int kUnitChunks, int kThreads, int kLanes>
 __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, int cta, int ctas) {
     int* pre = scratch + 64;  // inclusive prefix of the requests' units
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -159,8 +170,8 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
         int s = 0;
         if (b < a.requests) {
             const Request r = load_request(a, b);
-            const int n = Tiles<kRows, kIds>::count(a, r);
-            for (int t = tid % kLanes; t < n; t += kLanes) s += tile_keys<kRows, kIds, kChunk, kUnitChunks>(a, r, t).units;
+            const int n = Tiles<kRows, kLayout>::count(a, r);
+            for (int t = tid % kLanes; t < n; t += kLanes) s += tile_keys<kRows, kLayout, kChunk, kUnitChunks>(a, r, t).units;
         }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -201,11 +212,11 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
     if (lo > 0) rest -= pre[lo - 1];
     const Request r = load_request(a, lo);
     // the tile that holds unit `rest` of the request, 32 tiles at a time, in every warp
-    const int tiles = Tiles<kRows, kIds>::count(a, r);
+    const int tiles = Tiles<kRows, kLayout>::count(a, r);
     int t = 0;
     for (int t0 = 0; t0 < tiles; t0 += 32) {
         const int mine = t0 + lane;
-        const int u = mine < tiles ? tile_keys<kRows, kIds, kChunk, kUnitChunks>(a, r, mine).units : 0;
+        const int u = mine < tiles ? tile_keys<kRows, kLayout, kChunk, kUnitChunks>(a, r, mine).units : 0;
         int s = u;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -228,9 +239,9 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
 }
 
 // The next tile in the numbering after (head, request, tile); false after the last.
-template <int kRows, bool kIds>
+template <int kRows, Layout kLayout>
 __device__ __forceinline__ bool next_tile(const AttentionParams& a, Request* r, int* head, int* request, int* tile) {
-    if (++*tile < Tiles<kRows, kIds>::count(a, *r)) return true;
+    if (++*tile < Tiles<kRows, kLayout>::count(a, *r)) return true;
     *tile = 0;
     do {
         if (++*request == a.requests) {
@@ -278,7 +289,7 @@ struct Half2<__nv_bfloat16> {
 // if c is the first such CTA.  Bandwidth-bound and tiny: at most 2 partials
 // per main CTA; launched as a dependent of the main kernel so that its start
 // overlaps the main kernel's tail.
-template <typename T, int kRows, int kDim, bool kIds>
+template <typename T, int kRows, int kDim, Layout kLayout>
 __global__ void __launch_bounds__(128) attention_combine_kernel(const AttentionParams a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const char* ws = static_cast<const char*>(a.workspace);
@@ -300,7 +311,7 @@ __global__ void __launch_bounds__(128) attention_combine_kernel(const AttentionP
     const int per = (kRows + a.combine_split - 1) / a.combine_split;
     for (int row = part * per + warp; row < min(kRows, (part + 1) * per); row += 4) {
         int i, g;
-        if (!Tiles<kRows, kIds>::row(a, r, rec.tile, row, &i, &g)) continue;
+        if (!Tiles<kRows, kLayout>::row(a, r, rec.tile, row, &i, &g)) continue;
         float m = p0[kRows * kDim + row], l = p0[kRows * kDim + kRows + row];
         const int d = lane * 4;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);

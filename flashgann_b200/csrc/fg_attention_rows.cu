@@ -128,13 +128,13 @@ struct Warp {
         table = a.block_table + request * a.table_stride;
         head_off = head * a.head_stride;
         int i0, i1;
-        Tiles<kRows, kIds>::tokens(a, req, tile, &i0, &i1);
+        Tiles<kRows, kIds ? kToken : kPacked>::tokens(a, req, tile, &i0, &i1);
         p0 = req.kv_len - req.rows + i0;
         p1 = req.kv_len - req.rows + i1;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             int i, g;
-            const bool ok = Tiles<kRows, kIds>::row(a, req, tile, (lane >> 2) + 8 * x, &i, &g);
+            const bool ok = Tiles<kRows, kIds ? kToken : kPacked>::row(a, req, tile, (lane >> 2) + 8 * x, &i, &g);
             prow[x] = ok ? req.kv_len - req.rows + i : -1;
             const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(req.start + i) * a.q_token_stride +
                            static_cast<int64_t>(head * a.group + g) * a.q_head_stride + (lane & 3) * 2;
@@ -146,7 +146,7 @@ struct Warp {
         }
         if (kIds) {
             int i, g;
-            Tiles<kRows, kIds>::row(a, req, tile, 0, &i, &g);
+            Tiles<kRows, kIds ? kToken : kPacked>::row(a, req, tile, 0, &i, &g);
             ids = a.ids + static_cast<int64_t>(req.start + i) * a.ids_token_stride +
                   static_cast<int64_t>(head * a.group + g) * a.ids_head_stride;
         }
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     char* ws = static_cast<char*>(a.workspace);
 
-    const Place pl = locate<kRows, kIds, kChunk, kWarps, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kWarps, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
     __syncthreads();  // the rings overlay the scan
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
     if (pl.unit >= pl.end) return;
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
     int head = pl.head, request = pl.request, tile = pl.tile;
     int64_t unit = pl.unit, tile_first = pl.unit - pl.offset;
     w.req = load_request(a, request);
-    w.keys = tile_keys<kRows, kIds, kChunk, kWarps>(a, w.req, tile);
+    w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk, kWarps>(a, w.req, tile);
     if (threadIdx.x == 0) {
         TileRecord rec;
         rec.first = tile_first;
@@ -464,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
             }
             if (whole_tile) {
                 int i, g;
-                if (Tiles<kRows, kIds>::row(a, w.req, tile, row, &i, &g)) {
+                if (Tiles<kRows, kIds ? kToken : kPacked>::row(a, w.req, tile, row, &i, &g)) {
                     const float inv = ll == 0.f ? 1.f : 1.f / ll;
                     const int64_t token = w.req.start + i;
                     const int h = head * a.group + g;
@@ -484,8 +484,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
         unit = tile_first + u1;
         if (unit >= pl.end) break;
         tile_first = tile_last;
-        if (!next_tile<kRows, kIds>(a, &w.req, &head, &request, &tile)) break;
-        w.keys = tile_keys<kRows, kIds, kChunk, kWarps>(a, w.req, tile);
+        if (!next_tile<kRows, kIds ? kToken : kPacked>(a, &w.req, &head, &request, &tile)) break;
+        w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk, kWarps>(a, w.req, tile);
         first_segment = false;
         __syncthreads();  // the join's reads end before the next tile's copies
     }
@@ -494,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
 template <typename T, int kDim, bool kIds>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = Smem<kDim>::kBytes;
+    a.base_align = kChunk;
     cudaError_t e = cudaFuncSetAttribute(attention_rows_kernel<T, kDim, kIds>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
     attention_rows_kernel<T, kDim, kIds><<<a.ctas, kThreads, bytes, stream>>>(a);
@@ -508,7 +509,7 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_combine_kernel<T, kRows, kDim, kIds>, a);
+    return cudaLaunchKernelEx(&cfg, attention_combine_kernel<T, kRows, kDim, kIds ? kToken : kPacked>, a);
 }
 
 template <typename T, int kDim>

@@ -137,6 +137,7 @@ struct AttentionParams {
     int64_t ids_token_stride = 0, ids_head_stride = 0;
     void* workspace = nullptr;
     int ctas = 0;           // CTAs that share the work
+    int base_align = 16;    // power of two that windows' key chunks start at multiples of
     int combine_split = 1;  // CTAs that join one tile's partials
 };
 int attention_max_requests();
