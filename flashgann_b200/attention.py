@@ -13,14 +13,30 @@ tensors, run in libflashgann.so (include/flashgann.h has the exact rules) on
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _capi
-from ._capi import FG_ERR_ARG, FG_OK, AttentionArgs, FlashGANNError, KVCacheArgs, lib
+from ._capi import FG_ERR_ARG, FG_OK, FlashGANNError, lib
 
 _DTYPES = {torch.float16: _capi.FG_DTYPE_F16, torch.bfloat16: _capi.FG_DTYPE_BF16}
+
+# A decode step makes these calls once for each layer, so the calls themselves are kept short: the two argument structs
+# are packed into bytes (a ctypes.Structure takes several times as long to fill), their layout is _capi's.
+_CACHE = struct.Struct("@PPqqqiiiii4x")
+_ARGS = struct.Struct("@PqqPqqPPqPPPqqPQiiiiiiiif4x")
+assert _CACHE.size == ctypes.sizeof(_capi.KVCacheArgs) and _ARGS.size == ctypes.sizeof(_capi.AttentionArgs)
+_calls = {}
+
+
+def _call(name: str, *argtypes):
+    """The library's entry point `name`, taking packed structs as bytes."""
+    f = _calls.get(name)
+    if f is None:
+        f = _calls[name] = ctypes.CFUNCTYPE(ctypes.c_int, *argtypes)((name, lib()))
+    return f
 
 
 class KVPlan(NamedTuple):
@@ -47,25 +63,21 @@ class _On:
     inside belong to that stream; inputs that live on another one are marked
     as in use there, so that the caller may drop them right after the call."""
 
-    __slots__ = ("device", "handle", "guard")
+    __slots__ = ("index", "handle", "guard")
 
     def __init__(self, like: torch.Tensor, stream):
         if not like.is_cuda:
             _fail("expected a CUDA tensor")
-        index = like.device.index
-        current = torch.cuda.current_stream(index)
+        self.index = index = like.get_device()
         self.guard = None
-        if stream is None or getattr(stream, "cuda_stream", stream) == current.cuda_stream:
-            self.handle = current.cuda_stream
-            if torch.cuda.current_device() != index:
-                self.guard = torch.cuda.device(index)
-        else:
-            handle = getattr(stream, "cuda_stream", stream) or 0
+        self.handle = torch._C._cuda_getCurrentRawStream(index)
+        if stream is not None and getattr(stream, "cuda_stream", stream) != self.handle:
+            self.handle = handle = getattr(stream, "cuda_stream", stream) or 0
             s = stream if isinstance(stream, torch.cuda.Stream) else (
                 torch.cuda.ExternalStream(handle, device=index) if handle else torch.cuda.default_stream(index))
-            self.handle = handle
             self.guard = torch.cuda.stream(s)
-        self.device = like.device
+        elif torch.cuda.current_device() != index:
+            self.guard = torch.cuda.device(index)
 
     def __enter__(self):
         if self.guard is not None:
@@ -77,43 +89,45 @@ class _On:
             self.guard.__exit__(*exc)
 
     def uses(self, *tensors):
+        index = self.index
         for t in tensors:
             if t is None:
                 continue
-            if t.device != self.device:
-                _fail(f"a tensor is on {t.device}, not on {self.device}")
+            if t.get_device() != index:
+                _fail(f"a tensor is on {t.device}, not on device {index}")
             if self.guard is not None:
-                t.record_stream(torch.cuda.current_stream(self.device))
+                t.record_stream(torch.cuda.current_stream(index))
 
 
 def _ints(t: torch.Tensor, dims: int, name: str, dtype=torch.int32) -> torch.Tensor:
     if t.dtype != dtype or t.dim() != dims:
         _fail(f"{name} must be {dtype} with {dims} dimension(s), not {t.dtype} {tuple(t.shape)}")
-    return t if dims == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     """[tokens, heads, dim] with a contiguous last axis and 16-byte aligned rows (a copy where it is not)."""
     if t.dim() != 3:
         _fail(f"{name} must be [tokens, heads, dim], not {tuple(t.shape)}")
-    s = t.stride()
-    if (s[2] != 1 and t.shape[2] > 1) or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and t.shape[2] > 1) or (s0 | s1) % 8 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> KVCacheArgs:
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
-        _fail(f"caches must be [pages, page_size, heads, dim] alike, not {tuple(k_cache.shape)} and "
-              f"{tuple(v_cache.shape)}")
-    if k_cache.dtype not in _DTYPES or v_cache.dtype != k_cache.dtype:
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor):
+    """(fg_kv_cache as bytes, kv heads, dim)"""
+    shape, s = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape:
+        _fail(f"caches must be [pages, page_size, heads, dim] alike, not {tuple(shape)} and {tuple(v_cache.shape)}")
+    dtype = _DTYPES.get(k_cache.dtype)
+    if dtype is None or v_cache.dtype != k_cache.dtype:
         _fail(f"caches must both be float16 or bfloat16, not {k_cache.dtype} and {v_cache.dtype}")
-    s = k_cache.stride()
     if s != v_cache.stride() or s[3] != 1:
         _fail(f"caches must have the same strides and a contiguous last axis, not {s} and {v_cache.stride()}")
-    pages, page_size, heads, dim = k_cache.shape
-    return KVCacheArgs(k_cache.data_ptr(), v_cache.data_ptr(), s[0], s[1], s[2], pages, page_size, heads, dim,
-                       _DTYPES[k_cache.dtype])
+    pages, page_size, heads, dim = shape
+    return _CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), s[0], s[1], s[2], pages, page_size, heads, dim,
+                       dtype), heads, dim
 
 
 def kv_plan(ctx_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor, *,
@@ -137,11 +151,11 @@ def kv_plan(ctx_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Ten
             _fail(f"block_table must be int32 [{R}, width] with contiguous rows")
         if free_head is not None and (free_head.dtype != torch.int32 or free_head.numel() != 1):
             _fail("free_head must be int32 [1]")
-        heads = torch.empty(3 * R + 2 + max(tokens, 0), dtype=torch.int32, device=on.device)
-        slot = torch.empty(max(tokens, 0), dtype=torch.int64, device=on.device)
-        plan = KVPlan(heads[:R + 1], heads[R + 1:2 * R + 1], heads[3 * R + 2:], slot, heads[2 * R + 1:2 * R + 2],
-                      heads[2 * R + 2:3 * R + 2])
-        base = heads.data_ptr()
+        T = max(tokens, 0)
+        slot = torch.empty(T, dtype=torch.int64, device=ctx_len.device)
+        ints = torch.empty(3 * R + 2 + T, dtype=torch.int32, device=ctx_len.device)
+        base = ints.data_ptr()
+        query_start, kv_len, head, refused, position = ints.split_with_sizes((R + 1, R, 1, R, T))
         rc = lib().fg_kv_plan_device(ctx_len.data_ptr(), new_len.data_ptr(), R, free_pages.data_ptr(),
                                      free_pages.shape[0], None if free_head is None else free_head.data_ptr(),
                                      page_size, block_table.data_ptr(), block_table.shape[1], block_table.stride(0),
@@ -149,7 +163,7 @@ def kv_plan(ctx_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Ten
                                      base + 4 * (2 * R + 1), base + 4 * (2 * R + 2), on.handle)
         if rc != FG_OK:
             _raise(rc, "fg_kv_plan_device")
-        return plan
+        return KVPlan(query_start, kv_len, position, slot, head, refused)
 
 
 def kv_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, *,
@@ -159,27 +173,33 @@ def kv_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: 
     (fg_kv_append_device)."""
     with _On(k_cache, stream) as on:
         on.uses(k_cache, v_cache, k, v, slot)
-        c = _cache(k_cache, v_cache)
-        want = (slot.shape[0], c.heads, c.dim)
+        c, heads, dim = _cache(k_cache, v_cache)
+        want = (slot.shape[0], heads, dim)
         if k.shape != want or v.shape != want or k.dtype != k_cache.dtype or v.dtype != k_cache.dtype:
             _fail(f"k and v must be {k_cache.dtype} {want}, not {k.dtype} {tuple(k.shape)} and {v.dtype} "
                   f"{tuple(v.shape)}")
         slot, k, v = _ints(slot, 1, "slot", torch.int64), _rows(k, "k"), _rows(v, "v")
-        rc = lib().fg_kv_append_device(c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                       v.stride(1), slot.data_ptr(), want[0], on.handle)
+        k0, k1, _ = k.stride()
+        v0, v1, _ = v.stride()
+        i64, ptr = ctypes.c_int64, ctypes.c_void_p
+        rc = _call("fg_kv_append_device", ctypes.c_char_p, ptr, i64, i64, ptr, i64, i64, ptr, ctypes.c_int32, ptr)(
+            c, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, slot.data_ptr(), want[0], on.handle)
         if rc != FG_OK:
             _raise(rc, "fg_kv_append_device")
+
+
+_workspace = {}  # bytes that a call needs: by device, entry point, head size and whether requests have many rows
 
 
 def _attend(call: str, q, k_cache, v_cache, block_table, query_start, kv_len, max_new, ids, window, sinks, scale, out,
             return_lse, stream):
     with _On(q, stream) as on:
         on.uses(q, k_cache, v_cache, block_table, query_start, kv_len, out, ids)
-        c = _cache(k_cache, v_cache)
+        c, kv_heads, cache_dim = _cache(k_cache, v_cache)
         q = _rows(q, "q")
         T, heads, dim = q.shape
-        if q.dtype != k_cache.dtype or dim != c.dim:
-            _fail(f"q must be {k_cache.dtype} [tokens, heads, {c.dim}], not {q.dtype} {tuple(q.shape)}")
+        if q.dtype != k_cache.dtype or dim != cache_dim:
+            _fail(f"q must be {k_cache.dtype} [tokens, heads, {cache_dim}], not {q.dtype} {tuple(q.shape)}")
         block_table = _ints(block_table, 2, "block_table")
         query_start, kv_len = _ints(query_start, 1, "query_start"), _ints(kv_len, 1, "kv_len")
         R = kv_len.shape[0]
@@ -187,29 +207,36 @@ def _attend(call: str, q, k_cache, v_cache, block_table, query_start, kv_len, ma
             _fail(f"{R} lengths need {R + 1} query_start entries and {R} table rows, not {query_start.shape[0]} and "
                   f"{block_table.shape[0]}")
         if out is None:
-            out = torch.empty((T, heads, dim), dtype=q.dtype, device=on.device)
+            out = torch.empty((T, heads, dim), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
             _fail(f"out must be {q.dtype} {tuple(q.shape)} with a contiguous last axis")
-        lse = torch.empty((T, heads), dtype=torch.float32, device=on.device) if return_lse else None
-        a = AttentionArgs(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-                          lse.data_ptr() if return_lse else None, block_table.data_ptr(), block_table.stride(0),
-                          query_start.data_ptr(), kv_len.data_ptr(), None, 0, 0, None, 0, T, heads, R,
-                          block_table.shape[1], max_new, -1 if window is None else window, sinks, 0,
-                          dim ** -0.5 if scale is None else scale)
+        lse = torch.empty((T, heads), dtype=torch.float32, device=q.device) if return_lse else None
+        id_ptr = id_token = id_head = count = 0
         if ids is not None:
             if ids.dtype != torch.int32 or ids.dim() != 3 or ids.shape[:2] != q.shape[:2]:
                 _fail(f"ids must be int32 [{T}, {heads}, count], not {ids.dtype} {tuple(ids.shape)}")
             if ids.stride(2) != 1 and ids.shape[2] > 1:
                 ids = ids.contiguous()
-            a.ids, a.ids_token_stride, a.ids_head_stride = ids.data_ptr(), ids.stride(0), ids.stride(1)
-            a.ids_count = ids.shape[2]
-        L = lib()
-        need = ctypes.c_uint64()
-        rc = L.fg_attention_workspace_bytes(c, a, need)
-        if rc == FG_OK:
-            work = torch.empty(need.value, dtype=torch.uint8, device=on.device)
-            a.workspace, a.workspace_bytes = work.data_ptr(), need.value
-            rc = getattr(L, call)(c, a, on.handle)
+            id_ptr, count = ids.data_ptr(), ids.shape[2]
+            id_token, id_head, _ = ids.stride()
+        q0, q1, _ = q.stride()
+        o0, o1, _ = out.stride()
+        args = [q.data_ptr(), q0, q1, out.data_ptr(), o0, o1, lse.data_ptr() if return_lse else 0,
+                block_table.data_ptr(), block_table.stride(0), query_start.data_ptr(), kv_len.data_ptr(), id_ptr,
+                id_token, id_head, 0, 0, T, heads, R, block_table.shape[1], max_new, -1 if window is None else window,
+                sinks, count, dim ** -0.5 if scale is None else scale]
+        key = (on.index, call, dim, max_new * heads > 16 * kv_heads)
+        need = _workspace.get(key)
+        if need is None:
+            size = ctypes.c_uint64()
+            rc = _call("fg_attention_workspace_bytes", ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p)(
+                c, _ARGS.pack(*args), ctypes.addressof(size))
+            if rc != FG_OK:
+                _raise(rc, call)
+            need = _workspace[key] = size.value
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        args[14], args[15] = work.data_ptr(), need
+        rc = _call(call, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p)(c, _ARGS.pack(*args), on.handle)
         if rc != FG_OK:
             _raise(rc, call)
         return (out, lse) if return_lse else out

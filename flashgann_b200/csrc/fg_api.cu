@@ -855,9 +855,11 @@ int sm_count(int* sms) {
 // would read the keys once for each 16 rows, and the tiles kernel takes them
 // 256 at a time.  That one folds the scale into its maxima, so it needs a
 // positive one, and its copies are whole groups of 8 rows of a page.
+bool many_rows(const fg_kv_cache* c, const fg_attention* x) {
+    return static_cast<int64_t>(x->max_new) * (x->heads / c->heads) > 16;
+}
 bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
-    return !retrieved && x->scale > 0.f && c->page_size >= 8 &&
-           static_cast<int64_t>(x->max_new) * (x->heads / c->heads) > 16;
+    return !retrieved && many_rows(c, x) && x->scale > 0.f && c->page_size >= 8;
 }
 
 int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void* stream) {
@@ -1025,8 +1027,8 @@ int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* a
     if ((rc = sm_count(&sms))) return rc;
     if (args->heads < 1 || args->heads % cache->heads)
         return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", args->heads, cache->heads);
-    *bytes = takes_tiles(cache, args, args->ids != nullptr) ? fg::attention_tiles_workspace(sms, cache->dim)
-                                                            : fg::attention_rows_workspace(sms, cache->dim);
+    // by the number of rows alone: what else decides between the kernels must not change the answer for like calls
+    *bytes = many_rows(cache, args) ? fg::attention_tiles_workspace(sms, cache->dim) : fg::attention_rows_workspace(sms, cache->dim);
     return FG_OK;
 }
 

@@ -495,7 +495,8 @@ template <typename T, int kDim, bool kIds>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = Smem<kDim>::kBytes;
     a.base_align = kChunk;
-    cudaError_t e = cudaFuncSetAttribute(attention_rows_kernel<T, kDim, kIds>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static SmemOnce once;
+    cudaError_t e = once.set(reinterpret_cast<const void*>(attention_rows_kernel<T, kDim, kIds>), bytes);
     if (e != cudaSuccess) return e;
     attention_rows_kernel<T, kDim, kIds><<<a.ctas, kThreads, bytes, stream>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;

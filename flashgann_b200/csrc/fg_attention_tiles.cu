@@ -931,7 +931,8 @@ bool encode(CUtensorMap* map, const AttentionParams& a, const void* data, const 
 template <typename T, int kDim>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = Smem<kDim>::kBytes;
-    cudaError_t e = cudaFuncSetAttribute(attention_tiles_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static SmemOnce once;
+    cudaError_t e = once.set(reinterpret_cast<const void*>(attention_tiles_kernel<T, kDim>), bytes);
     if (e != cudaSuccess) return e;
     // A box is as much of a page as a block takes, so that the copies are few; with a window 64 rows at most, because
     // blocks then start at multiples of it and begin with that many keys less one that no row sees.  (16 rows always:
