@@ -14,7 +14,7 @@
 //
 // Work split.  Tiles (kv head, request, row tile) differ in length by orders
 // of magnitude (one short decode beside a chunk over a long context), so the
-// unit of work is not the tile but `kUnitChunks` chunks of keys of one tile.
+// unit of work is not the tile but 2^unit_shift chunks of keys of one tile.
 // All units are numbered in tile order and CTA c of P takes the contiguous
 // range [c*W/P, (c+1)*W/P) of the W units: every CTA gets the same amount of
 // key traffic to within one unit whatever the lengths, and at most its first
@@ -126,7 +126,7 @@ struct Tiles {
     }
 };
 
-template <int kRows, Layout kLayout, int kChunk, int kUnitChunks>
+template <int kRows, Layout kLayout, int kChunk>
 __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Request& r, int t) {
     TileKeys k;
     int i0, i1;
@@ -145,7 +145,7 @@ __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Re
         k.id_chunks = heads * ((a.ids_count + kChunk - 1) / kChunk);
     }
     k.chunks = k.sink_chunks + k.near_chunks + k.id_chunks;
-    k.units = max(1, (k.chunks + kUnitChunks - 1) / kUnitChunks);  // a tile that sees nothing still writes its rows
+    k.units = max(1, (k.chunks + (1 << a.unit_shift) - 1) >> a.unit_shift);  // a tile that sees nothing still writes its rows
     return k;
 }
 
@@ -160,7 +160,7 @@ struct Place {
 // Called by all kThreads threads; scratch holds requests + 64 ints.  kLanes
 // threads count the tiles of a request: 1 where requests are short, 8 where
 // they have many tiles.
-template <int kRows, Layout kLayout, int kChunk, int kUnitChunks, int kThreads, int kLanes>
+template <int kRows, Layout kLayout, int kChunk, int kThreads, int kLanes>
 __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, int cta, int ctas) {
     int* pre = scratch + 64;  // inclusive prefix of the requests' units
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -172,7 +172,7 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
         if (b < a.requests) {
             const Request r = load_request(a, b);
             const int n = Tiles<kRows, kLayout>::count(a, r);
-            for (int t = tid % kLanes; t < n; t += kLanes) s += tile_keys<kRows, kLayout, kChunk, kUnitChunks>(a, r, t).units;
+            for (int t = tid % kLanes; t < n; t += kLanes) s += tile_keys<kRows, kLayout, kChunk>(a, r, t).units;
         }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -217,7 +217,7 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
     int t = 0;
     for (int t0 = 0; t0 < tiles; t0 += 32) {
         const int mine = t0 + lane;
-        const int u = mine < tiles ? tile_keys<kRows, kLayout, kChunk, kUnitChunks>(a, r, mine).units : 0;
+        const int u = mine < tiles ? tile_keys<kRows, kLayout, kChunk>(a, r, mine).units : 0;
         int s = u;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {

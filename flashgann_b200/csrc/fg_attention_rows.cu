@@ -11,7 +11,8 @@
 // Layout.  One CTA of 8 warps per SM.  A chunk is 16 keys; warp w of a CTA
 // takes chunks w, w+8, ... of the CTA's range and is on its own until the tile
 // ends: it looks the keys' pages up, copies their K and V rows to its own ring
-// of shared memory with 16-byte cp.async (kStages - 1 chunks ahead), and keeps
+// of shared memory with 16-byte cp.async (kStages - 1 chunks ahead, the pages
+// one more), and keeps
 // its own running maximum, sum and 16 x dim output in registers, so no barrier
 // sits between a load and its use.  Gathering by row costs nothing extra over
 // a tile copy here, and makes pages of any size, any strides, windows that
@@ -20,7 +21,15 @@
 //
 // Retrieved ids are chunks like the others: 16 ids of one head, whose scores
 // count in that head's row alone.  The other rows' share of the product is
-// waste on a pipe that idles anyway.
+// waste on a pipe that idles anyway.  At a tile's start the warps read the
+// heads' lists once, drop the ids that do not count (out of range, in the window,
+// repeated) and leave the rest in shared memory, see stage_ids.
+//
+// Tiles that are short whatever the lengths are (a narrow table, or a window and
+// a few ids: up to kShort chunks, a bound that the host knows) are not split:
+// there are no partials and no second kernel, which costs more than it saves.
+#include <algorithm>
+
 #include "fg_attention.cuh"
 
 namespace fg {
@@ -31,6 +40,9 @@ constexpr int kRows = 16;
 constexpr int kChunk = 16;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
+constexpr int kShort = 64;       // chunks of a tile that is not split
+constexpr int kMaxIds = 4096;    // ids of a tile's heads that are kept in shared memory
+constexpr int kMarkWords = 64;   // 2048 marks for each head, see stage_ids
 
 template <int kDim>
 struct Smem {
@@ -39,7 +51,9 @@ struct Smem {
     static constexpr int kStages = 3;
     static constexpr int kRing = kStages * 2 * kTile;  // K and V of each stage
     static constexpr int kWarpBytes = kRing;
-    static constexpr int kBytes = kWarps * kWarpBytes;
+    static constexpr int kIdsAt = kWarps * kWarpBytes;  // retrieved form: the tile's ids and their marks
+    static constexpr int kBytes = kIdsAt;
+    static constexpr int kBytesIds = kIdsAt + kMaxIds * 4 + kRows * kMarkWords * 4;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -82,15 +96,21 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], const uint32_t
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The element offset of key j's row in the cache (either half), or -1 where
-// the table has no page for it.
-__device__ __forceinline__ int64_t key_offset(const AttentionParams& a, const int32_t* table, int j, int64_t head_off) {
-    const int page = j >> a.page_shift;
-    if (page >= a.table_width) return -1;
-    const int id = __ldg(table + page);
-    if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(a.pages)) return -1;
-    return id * a.page_stride + (j & (a.page_size - 1)) * a.token_stride + head_off;
+// The element offset of key j's row in the cache (either half) given its page, or -1 where there is no such page.
+__device__ __forceinline__ int64_t key_offset(const AttentionParams& a, int page, int j, int64_t head_off) {
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) return -1;
+    return page * a.page_stride + (j & (a.page_size - 1)) * a.token_stride + head_off;
 }
+__device__ __forceinline__ int key_page(const AttentionParams& a, const int32_t* table, int j) {
+    const int at = j >> a.page_shift;
+    return at < a.table_width ? __ldg(table + at) : -1;
+}
+
+// A chunk whose keys' pages are being looked up; one key to a lane (lanes 16-31 repeat them).
+struct Found {
+    int key, row;  // as in Chunk
+    int j, page;   // this lane's key and, when it arrives, its page
+};
 
 // One chunk in flight.
 struct Chunk {
@@ -116,6 +136,7 @@ struct Warp {
     int p0, p1;        // positions of the tile's first and last row
     int prow[2];       // positions of this lane's two rows (-1: no row)
     const int32_t* ids;  // retrieved ids of the tile's first row
+    const int* staged;   // those of all its rows that count, in shared memory; null: too many
     // running state
     uint32_t q[kDim / 16][4];
     float o[kDim / 8][4];
@@ -156,44 +177,98 @@ struct Warp {
         l[0] = l[1] = 0.f;
     }
 
-    // Looks chunk c's keys up and starts its copies into stage s.
-    __device__ __forceinline__ Chunk load(int c, int s) {
-        Chunk ch;
-        ch.row = -1;
-        ch.key = 0;
+    // Starts looking chunk c's keys up.
+    __device__ __forceinline__ Found find(int c) const {
+        Found f;
+        f.row = -1;
+        f.key = 0;
+        f.j = f.page = -1;
         const int x = lane & 15;
-        int64_t off = -1;
         if (c < keys.sink_chunks) {
-            ch.key = c * kChunk;
-            if (ch.key + x < keys.sink_hi) off = key_offset(a, table, ch.key + x, head_off);
+            f.key = c * kChunk;
+            if (f.key + x < keys.sink_hi) f.j = f.key + x;
         } else if (c < keys.sink_chunks + keys.near_chunks) {
-            ch.key = keys.base + (c - keys.sink_chunks) * kChunk;
-            const int j = ch.key + x;
-            if (j < keys.hi && (j >= keys.lo || j < a.sinks)) off = key_offset(a, table, j, head_off);
+            f.key = keys.base + (c - keys.sink_chunks) * kChunk;
+            const int j = f.key + x;
+            if (j < keys.hi && (j >= keys.lo || j < a.sinks)) f.j = j;
         } else if (kIds) {
             const int per = (a.ids_count + kChunk - 1) / kChunk;
             const int at = c - keys.sink_chunks - keys.near_chunks;
-            ch.row = at / per;
-            const int n = (at % per) * kChunk + x;
-            const int32_t* list = ids + ch.row * a.ids_head_stride;
-            const int id = n < a.ids_count ? __ldg(list + n) : -1;
-            // visible by the mask already (window, first tokens), beyond the row's position, or an empty place
-            bool fresh = id >= a.sinks && id <= p0 && p0 - id >= a.window && id >= 0;
-            // an id that stands earlier in the list counts there
-            const int stop = (at % per) * kChunk + kChunk;
-            for (int e0 = 0; e0 < stop; e0 += 32) {
-                const int e = e0 + lane;
-                const int other = e < a.ids_count ? __ldg(list + e) : -1;
+            f.row = at / per;
+            f.j = listed(f.row, (at - f.row * per) * kChunk);
+        }
+        if (f.j >= 0) f.page = key_page(a, table, f.j);
+        return f;
+    }
+
+    // Whether a retrieved id counts, repeats aside: in range, and not visible by the mask already.
+    __device__ __forceinline__ bool counts(int id) const { return id >= a.sinks && id <= p0 && p0 - id >= a.window; }
+
+    // Ids first .. first + 15 of a head's list, one to a lane; -1 for those that do not count.
+    __device__ __forceinline__ int listed(int row, int first) const {
+        const int n = first + (lane & 15);
+        if (staged) return n < a.ids_count ? staged[row * a.ids_count + n] : -1;
+        const int32_t* list = ids + row * a.ids_head_stride;
+        const int id = n < a.ids_count ? __ldg(list + n) : -1;
+        bool fresh = counts(id);
+        // an id that stands earlier in the list counts there
+        for (int e0 = 0; e0 < first + kChunk; e0 += 32) {
+            const int e = e0 + lane;
+            const int other = e < a.ids_count ? __ldg(list + e) : -1;
 #pragma unroll
-                for (int y = 0; y < kChunk; ++y) {
-                    const int idy = __shfl_sync(0xFFFFFFFFu, id, y);
-                    const int ny = (at % per) * kChunk + y;
-                    const bool hit = __any_sync(0xFFFFFFFFu, other == idy && e < ny);
-                    if (x == y && hit) fresh = false;
+            for (int y = 0; y < kChunk; ++y) {
+                const int idy = __shfl_sync(0xFFFFFFFFu, id, y);
+                const bool hit = __any_sync(0xFFFFFFFFu, other == idy && e < first + y);
+                if ((lane & 15) == y && hit) fresh = false;
+            }
+        }
+        return fresh ? id : -1;
+    }
+
+    // Reads the lists of the tile's heads into shared memory, a head to a warp,
+    // with -1 in the place of ids that do not count.  Repeats: every id sets one
+    // of 2048 marks by its hash; only one that finds its mark set is compared
+    // with the list so far.  Of equal ids the first stays.
+    __device__ __forceinline__ void stage_ids(int* list, uint32_t* marks, int heads) const {
+        for (int h = threadIdx.x >> 5; h < heads; h += kWarps) {
+            uint32_t* mark = marks + h * kMarkWords;
+            int* mine = list + h * a.ids_count;
+            const int32_t* from = ids + h * a.ids_head_stride;
+            mark[lane] = mark[lane + 32] = 0;
+            __syncwarp();
+            for (int n0 = 0; n0 < a.ids_count; n0 += 32) {
+                const int n = n0 + lane;
+                int id = n < a.ids_count ? __ldg(from + n) : -1;
+                if (!counts(id)) id = -1;
+                bool met = false;
+                if (id >= 0) {
+                    const uint32_t hash = (static_cast<uint32_t>(id) * 2654435761u) >> 21, bit = 1u << (hash & 31);
+                    met = atomicOr(mark + (hash >> 5), bit) & bit;
+                }
+                if (n < a.ids_count) mine[n] = id;
+                __syncwarp();
+                for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, met); todo; todo &= todo - 1) {
+                    const int same = __shfl_sync(0xFFFFFFFFu, id, __ffs(todo) - 1);
+                    int first = -1;
+                    for (int e0 = 0; first < 0 && e0 <= n0; e0 += 32) {
+                        const bool eq = e0 + lane < a.ids_count && mine[e0 + lane] == same;
+                        const uint32_t at = __ballot_sync(0xFFFFFFFFu, eq);
+                        if (at) first = e0 + __ffs(at) - 1;
+                    }
+                    __syncwarp();
+                    if (id == same && n != first && n < a.ids_count) mine[n] = -1;
+                    __syncwarp();
                 }
             }
-            if (fresh) off = key_offset(a, table, id, head_off);
         }
+    }
+
+    // Starts the copies of a chunk into stage s.
+    __device__ __forceinline__ Chunk load(const Found& f, int s) const {
+        Chunk ch;
+        ch.key = f.key;
+        ch.row = f.row;
+        const int64_t off = f.j >= 0 ? key_offset(a, f.page, f.j, head_off) : -1;
         ch.ok = __ballot_sync(0xFFFFFFFFu, off >= 0) & 0xFFFFu;
         const uint32_t dst = ring + s * 2 * S::kTile;
         const T* kc = static_cast<const T*>(a.k_cache);
@@ -267,7 +342,7 @@ struct Warp {
                 const int per = (a.ids_count + kChunk - 1) / kChunk;
                 j = __ldg(ids + ch.row * a.ids_head_stride + (id_chunk % per) * kChunk + col);
             }
-            const T* src = vc + key_offset(a, table, j, head_off) + (lane & 3) * 2;
+            const T* src = vc + key_offset(a, key_page(a, table, j), j, head_off) + (lane & 3) * 2;
 #pragma unroll
             for (int n = 0; n < kDim / 8; ++n) {
                 const uint32_t w = *reinterpret_cast<const uint32_t*>(src + n * 8);
@@ -360,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     char* ws = static_cast<char*>(a.workspace);
 
-    const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kWarps, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
     __syncthreads();  // the rings overlay the scan
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
     if (pl.unit >= pl.end) return;
@@ -369,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
     int head = pl.head, request = pl.request, tile = pl.tile;
     int64_t unit = pl.unit, tile_first = pl.unit - pl.offset;
     w.req = load_request(a, request);
-    w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk, kWarps>(a, w.req, tile);
+    w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk>(a, w.req, tile);
     if (threadIdx.x == 0) {
         TileRecord rec;
         rec.first = tile_first;
@@ -385,15 +460,35 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
         const int64_t tile_last = tile_first + w.keys.units;
         const int u0 = static_cast<int>(unit - tile_first);
         const int u1 = static_cast<int>(min(tile_last, pl.end) - tile_first);
-        const int c1 = min(u1 * kWarps, w.keys.chunks);
+        const int c1 = min(u1 << a.unit_shift, w.keys.chunks);
         w.begin(head, request, tile);
-        // the chunks in flight: a shift register of kStages - 1 descriptors
+        int c = (u0 << a.unit_shift) + warp;
+        const int window_end = w.keys.sink_chunks + w.keys.near_chunks;  // chunks from here on need the tile's ids
+        // the chunks in flight: a shift register of kStages - 1 descriptors, and one chunk whose pages are looked up
         Chunk flight[S::kStages - 1];
-        int c = u0 * kWarps + warp;
+        Found next_up;
+        bool ids_ready = !kIds;
 #pragma unroll
-        for (int s = 0; s < S::kStages - 1; ++s) {
-            if (c + s * kWarps < c1) flight[s] = w.load(c + s * kWarps, s);
-            copy_commit();
+        for (int s = 0; s < S::kStages; ++s) {
+            const int cs = c + s * kWarps;
+            if (kIds && !ids_ready && (s == S::kStages - 1 || (u0 << a.unit_shift) + s * kWarps + kWarps > window_end)) {
+                // first when a warp may need one, so that the copies of the window are under way meanwhile
+                w.staged = nullptr;
+                const int heads = min(kRows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * kRows);
+                if (w.keys.id_chunks > 0 && heads * a.ids_count <= kMaxIds) {
+                    int* list = reinterpret_cast<int*>(smem + S::kIdsAt);
+                    w.stage_ids(list, reinterpret_cast<uint32_t*>(list + kMaxIds), heads);
+                    w.staged = list;
+                }
+                __syncthreads();
+                ids_ready = true;
+            }
+            if (s < S::kStages - 1) {
+                if (cs < c1) flight[s] = w.load(w.find(cs), s);
+                copy_commit();
+            } else if (cs < c1) {
+                next_up = w.find(cs);
+            }
         }
         int stage = 0;
         for (; c < c1; c += kWarps) {
@@ -405,9 +500,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
             const int ahead = c + (S::kStages - 1) * kWarps;
             int next = stage + S::kStages - 1;
             if (next >= S::kStages) next -= S::kStages;
-            if (ahead < c1) flight[S::kStages - 2] = w.load(ahead, next);
+            if (ahead < c1) {
+                flight[S::kStages - 2] = w.load(next_up, next);
+                if (ahead + kWarps < c1) next_up = w.find(ahead + kWarps);
+            }
             copy_commit();
-            w.id_chunk = c - w.keys.sink_chunks - w.keys.near_chunks;
+            w.id_chunk = c - window_end;
             w.compute(now, stage);
             if (++stage == S::kStages) stage = 0;
             __syncwarp();
@@ -485,24 +583,36 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
         if (unit >= pl.end) break;
         tile_first = tile_last;
         if (!next_tile<kRows, kIds ? kToken : kPacked>(a, &w.req, &head, &request, &tile)) break;
-        w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk, kWarps>(a, w.req, tile);
+        w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk>(a, w.req, tile);
         first_segment = false;
         __syncthreads();  // the join's reads end before the next tile's copies
     }
 }
 
+// Chunks that no tile has more of, as far as the host can tell.
+int64_t most_chunks(const AttentionParams& a) {
+    int64_t keys = static_cast<int64_t>(a.table_width) * a.page_size;
+    if (a.window >= 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + kRows + a.sinks);
+    int64_t chunks = keys / kChunk + 3;
+    if (a.ids) chunks += static_cast<int64_t>(std::min(a.group, kRows)) * ((a.ids_count + kChunk - 1) / kChunk);
+    return chunks;
+}
+
 template <typename T, int kDim, bool kIds>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
-    constexpr int bytes = Smem<kDim>::kBytes;
+    constexpr int bytes = kIds ? Smem<kDim>::kBytesIds : Smem<kDim>::kBytes;
+    static_assert(bytes <= 227 * 1024, "one CTA's shared memory");
     a.base_align = kChunk;
+    const bool split = most_chunks(a) > kShort;
+    a.unit_shift = split ? 3 : 24;  // a unit: one chunk for each warp, or a tile
     static SmemOnce once;
     cudaError_t e = once.set(reinterpret_cast<const void*>(attention_rows_kernel<T, kDim, kIds>), bytes);
     if (e != cudaSuccess) return e;
     attention_rows_kernel<T, kDim, kIds><<<a.ctas, kThreads, bytes, stream>>>(a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if ((e = cudaGetLastError()) != cudaSuccess || !split) return e;
     a.combine_split = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(max(1, a.ctas - 1)));
+    cfg.gridDim = dim3(static_cast<unsigned>(std::max(1, a.ctas - 1)));
     cfg.blockDim = dim3(128);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

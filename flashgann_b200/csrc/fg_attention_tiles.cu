@@ -239,7 +239,7 @@ struct Walk {
         set();
     }
     __device__ __forceinline__ void set() {
-        keys = tile_keys<kRows, kTokens, kBlock, 1>(a, req, tile);
+        keys = tile_keys<kRows, kTokens, kBlock>(a, req, tile);
         int i0, i1;
         Tiles<kRows, kTokens>::tokens(a, req, tile, &i0, &i1);
         p0 = req.kv_len - req.rows + i0;
@@ -687,7 +687,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     char* ws = static_cast<char*>(a.workspace);
 
-    const Place pl = locate<kRows, kTokens, kBlock, 1, kThreads, 8>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, kTokens, kBlock, kThreads, 8>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
     if (pl.unit >= pl.end) return;
     if (threadIdx.x == 0) {
@@ -939,6 +939,7 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     // 2048 tokens on 8192 20 % slower with pages of 64.)
     const int box_shift = min(a.page_shift, a.window < 0 ? 7 : 6);
     a.base_align = 1 << box_shift;
+    a.unit_shift = 0;
     const int64_t cache_size[3] = {a.page_size, a.kv_heads, a.pages}, cache_stride[3] = {a.token_stride, a.head_stride, a.page_stride};
     const int64_t q_size[3] = {a.heads, a.tokens, 1}, q_stride[3] = {a.q_head_stride, a.q_token_stride, 0};
     CUtensorMap q_map, k_map, v_map;

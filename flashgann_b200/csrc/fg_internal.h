@@ -138,6 +138,7 @@ struct AttentionParams {
     void* workspace = nullptr;
     int ctas = 0;           // CTAs that share the work
     int base_align = 16;    // power of two that windows' key chunks start at multiples of
+    int unit_shift = 0;     // log2 of the key chunks in a unit of work
     int combine_split = 1;  // CTAs that join one tile's partials
 };
 int attention_max_requests();
