@@ -882,7 +882,8 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
         if (x->window < 0) return fail(FG_ERR_ARG, "retrieved attention needs a window >= 0");
         if (x->ids_count < 0 || x->ids_token_stride < 0 || x->ids_head_stride < 0)
             return fail(FG_ERR_ARG, "bad ids: count %d, or a negative stride", x->ids_count);
-        if (x->ids_count > 65536) return fail(FG_ERR_UNSUPPORTED, "%d ids for each row, at most 65536", x->ids_count);
+        if (x->ids_count > fg::attention_max_ids())
+            return fail(FG_ERR_UNSUPPORTED, "%d ids for each row, at most %d", x->ids_count, fg::attention_max_ids());
     }
     if (x->tokens == 0 || x->requests == 0) return FG_OK;
     if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, "q"))) return rc;

@@ -85,14 +85,14 @@ __device__ __forceinline__ int div_group(const AttentionParams& a, int n) {
 // The query rows of a tile of one kv head.
 //   kPacked  kRows consecutive (token, head of the group) pairs of a request
 //   kTokens  the group's heads of as many tokens as fit kRows rows
-//   kToken   one token, kRows heads of the group (what each head retrieved is its own)
+//   kToken   one token, tile_rows heads of the group (what each head retrieved is its own)
 enum Layout { kPacked, kTokens, kToken };
 
 template <int kRows, Layout kLayout>
 struct Tiles {
     // tokens of a tile, or tiles of a token
     __device__ static __forceinline__ int per(const AttentionParams& a) {
-        return kLayout == kTokens ? div_group(a, kRows) : (a.group + kRows - 1) / kRows;
+        return kLayout == kTokens ? div_group(a, kRows) : (a.group + a.tile_rows - 1) / a.tile_rows;
     }
     __device__ static __forceinline__ int count(const AttentionParams& a, const Request& r) {
         if (kLayout == kToken) return r.rows * per(a);
@@ -115,8 +115,8 @@ struct Tiles {
         if (kLayout == kToken) {
             const int n = per(a);
             *i = t / n;
-            *g = (t - *i * n) * kRows + row;
-            return *g < a.group;
+            *g = (t - *i * n) * a.tile_rows + row;
+            return row < a.tile_rows && *g < a.group;
         }
         const int R = kLayout == kTokens ? row : t * kRows + row;
         const int x = div_group(a, R);
@@ -141,7 +141,7 @@ __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Re
     k.near_chunks = (k.hi - k.base + kChunk - 1) / kChunk;
     k.id_chunks = 0;
     if (kLayout == kToken && a.ids_count > 0 && k.lo > 0) {
-        const int heads = min(kRows, a.group - (t % Tiles<kRows, kLayout>::per(a)) * kRows);
+        const int heads = min(a.tile_rows, a.group - (t % Tiles<kRows, kLayout>::per(a)) * a.tile_rows);
         k.id_chunks = heads * ((a.ids_count + kChunk - 1) / kChunk);
     }
     k.chunks = k.sink_chunks + k.near_chunks + k.id_chunks;
@@ -311,40 +311,50 @@ __global__ void __launch_bounds__(128) attention_combine_kernel(const AttentionP
     const char* ws = static_cast<const char*>(a.workspace);
     const int64_t total = *reinterpret_cast<const int64_t*>(ws);
     const int ctas = static_cast<int>(min(static_cast<int64_t>(a.ctas), total));
-    const int c = blockIdx.x / a.combine_split + 1, part = blockIdx.x % a.combine_split;
+    constexpr int kBlocks = kRows / 4;  // 4 rows to a block
+    const int c = blockIdx.x / kBlocks + 1, part = blockIdx.x % kBlocks;
     if (c >= ctas) return;
     const TileRecord rec = reinterpret_cast<const TileRecord*>(ws + kHeaderBytes)[c];
     const int64_t begin = total * c / ctas, before = total * (c - 1) / ctas;
     if (begin == rec.first || before > rec.first) return;
     const float* partials = reinterpret_cast<const float*>(ws + workspace_records_bytes(a.ctas));
     const size_t psize = partial_floats(kRows, kDim);
-    const float* p0 = partials + (2 * static_cast<size_t>(c - 1) + (before == rec.first ? 0 : 1)) * psize;
-    int last = c;
-    while (last + 1 < ctas && total * (last + 1) / ctas < rec.last) ++last;
+    const int last = static_cast<int>((rec.last * ctas - 1) / total);  // the CTA whose range holds the tile's last unit
+    const int parts = last - c + 2;  // CTAs c - 1 .. last
+    const auto partial = [&](int x) {  // the first CTA's is its second segment unless its range starts with this tile
+        return partials + (x == 0 ? 2 * static_cast<size_t>(c - 1) + (before == rec.first ? 0 : 1) : 2 * static_cast<size_t>(c - 1 + x)) * psize;
+    };
     const Request r = load_request(a, rec.request);
-    // each warp joins whole rows: lane owns 4-float pieces of the row
+    // a warp joins a row: the maximum first, a partial to a lane, then the sums with several loads under way, a lane's 4
+    // columns each
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per = (kRows + a.combine_split - 1) / a.combine_split;
-    for (int row = part * per + warp; row < min(kRows, (part + 1) * per); row += 4) {
-        int i, g;
-        if (!Tiles<kRows, kLayout>::row(a, r, rec.tile, row, &i, &g)) continue;
-        float m = p0[kRows * kDim + row], l = p0[kRows * kDim + kRows + row];
+    const int row = part * 4 + warp;
+    int i, g;
+    if (Tiles<kRows, kLayout>::row(a, r, rec.tile, row, &i, &g)) {
+        float m = -INFINITY;
+        bool nan = false;  // left by a main kernel that gave up
+        for (int x = lane; x < parts; x += 32) {
+            const float v = partial(x)[kRows * kDim + row];
+            m = fmaxf(m, v);
+            nan = nan || v != v;
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+        const float ref = __any_sync(0xFFFFFFFFu, nan) ? NAN : m == -INFINITY ? 0.f : m;
         const int d = lane * 4;
+        float l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (d < kDim) o = *reinterpret_cast<const float4*>(p0 + row * kDim + d);
-        for (int x = c; x <= last; ++x) {
-            const float* p = partials + 2 * static_cast<size_t>(x) * psize;
-            const float m2 = p[kRows * kDim + row], l2 = p[kRows * kDim + kRows + row];
-            const float mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
-            const float s1 = exp2_fast(m - ref), s2 = exp2_fast(m2 - ref);
-            l = l * s1 + l2 * s2;
-            m = mn;
+#pragma unroll 8
+        for (int x = 0; x < parts; ++x) {
+            const float* p = partial(x);
+            const float f = exp2_fast(p[kRows * kDim + row] - ref);
+            l += p[kRows * kDim + kRows + row] * f;
             if (d < kDim) {
                 const float4 q = *reinterpret_cast<const float4*>(p + row * kDim + d);
-                o.x = o.x * s1 + q.x * s2;
-                o.y = o.y * s1 + q.y * s2;
-                o.z = o.z * s1 + q.z * s2;
-                o.w = o.w * s1 + q.w * s2;
+                o.x += q.x * f;
+                o.y += q.y * f;
+                o.z += q.z * f;
+                o.w += q.w * f;
             }
         }
         const float inv = l == 0.f ? 1.f : 1.f / l;
@@ -357,6 +367,22 @@ __global__ void __launch_bounds__(128) attention_combine_kernel(const AttentionP
         }
         if (lane == 0 && a.lse) a.lse[token * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
     }
+}
+
+// After a main kernel that may have left partials; the main kernel lets it start early.
+template <typename T, int kRows, int kDim, Layout kLayout>
+cudaError_t launch_combine(const AttentionParams& a, cudaStream_t stream) {
+    if (a.ctas < 2) return cudaSuccess;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((a.ctas - 1) * (kRows / 4)));
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_combine_kernel<T, kRows, kDim, kLayout>, a);
 }
 
 }  // namespace attn

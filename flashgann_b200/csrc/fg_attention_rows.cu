@@ -8,15 +8,16 @@
 // bytes: the kernel is bound by bandwidth, and everything serves keeping loads
 // in flight.
 //
-// Layout.  One CTA of 8 warps per SM.  A chunk is 16 keys; warp w of a CTA
-// takes chunks w, w+8, ... of the CTA's range and is on its own until the tile
+// Layout.  Two CTAs of 4 warps per SM, so that one's start, list of ids and join
+// pass beside the other's loads.  A chunk is 16 keys; warp w of a CTA takes
+// chunks w, w+4, ... of the CTA's range and is on its own until the tile
 // ends: it looks the keys' pages up, copies their K and V rows to its own ring
 // of shared memory with 16-byte cp.async (kStages - 1 chunks ahead, the pages
 // one more), and keeps
 // its own running maximum, sum and 16 x dim output in registers, so no barrier
 // sits between a load and its use.  Gathering by row costs nothing extra over
 // a tile copy here, and makes pages of any size, any strides, windows that
-// start inside a page and retrieved ids the same code.  At a tile's end the 8
+// start inside a page and retrieved ids the same code.  At a tile's end the
 // warps join through shared memory.
 //
 // Retrieved ids are chunks like the others: 16 ids of one head, whose scores
@@ -38,22 +39,29 @@ namespace {
 
 constexpr int kRows = 16;
 constexpr int kChunk = 16;
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
+constexpr int kCtasPerSm = 2;
 constexpr int kThreads = kWarps * 32;
 constexpr int kShort = 64;       // chunks of a tile that is not split
-constexpr int kMaxIds = 4096;    // ids of a tile's heads that are kept in shared memory
-constexpr int kMarkWords = 64;   // 2048 marks for each head, see stage_ids
+constexpr int kMaxIds = 2048;    // ids of a tile's heads, in shared memory
+constexpr int kTable = 4096;     // places of the hash table over them
 
 template <int kDim>
 struct Smem {
-    static constexpr int kPitch = kDim * 2 + 16;  // odd multiple of 16 bytes: ldmatrix reads 8 rows without conflicts
+    // ldmatrix reads 8 rows without bank conflicts: rows of 128 or 256 bytes with their 16-byte pieces exchanged by the
+    // row's number, rows of 192 bytes padded to an odd multiple of 16
+    static constexpr bool kExchange = kDim % 64 == 0;
+    static constexpr int kPitch = kExchange ? kDim * 2 : kDim * 2 + 16;
+    __device__ static __forceinline__ uint32_t at(int row, int piece) {
+        return row * kPitch + (kExchange ? piece ^ (row & 7) : piece) * 16;
+    }
     static constexpr int kTile = kChunk * kPitch;
     static constexpr int kStages = 3;
     static constexpr int kRing = kStages * 2 * kTile;  // K and V of each stage
     static constexpr int kWarpBytes = kRing;
-    static constexpr int kIdsAt = kWarps * kWarpBytes;  // retrieved form: the tile's ids and their marks
+    static constexpr int kIdsAt = kWarps * kWarpBytes;  // retrieved form: the tile's ids and the table
     static constexpr int kBytes = kIdsAt;
-    static constexpr int kBytesIds = kIdsAt + kMaxIds * 4 + kRows * kMarkWords * 4;
+    static constexpr int kBytesIds = kIdsAt + kMaxIds * 4 + kTable * 2;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -136,7 +144,7 @@ struct Warp {
     int p0, p1;        // positions of the tile's first and last row
     int prow[2];       // positions of this lane's two rows (-1: no row)
     const int32_t* ids;  // retrieved ids of the tile's first row
-    const int* staged;   // those of all its rows that count, in shared memory; null: too many
+    const int* staged;   // those of all its rows that count, in shared memory
     // running state
     uint32_t q[kDim / 16][4];
     float o[kDim / 8][4];
@@ -195,7 +203,8 @@ struct Warp {
             const int per = (a.ids_count + kChunk - 1) / kChunk;
             const int at = c - keys.sink_chunks - keys.near_chunks;
             f.row = at / per;
-            f.j = listed(f.row, (at - f.row * per) * kChunk);
+            const int n = (at - f.row * per) * kChunk + x;
+            if (n < a.ids_count) f.j = staged[f.row * staged_pitch(a.ids_count) + n];
         }
         if (f.j >= 0) f.page = key_page(a, table, f.j);
         return f;
@@ -204,63 +213,59 @@ struct Warp {
     // Whether a retrieved id counts, repeats aside: in range, and not visible by the mask already.
     __device__ __forceinline__ bool counts(int id) const { return id >= a.sinks && id <= p0 && p0 - id >= a.window; }
 
-    // Ids first .. first + 15 of a head's list, one to a lane; -1 for those that do not count.
-    __device__ __forceinline__ int listed(int row, int first) const {
-        const int n = first + (lane & 15);
-        if (staged) return n < a.ids_count ? staged[row * a.ids_count + n] : -1;
-        const int32_t* list = ids + row * a.ids_head_stride;
-        const int id = n < a.ids_count ? __ldg(list + n) : -1;
-        bool fresh = counts(id);
-        // an id that stands earlier in the list counts there
-        for (int e0 = 0; e0 < first + kChunk; e0 += 32) {
-            const int e = e0 + lane;
-            const int other = e < a.ids_count ? __ldg(list + e) : -1;
-#pragma unroll
-            for (int y = 0; y < kChunk; ++y) {
-                const int idy = __shfl_sync(0xFFFFFFFFu, id, y);
-                const bool hit = __any_sync(0xFFFFFFFFu, other == idy && e < first + y);
-                if ((lane & 15) == y && hit) fresh = false;
-            }
-        }
-        return fresh ? id : -1;
-    }
+    // Places of a list in shared memory: whole groups of 128.
+    __host__ __device__ static __forceinline__ int staged_pitch(int count) { return (count + 127) & ~127; }
 
-    // Reads the lists of the tile's heads into shared memory, a head to a warp,
-    // with -1 in the place of ids that do not count.  Repeats: every id sets one
-    // of 2048 marks by its hash; only one that finds its mark set is compared
-    // with the list so far.  Of equal ids the first stays.
-    __device__ __forceinline__ void stage_ids(int* list, uint32_t* marks, int heads) const {
-        for (int h = threadIdx.x >> 5; h < heads; h += kWarps) {
-            uint32_t* mark = marks + h * kMarkWords;
-            int* mine = list + h * a.ids_count;
-            const int32_t* from = ids + h * a.ids_head_stride;
-            mark[lane] = mark[lane + 32] = 0;
-            __syncwarp();
-            for (int n0 = 0; n0 < a.ids_count; n0 += 32) {
-                const int n = n0 + lane;
-                int id = n < a.ids_count ? __ldg(from + n) : -1;
-                if (!counts(id)) id = -1;
-                bool met = false;
-                if (id >= 0) {
-                    const uint32_t hash = (static_cast<uint32_t>(id) * 2654435761u) >> 21, bit = 1u << (hash & 31);
-                    met = atomicOr(mark + (hash >> 5), bit) & bit;
+    // Reads the lists of the tile's heads into shared memory, with -1 in the
+    // place of ids that do not count.  Of equal ids in a list the first stays: a
+    // hash table (open addressing, half full at most) holds for each id of each
+    // head the least of its places in the lists; an id whose place is another's
+    // goes.  The result does not depend on the order of the atomics.  Called by
+    // the whole CTA.
+    __device__ __forceinline__ void stage_ids(int* list, unsigned short* table, int heads) const {
+        constexpr unsigned short kFree = 0xFFFF;
+        const int pitch = staged_pitch(a.ids_count), all = heads * pitch;
+        for (int x = threadIdx.x; x < kTable / 2; x += kThreads) reinterpret_cast<uint32_t*>(table)[x] = 0xFFFFFFFFu;
+        for (int x0 = threadIdx.x; x0 < all; x0 += kThreads * 4) {
+            int id[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int x = x0 + y * kThreads, h = x / pitch, n = x - h * pitch;
+                id[y] = x < all && n < a.ids_count ? __ldg(ids + h * a.ids_head_stride + n) : -1;
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                if (x0 + y * kThreads < all) list[x0 + y * kThreads] = counts(id[y]) ? id[y] : -1;
+        }
+        __syncthreads();
+        const auto first_place = [&](int id, int h) {
+            return ((static_cast<uint32_t>(id) + static_cast<uint32_t>(h) * 0x9E3779B9u) * 2654435761u) >> 20;  // of 4096
+        };
+        const auto same = [&](int x, int id, int h) { return list[x] == id && x / pitch == h; };
+        for (int x = threadIdx.x; x < all; x += kThreads) {
+            const int id = list[x], h = x / pitch;
+            if (id < 0) continue;
+            for (uint32_t at = first_place(id, h);; at = (at + 1) % kTable) {
+                unsigned short old = atomicCAS(table + at, kFree, static_cast<unsigned short>(x));
+                if (old == kFree) break;
+                if (!same(old, id, h)) continue;  // another id's place
+                while (old > x) {
+                    const unsigned short was = atomicCAS(table + at, old, static_cast<unsigned short>(x));
+                    if (was == old) break;
+                    old = was;  // lowered by another thread with the same id
                 }
-                if (n < a.ids_count) mine[n] = id;
-                __syncwarp();
-                for (uint32_t todo = __ballot_sync(0xFFFFFFFFu, met); todo; todo &= todo - 1) {
-                    const int same = __shfl_sync(0xFFFFFFFFu, id, __ffs(todo) - 1);
-                    int first = -1;
-                    for (int e0 = 0; first < 0 && e0 <= n0; e0 += 32) {
-                        const bool eq = e0 + lane < a.ids_count && mine[e0 + lane] == same;
-                        const uint32_t at = __ballot_sync(0xFFFFFFFFu, eq);
-                        if (at) first = e0 + __ffs(at) - 1;
-                    }
-                    __syncwarp();
-                    if (id == same && n != first && n < a.ids_count) mine[n] = -1;
-                    __syncwarp();
-                }
+                break;
             }
         }
+        __syncthreads();
+        for (int x = threadIdx.x; x < all; x += kThreads) {
+            const int id = list[x], h = x / pitch;
+            if (id < 0) continue;
+            uint32_t at = first_place(id, h);
+            while (!same(table[at], id, h)) at = (at + 1) % kTable;
+            if (table[at] != x) list[x] = -1;  // no place that the table holds
+        }
+        __syncthreads();
     }
 
     // Starts the copies of a chunk into stage s.
@@ -279,7 +284,7 @@ struct Warp {
             const int64_t ro = __shfl_sync(0xFFFFFFFFu, off, r);
             const bool ok = ro >= 0;
             const int64_t from = ok ? ro + p * 8 : 0;
-            const uint32_t to = dst + r * S::kPitch + p * 16;
+            const uint32_t to = dst + S::at(r, p);
             copy16(to, kc + from, ok);
             copy16(to + S::kTile, vc + from, ok);
         }
@@ -302,7 +307,7 @@ struct Warp {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             const int idx = i * 32 + lane, r = idx / kPieces, p = idx % kPieces;
-            const uint32_t at = dst + r * S::kPitch + p * 16;
+            const uint32_t at = dst + S::at(r, p);
             uint32_t w[4];
             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                          : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
@@ -366,11 +371,11 @@ struct Warp {
 #pragma unroll
         for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
         // keys (lane & 7) + 8 * (lane >= 16), k offset 8 * ((lane >> 3) & 1)
-        const uint32_t kaddr = kt + ((lane & 7) + ((lane >> 4) << 3)) * S::kPitch + ((lane >> 3) & 1) * 16;
+        const int krow = (lane & 7) + ((lane >> 4) << 3), kpiece = (lane >> 3) & 1;
 #pragma unroll
         for (int k = 0; k < kDim / 16; ++k) {
             uint32_t b[4];
-            ldmatrix4(kaddr + k * 32, b);
+            ldmatrix4(kt + S::at(krow, 2 * k + kpiece), b);
             mma<T>(sc[0], q[k], b[0], b[1]);
             mma<T>(sc[1], q[k], b[2], b[3]);
         }
@@ -416,11 +421,11 @@ struct Warp {
             pa[x + 2] = Half2<T>::pack(e2, e3);
         }
         // keys (lane & 15), dims 8 * (lane >= 16)
-        const uint32_t vaddr = vt + (lane & 15) * S::kPitch + (lane >> 4) * 16;
+        const int vrow = lane & 15, vpiece = lane >> 4;
 #pragma unroll
         for (int n = 0; n < kDim / 16; ++n) {
             uint32_t b[4];
-            ldmatrix4_trans(vaddr + n * 32, b);
+            ldmatrix4_trans(vt + S::at(vrow, 2 * n + vpiece), b);
             mma<T>(o[2 * n], pa, b[0], b[1]);
             mma<T>(o[2 * n + 1], pa, b[2], b[3]);
         }
@@ -429,12 +434,13 @@ struct Warp {
 };
 
 template <typename T, int kDim, bool kIds>
-__global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const AttentionParams a) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(const AttentionParams a) {
     using S = Smem<kDim>;
     extern __shared__ __align__(128) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     char* ws = static_cast<char*>(a.workspace);
 
+    asm volatile("griddepcontrol.launch_dependents;");
     const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
     __syncthreads();  // the rings overlay the scan
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
@@ -473,14 +479,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
             const int cs = c + s * kWarps;
             if (kIds && !ids_ready && (s == S::kStages - 1 || (u0 << a.unit_shift) + s * kWarps + kWarps > window_end)) {
                 // first when a warp may need one, so that the copies of the window are under way meanwhile
-                w.staged = nullptr;
-                const int heads = min(kRows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * kRows);
-                if (w.keys.id_chunks > 0 && heads * a.ids_count <= kMaxIds) {
+                if (w.keys.id_chunks > 0) {
                     int* list = reinterpret_cast<int*>(smem + S::kIdsAt);
-                    w.stage_ids(list, reinterpret_cast<uint32_t*>(list + kMaxIds), heads);
+                    const int heads = min(a.tile_rows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * a.tile_rows);
+                    w.stage_ids(list, reinterpret_cast<unsigned short*>(list + kMaxIds), heads);
                     w.staged = list;
                 }
-                __syncthreads();
                 ids_ready = true;
             }
             if (s < S::kStages - 1) {
@@ -512,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_rows_kernel(const Atten
         }
         copy_wait<0>();
 
-        // join the 8 warps: rows of (m, l) and sums, over the rings
+        // join the warps: rows of (m, l) and sums, over the rings
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             w.l[x] += __shfl_xor_sync(0xFFFFFFFFu, w.l[x], 1);
@@ -601,26 +605,18 @@ int64_t most_chunks(const AttentionParams& a) {
 template <typename T, int kDim, bool kIds>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = kIds ? Smem<kDim>::kBytesIds : Smem<kDim>::kBytes;
-    static_assert(bytes <= 227 * 1024, "one CTA's shared memory");
+    static_assert((bytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
     a.base_align = kChunk;
+    if (kIds) a.tile_rows = std::min(kRows, kMaxIds / Warp<T, kDim, kIds>::staged_pitch(a.ids_count));
     const bool split = most_chunks(a) > kShort;
-    a.unit_shift = split ? 3 : 24;  // a unit: one chunk for each warp, or a tile
+    a.ctas *= kCtasPerSm;
+    a.unit_shift = split ? 2 : 24;  // a unit: one chunk for each warp, or a tile
     static SmemOnce once;
     cudaError_t e = once.set(reinterpret_cast<const void*>(attention_rows_kernel<T, kDim, kIds>), bytes);
     if (e != cudaSuccess) return e;
     attention_rows_kernel<T, kDim, kIds><<<a.ctas, kThreads, bytes, stream>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess || !split) return e;
-    a.combine_split = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::max(1, a.ctas - 1)));
-    cfg.blockDim = dim3(128);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_combine_kernel<T, kRows, kDim, kIds ? kToken : kPacked>, a);
+    return launch_combine<T, kRows, kDim, kIds ? kToken : kPacked>(a, stream);
 }
 
 template <typename T, int kDim>
@@ -639,10 +635,12 @@ cudaError_t by_dim(const AttentionParams& a, cudaStream_t s) {
 }  // namespace
 }  // namespace attn
 
-size_t attention_rows_workspace(int ctas, int dim) {
+size_t attention_rows_workspace(int sms, int dim) {
+    const int ctas = sms * attn::kCtasPerSm;
     return attn::workspace_records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * attn::partial_floats(attn::kRows, dim) * sizeof(float);
 }
 int attention_max_requests() { return 16384; }
+int attention_max_ids() { return attn::kMaxIds; }
 
 cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream) {
     return a.dtype == FG_DTYPE_BF16 ? attn::by_dim<__nv_bfloat16>(a, stream) : attn::by_dim<__half>(a, stream);

@@ -687,6 +687,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     char* ws = static_cast<char*>(a.workspace);
 
+    asm volatile("griddepcontrol.launch_dependents;");
     const Place pl = locate<kRows, kTokens, kBlock, kThreads, 8>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
     if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
     if (pl.unit >= pl.end) return;
@@ -949,17 +950,7 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
         return cudaErrorInvalidValue;
     attention_tiles_kernel<T, kDim><<<a.ctas, kThreads, bytes, stream>>>(a, q_map, k_map, v_map, box_shift);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    a.combine_split = 8;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(max(1, (a.ctas - 1) * a.combine_split)));
-    cfg.blockDim = dim3(128);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_combine_kernel<T, kRows, kDim, kTokens>, a);
+    return launch_combine<T, kRows, kDim, kTokens>(a, stream);
 }
 
 template <typename T>
@@ -974,7 +965,8 @@ cudaError_t by_dim(const AttentionParams& a, cudaStream_t s) {
 }  // namespace
 }  // namespace attn
 
-size_t attention_tiles_workspace(int ctas, int dim) {
+size_t attention_tiles_workspace(int sms, int dim) {
+    const int ctas = sms;
     return attn::workspace_records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * attn::partial_floats(attn::kRows, dim) * sizeof(float);
 }
 

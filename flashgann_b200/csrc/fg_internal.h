@@ -136,15 +136,16 @@ struct AttentionParams {
     int ids_count = 0;
     int64_t ids_token_stride = 0, ids_head_stride = 0;
     void* workspace = nullptr;
-    int ctas = 0;           // CTAs that share the work
+    int ctas = 0;           // CTAs that share the work (to the launchers: SMs)
     int base_align = 16;    // power of two that windows' key chunks start at multiples of
     int unit_shift = 0;     // log2 of the key chunks in a unit of work
-    int combine_split = 1;  // CTAs that join one tile's partials
+    int tile_rows = 16;     // retrieved form: heads to a tile
 };
 int attention_max_requests();
-size_t attention_rows_workspace(int ctas, int dim);
+int attention_max_ids();
+size_t attention_rows_workspace(int sms, int dim);
 cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream);
-size_t attention_tiles_workspace(int ctas, int dim);
+size_t attention_tiles_workspace(int sms, int dim);
 cudaError_t launch_attention_tiles(const AttentionParams& a, cudaStream_t stream);
 
 // Host restatements shared with the CLI and the API.
