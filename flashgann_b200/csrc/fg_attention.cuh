@@ -39,15 +39,18 @@ namespace attn {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Header of the workspace and one record per CTA: the tile its range starts in.
+// The workspace: a record for each CTA, then its partials.  A CTA whose range
+// starts inside a tile that the CTA before it began has the tile to be joined.
 struct alignas(16) TileRecord {
-    int64_t first, last;  // the tile's units [first, last) in the global numbering
-    int32_t head, request, tile, pad;
+    int32_t parts;   // CTAs that share the tile, 0: nothing to join here
+    int32_t before;  // number of the first one's partial; the others' are 2c, 2c + 2, ...
+    int32_t head, tile;
+    int32_t start, rows;  // the request's first query row and its new tokens
+    int32_t pad[2];
 };
-constexpr size_t kHeaderBytes = 256;  // int64 W, then padding
 
 __host__ __device__ inline size_t workspace_records_bytes(int ctas) {
-    return kHeaderBytes + ((static_cast<size_t>(ctas) * sizeof(TileRecord) + 255) & ~static_cast<size_t>(255));
+    return (static_cast<size_t>(ctas) * sizeof(TileRecord) + 255) & ~static_cast<size_t>(255);
 }
 // one partial: rows x dim sums, then rows maxima and rows sums
 __host__ __device__ inline size_t partial_floats(int rows, int dim) { return static_cast<size_t>(rows) * (dim + 2); }
@@ -239,6 +242,23 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
     return x;
 }
 
+// The record of CTA c, whose range starts in tile units [first, last) of the given request.
+__device__ __forceinline__ TileRecord tile_record(const AttentionParams& a, const Place& x, int c, const Request& r, int units) {
+    TileRecord rec = {};
+    const int64_t first = x.unit - x.offset, last = first + units;
+    if (c == 0 || x.unit >= x.end || x.offset == 0) return rec;
+    const int64_t before = x.total * (c - 1) / x.ctas;  // where the CTA before starts
+    if (before > first) return rec;                     // an earlier CTA's range starts inside the tile too
+    const int end = static_cast<int>((last * x.ctas - 1) / x.total);  // the CTA whose range holds the tile's last unit
+    rec.parts = end - c + 2;
+    rec.before = 2 * (c - 1) + (before == first ? 0 : 1);  // its second segment unless its range starts with this tile
+    rec.head = x.head;
+    rec.tile = x.tile;
+    rec.start = r.start;
+    rec.rows = r.rows;
+    return rec;
+}
+
 // The next tile in the numbering after (head, request, tile); false after the last.
 template <int kRows, Layout kLayout>
 __device__ __forceinline__ bool next_tile(const AttentionParams& a, Request* r, int* head, int* request, int* tile) {
@@ -301,72 +321,75 @@ struct SmemOnce {
 };
 
 // Joins the partials of every tile that two or more CTAs of the main kernel
-// shared.  CTA c handles the tile that main CTA c's range starts inside of,
-// if c is the first such CTA.  Bandwidth-bound and tiny: at most 2 partials
-// per main CTA; launched as a dependent of the main kernel so that its start
-// overlaps the main kernel's tail.
+// shared, by the records that those left; a warp joins a row, a lane 4 columns
+// of it.  The maximum first, a partial to a lane, then the sums with 8 partials'
+// loads under way.  Little data (at most 2 partials for each main CTA) and a
+// chain of three loads; launched as a dependent of the main kernel so that its
+// start overlaps the main kernel's tail.
+constexpr int kJoinRows = 8;
+
 template <typename T, int kRows, int kDim, Layout kLayout>
-__global__ void __launch_bounds__(128) attention_combine_kernel(const AttentionParams a) {
+__global__ void __launch_bounds__(kJoinRows * 32) attention_combine_kernel(const AttentionParams a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int kBlocks = kRows / kJoinRows;
     const char* ws = static_cast<const char*>(a.workspace);
-    const int64_t total = *reinterpret_cast<const int64_t*>(ws);
-    const int ctas = static_cast<int>(min(static_cast<int64_t>(a.ctas), total));
-    constexpr int kBlocks = kRows / 4;  // 4 rows to a block
-    const int c = blockIdx.x / kBlocks + 1, part = blockIdx.x % kBlocks;
-    if (c >= ctas) return;
-    const TileRecord rec = reinterpret_cast<const TileRecord*>(ws + kHeaderBytes)[c];
-    const int64_t begin = total * c / ctas, before = total * (c - 1) / ctas;
-    if (begin == rec.first || before > rec.first) return;
+    const int c = blockIdx.x / kBlocks + 1;
+    const TileRecord rec = reinterpret_cast<const TileRecord*>(ws)[c];
+    if (rec.parts == 0) return;
     const float* partials = reinterpret_cast<const float*>(ws + workspace_records_bytes(a.ctas));
-    const size_t psize = partial_floats(kRows, kDim);
-    const int last = static_cast<int>((rec.last * ctas - 1) / total);  // the CTA whose range holds the tile's last unit
-    const int parts = last - c + 2;  // CTAs c - 1 .. last
-    const auto partial = [&](int x) {  // the first CTA's is its second segment unless its range starts with this tile
-        return partials + (x == 0 ? 2 * static_cast<size_t>(c - 1) + (before == rec.first ? 0 : 1) : 2 * static_cast<size_t>(c - 1 + x)) * psize;
-    };
-    const Request r = load_request(a, rec.request);
-    // a warp joins a row: the maximum first, a partial to a lane, then the sums with several loads under way, a lane's 4
-    // columns each
+    constexpr size_t kPartial = static_cast<size_t>(kRows) * (kDim + 2);
+    const auto partial = [&](int x) { return partials + (x == 0 ? rec.before : 2 * (c - 1 + x)) * kPartial; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = part * 4 + warp;
+    const int row = (blockIdx.x % kBlocks) * kJoinRows + warp;
+    const Request r = {rec.start, rec.rows, 0};
     int i, g;
-    if (Tiles<kRows, kLayout>::row(a, r, rec.tile, row, &i, &g)) {
-        float m = -INFINITY;
-        bool nan = false;  // left by a main kernel that gave up
-        for (int x = lane; x < parts; x += 32) {
-            const float v = partial(x)[kRows * kDim + row];
-            m = fmaxf(m, v);
-            nan = nan || v != v;
-        }
+    if (!Tiles<kRows, kLayout>::row(a, r, rec.tile, row, &i, &g)) return;
+    float m = -INFINITY;
+    bool nan = false;  // a row that holds NaN, or left by a main kernel that gave up
+    for (int x = lane; x < rec.parts; x += 32) {
+        const float v = partial(x)[kRows * kDim + row];
+        m = fmaxf(m, v);
+        nan = nan || v != v;
+    }
 #pragma unroll
-        for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-        const float ref = __any_sync(0xFFFFFFFFu, nan) ? NAN : m == -INFINITY ? 0.f : m;
-        const int d = lane * 4;
-        float l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int x = 0; x < parts; ++x) {
-            const float* p = partial(x);
-            const float f = exp2_fast(p[kRows * kDim + row] - ref);
-            l += p[kRows * kDim + kRows + row] * f;
-            if (d < kDim) {
-                const float4 q = *reinterpret_cast<const float4*>(p + row * kDim + d);
-                o.x += q.x * f;
-                o.y += q.y * f;
-                o.z += q.z * f;
-                o.w += q.w * f;
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    const float ref = __any_sync(0xFFFFFFFFu, nan) ? NAN : m == -INFINITY ? 0.f : m;
+    const int d = lane * 4;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x0 = 0; x0 < rec.parts; x0 += 8) {
+        float pm[8], pl[8];
+        float4 q[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            pm[y] = -INFINITY;
+            pl[y] = 0.f;
+            q[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (x0 + y < rec.parts) {
+                const float* p = partial(x0 + y);
+                pm[y] = p[kRows * kDim + row];
+                pl[y] = p[kRows * kDim + kRows + row];
+                if (d < kDim) q[y] = *reinterpret_cast<const float4*>(p + row * kDim + d);
             }
         }
-        const float inv = l == 0.f ? 1.f : 1.f / l;
-        const int64_t token = r.start + i;
-        const int head = rec.head * a.group + g;
-        if (d < kDim) {
-            T* out = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride + d;
-            *reinterpret_cast<uint2*>(out) =
-                make_uint2(Half2<T>::pack(o.x * inv, o.y * inv), Half2<T>::pack(o.z * inv, o.w * inv));
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            const float f = exp2_fast(pm[y] - ref);
+            l += pl[y] * f;
+            o.x += q[y].x * f;
+            o.y += q[y].y * f;
+            o.z += q[y].z * f;
+            o.w += q[y].w * f;
         }
-        if (lane == 0 && a.lse) a.lse[token * a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
     }
+    const float inv = l == 0.f ? 1.f : 1.f / l;
+    const int64_t token = r.start + i;
+    const int head = rec.head * a.group + g;
+    if (d < kDim) {
+        T* out = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride + d;
+        *reinterpret_cast<uint2*>(out) = make_uint2(Half2<T>::pack(o.x * inv, o.y * inv), Half2<T>::pack(o.z * inv, o.w * inv));
+    }
+    if (lane == 0 && a.lse) a.lse[token * a.heads + head] = l == 0.f ? -INFINITY : (ref + log2f(l)) * kLn2;
 }
 
 // After a main kernel that may have left partials; the main kernel lets it start early.
@@ -374,8 +397,8 @@ template <typename T, int kRows, int kDim, Layout kLayout>
 cudaError_t launch_combine(const AttentionParams& a, cudaStream_t stream) {
     if (a.ctas < 2) return cudaSuccess;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((a.ctas - 1) * (kRows / 4)));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(static_cast<unsigned>((a.ctas - 1) * (kRows / kJoinRows)));
+    cfg.blockDim = dim3(kJoinRows * 32);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

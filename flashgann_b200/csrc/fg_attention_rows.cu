@@ -443,24 +443,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     asm volatile("griddepcontrol.launch_dependents;");
     const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
     __syncthreads();  // the rings overlay the scan
-    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
-    if (pl.unit >= pl.end) return;
+    if (pl.unit >= pl.end) {
+        if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
+        return;
+    }
 
     Warp<T, kDim, kIds> w(a, smem_addr(smem) + warp * S::kWarpBytes);
     int head = pl.head, request = pl.request, tile = pl.tile;
     int64_t unit = pl.unit, tile_first = pl.unit - pl.offset;
     w.req = load_request(a, request);
     w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk>(a, w.req, tile);
-    if (threadIdx.x == 0) {
-        TileRecord rec;
-        rec.first = tile_first;
-        rec.last = tile_first + w.keys.units;
-        rec.head = head;
-        rec.request = request;
-        rec.tile = tile;
-        rec.pad = 0;
-        reinterpret_cast<TileRecord*>(ws + kHeaderBytes)[blockIdx.x] = rec;
-    }
+    if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = tile_record(a, pl, blockIdx.x, w.req, w.keys.units);
     bool first_segment = true;
     while (true) {
         const int64_t tile_last = tile_first + w.keys.units;
@@ -472,28 +465,30 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         const int window_end = w.keys.sink_chunks + w.keys.near_chunks;  // chunks from here on need the tile's ids
         // the chunks in flight: a shift register of kStages - 1 descriptors, and one chunk whose pages are looked up
         Chunk flight[S::kStages - 1];
-        Found next_up;
-        bool ids_ready = !kIds;
+        Found found[S::kStages];
+        // those of the first chunks that need no ids, so that their copies are under way while the ids are read
+        int ready = S::kStages;
+        if (kIds) ready = max(0, min(ready, (window_end - (u0 << a.unit_shift)) / kWarps));
+        const auto begin_stages = [&](int from, int to) {
 #pragma unroll
-        for (int s = 0; s < S::kStages; ++s) {
-            const int cs = c + s * kWarps;
-            if (kIds && !ids_ready && (s == S::kStages - 1 || (u0 << a.unit_shift) + s * kWarps + kWarps > window_end)) {
-                // first when a warp may need one, so that the copies of the window are under way meanwhile
-                if (w.keys.id_chunks > 0) {
-                    int* list = reinterpret_cast<int*>(smem + S::kIdsAt);
-                    const int heads = min(a.tile_rows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * a.tile_rows);
-                    w.stage_ids(list, reinterpret_cast<unsigned short*>(list + kMaxIds), heads);
-                    w.staged = list;
+            for (int s = 0; s < S::kStages; ++s)
+                if (s >= from && s < to && c + s * kWarps < c1) found[s] = w.find(c + s * kWarps);
+#pragma unroll
+            for (int s = 0; s < S::kStages - 1; ++s)
+                if (s >= from && s < to) {
+                    if (c + s * kWarps < c1) flight[s] = w.load(found[s], s);
+                    copy_commit();
                 }
-                ids_ready = true;
-            }
-            if (s < S::kStages - 1) {
-                if (cs < c1) flight[s] = w.load(w.find(cs), s);
-                copy_commit();
-            } else if (cs < c1) {
-                next_up = w.find(cs);
-            }
+        };
+        begin_stages(0, ready);
+        if (kIds && w.keys.id_chunks > 0) {
+            int* list = reinterpret_cast<int*>(smem + S::kIdsAt);
+            const int heads = min(a.tile_rows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * a.tile_rows);
+            w.stage_ids(list, reinterpret_cast<unsigned short*>(list + kMaxIds), heads);
+            w.staged = list;
         }
+        if (kIds) begin_stages(ready, S::kStages);
+        Found next_up = found[S::kStages - 1];
         int stage = 0;
         for (; c < c1; c += kWarps) {
             copy_wait<S::kStages - 2>();

@@ -689,8 +689,10 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
 
     asm volatile("griddepcontrol.launch_dependents;");
     const Place pl = locate<kRows, kTokens, kBlock, kThreads, 8>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int64_t*>(ws) = pl.total;
-    if (pl.unit >= pl.end) return;
+    if (pl.unit >= pl.end) {
+        if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
+        return;
+    }
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) {
             bar_init(&sh->full[i], 4);  // the four helper warps, or four times the loader
@@ -722,16 +724,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     tmem_fence_after();
     const uint32_t tmem = sh->tmem;
     Walk w(a, pl);
-    if (threadIdx.x == 0) {
-        TileRecord rec;
-        rec.first = w.first;
-        rec.last = w.first + w.keys.units;
-        rec.head = w.head;
-        rec.request = w.request;
-        rec.tile = w.tile;
-        rec.pad = 0;
-        reinterpret_cast<TileRecord*>(ws + kHeaderBytes)[blockIdx.x] = rec;
-    }
+    if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = tile_record(a, pl, blockIdx.x, w.req, w.keys.units);
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
