@@ -114,24 +114,26 @@ __device__ __forceinline__ int key_page(const AttentionParams& a, const int32_t*
     return at < a.table_width ? __ldg(table + at) : -1;
 }
 
-// A chunk whose keys' pages are being looked up; one key to a lane (lanes 16-31 repeat them).
+// A chunk whose keys' pages are being looked up.  A lane has two keys, number
+// lane / 4 and that + 8, and copies every fourth 16-byte piece of their rows:
+// 64 contiguous bytes to each 4 lanes, and addresses that differ by constants.
 struct Found {
-    int key, row;  // as in Chunk
-    int j, page;   // this lane's key and, when it arrives, its page
+    int key, row;          // as in Chunk
+    int j[2], page[2];     // this lane's keys (-1: none) and, when they arrive, their pages
 };
 
 // One chunk in flight.
 struct Chunk {
-    int key;        // first key (contiguous chunks)
-    int row;        // row that alone sees it (retrieved ids), or -1
-    uint32_t ok;    // bit i: key i is loaded and may be visible
+    int key;         // first key (contiguous chunks)
+    int row;         // row that alone sees it (retrieved ids), or -1
+    uint32_t ok[2];  // bits 4 i .. 4 i + 3: key i (and 8 + i) is loaded and may be visible
+    __device__ __forceinline__ bool has(int col) const { return (ok[col >> 3] >> ((col & 7) * 4)) & 1u; }
 };
 
 template <typename T, int kDim, bool kIds>
 struct Warp {
     using S = Smem<kDim>;
     static constexpr int kPieces = kDim / 8;              // 16-byte pieces of a row
-    static constexpr int kCopies = kChunk * kPieces / 32;  // per lane and operand
 
     const AttentionParams& a;
     const int lane;
@@ -149,6 +151,7 @@ struct Warp {
     uint32_t q[kDim / 16][4];
     float o[kDim / 8][4];
     float m[2], l[2];
+    bool safe;
 
     __device__ __forceinline__ Warp(const AttentionParams& args, uint32_t ring_addr)
         : a(args), lane(threadIdx.x & 31), ring(ring_addr) {}
@@ -179,6 +182,10 @@ struct Warp {
             ids = a.ids + static_cast<int64_t>(req.start + i) * a.ids_token_stride +
                   static_cast<int64_t>(head * a.group + g) * a.ids_head_stride;
         }
+        safe = false;
+        clear();
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int n = 0; n < kDim / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
         m[0] = m[1] = -INFINITY;
@@ -190,23 +197,32 @@ struct Warp {
         Found f;
         f.row = -1;
         f.key = 0;
-        f.j = f.page = -1;
-        const int x = lane & 15;
+        f.j[0] = f.j[1] = f.page[0] = f.page[1] = -1;
+        const int x = lane >> 2;
         if (c < keys.sink_chunks) {
             f.key = c * kChunk;
-            if (f.key + x < keys.sink_hi) f.j = f.key + x;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+                if (f.key + x + 8 * y < keys.sink_hi) f.j[y] = f.key + x + 8 * y;
         } else if (c < keys.sink_chunks + keys.near_chunks) {
             f.key = keys.base + (c - keys.sink_chunks) * kChunk;
-            const int j = f.key + x;
-            if (j < keys.hi && (j >= keys.lo || j < a.sinks)) f.j = j;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int j = f.key + x + 8 * y;
+                if (j < keys.hi && (j >= keys.lo || j < a.sinks)) f.j[y] = j;
+            }
         } else if (kIds) {
             const int per = (a.ids_count + kChunk - 1) / kChunk;
             const int at = c - keys.sink_chunks - keys.near_chunks;
             f.row = at / per;
-            const int n = (at - f.row * per) * kChunk + x;
-            if (n < a.ids_count) f.j = staged[f.row * staged_pitch(a.ids_count) + n];
+            const int n = (at - f.row * per) * kChunk + x;  // the list is padded to whole chunks
+            const int* list = staged + f.row * staged_pitch(a.ids_count);
+            f.j[0] = list[n];
+            f.j[1] = list[n + 8];
         }
-        if (f.j >= 0) f.page = key_page(a, table, f.j);
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+            if (f.j[y] >= 0) f.page[y] = key_page(a, table, f.j[y]);
         return f;
     }
 
@@ -273,79 +289,81 @@ struct Warp {
         Chunk ch;
         ch.key = f.key;
         ch.row = f.row;
-        const int64_t off = f.j >= 0 ? key_offset(a, f.page, f.j, head_off) : -1;
-        ch.ok = __ballot_sync(0xFFFFFFFFu, off >= 0) & 0xFFFFu;
         const uint32_t dst = ring + s * 2 * S::kTile;
-        const T* kc = static_cast<const T*>(a.k_cache);
-        const T* vc = static_cast<const T*>(a.v_cache);
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            const int idx = i * 32 + lane, r = idx / kPieces, p = idx % kPieces;
-            const int64_t ro = __shfl_sync(0xFFFFFFFFu, off, r);
-            const bool ok = ro >= 0;
-            const int64_t from = ok ? ro + p * 8 : 0;
-            const uint32_t to = dst + S::at(r, p);
-            copy16(to, kc + from, ok);
-            copy16(to + S::kTile, vc + from, ok);
+        for (int y = 0; y < 2; ++y) {
+            const int64_t off = f.j[y] >= 0 ? key_offset(a, f.page[y], f.j[y], head_off) : -1;
+            const bool ok = off >= 0;
+            ch.ok[y] = __ballot_sync(0xFFFFFFFFu, ok);
+            const T* k = static_cast<const T*>(a.k_cache) + (ok ? off + (lane & 3) * 8 : 0);
+            const T* v = static_cast<const T*>(a.v_cache) + (ok ? off + (lane & 3) * 8 : 0);
+#pragma unroll
+            for (int i = 0; i < kPieces / 4; ++i) {
+                const uint32_t to = dst + S::at((lane >> 2) + 8 * y, 4 * i + (lane & 3));
+                copy16(to, k + i * 32, ok);
+                copy16(to + S::kTile, v + i * 32, ok);
+            }
         }
         return ch;
     }
 
     __device__ __forceinline__ bool sees(const Chunk& ch, int x, int col) const {
-        if (!((ch.ok >> col) & 1u)) return false;
-        if (kIds && ch.row >= 0) return (lane >> 2) + 8 * x == ch.row;
+        if (!ch.has(col)) return false;
+        if (kIds) return ch.row < 0 || (lane >> 2) + 8 * x == ch.row;  // one token: what is loaded is visible
         const int j = ch.key + col, p = prow[x];
         return j <= p && (a.window < 0 || p - j < a.window || j < a.sinks);
     }
 
     // V rows that some rows of the tile see and others do not: 0 * inf and
-    // 0 * NaN must not reach the ones that do not.  Each lane checks and clears
-    // the pieces that it copied itself.
+    // 0 * NaN must not reach the ones that do not.  That is rare, and shows in
+    // the sums: only where a tile's sums are not finite (or the values that
+    // belong there are not) its chunks are done once more with `safe` set.  Then
+    // each lane clears such values from the pieces that it copied itself,
     __device__ __forceinline__ bool clear_nonfinite(int s) {
-        const uint32_t dst = ring + s * 2 * S::kTile + S::kTile;
         bool bad = false;
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            const int idx = i * 32 + lane, r = idx / kPieces, p = idx % kPieces;
-            const uint32_t at = dst + S::at(r, p);
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                         : "r"(at)
-                         : "memory");
-            bool here = false;
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                constexpr uint32_t kE = Half2<T>::kExpMask;
-                if ((w[e] & kE) == kE) {
-                    w[e] &= 0xFFFF0000u;
-                    here = true;
-                }
-                if ((w[e] & (kE << 16)) == (kE << 16)) {
-                    w[e] &= 0x0000FFFFu;
-                    here = true;
-                }
-            }
-            if (here) {
-                bad = true;
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+            for (int i = 0; i < kPieces / 4; ++i) {
+                const uint32_t at = ring + s * 2 * S::kTile + S::kTile + S::at((lane >> 2) + 8 * y, 4 * i + (lane & 3));
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                             : "r"(at)
                              : "memory");
+                bool here = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    constexpr uint32_t kE = Half2<T>::kExpMask;
+                    if ((w[e] & kE) == kE) {
+                        w[e] &= 0xFFFF0000u;
+                        here = true;
+                    }
+                    if ((w[e] & (kE << 16)) == (kE << 16)) {
+                        w[e] &= 0x0000FFFFu;
+                        here = true;
+                    }
+                }
+                if (here) {
+                    bad = true;
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                 : "memory");
+                }
             }
-        }
         return __any_sync(0xFFFFFFFFu, bad);
     }
 
-    // ... and the rows that do see them get them back.
-    __device__ __forceinline__ void add_nonfinite(const Chunk ch) {
+    // and the rows that do see them get them back.  id_chunk: number of the chunk among the retrieved ones.
+    __device__ __forceinline__ void add_nonfinite(const Chunk ch, int id_chunk) {
         const T* vc = static_cast<const T*>(a.v_cache);
 #pragma unroll 1
         for (int col = 0; col < kChunk; ++col) {
-            if (!((ch.ok >> col) & 1u)) continue;
+            if (!ch.has(col)) continue;
             const bool see0 = sees(ch, 0, col), see1 = sees(ch, 1, col);
             int j = ch.key + col;
             if (kIds && ch.row >= 0) {
                 const int per = (a.ids_count + kChunk - 1) / kChunk;
-                j = __ldg(ids + ch.row * a.ids_head_stride + (id_chunk % per) * kChunk + col);
+                j = staged[ch.row * staged_pitch(a.ids_count) + (id_chunk % per) * kChunk + col];
             }
             const T* src = vc + key_offset(a, key_page(a, table, j), j, head_off) + (lane & 3) * 2;
 #pragma unroll
@@ -363,9 +381,19 @@ struct Warp {
             }
         }
     }
-    int id_chunk;  // number among the retrieved chunks of the chunk in work
 
-    __device__ __forceinline__ void compute(const Chunk& ch, int s) {
+    // Rows of the tile differ in what they see, and a sum is not finite.
+    __device__ __forceinline__ bool tainted() const {
+        if (!kIds && p0 == p1) return false;
+        float t = 0.f;
+#pragma unroll
+        for (int n = 0; n < kDim / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t = fmaf(o[n][e], 0.f, t);
+        return __any_sync(0xFFFFFFFFu, t != 0.f);
+    }
+
+    __device__ __forceinline__ void compute(const Chunk& ch, int s, int id_chunk) {
         const uint32_t kt = ring + s * 2 * S::kTile, vt = kt + S::kTile;
         float sc[2][4];
 #pragma unroll
@@ -379,8 +407,9 @@ struct Warp {
             mma<T>(sc[0], q[k], b[0], b[1]);
             mma<T>(sc[1], q[k], b[2], b[3]);
         }
-        const bool whole = ch.ok == 0xFFFFu && ch.row < 0 && ch.key + kChunk - 1 <= p0 &&
-                           (a.window < 0 || p1 - ch.key < a.window || ch.key + kChunk - 1 < a.sinks);
+        const bool whole = (ch.ok[0] & ch.ok[1]) == 0xFFFFFFFFu && ch.row < 0 &&
+                           (kIds || p0 == p1 || (ch.key + kChunk - 1 <= p0 && (a.window < 0 || p1 - ch.key < a.window ||
+                                                                              ch.key + kChunk - 1 < a.sinks)));
         bool poison = false;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -392,8 +421,10 @@ struct Warp {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (!sees(ch, e >> 1, n * 8 + (lane & 3) * 2 + (e & 1))) sc[n][e] = -INFINITY;
-            if (p0 != p1 || ch.row >= 0) poison = clear_nonfinite(s);
-            __syncwarp();
+            if (safe) {
+                poison = clear_nonfinite(s);
+                __syncwarp();
+            }
         }
         uint32_t pa[4];
 #pragma unroll
@@ -429,7 +460,7 @@ struct Warp {
             mma<T>(o[2 * n], pa, b[0], b[1]);
             mma<T>(o[2 * n + 1], pa, b[2], b[3]);
         }
-        if (poison) add_nonfinite(ch);
+        if (poison) add_nonfinite(ch, id_chunk);
     }
 };
 
@@ -461,55 +492,63 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         const int u1 = static_cast<int>(min(tile_last, pl.end) - tile_first);
         const int c1 = min(u1 << a.unit_shift, w.keys.chunks);
         w.begin(head, request, tile);
-        int c = (u0 << a.unit_shift) + warp;
         const int window_end = w.keys.sink_chunks + w.keys.near_chunks;  // chunks from here on need the tile's ids
-        // the chunks in flight: a shift register of kStages - 1 descriptors, and one chunk whose pages are looked up
-        Chunk flight[S::kStages - 1];
-        Found found[S::kStages];
-        // those of the first chunks that need no ids, so that their copies are under way while the ids are read
-        int ready = S::kStages;
-        if (kIds) ready = max(0, min(ready, (window_end - (u0 << a.unit_shift)) / kWarps));
-        const auto begin_stages = [&](int from, int to) {
+        const int c0 = u0 << a.unit_shift;
+        while (true) {
+            int c = c0 + warp;
+            // the chunks in flight: a shift register of kStages - 1 descriptors, and one chunk whose pages are looked up
+            Chunk flight[S::kStages - 1];
+            Found found[S::kStages];
+            const auto begin_stages = [&](int from, int to) {
 #pragma unroll
-            for (int s = 0; s < S::kStages; ++s)
-                if (s >= from && s < to && c + s * kWarps < c1) found[s] = w.find(c + s * kWarps);
+                for (int s = 0; s < S::kStages; ++s)
+                    if (s >= from && s < to && c + s * kWarps < c1) found[s] = w.find(c + s * kWarps);
 #pragma unroll
-            for (int s = 0; s < S::kStages - 1; ++s)
-                if (s >= from && s < to) {
-                    if (c + s * kWarps < c1) flight[s] = w.load(found[s], s);
-                    copy_commit();
-                }
-        };
-        begin_stages(0, ready);
-        if (kIds && w.keys.id_chunks > 0) {
-            int* list = reinterpret_cast<int*>(smem + S::kIdsAt);
-            const int heads = min(a.tile_rows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * a.tile_rows);
-            w.stage_ids(list, reinterpret_cast<unsigned short*>(list + kMaxIds), heads);
-            w.staged = list;
-        }
-        if (kIds) begin_stages(ready, S::kStages);
-        Found next_up = found[S::kStages - 1];
-        int stage = 0;
-        for (; c < c1; c += kWarps) {
-            copy_wait<S::kStages - 2>();
-            __syncwarp();
-            const Chunk now = flight[0];
-#pragma unroll
-            for (int s = 0; s + 1 < S::kStages - 1; ++s) flight[s] = flight[s + 1];
-            const int ahead = c + (S::kStages - 1) * kWarps;
-            int next = stage + S::kStages - 1;
-            if (next >= S::kStages) next -= S::kStages;
-            if (ahead < c1) {
-                flight[S::kStages - 2] = w.load(next_up, next);
-                if (ahead + kWarps < c1) next_up = w.find(ahead + kWarps);
+                for (int s = 0; s < S::kStages - 1; ++s)
+                    if (s >= from && s < to) {
+                        if (c + s * kWarps < c1) flight[s] = w.load(found[s], s);
+                        copy_commit();
+                    }
+            };
+            int ready = S::kStages;
+            if (kIds && !w.safe && c1 > window_end) {
+                // those of the first chunks that need no ids, so that their copies are under way while the ids are read
+                ready = max(0, min(ready, (window_end - c0) / kWarps));
+                begin_stages(0, ready);
+                int* list = reinterpret_cast<int*>(smem + S::kIdsAt);
+                const int heads = min(a.tile_rows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * a.tile_rows);
+                w.stage_ids(list, reinterpret_cast<unsigned short*>(list + kMaxIds), heads);
+                w.staged = list;
+                begin_stages(ready, S::kStages);
+            } else {
+                begin_stages(0, S::kStages);
             }
-            copy_commit();
-            w.id_chunk = c - window_end;
-            w.compute(now, stage);
-            if (++stage == S::kStages) stage = 0;
+            Found next_up = found[S::kStages - 1];
+            int stage = 0;
+            for (; c < c1; c += kWarps) {
+                copy_wait<S::kStages - 2>();
+                __syncwarp();
+                const Chunk now = flight[0];
+#pragma unroll
+                for (int s = 0; s + 1 < S::kStages - 1; ++s) flight[s] = flight[s + 1];
+                const int ahead = c + (S::kStages - 1) * kWarps;
+                int next = stage + S::kStages - 1;
+                if (next >= S::kStages) next -= S::kStages;
+                if (ahead < c1) {
+                    flight[S::kStages - 2] = w.load(next_up, next);
+                    if (ahead + kWarps < c1) next_up = w.find(ahead + kWarps);
+                }
+                copy_commit();
+                w.compute(now, stage, c - window_end);
+                if (++stage == S::kStages) stage = 0;
+                __syncwarp();
+            }
+            copy_wait<0>();
+            if (w.safe || !w.tainted()) break;
+            w.safe = true;
+            w.clear();
             __syncwarp();
         }
-        copy_wait<0>();
 
         // join the warps: rows of (m, l) and sums, over the rings
 #pragma unroll
