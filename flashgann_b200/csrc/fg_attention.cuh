@@ -168,31 +168,45 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
     int* pre = scratch + 64;  // inclusive prefix of the requests' units
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kWarps = kThreads / 32;
-    int carry = 0;
-    for (int b0 = 0; b0 < a.requests; b0 += kThreads / kLanes) {
-        const int b = b0 + tid / kLanes;
-        int s = 0;
-        if (b < a.requests) {
-            const Request r = load_request(a, b);
+    int carry = 0, few = 0;
+    if (a.requests <= 32 / kLanes) {  // every warp on its own, without a barrier
+        if (lane / kLanes < a.requests) {
+            const Request r = load_request(a, lane / kLanes);
             const int n = Tiles<kRows, kLayout>::count(a, r);
-            for (int t = tid % kLanes; t < n; t += kLanes) s += tile_keys<kRows, kLayout, kChunk>(a, r, t).units;
+            for (int t = lane % kLanes; t < n; t += kLanes) few += tile_keys<kRows, kLayout, kChunk>(a, r, t).units;
         }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(0xFFFFFFFFu, s, d);
-            if (lane >= d) s += v;
+            const int v = __shfl_up_sync(0xFFFFFFFFu, few, d);
+            if (lane >= d) few += v;
         }
-        if (lane == 31) scratch[warp] = s;
-        __syncthreads();
-        int before = carry, sum = 0;
-        for (int w = 0; w < kWarps; ++w) {
-            const int v = scratch[w];
-            if (w < warp) before += v;
-            sum += v;
+        carry = __shfl_sync(0xFFFFFFFFu, few, 31);
+    } else {
+        for (int b0 = 0; b0 < a.requests; b0 += kThreads / kLanes) {
+            const int b = b0 + tid / kLanes;
+            int s = 0;
+            if (b < a.requests) {
+                const Request r = load_request(a, b);
+                const int n = Tiles<kRows, kLayout>::count(a, r);
+                for (int t = tid % kLanes; t < n; t += kLanes) s += tile_keys<kRows, kLayout, kChunk>(a, r, t).units;
+            }
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, s, d);
+                if (lane >= d) s += v;
+            }
+            if (lane == 31) scratch[warp] = s;
+            __syncthreads();
+            int before = carry, sum = 0;
+            for (int w = 0; w < kWarps; ++w) {
+                const int v = scratch[w];
+                if (w < warp) before += v;
+                sum += v;
+            }
+            if (b < a.requests && tid % kLanes == kLanes - 1) pre[b] = before + s;
+            carry += sum;
+            __syncthreads();
         }
-        if (b < a.requests && tid % kLanes == kLanes - 1) pre[b] = before + s;
-        carry += sum;
-        __syncthreads();
     }
     Place x;
     const int64_t per_head = carry;
@@ -207,13 +221,19 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
     x.head = static_cast<int>(x.unit / per_head);
     int rest = static_cast<int>(x.unit - x.head * per_head);
     int lo = 0, hi = a.requests - 1;  // first request whose inclusive prefix exceeds rest
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (pre[mid] > rest) hi = mid;
-        else lo = mid + 1;
+    if (a.requests <= 32 / kLanes) {
+        lo = (__ffs(__ballot_sync(0xFFFFFFFFu, few > rest)) - 1) / kLanes;
+        const int before = __shfl_sync(0xFFFFFFFFu, few, max(lo * kLanes - 1, 0));
+        if (lo > 0) rest -= before;
+    } else {
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (pre[mid] > rest) hi = mid;
+            else lo = mid + 1;
+        }
+        if (lo > 0) rest -= pre[lo - 1];
     }
     x.request = lo;
-    if (lo > 0) rest -= pre[lo - 1];
     const Request r = load_request(a, lo);
     // the tile that holds unit `rest` of the request, 32 tiles at a time, in every warp
     const int tiles = Tiles<kRows, kLayout>::count(a, r);

@@ -145,7 +145,7 @@ struct Warp {
     int64_t head_off;
     int p0, p1;        // positions of the tile's first and last row
     int prow[2];       // positions of this lane's two rows (-1: no row)
-    const int32_t* ids;  // retrieved ids of the tile's first row
+    const int32_t* ids;  // the tile's lists of retrieved ids
     const int* staged;   // those of all its rows that count, in shared memory
     // running state
     uint32_t q[kDim / 16][4];
@@ -176,12 +176,6 @@ struct Warp {
                 q[k][x + 2] = ok ? *reinterpret_cast<const uint32_t*>(src + k * 16 + 8) : 0u;
             }
         }
-        if (kIds) {
-            int i, g;
-            Tiles<kRows, kIds ? kToken : kPacked>::row(a, req, tile, 0, &i, &g);
-            ids = a.ids + static_cast<int64_t>(req.start + i) * a.ids_token_stride +
-                  static_cast<int64_t>(head * a.group + g) * a.ids_head_stride;
-        }
         safe = false;
         clear();
     }
@@ -191,6 +185,31 @@ struct Warp {
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = 0.f;
     }
+
+    // The lists of a tile's heads.
+    __device__ __forceinline__ const int32_t* lists(const Request& r, int head, int tile) const {
+        int i, g;
+        Tiles<kRows, kIds ? kToken : kPacked>::row(a, r, tile, 0, &i, &g);
+        return a.ids + static_cast<int64_t>(r.start + i) * a.ids_token_stride + static_cast<int64_t>(head * a.group + g) * a.ids_head_stride;
+    }
+    // This thread's places x, x + kThreads, ... of the tile's lists.
+    __device__ __forceinline__ void read_places(const int32_t* from, int x0, int heads, int (&id)[4]) const {
+        const int pitch = staged_pitch(a.ids_count);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const int x = x0 + y * kThreads, h = x / pitch, n = x - h * pitch;
+            id[y] = h < heads && n < a.ids_count ? __ldg(from + h * a.ids_head_stride + n) : -1;
+        }
+    }
+    __device__ __forceinline__ int list_heads(int tile) const {
+        return min(a.tile_rows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * a.tile_rows);
+    }
+    // The first ids of a tile that comes next, into registers.
+    __device__ __forceinline__ void read_ids(const Request& r, int head, int tile) {
+        ids = lists(r, head, tile);
+        read_places(ids, threadIdx.x, list_heads(tile), early);
+    }
+    int early[4];
 
     // Starts looking chunk c's keys up.
     __device__ __forceinline__ Found find(int c) const {
@@ -242,13 +261,9 @@ struct Warp {
         constexpr unsigned short kFree = 0xFFFF;
         const int pitch = staged_pitch(a.ids_count), all = heads * pitch;
         for (int x = threadIdx.x; x < kTable / 2; x += kThreads) reinterpret_cast<uint32_t*>(table)[x] = 0xFFFFFFFFu;
+        int id[4] = {early[0], early[1], early[2], early[3]};
         for (int x0 = threadIdx.x; x0 < all; x0 += kThreads * 4) {
-            int id[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const int x = x0 + y * kThreads, h = x / pitch, n = x - h * pitch;
-                id[y] = x < all && n < a.ids_count ? __ldg(ids + h * a.ids_head_stride + n) : -1;
-            }
+            if (x0 != threadIdx.x) read_places(ids, x0, heads, id);
 #pragma unroll
             for (int y = 0; y < 4; ++y)
                 if (x0 + y * kThreads < all) list[x0 + y * kThreads] = counts(id[y]) ? id[y] : -1;
@@ -485,6 +500,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     w.req = load_request(a, request);
     w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk>(a, w.req, tile);
     if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = tile_record(a, pl, blockIdx.x, w.req, w.keys.units);
+    if (kIds) w.read_ids(w.req, head, tile);
     bool first_segment = true;
     while (true) {
         const int64_t tile_last = tile_first + w.keys.units;
@@ -516,8 +532,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                 ready = max(0, min(ready, (window_end - c0) / kWarps));
                 begin_stages(0, ready);
                 int* list = reinterpret_cast<int*>(smem + S::kIdsAt);
-                const int heads = min(a.tile_rows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * a.tile_rows);
-                w.stage_ids(list, reinterpret_cast<unsigned short*>(list + kMaxIds), heads);
+                w.stage_ids(list, reinterpret_cast<unsigned short*>(list + kMaxIds), w.list_heads(tile));
                 w.staged = list;
                 begin_stages(ready, S::kStages);
             } else {
@@ -549,6 +564,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             w.clear();
             __syncwarp();
         }
+
+        // the next tile's request and ids are read beside the join
+        Request next_req = w.req;
+        int next_head = head, next_request = request, next_number = tile;
+        const bool more = tile_first + u1 < pl.end && next_tile<kRows, kIds ? kToken : kPacked>(a, &next_req, &next_head, &next_request, &next_number);
+        if (kIds && more) w.read_ids(next_req, next_head, next_number);
 
         // join the warps: rows of (m, l) and sums, over the rings
 #pragma unroll
@@ -617,10 +638,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                 }
             }
         }
-        unit = tile_first + u1;
-        if (unit >= pl.end) break;
-        tile_first = tile_last;
-        if (!next_tile<kRows, kIds ? kToken : kPacked>(a, &w.req, &head, &request, &tile)) break;
+        if (!more) break;
+        unit = tile_first = tile_last;
+        w.req = next_req;
+        head = next_head;
+        request = next_request;
+        tile = next_number;
         w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk>(a, w.req, tile);
         first_segment = false;
         __syncthreads();  // the join's reads end before the next tile's copies
