@@ -160,6 +160,18 @@ struct Place {
     int head, request, tile, offset;  // the first unit: its tile and its place in it
 };
 
+// a / b, without a 64-bit division where 32 bits will do
+__device__ __forceinline__ int64_t divide(int64_t a, uint32_t b) {
+    if ((a >> 32) == 0) return static_cast<uint32_t>(a) / b;
+    return a / b;
+}
+// total * c / ctas
+__device__ __forceinline__ int64_t share(int64_t total, int c, int ctas) {
+    const int64_t each = divide(total, ctas);
+    const uint32_t rest = static_cast<uint32_t>(total - each * ctas);
+    return each * c + rest * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);  // both below 2^16
+}
+
 // Called by all kThreads threads; scratch holds requests + 64 ints.  kLanes
 // threads count the tiles of a request: 1 where requests are short, 8 where
 // they have many tiles.
@@ -216,9 +228,9 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
         x.unit = x.end = 0;
         return x;
     }
-    x.unit = x.total * cta / x.ctas;
-    x.end = x.total * (cta + 1) / x.ctas;
-    x.head = static_cast<int>(x.unit / per_head);
+    x.unit = share(x.total, cta, x.ctas);
+    x.end = share(x.total, cta + 1, x.ctas);
+    x.head = static_cast<int>(divide(x.unit, static_cast<uint32_t>(per_head)));
     int rest = static_cast<int>(x.unit - x.head * per_head);
     int lo = 0, hi = a.requests - 1;  // first request whose inclusive prefix exceeds rest
     if (a.requests <= 32 / kLanes) {
@@ -267,7 +279,7 @@ __device__ __forceinline__ TileRecord tile_record(const AttentionParams& a, cons
     TileRecord rec = {};
     const int64_t first = x.unit - x.offset, last = first + units;
     if (c == 0 || x.unit >= x.end || x.offset == 0) return rec;
-    const int64_t before = x.total * (c - 1) / x.ctas;  // where the CTA before starts
+    const int64_t before = share(x.total, c - 1, x.ctas);  // where the CTA before starts
     if (before > first) return rec;                     // an earlier CTA's range starts inside the tile too
     const int end = static_cast<int>((last * x.ctas - 1) / x.total);  // the CTA whose range holds the tile's last unit
     rec.parts = end - c + 2;

@@ -43,8 +43,8 @@ constexpr int kWarps = 4;
 constexpr int kCtasPerSm = 2;
 constexpr int kThreads = kWarps * 32;
 constexpr int kShort = 64;       // chunks of a tile that is not split
-constexpr int kMaxIds = 2048;    // ids of a tile's heads, in shared memory
-constexpr int kTable = 4096;     // places of the hash table over them
+constexpr int kMaxIds = 1024;    // ids of a tile's heads, in shared memory
+constexpr int kTable = 2048;     // places of the hash table over them
 
 template <int kDim>
 struct Smem {
@@ -61,7 +61,7 @@ struct Smem {
     static constexpr int kWarpBytes = kRing;
     static constexpr int kIdsAt = kWarps * kWarpBytes;  // retrieved form: the tile's ids and the table
     static constexpr int kBytes = kIdsAt;
-    static constexpr int kBytesIds = kIdsAt + kMaxIds * 4 + kTable * 2;
+    static constexpr int kBytesIds = kIdsAt + kMaxIds * 4 + kTable * 4;
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -257,10 +257,10 @@ struct Warp {
     // head the least of its places in the lists; an id whose place is another's
     // goes.  The result does not depend on the order of the atomics.  Called by
     // the whole CTA.
-    __device__ __forceinline__ void stage_ids(int* list, unsigned short* table, int heads) const {
-        constexpr unsigned short kFree = 0xFFFF;
+    __device__ __forceinline__ void stage_ids(int* list, int* table, int heads) const {
+        constexpr int kFree = -1;  // (16-bit places would do, but their atomics are ten times as slow)
         const int pitch = staged_pitch(a.ids_count), all = heads * pitch;
-        for (int x = threadIdx.x; x < kTable / 2; x += kThreads) reinterpret_cast<uint32_t*>(table)[x] = 0xFFFFFFFFu;
+        for (int x = threadIdx.x; x < kTable; x += kThreads) table[x] = kFree;
         int id[4] = {early[0], early[1], early[2], early[3]};
         for (int x0 = threadIdx.x; x0 < all; x0 += kThreads * 4) {
             if (x0 != threadIdx.x) read_places(ids, x0, heads, id);
@@ -270,21 +270,17 @@ struct Warp {
         }
         __syncthreads();
         const auto first_place = [&](int id, int h) {
-            return ((static_cast<uint32_t>(id) + static_cast<uint32_t>(h) * 0x9E3779B9u) * 2654435761u) >> 20;  // of 4096
+            return ((static_cast<uint32_t>(id) + static_cast<uint32_t>(h) * 0x9E3779B9u) * 2654435761u) >> 21;  // of 2048
         };
         const auto same = [&](int x, int id, int h) { return list[x] == id && x / pitch == h; };
         for (int x = threadIdx.x; x < all; x += kThreads) {
             const int id = list[x], h = x / pitch;
             if (id < 0) continue;
             for (uint32_t at = first_place(id, h);; at = (at + 1) % kTable) {
-                unsigned short old = atomicCAS(table + at, kFree, static_cast<unsigned short>(x));
+                int old = atomicCAS(table + at, kFree, x);
                 if (old == kFree) break;
                 if (!same(old, id, h)) continue;  // another id's place
-                while (old > x) {
-                    const unsigned short was = atomicCAS(table + at, old, static_cast<unsigned short>(x));
-                    if (was == old) break;
-                    old = was;  // lowered by another thread with the same id
-                }
+                atomicMin(table + at, x);  // the same id's
                 break;
             }
         }
@@ -532,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                 ready = max(0, min(ready, (window_end - c0) / kWarps));
                 begin_stages(0, ready);
                 int* list = reinterpret_cast<int*>(smem + S::kIdsAt);
-                w.stage_ids(list, reinterpret_cast<unsigned short*>(list + kMaxIds), w.list_heads(tile));
+                w.stage_ids(list, list + kMaxIds, w.list_heads(tile));
                 w.staged = list;
                 begin_stages(ready, S::kStages);
             } else {

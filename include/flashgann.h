@@ -347,8 +347,8 @@ int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args
  * ids[token, head, :] that are in [0, p].  The visible keys are a set: an id
  * that repeats, or that the window or the first tokens hold already, counts
  * once; ids outside [0, p] (such as the search's padding, 0xFFFFFFFF) count
- * nothing.  Needs a window >= 0; at most 2048 ids for each row (a search
- * returns up to 1024). */
+ * nothing.  Needs a window >= 0; at most 1024 ids for each row (more
+ * than a search finds). */
 int fg_retrieved_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream);
 
 /* ---- host helpers of the reference CLI ---- */

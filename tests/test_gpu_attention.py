@@ -332,9 +332,9 @@ def test_long_axes_split_over_ctas(ctx, new, heads, kv_heads):
     ([900, 2], [1, 2], 12, 4, 128, 64, 512, 16, 1, "bf16"),
     ([10], [1], 4, 4, 96, 16, 200, 100, 4, "fp16"),         # the window holds all
     ([250], [1], 3, 1, 128, 1, 1, 5, 2, "bf16"),
-    ([3000, 900], [1, 2], 6, 2, 64, 16, 2000, 30, 3, "fp16"),   # a tile to a head
-    ([5000], [1], 4, 1, 128, 32, 1024, 0, 0, "bf16"),           # two heads to a tile
-    ([100, 40], [1, 1], 6, 1, 64, 16, 2048, 3, 0, "fp16"),      # as many ids as there may be, most of them repeats
+    ([3000, 900], [1, 2], 6, 2, 64, 16, 1000, 30, 3, "fp16"),   # a tile to a head
+    ([5000], [1], 4, 1, 128, 32, 500, 0, 0, "bf16"),            # two heads to a tile
+    ([100, 40], [1, 1], 6, 1, 64, 16, 1024, 3, 0, "fp16"),      # as many ids as there may be, most of them repeats
     ([2000], [3], 8, 8, 96, 16, 40, 700, 0, "bf16"),
 ])
 def test_retrieved_attention(ctx, new, heads, kv_heads, dim, page, count, window, sinks, dtype):
