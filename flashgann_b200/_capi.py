@@ -102,7 +102,7 @@ SIGNATURES = [
     ("fg_kv_append_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32,
                                            _vp]),
     ("fg_attention_workspace_bytes", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs),
-                                                    ctypes.POINTER(_u64)]),
+                                                    _i32, ctypes.POINTER(_u64)]),
     ("fg_paged_attention_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs), _vp]),
     ("fg_retrieved_attention_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs),
                                                      _vp]),

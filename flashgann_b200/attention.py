@@ -153,7 +153,7 @@ def kv_plan(ctx_len: torch.Tensor, new_len: torch.Tensor, block_table: torch.Ten
             _fail("free_head must be int32 [1]")
         T = max(tokens, 0)
         slot = torch.empty(T, dtype=torch.int64, device=ctx_len.device)
-        ints = torch.empty(3 * R + 2 + T, dtype=torch.int32, device=ctx_len.device)
+        ints = ctx_len.new_empty(3 * R + 2 + T)
         base = ints.data_ptr()
         query_start, kv_len, head, refused, position = ints.split_with_sizes((R + 1, R, 1, R, T))
         rc = lib().fg_kv_plan_device(ctx_len.data_ptr(), new_len.data_ptr(), R, free_pages.data_ptr(),
@@ -188,10 +188,10 @@ def kv_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: 
             _raise(rc, "fg_kv_append_device")
 
 
-_workspace = {}  # bytes that a call needs: by device, entry point, head size and whether requests have many rows
+_workspace = {}  # bytes that a call needs, by what they depend on
 
 
-def _attend(call: str, q, k_cache, v_cache, block_table, query_start, kv_len, max_new, ids, window, sinks, scale, out,
+def _attend(retrieved: bool, q, k_cache, v_cache, block_table, query_start, kv_len, max_new, ids, window, sinks, scale, out,
             return_lse, stream):
     with _On(q, stream) as on:
         on.uses(q, k_cache, v_cache, block_table, query_start, kv_len, out, ids)
@@ -207,7 +207,7 @@ def _attend(call: str, q, k_cache, v_cache, block_table, query_start, kv_len, ma
             _fail(f"{R} lengths need {R + 1} query_start entries and {R} table rows, not {query_start.shape[0]} and "
                   f"{block_table.shape[0]}")
         if out is None:
-            out = torch.empty((T, heads, dim), dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty((T, heads, dim), dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
             _fail(f"out must be {q.dtype} {tuple(q.shape)} with a contiguous last axis")
         lse = torch.empty((T, heads), dtype=torch.float32, device=q.device) if return_lse else None
@@ -225,17 +225,21 @@ def _attend(call: str, q, k_cache, v_cache, block_table, query_start, kv_len, ma
                 block_table.data_ptr(), block_table.stride(0), query_start.data_ptr(), kv_len.data_ptr(), id_ptr,
                 id_token, id_head, 0, 0, T, heads, R, block_table.shape[1], max_new, -1 if window is None else window,
                 sinks, count, dim ** -0.5 if scale is None else scale]
-        key = (on.index, call, dim, max_new * heads > 16 * kv_heads)
+        key = (on.index, retrieved, c[40:], heads, max_new, block_table.shape[1], window, sinks, count, args[-1] > 0)
         need = _workspace.get(key)
         if need is None:
             size = ctypes.c_uint64()
-            rc = _call("fg_attention_workspace_bytes", ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p)(
-                c, _ARGS.pack(*args), ctypes.addressof(size))
+            rc = _call("fg_attention_workspace_bytes", ctypes.c_char_p, ctypes.c_char_p, ctypes.c_int32,
+                       ctypes.c_void_p)(c, _ARGS.pack(*args), retrieved, ctypes.addressof(size))
             if rc != FG_OK:
-                _raise(rc, call)
+                _raise(rc, "fg_attention_workspace_bytes")
+            if len(_workspace) > 1000:  # table widths that never come back
+                _workspace.clear()
             need = _workspace[key] = size.value
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        args[14], args[15] = work.data_ptr(), need
+        if need:
+            work = torch.empty(need, dtype=torch.uint8, device=q.device)
+            args[14], args[15] = work.data_ptr(), need
+        call = "fg_retrieved_attention_device" if retrieved else "fg_paged_attention_device"
         rc = _call(call, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_void_p)(c, _ARGS.pack(*args), on.handle)
         if rc != FG_OK:
             _raise(rc, call)
@@ -257,8 +261,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     stay visible.  scale: default dim ** -0.5.  Returns out [T, heads, dim],
     with return_lse also the rows' log-sum-exp float32 [T, heads]; a row that
     sees nothing is 0 and -inf."""
-    return _attend("fg_paged_attention_device", q, k_cache, v_cache, block_table, query_start, kv_len, max_new, None,
-                   window, sinks, scale, out, return_lse, stream)
+    return _attend(False, q, k_cache, v_cache, block_table, query_start, kv_len, max_new, None, window, sinks, scale,
+                   out, return_lse, stream)
 
 
 def retrieved_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -270,5 +274,5 @@ def retrieved_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     of the request's context, in any order, as a search over its keys returns
     them (uint32 ids as int32 bits; negative, repeated, already visible and
     future ones count nothing)."""
-    return _attend("fg_retrieved_attention_device", q, k_cache, v_cache, block_table, query_start, kv_len, 1, ids,
-                   window, sinks, scale, out, return_lse, stream)
+    return _attend(True, q, k_cache, v_cache, block_table, query_start, kv_len, 1, ids, window, sinks, scale, out,
+                   return_lse, stream)

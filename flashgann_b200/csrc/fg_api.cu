@@ -862,6 +862,25 @@ bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
     return !retrieved && many_rows(c, x) && x->scale > 0.f && c->page_size >= 8;
 }
 
+int workspace_bytes(const fg_kv_cache* c, const fg_attention* x, bool retrieved, uint64_t* bytes) {
+    int sms = 0;
+    const int rc = sm_count(&sms);
+    if (rc) return rc;
+    if (takes_tiles(c, x, retrieved)) {
+        *bytes = fg::attention_tiles_workspace(sms, c->dim);
+        return FG_OK;
+    }
+    fg::AttentionParams a;  // what decides whether tiles are split
+    a.table_width = x->table_width;
+    a.page_size = c->page_size;
+    a.window = x->window;
+    a.sinks = x->sinks;
+    a.group = x->heads / c->heads;
+    a.ids_count = retrieved ? x->ids_count : 0;
+    *bytes = fg::attention_rows_workspace(a, sms, c->dim);
+    return FG_OK;
+}
+
 int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void* stream) {
     int rc = check_cache(c);
     if (rc) return rc;
@@ -891,10 +910,10 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     if (!x->query_start || !x->kv_len || (!x->block_table && x->table_width > 0) || (retrieved && !x->ids && x->ids_count))
         return fail(FG_ERR_ARG, "null buffer");
     if (x->table_stride < 0) return fail(FG_ERR_ARG, "negative table stride");
-    if (!x->workspace || (reinterpret_cast<uintptr_t>(x->workspace) & 255))
-        return fail(FG_ERR_ARG, "workspace is null or not 256-byte aligned");
     uint64_t need = 0;
-    if ((rc = fg_attention_workspace_bytes(c, x, &need))) return rc;
+    if ((rc = workspace_bytes(c, x, retrieved, &need))) return rc;
+    if (need && (!x->workspace || (reinterpret_cast<uintptr_t>(x->workspace) & 255)))
+        return fail(FG_ERR_ARG, "workspace is null or not 256-byte aligned");
     if (x->workspace_bytes < need)
         return fail(FG_ERR_ARG, "workspace of %llu bytes, %llu needed", (unsigned long long)x->workspace_bytes,
                     (unsigned long long)need);
@@ -938,7 +957,7 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
         a.ids_token_stride = x->ids_token_stride;
         a.ids_head_stride = x->ids_head_stride;
     }
-    a.workspace = x->workspace;
+    a.workspace = need ? x->workspace : nullptr;
     if ((rc = sm_count(&a.ctas))) return rc;
     const cudaError_t e = takes_tiles(c, x, retrieved) ? fg::launch_attention_tiles(a, static_cast<cudaStream_t>(stream))
                                                        : fg::launch_attention_rows(a, static_cast<cudaStream_t>(stream));
@@ -1019,18 +1038,14 @@ int fg_kv_append_device(const fg_kv_cache* cache, const void* d_k, int64_t k_tok
     return e == cudaSuccess ? FG_OK : cuda_fail(e, "append launch");
 }
 
-int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* args, uint64_t* bytes) {
+int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* args, int32_t retrieved, uint64_t* bytes) {
     g_err.clear();
     int rc = check_cache(cache);
     if (rc) return rc;
     if (!args || !bytes) return fail(FG_ERR_ARG, "null argument");
-    int sms = 0;
-    if ((rc = sm_count(&sms))) return rc;
     if (args->heads < 1 || args->heads % cache->heads)
         return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", args->heads, cache->heads);
-    // by the number of rows alone: what else decides between the kernels must not change the answer for like calls
-    *bytes = many_rows(cache, args) ? fg::attention_tiles_workspace(sms, cache->dim) : fg::attention_rows_workspace(sms, cache->dim);
-    return FG_OK;
+    return workspace_bytes(cache, args, retrieved != 0, bytes);
 }
 
 int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {

@@ -27,13 +27,26 @@
 // repeated) and leave the rest in shared memory, see stage_ids.
 //
 // Tiles that are short whatever the lengths are (a narrow table, or a window and
-// a few ids: up to kShort chunks, a bound that the host knows) are not split:
+// a few ids, see attention_rows_splits) are not split:
 // there are no partials and no second kernel, which costs more than it saves.
 #include <algorithm>
 
 #include "fg_attention.cuh"
 
 namespace fg {
+
+// Whether tiles may be split over CTAs.  The host knows how many chunks no tile has more of: from the table's width, or
+// from the window, the first tokens and the ids.
+bool attention_rows_splits(const AttentionParams& a) {
+    constexpr int kRows = 16, kChunk = 16;
+    constexpr int kShort = 64;  // chunks of a tile that is not split
+    int64_t keys = static_cast<int64_t>(a.table_width) * a.page_size;
+    if (a.window >= 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + kRows + a.sinks);
+    int64_t chunks = keys / kChunk + 3;
+    chunks += static_cast<int64_t>(std::min(a.group, kRows)) * ((a.ids_count + kChunk - 1) / kChunk);
+    return chunks > kShort;
+}
+
 namespace attn {
 namespace {
 
@@ -42,7 +55,6 @@ constexpr int kChunk = 16;
 constexpr int kWarps = 4;
 constexpr int kCtasPerSm = 2;
 constexpr int kThreads = kWarps * 32;
-constexpr int kShort = 64;       // chunks of a tile that is not split
 constexpr int kMaxIds = 1024;    // ids of a tile's heads, in shared memory
 constexpr int kTable = 2048;     // places of the hash table over them
 
@@ -486,7 +498,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
     __syncthreads();  // the rings overlay the scan
     if (pl.unit >= pl.end) {
-        if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
+        if (threadIdx.x == 0 && ws) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
         return;
     }
 
@@ -495,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     int64_t unit = pl.unit, tile_first = pl.unit - pl.offset;
     w.req = load_request(a, request);
     w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk>(a, w.req, tile);
-    if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = tile_record(a, pl, blockIdx.x, w.req, w.keys.units);
+    if (threadIdx.x == 0 && ws) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = tile_record(a, pl, blockIdx.x, w.req, w.keys.units);
     if (kIds) w.read_ids(w.req, head, tile);
     bool first_segment = true;
     while (true) {
@@ -646,22 +658,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     }
 }
 
-// Chunks that no tile has more of, as far as the host can tell.
-int64_t most_chunks(const AttentionParams& a) {
-    int64_t keys = static_cast<int64_t>(a.table_width) * a.page_size;
-    if (a.window >= 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + kRows + a.sinks);
-    int64_t chunks = keys / kChunk + 3;
-    if (a.ids) chunks += static_cast<int64_t>(std::min(a.group, kRows)) * ((a.ids_count + kChunk - 1) / kChunk);
-    return chunks;
-}
-
 template <typename T, int kDim, bool kIds>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = kIds ? Smem<kDim>::kBytesIds : Smem<kDim>::kBytes;
     static_assert((bytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
     a.base_align = kChunk;
     if (kIds) a.tile_rows = std::min(kRows, kMaxIds / Warp<T, kDim, kIds>::staged_pitch(a.ids_count));
-    const bool split = most_chunks(a) > kShort;
+    const bool split = attention_rows_splits(a);
     a.ctas *= kCtasPerSm;
     a.unit_shift = split ? 2 : 24;  // a unit: one chunk for each warp, or a tile
     static SmemOnce once;
@@ -688,7 +691,8 @@ cudaError_t by_dim(const AttentionParams& a, cudaStream_t s) {
 }  // namespace
 }  // namespace attn
 
-size_t attention_rows_workspace(int sms, int dim) {
+size_t attention_rows_workspace(const AttentionParams& a, int sms, int dim) {
+    if (!attention_rows_splits(a)) return 0;
     const int ctas = sms * attn::kCtasPerSm;
     return attn::workspace_records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * attn::partial_floats(attn::kRows, dim) * sizeof(float);
 }

@@ -143,7 +143,8 @@ struct AttentionParams {
 };
 int attention_max_requests();
 int attention_max_ids();
-size_t attention_rows_workspace(int sms, int dim);
+bool attention_rows_splits(const AttentionParams& a);
+size_t attention_rows_workspace(const AttentionParams& a, int sms, int dim);  // 0 where nothing is split
 cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream);
 size_t attention_tiles_workspace(int sms, int dim);
 cudaError_t launch_attention_tiles(const AttentionParams& a, cudaStream_t stream);

@@ -26,7 +26,7 @@ namespace {
 // memory, and then maps its own share of tokens and pages back to requests by
 // bisection.  A fresh page is taken from the free list by index, never read
 // back from the table that another thread may be writing.
-constexpr int kPlanThreads = 256;
+constexpr int kPlanThreads = 512;
 
 struct Need {
     int64_t pages;  // fresh pages, 0 for a request that is too long for the table
@@ -60,6 +60,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
     extern __shared__ int64_t plan_smem[];
     int64_t* page_end = plan_smem;                // inclusive sum of need
     int64_t* token_end = page_end + a.requests;   // inclusive sum of new
+    int32_t* ctx_of = reinterpret_cast<int32_t*>(token_end + a.requests);
     __shared__ int64_t warp_pages[kPlanThreads / 32], warp_tokens[kPlanThreads / 32];
     __shared__ unsigned long long taken;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -67,12 +68,14 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
     const int b0 = min(tid * per, a.requests), b1 = min(b0 + per, a.requests);
     if (tid == 0) taken = 0;
     int64_t pages = 0, tokens = 0;
+#pragma unroll 4
     for (int b = b0; b < b1; ++b) {
-        const int64_t ctx = max(0, a.ctx_len[b]), add = max(0, a.new_len[b]);
+        const int64_t ctx = max(0, __ldg(a.ctx_len + b)), add = max(0, __ldg(a.new_len + b));
         pages += page_need(a, ctx, add).pages;
         tokens += add;
         page_end[b] = pages;
         token_end[b] = tokens;
+        ctx_of[b] = static_cast<int32_t>(ctx);
     }
     int64_t sp = pages, st = tokens;
 #pragma unroll
@@ -96,11 +99,12 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
     const int64_t head = a.free_head ? max(0, *a.free_head) : 0;
     const int64_t room = max(static_cast<int64_t>(0), a.free_count - head);
     const bool writes = blockIdx.x == 0;  // the outputs for each request
-    int64_t last = 0;
+    int64_t last = 0, tokens_before = bt;
     for (int b = b0; b < b1; ++b) {
         const int64_t pe = page_end[b] += bp, te = token_end[b] += bt;
         if (!writes) continue;
-        const int64_t ctx = max(0, a.ctx_len[b]), add = max(0, a.new_len[b]);
+        const int64_t ctx = ctx_of[b], add = te - tokens_before;
+        tokens_before = te;
         const Need n = page_need(a, ctx, add);
         const bool refused = n.wide || (n.pages > 0 && pe > room);
         if (!refused && n.pages > 0) last = pe;  // the admitted ones are a prefix of those that need pages
@@ -122,7 +126,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
         int64_t slot = -1;
         if (t < all_tokens) {
             const int b = owner(token_end, a.requests, t);
-            const int64_t ctx = max(0, a.ctx_len[b]), add = max(0, a.new_len[b]);
+            const int64_t ctx = ctx_of[b], add = token_end[b] - (b ? token_end[b - 1] : 0);
             const Need n = page_need(a, ctx, add);
             if (!(n.wide || (n.pages > 0 && page_end[b] > room))) {
                 const int64_t p = ctx + t - (token_end[b] - add);
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
     for (int64_t x = first; x < all_pages; x += threads) {
         const int b = owner(page_end, a.requests, x);
         if (page_end[b] > room) continue;  // the pool ends inside this request: it is refused whole
-        const int64_t ctx = max(0, a.ctx_len[b]), add = max(0, a.new_len[b]);
+        const int64_t ctx = ctx_of[b], add = token_end[b] - (b ? token_end[b - 1] : 0);
         const Need n = page_need(a, ctx, add);
         a.block_table[b * a.table_stride + n.had + x - (page_end[b] - n.pages)] = a.free_pages[head + x];
     }
@@ -187,10 +191,10 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendA
 
 }  // namespace
 
-int kv_plan_max_requests() { return 8192; }  // two 8-byte prefixes of each in one CTA's shared memory
+int kv_plan_max_requests() { return 8192; }  // 20 bytes of each in one CTA's shared memory
 
 cudaError_t launch_kv_plan(const PlanArgs& a, cudaStream_t stream) {
-    const size_t smem = static_cast<size_t>(a.requests) * 2 * sizeof(int64_t);
+    const size_t smem = static_cast<size_t>(a.requests) * (2 * sizeof(int64_t) + sizeof(int32_t));
     if (smem > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return e;

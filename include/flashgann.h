@@ -316,7 +316,8 @@ typedef struct fg_attention {
     const int32_t* kv_len;                      /* [requests], new tokens included */
     const int32_t* ids;                         /* fg_retrieved_attention_device: [tokens, heads, ids_count] */
     int64_t ids_token_stride, ids_head_stride;
-    void* workspace;                            /* fg_attention_workspace_bytes, 256-byte aligned; contents do not matter */
+    void* workspace;                            /* fg_attention_workspace_bytes, 256-byte aligned; contents do not matter;
+                                                 * NULL where 0 bytes are needed */
     uint64_t workspace_bytes;
     int32_t tokens, heads, requests, table_width;
     int32_t max_new;                            /* most new tokens of a request: picks the kernel, not the result */
@@ -326,9 +327,13 @@ typedef struct fg_attention {
     float scale;
 } fg_attention;
 
-/* Bytes of workspace that an attention call needs on the current device
- * (partial results of rows whose keys are split over CTAs). */
-int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* args, uint64_t* bytes);
+/* Bytes of workspace that a call needs on the current device, for partial
+ * results of rows whose keys are split over CTAs (0: none, where no row can
+ * have many keys).  retrieved: 1 for fg_retrieved_attention_device.  Depends
+ * on args' heads, max_new, table_width, window, sinks, ids_count and scale
+ * only, on no pointer. */
+int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* args, int32_t retrieved,
+                                 uint64_t* bytes);
 
 /* Causal attention of a batch's new tokens over the cache.  Token i of
  * request b (row query_start[b] + i) stands at p = kv_len[b] - new_b + i and

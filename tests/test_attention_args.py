@@ -38,7 +38,7 @@ ARGS = [(dict(tokens=-1), "tokens=-1"), (dict(requests=-2), "requests=-2"), (dic
         (dict(scale=float("inf")), "scale"), (dict(q=None), "null q"), (dict(q=PTR + 2), "q is not"),
         (dict(q_head_stride=68), "strides of q"), (dict(out=None), "null out"), (dict(out_token_stride=-8), "negative"),
         (dict(query_start=None), "null buffer"), (dict(kv_len=None), "null buffer"), (dict(block_table=None), "null"),
-        (dict(workspace=None), "workspace"), (dict(workspace=PTR + 16), "workspace"), (dict(table_stride=-1), "table")]
+        (dict(table_stride=-1), "table")]
 IDS = [(dict(window=-1), "window"), (dict(ids_count=-1), "count -1"), (dict(ids=None), "null"),
        (dict(ids_head_stride=-10), "negative"), (dict(ids_count=70000), "70000 ids")]
 
@@ -74,7 +74,7 @@ def test_null_structs_and_empty_calls():
     L = fg.lib()
     assert L.fg_paged_attention_device(None, _args(), None) == fg.FG_ERR_ARG
     assert L.fg_paged_attention_device(_cache(), None, None) == fg.FG_ERR_ARG
-    assert L.fg_attention_workspace_bytes(None, None, None) == fg.FG_ERR_ARG
+    assert L.fg_attention_workspace_bytes(None, None, 0, None) == fg.FG_ERR_ARG
     # nothing to do: no device is needed
     assert L.fg_paged_attention_device(_cache(), _args(tokens=0, workspace=None), None) == fg.FG_OK
     assert L.fg_retrieved_attention_device(_cache(), _args(requests=0, workspace=None), None) == fg.FG_OK
