@@ -353,17 +353,15 @@ struct SmemOnce {
 };
 
 // Joins the partials of every tile that two or more CTAs of the main kernel
-// shared, by the records that those left; a warp joins a row, a lane 4 columns
-// of it.  The maximum first, a partial to a lane, then the sums with 8 partials'
-// loads under way.  Little data (at most 2 partials for each main CTA) and a
-// chain of three loads; launched as a dependent of the main kernel so that its
-// start overlaps the main kernel's tail.
-constexpr int kJoinRows = 8;
-
-template <typename T, int kRows, int kDim, Layout kLayout>
-__global__ void __launch_bounds__(kJoinRows * 32) attention_combine_kernel(const AttentionParams a) {
+// shared, by the records that those left; a warp joins kJoin rows, a lane 4
+// columns of them.  The maxima first, then the sums, with the loads of 8 rows
+// of partials under way together.  Launched as a dependent of the main kernel
+// so that its start overlaps the main kernel's tail.
+template <typename T, int kRows, int kDim, Layout kLayout, int kJoin>
+__global__ void __launch_bounds__(256) attention_combine_kernel(const AttentionParams a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    constexpr int kBlocks = kRows / kJoinRows;
+    constexpr int kBlocks = kRows / (8 * kJoin);
+    constexpr int kAhead = 8 / kJoin;  // partials under way
     const char* ws = static_cast<const char*>(a.workspace);
     const int c = blockIdx.x / kBlocks + 1;
     const TileRecord rec = reinterpret_cast<const TileRecord*>(ws)[c];
@@ -371,73 +369,91 @@ __global__ void __launch_bounds__(kJoinRows * 32) attention_combine_kernel(const
     const float* partials = reinterpret_cast<const float*>(ws + workspace_records_bytes(a.ctas));
     constexpr size_t kPartial = static_cast<size_t>(kRows) * (kDim + 2);
     const auto partial = [&](int x) { return partials + (x == 0 ? rec.before : 2 * (c - 1 + x)) * kPartial; };
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = (blockIdx.x % kBlocks) * kJoinRows + warp;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane * 4;
+    const int row = ((blockIdx.x % kBlocks) * 8 + warp) * kJoin;
     const Request r = {rec.start, rec.rows, 0};
-    int i, g;
-    if (!Tiles<kRows, kLayout>::row(a, r, rec.tile, row, &i, &g)) return;
-    float m = -INFINITY;
-    bool nan = false;  // a row that holds NaN, or left by a main kernel that gave up
-    for (int x = lane; x < rec.parts; x += 32) {
-        const float v = partial(x)[kRows * kDim + row];
-        m = fmaxf(m, v);
-        nan = nan || v != v;
-    }
+    int i[kJoin], g[kJoin];
+    bool valid[kJoin];
+    float m[kJoin], ref[kJoin], l[kJoin];
+    float4 o[kJoin];
 #pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    const float ref = __any_sync(0xFFFFFFFFu, nan) ? NAN : m == -INFINITY ? 0.f : m;
-    const int d = lane * 4;
-    float l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int x0 = 0; x0 < rec.parts; x0 += 8) {
+    for (int y = 0; y < kJoin; ++y) {
+        valid[y] = Tiles<kRows, kLayout>::row(a, r, rec.tile, row + y, &i[y], &g[y]);
+        m[y] = -INFINITY;
+        l[y] = 0.f;
+        o[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (!valid[0]) return;  // rows past the tile's end come last
+    bool nan[kJoin] = {};   // a row that holds NaN, or left by a main kernel that gave up
+    for (int x = lane; x < rec.parts; x += 32)
+#pragma unroll
+        for (int y = 0; y < kJoin; ++y) {
+            const float v = valid[y] ? partial(x)[kRows * kDim + row + y] : 0.f;
+            m[y] = fmaxf(m[y], v);
+            nan[y] = nan[y] || v != v;
+        }
+#pragma unroll
+    for (int y = 0; y < kJoin; ++y) {
+#pragma unroll
+        for (int b = 16; b; b >>= 1) m[y] = fmaxf(m[y], __shfl_xor_sync(0xFFFFFFFFu, m[y], b));
+        ref[y] = __any_sync(0xFFFFFFFFu, nan[y]) ? NAN : m[y] == -INFINITY ? 0.f : m[y];
+    }
+    for (int x0 = 0; x0 < rec.parts; x0 += kAhead) {
         float pm[8], pl[8];
         float4 q[8];
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-            pm[y] = -INFINITY;
-            pl[y] = 0.f;
-            q[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (x0 + y < rec.parts) {
-                const float* p = partial(x0 + y);
-                pm[y] = p[kRows * kDim + row];
-                pl[y] = p[kRows * kDim + kRows + row];
-                if (d < kDim) q[y] = *reinterpret_cast<const float4*>(p + row * kDim + d);
+        for (int z = 0; z < 8; ++z) {
+            const int x = x0 + z / kJoin, y = z % kJoin;
+            pm[z] = -INFINITY;
+            pl[z] = 0.f;
+            q[z] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (x < rec.parts && valid[y]) {
+                const float* p = partial(x);
+                pm[z] = p[kRows * kDim + row + y];
+                pl[z] = p[kRows * kDim + kRows + row + y];
+                if (d < kDim) q[z] = *reinterpret_cast<const float4*>(p + (row + y) * kDim + d);
             }
         }
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-            const float f = exp2_fast(pm[y] - ref);
-            l += pl[y] * f;
-            o.x += q[y].x * f;
-            o.y += q[y].y * f;
-            o.z += q[y].z * f;
-            o.w += q[y].w * f;
+        for (int z = 0; z < 8; ++z) {
+            const int y = z % kJoin;
+            const float f = exp2_fast(pm[z] - ref[y]);
+            l[y] += pl[z] * f;
+            o[y].x += q[z].x * f;
+            o[y].y += q[z].y * f;
+            o[y].z += q[z].z * f;
+            o[y].w += q[z].w * f;
         }
     }
-    const float inv = l == 0.f ? 1.f : 1.f / l;
-    const int64_t token = r.start + i;
-    const int head = rec.head * a.group + g;
-    if (d < kDim) {
-        T* out = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride + d;
-        *reinterpret_cast<uint2*>(out) = make_uint2(Half2<T>::pack(o.x * inv, o.y * inv), Half2<T>::pack(o.z * inv, o.w * inv));
+#pragma unroll
+    for (int y = 0; y < kJoin; ++y) {
+        if (!valid[y]) continue;
+        const float inv = l[y] == 0.f ? 1.f : 1.f / l[y];
+        const int64_t token = r.start + i[y];
+        const int head = rec.head * a.group + g[y];
+        if (d < kDim) {
+            T* out = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride + d;
+            *reinterpret_cast<uint2*>(out) =
+                make_uint2(Half2<T>::pack(o[y].x * inv, o[y].y * inv), Half2<T>::pack(o[y].z * inv, o[y].w * inv));
+        }
+        if (lane == 0 && a.lse) a.lse[token * a.heads + head] = l[y] == 0.f ? -INFINITY : (ref[y] + log2f(l[y])) * kLn2;
     }
-    if (lane == 0 && a.lse) a.lse[token * a.heads + head] = l == 0.f ? -INFINITY : (ref + log2f(l)) * kLn2;
 }
 
 // After a main kernel that may have left partials; the main kernel lets it start early.
-template <typename T, int kRows, int kDim, Layout kLayout>
+template <typename T, int kRows, int kDim, Layout kLayout, int kJoin>
 cudaError_t launch_combine(const AttentionParams& a, cudaStream_t stream) {
     if (a.ctas < 2) return cudaSuccess;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>((a.ctas - 1) * (kRows / kJoinRows)));
-    cfg.blockDim = dim3(kJoinRows * 32);
+    cfg.gridDim = dim3(static_cast<unsigned>((a.ctas - 1) * (kRows / (8 * kJoin))));
+    cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_combine_kernel<T, kRows, kDim, kLayout>, a);
+    return cudaLaunchKernelEx(&cfg, attention_combine_kernel<T, kRows, kDim, kLayout, kJoin>, a);
 }
 
 }  // namespace attn

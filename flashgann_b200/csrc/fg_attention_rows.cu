@@ -672,7 +672,7 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     attention_rows_kernel<T, kDim, kIds><<<a.ctas, kThreads, bytes, stream>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess || !split) return e;
-    return launch_combine<T, kRows, kDim, kIds ? kToken : kPacked>(a, stream);
+    return launch_combine<T, kRows, kDim, kIds ? kToken : kPacked, 1>(a, stream);
 }
 
 template <typename T, int kDim>

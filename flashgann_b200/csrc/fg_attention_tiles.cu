@@ -943,7 +943,7 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
         return cudaErrorInvalidValue;
     attention_tiles_kernel<T, kDim><<<a.ctas, kThreads, bytes, stream>>>(a, q_map, k_map, v_map, box_shift);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return launch_combine<T, kRows, kDim, kTokens>(a, stream);
+    return launch_combine<T, kRows, kDim, kTokens, 4>(a, stream);
 }
 
 template <typename T>

@@ -152,41 +152,28 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
 // ---- append ----
 //
 // A copy of tokens * heads rows of K and of V: 2 * 2 bytes of traffic for each
-// element, nothing else.  A thread moves kUnroll 16-byte pieces of each, all
-// loads before the first store; consecutive threads take consecutive pieces of
-// a row, so that a row is whole 128-byte lines on both sides.
+// element, nothing else.  A thread moves one 16-byte piece of each; consecutive
+// threads take consecutive pieces of a row, so that a row is whole 128-byte
+// lines on both sides.  (2, 4 and 8 pieces to a thread: 1, 11 and 48 % slower
+// for 16001 tokens of 4 x 96; what hides the latency is the number of CTAs.)
 constexpr int kAppendThreads = 256;
 
-template <int kUnroll>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendArgs a) {
     const int64_t slots = static_cast<int64_t>(a.pages) << a.page_shift;
     const uint32_t per = static_cast<uint32_t>(a.heads) * a.pieces;  // pieces of a token
     const int64_t total = static_cast<int64_t>(a.tokens) * per;
-    const int64_t base = static_cast<int64_t>(blockIdx.x) * kAppendThreads * kUnroll + threadIdx.x;
-    uint4 kv[kUnroll], vv[kUnroll];
-    int64_t to[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const int64_t idx = base + u * kAppendThreads;
-        to[u] = -1;
-        if (idx >= total) continue;
-        // a token's pieces are far below 2^32, so one 64-bit division at most
-        const int64_t t = total <= UINT32_MAX ? static_cast<uint32_t>(idx) / per : idx / per;
-        const uint32_t rest = static_cast<uint32_t>(idx - t * per);
-        const uint32_t h = rest / a.pieces, p = rest % a.pieces;
-        const int64_t slot = a.slot[t];
-        kv[u] = __ldg(static_cast<const uint4*>(a.k) + t * a.k_token_stride + h * a.k_head_stride + p);
-        vv[u] = __ldg(static_cast<const uint4*>(a.v) + t * a.v_token_stride + h * a.v_head_stride + p);
-        if (slot >= 0 && slot < slots)
-            to[u] = (slot >> a.page_shift) * a.page_stride + (slot & ((1 << a.page_shift) - 1)) * a.token_stride +
-                    h * a.head_stride + p;
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        if (to[u] < 0) continue;
-        static_cast<uint4*>(a.k_cache)[to[u]] = kv[u];
-        static_cast<uint4*>(a.v_cache)[to[u]] = vv[u];
-    }
+    const int64_t idx = static_cast<int64_t>(blockIdx.x) * kAppendThreads + threadIdx.x;
+    if (idx >= total) return;
+    const int64_t t = total <= UINT32_MAX ? static_cast<uint32_t>(idx) / per : idx / per;
+    const uint32_t rest = static_cast<uint32_t>(idx - t * per);
+    const uint32_t h = rest / a.pieces, p = rest % a.pieces;
+    const int64_t slot = __ldg(a.slot + t);
+    const uint4 k = __ldg(static_cast<const uint4*>(a.k) + t * a.k_token_stride + h * a.k_head_stride + p);
+    const uint4 v = __ldg(static_cast<const uint4*>(a.v) + t * a.v_token_stride + h * a.v_head_stride + p);
+    if (slot < 0 || slot >= slots) return;
+    const int64_t to = (slot >> a.page_shift) * a.page_stride + (slot & ((1 << a.page_shift) - 1)) * a.token_stride + h * a.head_stride + p;
+    static_cast<uint4*>(a.k_cache)[to] = k;
+    static_cast<uint4*>(a.v_cache)[to] = v;
 }
 
 }  // namespace
@@ -208,13 +195,9 @@ cudaError_t launch_kv_plan(const PlanArgs& a, cudaStream_t stream) {
 
 cudaError_t launch_kv_append(const AppendArgs& a, cudaStream_t stream) {
     const int64_t total = static_cast<int64_t>(a.tokens) * a.heads * a.pieces;
-    if (total <= 148ll * 4 * kAppendThreads) {  // few pieces: one each, for the shortest chain
-        const int64_t grid = (total + kAppendThreads - 1) / kAppendThreads;
-        kv_append_kernel<1><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(a);
-    } else {
-        const int64_t grid = (total + 4 * kAppendThreads - 1) / (4 * kAppendThreads);
-        kv_append_kernel<4><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(a);
-    }
+    const int64_t grid = (total + kAppendThreads - 1) / kAppendThreads;
+    if (grid > INT32_MAX) return cudaErrorInvalidConfiguration;
+    kv_append_kernel<<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
