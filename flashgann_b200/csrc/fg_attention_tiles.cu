@@ -632,6 +632,24 @@ struct Softmax {
         }
     }
 
+    // Piece k of quad thread j becomes piece j of thread k.
+    __device__ static __forceinline__ void exchange(uint4 (&v)[4], int mate) {
+#pragma unroll
+        for (int bit = 1; bit < 4; bit <<= 1)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (k & bit) continue;
+                const bool high = mate & bit;  // gives the lower of the two pieces and keeps the upper
+                uint4 give = high ? v[k] : v[k + bit];
+                give.x = __shfl_xor_sync(0xFFFFFFFFu, give.x, bit);
+                give.y = __shfl_xor_sync(0xFFFFFFFFu, give.y, bit);
+                give.z = __shfl_xor_sync(0xFFFFFFFFu, give.z, bit);
+                give.w = __shfl_xor_sync(0xFFFFFFFFu, give.w, bit);
+                if (high) v[k] = give;
+                else v[k + bit] = give;
+            }
+    }
+
     // The segment's end: this thread's row of O to the output or, for part of a tile, to the workspace.
     __device__ __forceinline__ bool store(const Walk& w, bool ok) {
         if (ok) ok = bar_wait(&sh->pv_done[half], (settled - 1) & 1, sh);
@@ -644,23 +662,48 @@ struct Softmax {
         float* part = reinterpret_cast<float*>(ws + workspace_records_bytes(a.ctas)) +
                       (2 * static_cast<size_t>(blockIdx.x) + (w.opening ? 0 : 1)) * partial_floats(kRows, kDim);
         const float inv = !ok ? NAN : l == 0.f ? 1.f : 1.f / l;
-        T* out = static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride;
+        // A row lies in one thread; the four threads of a quad exchange 16-byte pieces, so that each of them writes
+        // every fourth piece of each other's rows and a store is 64 contiguous bytes of 8 rows, not 16 of 32.
+        const int lane = threadIdx.x & 31, mate = lane & 3;
+        char* to[4];  // the quad's rows, null where there is none
+        {
+            char* mine = nullptr;
+            if (valid)
+                mine = w.whole ? reinterpret_cast<char*>(static_cast<T*>(a.out) + token * a.out_token_stride + head * a.out_head_stride)
+                               : reinterpret_cast<char*>(part + row * kDim);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                to[k] = reinterpret_cast<char*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(mine), (lane & ~3) + k));
+        }
 #pragma unroll 1
         for (int d = 0; d < kDim; d += 32) {
             float o[32];
             tmem_load32(output + d, o);
             tmem_load_wait();
-            if (!valid) continue;
             if (w.whole) {
+                uint4 v[4];
 #pragma unroll
-                for (int x = 0; x < 32; x += 8)
-                    *reinterpret_cast<uint4*>(out + d + x) =
-                        make_uint4(Half2<T>::pack(o[x] * inv, o[x + 1] * inv), Half2<T>::pack(o[x + 2] * inv, o[x + 3] * inv),
-                                   Half2<T>::pack(o[x + 4] * inv, o[x + 5] * inv), Half2<T>::pack(o[x + 6] * inv, o[x + 7] * inv));
+                for (int x = 0; x < 4; ++x)
+                    v[x] = make_uint4(Half2<T>::pack(o[8 * x] * inv, o[8 * x + 1] * inv), Half2<T>::pack(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
+                                      Half2<T>::pack(o[8 * x + 4] * inv, o[8 * x + 5] * inv),
+                                      Half2<T>::pack(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+                exchange(v, mate);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (to[k]) *reinterpret_cast<uint4*>(to[k] + d * 2 + mate * 16) = v[k];
             } else {
 #pragma unroll
-                for (int x = 0; x < 32; x += 4)
-                    *reinterpret_cast<float4*>(part + row * kDim + d + x) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+                for (int y = 0; y < 32; y += 16) {
+                    uint4 v[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        v[x] = make_uint4(__float_as_uint(o[y + 4 * x]), __float_as_uint(o[y + 4 * x + 1]), __float_as_uint(o[y + 4 * x + 2]),
+                                          __float_as_uint(o[y + 4 * x + 3]));
+                    exchange(v, mate);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (to[k]) *reinterpret_cast<uint4*>(to[k] + (d + y) * 4 + mate * 16) = v[k];
+                }
             }
         }
         if (valid && w.whole) {
