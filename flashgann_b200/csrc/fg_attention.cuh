@@ -16,7 +16,9 @@
 // of magnitude (one short decode beside a chunk over a long context), so the
 // unit of work is not the tile but 2^unit_shift chunks of keys of one tile.
 // All units are numbered in tile order and CTA c of P takes the contiguous
-// range [c*W/P, (c+1)*W/P) of the W units: every CTA gets the same amount of
+// range [c*W/P, (c+1)*W/P) of the W units.  A tile begins with `tile_units`
+// units without chunks, for what a CTA spends on any tile (queries, join,
+// output); a range that ends in them ends before the tile.  So every CTA gets the same amount of
 // key traffic to within one unit whatever the lengths, and at most its first
 // and its last tile are shared with a neighbour.  Those go to the workspace as
 // partial (o, m, l), which attention_combine_kernel joins in unit order: no
@@ -148,7 +150,8 @@ __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Re
         k.id_chunks = heads * ((a.ids_count + kChunk - 1) / kChunk);
     }
     k.chunks = k.sink_chunks + k.near_chunks + k.id_chunks;
-    k.units = max(1, (k.chunks + (1 << a.unit_shift) - 1) >> a.unit_shift);  // a tile that sees nothing still writes its rows
+    // a tile that sees nothing still writes its rows
+    k.units = a.tile_units + max(1, (k.chunks + (1 << a.unit_shift) - 1) >> a.unit_shift);
     return k;
 }
 
@@ -278,12 +281,12 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
 __device__ __forceinline__ TileRecord tile_record(const AttentionParams& a, const Place& x, int c, const Request& r, int units) {
     TileRecord rec = {};
     const int64_t first = x.unit - x.offset, last = first + units;
-    if (c == 0 || x.unit >= x.end || x.offset == 0) return rec;
+    if (c == 0 || x.unit >= x.end || x.offset <= a.tile_units) return rec;
     const int64_t before = share(x.total, c - 1, x.ctas);  // where the CTA before starts
-    if (before > first) return rec;                     // an earlier CTA's range starts inside the tile too
+    if (before > first + a.tile_units) return rec;      // an earlier CTA's range starts inside the tile too
     const int end = static_cast<int>((last * x.ctas - 1) / x.total);  // the CTA whose range holds the tile's last unit
     rec.parts = end - c + 2;
-    rec.before = 2 * (c - 1) + (before == first ? 0 : 1);  // its second segment unless its range starts with this tile
+    rec.before = 2 * (c - 1) + (before >= first ? 0 : 1);  // its second segment unless its range starts with this tile
     rec.head = x.head;
     rec.tile = x.tile;
     rec.start = r.start;

@@ -512,8 +512,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     bool first_segment = true;
     while (true) {
         const int64_t tile_last = tile_first + w.keys.units;
-        const int u0 = static_cast<int>(unit - tile_first);
-        const int u1 = static_cast<int>(min(tile_last, pl.end) - tile_first);
+        const int u0 = max(0, static_cast<int>(unit - tile_first) - a.tile_units);
+        const int u1 = static_cast<int>(min(tile_last, pl.end) - tile_first) - a.tile_units;
+        if (u1 <= 0) break;  // the range ends before the tile's first chunk
         const int c1 = min(u1 << a.unit_shift, w.keys.chunks);
         w.begin(head, request, tile);
         const int window_end = w.keys.sink_chunks + w.keys.near_chunks;  // chunks from here on need the tile's ids
@@ -576,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         // the next tile's request and ids are read beside the join
         Request next_req = w.req;
         int next_head = head, next_request = request, next_number = tile;
-        const bool more = tile_first + u1 < pl.end && next_tile<kRows, kIds ? kToken : kPacked>(a, &next_req, &next_head, &next_request, &next_number);
+        const bool more = pl.end - tile_last > a.tile_units && next_tile<kRows, kIds ? kToken : kPacked>(a, &next_req, &next_head, &next_request, &next_number);
         if (kIds && more) w.read_ids(next_req, next_head, next_number);
 
         // join the warps: rows of (m, l) and sums, over the rings
@@ -603,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             }
         }
         __syncthreads();
-        const bool whole_tile = u0 == 0 && u1 == w.keys.units;
+        const bool whole_tile = u0 == 0 && u1 == w.keys.units - a.tile_units;
         float* part = nullptr;
         if (!whole_tile) {
             const size_t slot = 2 * static_cast<size_t>(blockIdx.x) + (first_segment ? 0 : 1);
@@ -667,6 +668,7 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     const bool split = attention_rows_splits(a);
     a.ctas *= kCtasPerSm;
     a.unit_shift = split ? 2 : 24;  // a unit: one chunk for each warp, or a tile
+    a.tile_units = split ? 2 : 0;   // a tile's start and end take about as long as two chunks of each warp
     static SmemOnce once;
     cudaError_t e = once.set(reinterpret_cast<const void*>(attention_rows_kernel<T, kDim, kIds>), bytes);
     if (e != cudaSuccess) return e;

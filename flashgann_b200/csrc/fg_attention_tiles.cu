@@ -46,6 +46,7 @@ constexpr int kHalf = 128;
 constexpr int kBlock = 128;  // keys
 constexpr int kThreads = 512;
 constexpr int kSlots = 5;    // see Loader::block; K and V tiles in the ring: two blocks and a half
+constexpr int kTileBlocks = 3;  // a tile costs about as much as that many blocks beside its own (1 to 4 measured)
 constexpr float kRaise = 8.f;
 constexpr int kPolyPairs = 1;  // of 8 pairs of weights, see exp2_poly
 
@@ -247,15 +248,15 @@ struct Walk {
         rows = (i1 - i0 + 1) * a.group;
         token = req.start + i0;
         const int64_t last = first + keys.units;
-        u0 = static_cast<int>(unit - first);
-        u1 = static_cast<int>(min(last, end) - first);
-        whole = u0 == 0 && u1 == keys.units;
+        u0 = max(0, static_cast<int>(unit - first) - a.tile_units);
+        u1 = static_cast<int>(min(last, end) - first) - a.tile_units;
+        whole = u0 == 0 && u1 == keys.units - a.tile_units;
         all = seen(p0, p1);
     }
     __device__ __forceinline__ bool next() {
-        unit = first + u1;
-        if (unit >= end) return false;
         first += keys.units;
+        unit = first;
+        if (end - first <= a.tile_units) return false;
         if (!next_tile<kRows, kTokens>(a, &req, &head, &request, &tile)) return false;
         opening = false;
         set();
@@ -736,6 +737,9 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
         if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
         return;
     }
+    Walk w(a, pl);
+    if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = tile_record(a, pl, blockIdx.x, w.req, w.keys.units);
+    if (w.u1 <= 0) return;  // the range ends before the tile's first block
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) {
             bar_init(&sh->full[i], 4);  // the four helper warps, or four times the loader
@@ -766,9 +770,6 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = sh->tmem;
-    Walk w(a, pl);
-    if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = tile_record(a, pl, blockIdx.x, w.req, w.keys.units);
-
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         Softmax<T, kDim> sm(a, sh, tmem, box_shift);
@@ -977,6 +978,7 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     const int box_shift = min(a.page_shift, a.window < 0 ? 7 : 6);
     a.base_align = 1 << box_shift;
     a.unit_shift = 0;
+    a.tile_units = kTileBlocks;
     const int64_t cache_size[3] = {a.page_size, a.kv_heads, a.pages}, cache_stride[3] = {a.token_stride, a.head_stride, a.page_stride};
     const int64_t q_size[3] = {a.heads, a.tokens, 1}, q_stride[3] = {a.q_head_stride, a.q_token_stride, 0};
     CUtensorMap q_map, k_map, v_map;

@@ -139,6 +139,7 @@ struct AttentionParams {
     int ctas = 0;           // CTAs that share the work (to the launchers: SMs)
     int base_align = 16;    // power of two that windows' key chunks start at multiples of
     int unit_shift = 0;     // log2 of the key chunks in a unit of work
+    int tile_units = 0;     // what a tile costs beside its chunks, in units
     int tile_rows = 16;     // retrieved form: heads to a tile
 };
 int attention_max_requests();
