@@ -461,3 +461,52 @@ def test_step_of_a_batch():
             at += n
         ctx = ctx + np.array(new, np.int32)
     assert plan.refused.sum().item() == 0
+
+
+def test_workspace_refusals():
+    """A call whose rows may be split refuses a missing, misaligned or short workspace; a short table needs none."""
+    import ctypes
+    import torch
+    import flashgann_b200 as fg
+    from flashgann_b200 import _capi
+    L = fg.lib()
+    z = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    p = z.data_ptr()
+
+    def args(width, **kw):
+        cache = _capi.KVCacheArgs(k=p, v=p, page_stride=1024, token_stride=64, head_stride=64, pages=4, page_size=16,
+                                  heads=1, dim=64, dtype=_capi.FG_DTYPE_F16)
+        a = _capi.AttentionArgs(q=p, q_token_stride=64, q_head_stride=64, out=p + 4096, out_token_stride=64,
+                                out_head_stride=64, block_table=p + 8192, table_stride=width, query_start=p + 16384,
+                                kv_len=p + 16448, tokens=1, heads=1, requests=1, table_width=width, max_new=1, window=-1,
+                                scale=0.125, **kw)
+        return cache, a
+
+    need = ctypes.c_uint64()
+    c, a = args(1000)
+    assert L.fg_attention_workspace_bytes(c, a, 0, ctypes.byref(need)) == fg.FG_OK and need.value > 0
+    for kw in (dict(), dict(workspace=p + 16, workspace_bytes=1 << 40), dict(workspace=p, workspace_bytes=need.value - 1)):
+        c, a = args(1000, **kw)
+        assert L.fg_paged_attention_device(c, a, None) == fg.FG_ERR_ARG
+        assert "workspace" in L.fg_last_error().decode()
+    c, a = args(4)
+    assert L.fg_attention_workspace_bytes(c, a, 0, ctypes.byref(need)) == fg.FG_OK and need.value == 0
+    assert L.fg_paged_attention_device(c, a, None) == fg.FG_OK
+    torch.cuda.synchronize()
+
+
+def test_example_of_a_decode_over_retrieved_keys():
+    """The example runs all four operators with the search; its last step's output is the formula's for the ids that
+    the search returned, over the cache as plan and append left it."""
+    import importlib.util
+    import os
+    from tests.common import ROOT
+    spec = importlib.util.spec_from_file_location("retrieval_decode", os.path.join(ROOT, "examples", "retrieval_decode.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    r = m.run(context=4000, steps=2)
+    assert r["refused"] == 0 and r["tokens"] == 4002 and 0 < r["weight_seen"] <= 1 + 1e-3
+    x = {k: v.float().cpu().numpy() if hasattr(v, "cpu") and v.is_floating_point() else v for k, v in r["last"].items()}
+    ref = attention_ref(x["q"], x["k_cache"], x["v_cache"], x["table"].cpu().numpy(), [0, 1], [4002],
+                        window=x["window"], sinks=x["sinks"], ids=x["ids"].cpu().numpy())
+    _check(r["last"]["out"], r["last"]["lse"], ref, "bf16")
