@@ -23,8 +23,9 @@
 //
 // What bounds it: per block and half 4 * 128 * 128 * dim operations, 1024
 // cycles of the tensor pipe at dim 128, and 128 * 128 exponentials, 1024
-// cycles of the SM's special-function units: both pipes are needed for the
-// whole time, see exp2_mixed.
+// cycles of the SM's special-function units.  (A polynomial for some of them
+// was slower: the special-function units are not what is short, issue slots and
+// latencies are.)
 //
 // The running maximum that the weights are relative to is raised only when it
 // grows by more than 2^8: then O and the sum are scaled, which costs a round
@@ -48,7 +49,6 @@ constexpr int kThreads = 512;
 constexpr int kSlots = 5;    // see Loader::block; K and V tiles in the ring: two blocks and a half
 constexpr int kTileBlocks = 3;  // a tile costs about as much as that many blocks beside its own (1 to 4 measured)
 constexpr float kRaise = 8.f;
-constexpr int kPolyPairs = 1;  // of 8 pairs of weights, see exp2_poly
 
 template <int kDim>
 struct Smem {
@@ -447,26 +447,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// 2^x for x in [-inf, 2^21], without the special-function units: x = n + f with
-// n the nearest integer (left in the low bits by adding 1.5 * 2^23), 2^f by the
-// polynomial of degree 4 with the least relative error on [-1/2, 1/2] (2.6e-6,
-// from a Remez exchange), n added to its exponent.  Below 2^-126 the result is
-// about 2^-126.  NaN is not kept.
-__device__ __forceinline__ Pair exp2_poly(Pair x) {
-    constexpr float kShift = 12582912.f;
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
-    const Pair t = add2(x, Pair{kShift, kShift});
-    const Pair n = add2(t, Pair{-kShift, -kShift});
-    const Pair f = fma2(n, Pair{-1.f, -1.f}, x);
-    Pair y = fma2(f, Pair{0.00957010221f, 0.00957010221f}, Pair{0.0559178591f, 0.0559178591f});
-    y = fma2(y, f, Pair{0.240247443f, 0.240247443f});
-    y = fma2(y, f, Pair{0.693121791f, 0.693121791f});
-    y = fma2(y, f, Pair{0.999999285f, 0.999999285f});
-    return Pair{__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
-                __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23))};
-}
-
 template <typename T, int kDim>
 struct Softmax {
     const AttentionParams& a;
@@ -484,25 +464,21 @@ struct Softmax {
           output(tmem + (((threadIdx.x >> 5) & 3) << 21) + output_column(threadIdx.x >> 7)), row(threadIdx.x & 255),
           box_shift(shift) {}
 
-    // The weights of 64 keys from key kFrom on from their scores, into place.
-    // kMixed: one pair in eight by exp2_poly, the others by the special-function
-    // units (measured: 0, 1, 2, 3, 4 in eight); only where no score is masked and
-    // the base is finite.
-    template <bool kMixed, int kFrom>
-    __device__ __forceinline__ void weights(const float (&s)[kBlock], float base, Pair (&sum)[2]) {
+    // The weights of 64 keys from their scores, into place from column `to` on.
+    __device__ __forceinline__ void weights(const float* s, float base, Pair (&sum)[2], uint32_t to) {
         const Pair scale{a.scale_log2, a.scale_log2}, shift{base, base};
 #pragma unroll
-        for (int c0 = kFrom; c0 < kFrom + 64; c0 += 32) {
+        for (int c0 = 0; c0 < 64; c0 += 32) {
             uint32_t pk[16];
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
                 const Pair x = fma2(Pair{s[c0 + c], s[c0 + c + 1]}, scale, shift);
-                const Pair e = kMixed && ((c / 2) & 7) < kPolyPairs ? exp2_poly(x) : Pair{exp2_fast(x.x), exp2_fast(x.y)};
+                const Pair e{exp2_fast(x.x), exp2_fast(x.y)};
                 sum[(c / 2) & 1] = add2(sum[(c / 2) & 1], e);
                 // weights go to the product in the cache's 16-bit type, as the tensor cores take them; the sum keeps 32 bits
                 pk[c / 2] = Half2<T>::pack(e.x, e.y);
             }
-            tmem_store16(score + c0 / 2, pk);
+            tmem_store16(to + c0 / 2, pk);
         }
     }
     __device__ __forceinline__ float row_max(const float (&s)[kBlock]) {
@@ -581,14 +557,12 @@ struct Softmax {
         }
         // a row without a visible key yet has no base; one with a score of +inf is NaN, as inf - inf
         const float base = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m;
-        const bool mixed = whole && __all_sync(0xFFFFFFFFu, m != -INFINITY);
         Pair sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-        if (mixed) weights<true, 0>(s, base, sum);
-        else weights<false, 0>(s, base, sum);
-        hand_over(0);
-        if (mixed) weights<true, 64>(s, base, sum);
-        else weights<false, 64>(s, base, sum);
-        hand_over(1);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            weights(s + part * 64, base, sum, score + part * 32);
+            hand_over(part);
+        }
         const Pair both = add2(sum[0], sum[1]);
         l += both.x + both.y;
         ++done;
@@ -836,7 +810,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                                  kPv, add || k > 0);
                 }
             };
-            struct Turn {  // place in the ring, and the parity of its use
+            struct Turn {  // a place in the ring, and the parity of its use
                 uint32_t slot;
                 int parity;
                 __device__ __forceinline__ void advance() {
@@ -857,33 +831,45 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                 if (halves == 2) scores(1, at.slot);
                 if (blocks == 1) commit(&sh->q_empty);
                 at.advance();
-                for (int b = 0; b < blocks; ++b, ++n) {
-                    const bool more = b + 1 < blocks, tell = !more || !w.all.has(w.u0 + b);
-                    const Turn v = at;
-                    at.advance();
-                    const Turn k = at;
-                    if (more) at.advance();
-                    ok = filled(v);
+                // V of the block in work and K of the next one; waited for a half block before they are used, so that
+                // nothing but the weights is waited for between two halves' products
+                Turn v = at, k = at;
+                k.advance();
+                ok = filled(v) && (blocks == 1 || filled(k));
+                bool tell = blocks == 1 || !w.all.has(w.u0);
+                for (int b = 0; ok && b < blocks; ++b, ++n) {
+                    const bool more = b + 1 < blocks;
                     const auto turn = [&](int h) {
-                        ok = ok && bar_wait(&sh->p_full[h][0], done[h] & 1, sh);
+                        ok = bar_wait(&sh->p_full[h][0], done[h] & 1, sh);
                         if (!ok) return;
                         tmem_fence_after();
                         output(h, v.slot, 0, b > 0);
+                        // the block before, told late: a commit takes its time, and here the tensor cores have work
+                        if (h == 0 && b > 0) commit(&sh->used[(n - 1) & 3]);
                         ok = bar_wait(&sh->p_full[h][1], done[h] & 1, sh);
                         if (!ok) return;
                         tmem_fence_after();
                         output(h, v.slot, 1, true);
                         if (tell) commit(&sh->pv_done[h]);
                         ++done[h];
-                        if (!more) return;
-                        if (h == 0) ok = filled(k);
-                        if (ok) scores(h, k.slot);
+                        if (more) scores(h, k.slot);
                     };
                     turn(0);
-                    if (halves == 2) turn(1);
                     if (!ok) break;
-                    commit(&sh->used[n & 3]);
+                    Turn next_v = k, next_k = k;
+                    next_v.advance();
+                    next_k = next_v;
+                    next_k.advance();
+                    if (more) ok = filled(next_v) && (b + 2 >= blocks || filled(next_k));
+                    const bool next_tell = b + 2 >= blocks || !w.all.has(w.u0 + b + 1);
+                    if (ok && halves == 2) turn(1);
+                    if (!ok) break;
                     if (b + 2 == blocks) commit(&sh->q_empty);
+                    if (!more) commit(&sh->used[n & 3]);
+                    at = more ? next_v : k;
+                    v = next_v;
+                    k = next_k;
+                    tell = next_tell;
                 }
                 ++segment;
             } while (ok && w.next());
