@@ -877,6 +877,10 @@ int workspace_bytes(const fg_kv_cache* c, const fg_attention* x, bool retrieved,
     a.sinks = x->sinks;
     a.group = x->heads / c->heads;
     a.ids_count = retrieved ? x->ids_count : 0;
+    a.requests = x->requests;
+    a.tokens = x->tokens;
+    a.kv_heads = c->heads;
+    a.ctas = sms;
     *bytes = fg::attention_rows_workspace(a, sms, c->dim);
     return FG_OK;
 }

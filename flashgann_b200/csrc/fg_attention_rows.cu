@@ -27,35 +27,56 @@
 // repeated) and leave the rest in shared memory, see stage_ids.
 //
 // Tiles that are short whatever the lengths are (a narrow table, or a window and
-// a few ids, see attention_rows_splits) are not split:
-// there are no partials and no second kernel, which costs more than it saves.
+// a few ids) are not split where that leaves the CTAs evenly filled, see
+// attention_rows_splits.
 #include <algorithm>
 
 #include "fg_attention.cuh"
 
 namespace fg {
 
-// Whether tiles may be split over CTAs.  The host knows how many chunks no tile has more of: from the table's width, or
-// from the window, the first tokens and the ids.
+namespace {
+constexpr int kRows = 16;
+constexpr int kChunk = 16;
+constexpr int kCtasPerSm = 2;
+constexpr int kMaxIds = 1024;  // ids of a tile's heads, in shared memory
+
+// Places of a list of ids in shared memory: whole groups of 128.
+__host__ __device__ __forceinline__ int staged_pitch(int count) { return (count + 127) & ~127; }
+
+// Heads to a tile: with ids as many as have room for theirs.
+int tile_rows(const AttentionParams& a) { return a.ids_count > 0 ? std::min(kRows, kMaxIds / staged_pitch(a.ids_count)) : kRows; }
+}  // namespace
+
+// Whether tiles are split over CTAs (a.ctas: SMs).  The host knows how many
+// chunks no tile has more of (from the table's width, or from the window, the
+// first tokens and the ids) and about how many tiles there are.  Not split:
+// no partials, no second kernel (4 us on the host), and every tile's ids are
+// read once; but the CTAs are as unevenly filled as the tiles fall.  Measured,
+// whole / split, us: 2 tiles of 37 chunks 10.3 / 8.2 and 15.7 / 19.5 with the
+// host's part; 8 of 57 18.5 / 10.2; 160 of 46 with ids 29 / 32; 296 of 57 30 / 34;
+// 320 of 46 with ids 56 / 45; 512 of them 62 / 65.
 bool attention_rows_splits(const AttentionParams& a) {
-    constexpr int kRows = 16, kChunk = 16;
-    constexpr int kShort = 64;  // chunks of a tile that is not split
     int64_t keys = static_cast<int64_t>(a.table_width) * a.page_size;
     if (a.window >= 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + kRows + a.sinks);
     int64_t chunks = keys / kChunk + 3;
-    chunks += static_cast<int64_t>(std::min(a.group, kRows)) * ((a.ids_count + kChunk - 1) / kChunk);
-    return chunks > kShort;
+    int64_t tiles = static_cast<int64_t>(a.requests) * a.kv_heads;
+    if (a.ids_count > 0) {
+        const int rows = tile_rows(a);
+        chunks += static_cast<int64_t>(std::min(a.group, rows)) * ((a.ids_count + kChunk - 1) / kChunk);
+        tiles = static_cast<int64_t>(a.tokens) * a.kv_heads * ((a.group + rows - 1) / rows);
+    }
+    const int64_t ctas = static_cast<int64_t>(a.ctas) * kCtasPerSm;
+    if (chunks > 64) return true;
+    if (tiles <= ctas) return chunks > 40 && tiles * 3 < ctas;
+    return chunks > 24 && tiles * 10 < (tiles + ctas - 1) / ctas * ctas * 8;
 }
 
 namespace attn {
 namespace {
 
-constexpr int kRows = 16;
-constexpr int kChunk = 16;
 constexpr int kWarps = 4;
-constexpr int kCtasPerSm = 2;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxIds = 1024;    // ids of a tile's heads, in shared memory
 constexpr int kTable = 2048;     // places of the hash table over them
 
 template <int kDim>
@@ -259,9 +280,6 @@ struct Warp {
 
     // Whether a retrieved id counts, repeats aside: in range, and not visible by the mask already.
     __device__ __forceinline__ bool counts(int id) const { return id >= a.sinks && id <= p0 && p0 - id >= a.window; }
-
-    // Places of a list in shared memory: whole groups of 128.
-    __host__ __device__ static __forceinline__ int staged_pitch(int count) { return (count + 127) & ~127; }
 
     // Reads the lists of the tile's heads into shared memory, with -1 in the
     // place of ids that do not count.  Of equal ids in a list the first stays: a
@@ -664,7 +682,7 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = kIds ? Smem<kDim>::kBytesIds : Smem<kDim>::kBytes;
     static_assert((bytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
     a.base_align = kChunk;
-    if (kIds) a.tile_rows = std::min(kRows, kMaxIds / Warp<T, kDim, kIds>::staged_pitch(a.ids_count));
+    a.tile_rows = tile_rows(a);
     const bool split = attention_rows_splits(a);
     a.ctas *= kCtasPerSm;
     a.unit_shift = split ? 2 : 24;  // a unit: one chunk for each warp, or a tile
@@ -695,11 +713,11 @@ cudaError_t by_dim(const AttentionParams& a, cudaStream_t s) {
 
 size_t attention_rows_workspace(const AttentionParams& a, int sms, int dim) {
     if (!attention_rows_splits(a)) return 0;
-    const int ctas = sms * attn::kCtasPerSm;
-    return attn::workspace_records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * attn::partial_floats(attn::kRows, dim) * sizeof(float);
+    const int ctas = sms * kCtasPerSm;
+    return attn::workspace_records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * attn::partial_floats(kRows, dim) * sizeof(float);
 }
 int attention_max_requests() { return 16384; }
-int attention_max_ids() { return attn::kMaxIds; }
+int attention_max_ids() { return kMaxIds; }
 
 cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream) {
     return a.dtype == FG_DTYPE_BF16 ? attn::by_dim<__nv_bfloat16>(a, stream) : attn::by_dim<__half>(a, stream);

@@ -330,8 +330,8 @@ typedef struct fg_attention {
 /* Bytes of workspace that a call needs on the current device, for partial
  * results of rows whose keys are split over CTAs (0: none, where no row can
  * have many keys).  retrieved: 1 for fg_retrieved_attention_device.  Depends
- * on args' heads, max_new, table_width, window, sinks, ids_count and scale
- * only, on no pointer. */
+ * on args' counts (tokens, heads, requests, table_width, max_new, window,
+ * sinks, ids_count) and the scale's sign only, on no pointer. */
 int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* args, int32_t retrieved,
                                  uint64_t* bytes);
 
