@@ -225,7 +225,7 @@ def _attend(retrieved: bool, q, k_cache, v_cache, block_table, query_start, kv_l
                 block_table.data_ptr(), block_table.stride(0), query_start.data_ptr(), kv_len.data_ptr(), id_ptr,
                 id_token, id_head, 0, 0, T, heads, R, block_table.shape[1], max_new, -1 if window is None else window,
                 sinks, count, dim ** -0.5 if scale is None else scale]
-        key = (on.index, retrieved, c[40:], T, heads, R, max_new, block_table.shape[1], window, sinks, count, args[-1] > 0)
+        key = (on.index, retrieved, c[16:], q0 == 0, q1 == 0, T, heads, R, max_new, block_table.shape[1], window, sinks, count, args[-1] > 0)
         need = _workspace.get(key)
         if need is None:
             size = ctypes.c_uint64()

@@ -854,12 +854,16 @@ int sm_count(int* sms) {
 // tokens x heads of the group) fill one tile of the rows kernel; above that it
 // would read the keys once for each 16 rows, and the tiles kernel takes them
 // 256 at a time.  That one folds the scale into its maxima, so it needs a
-// positive one, and its copies are whole groups of 8 rows of a page.
+// positive one; its copies are whole groups of 8 rows of a page, and take no
+// axis of stride 0 (an expanded tensor).
 bool many_rows(const fg_kv_cache* c, const fg_attention* x) {
     return static_cast<int64_t>(x->max_new) * (x->heads / c->heads) > 16;
 }
 bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
-    return !retrieved && many_rows(c, x) && x->scale > 0.f && c->page_size >= 8;
+    const bool expanded = (c->token_stride == 0 && c->page_size > 1) || (c->head_stride == 0 && c->heads > 1) ||
+                          (c->page_stride == 0 && c->pages > 1) || (x->q_token_stride == 0 && x->tokens > 1) ||
+                          (x->q_head_stride == 0 && x->heads > 1);
+    return !retrieved && many_rows(c, x) && x->scale > 0.f && c->page_size >= 8 && !expanded;
 }
 
 int workspace_bytes(const fg_kv_cache* c, const fg_attention* x, bool retrieved, uint64_t* bytes) {

@@ -137,7 +137,8 @@ __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Re
     int i0, i1;
     Tiles<kRows, kLayout>::tokens(a, r, t, &i0, &i1);
     const int p0 = r.kv_len - r.rows + i0, p1 = r.kv_len - r.rows + i1;
-    const int64_t room = static_cast<int64_t>(a.table_width) * a.page_size;  // keys that the table can address
+    // keys that the table can address, and that chunk numbers in 32 bits can
+    const int64_t room = min(static_cast<int64_t>(a.table_width) * a.page_size, static_cast<int64_t>(INT32_MAX - 1023));
     k.hi = p1 < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(p1) + 1, room));
     k.lo = (a.window < 0 || p0 < a.window) ? 0 : min(p0 - a.window + 1, k.hi);
     k.base = k.lo & -a.base_align;

@@ -110,10 +110,12 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, int parity, Shared* sh) {
         }
     return true;
 }
-// for waits that nothing hurries: leaves the issue slots to the other warps
+// For waits that nothing hurries: leaves the issue slots to the other warps.
+// They may last as long as a tile (a V tile to be looked through comes after
+// all others: 16 ms in a context of a million keys), the limit is seconds.
 __device__ __forceinline__ bool bar_wait_idle(uint64_t* b, int parity, Shared* sh) {
     for (int i = 0; !bar_try(b, parity); ++i) {
-        if (i == (1 << 18)) {
+        if (i == (1 << 26)) {
             *reinterpret_cast<volatile int*>(&sh->stalled) = 1;
             return false;
         }

@@ -331,7 +331,7 @@ typedef struct fg_attention {
  * results of rows whose keys are split over CTAs (0: none, where no row can
  * have many keys).  retrieved: 1 for fg_retrieved_attention_device.  Depends
  * on args' counts (tokens, heads, requests, table_width, max_new, window,
- * sinks, ids_count) and the scale's sign only, on no pointer. */
+ * sinks, ids_count), the scale's sign and which strides are 0 only. */
 int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* args, int32_t retrieved,
                                  uint64_t* bytes);
 

@@ -463,6 +463,26 @@ def test_step_of_a_batch():
     assert plan.refused.sum().item() == 0
 
 
+@pytest.mark.parametrize("new", [1, 60])
+def test_expanded_tensors(new):
+    """Axes of stride 0: one kv head's cache shown as four, one query shown as all."""
+    import torch
+    import flashgann_b200 as fg
+    x = make(np.random.default_rng(30 + new), ctx=[70, 40], new=[new, new], heads=8, kv_heads=1, dim=64, page=16)
+    x["q"][:] = x["q"][:, :1]
+    dt = torch.float16
+    k, v, q = _cuda(x["k"], dt).expand(-1, -1, 4, -1), _cuda(x["v"], dt).expand(-1, -1, 4, -1), _cuda(x["q"][:, :1], dt)
+    rest = (_cuda(x["table"]), _cuda(x["start"]), _cuda(x["kv_len"]), new)
+    for qq in (q.expand(-1, 8, -1), q.repeat(1, 8, 1)):
+        for kk, vv in ((k, v), (k.contiguous(), v.contiguous())):
+            out, lse = fg.paged_attention(qq, kk, vv, *rest, return_lse=True)
+            _check(out, lse, _ref(x), "fp16")
+    one = _cuda(x["q"][:1, :1], dt).expand(2 * new, 8, -1)
+    x["q"][:] = x["q"][:1, :1]
+    out, lse = fg.paged_attention(one, k, v, *rest, return_lse=True)
+    _check(out, lse, _ref(x), "fp16")
+
+
 def test_workspace_refusals():
     """A call whose rows may be split refuses a missing, misaligned or short workspace; a short table needs none."""
     import ctypes
