@@ -77,9 +77,10 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTable = 2048;     // places of the hash table over them
+static_assert(kThreads == 128, "lists of ids lie in groups of 128");
+constexpr int kTable = 8192;     // places of the hash table over them: with 2048 or 4096 staging takes twice or 1.3 times as long
 
-template <int kDim>
+template <int kDim, bool kIds>
 struct Smem {
     // ldmatrix reads 8 rows without bank conflicts: rows of 128 or 256 bytes with their 16-byte pieces exchanged by the
     // row's number, rows of 192 bytes padded to an odd multiple of 16
@@ -89,12 +90,11 @@ struct Smem {
         return row * kPitch + (kExchange ? piece ^ (row & 7) : piece) * 16;
     }
     static constexpr int kTile = kChunk * kPitch;
-    static constexpr int kStages = 3;
+    static constexpr int kStages = kIds ? 2 : 3;  // of the ring; with ids the third one's room is the table's (3 % for decodes)
     static constexpr int kRing = kStages * 2 * kTile;  // K and V of each stage
     static constexpr int kWarpBytes = kRing;
     static constexpr int kIdsAt = kWarps * kWarpBytes;  // retrieved form: the tile's ids and the table
-    static constexpr int kBytes = kIdsAt;
-    static constexpr int kBytesIds = kIdsAt + kMaxIds * 4 + kTable * 4;
+    static constexpr int kBytes = kIdsAt + (kIds ? kMaxIds * 4 + kTable * 4 : 0);
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -165,7 +165,7 @@ struct Chunk {
 
 template <typename T, int kDim, bool kIds>
 struct Warp {
-    using S = Smem<kDim>;
+    using S = Smem<kDim, kIds>;
     static constexpr int kPieces = kDim / 8;              // 16-byte pieces of a row
 
     const AttentionParams& a;
@@ -225,13 +225,13 @@ struct Warp {
         Tiles<kRows, kIds ? kToken : kPacked>::row(a, r, tile, 0, &i, &g);
         return a.ids + static_cast<int64_t>(r.start + i) * a.ids_token_stride + static_cast<int64_t>(head * a.group + g) * a.ids_head_stride;
     }
-    // This thread's places x, x + kThreads, ... of the tile's lists.
-    __device__ __forceinline__ void read_places(const int32_t* from, int x0, int heads, int (&id)[4]) const {
-        const int pitch = staged_pitch(a.ids_count);
+    // The lists lie in shared memory in groups of kThreads places, each of one head; group `at` and the three after it.
+    __device__ __forceinline__ void read_groups(const int32_t* from, int at, int groups, int (&id)[4]) const {
+        const int per = staged_pitch(a.ids_count) / kThreads;
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-            const int x = x0 + y * kThreads, h = x / pitch, n = x - h * pitch;
-            id[y] = h < heads && n < a.ids_count ? __ldg(from + h * a.ids_head_stride + n) : -1;
+            const int h = (at + y) / per, n = (at + y - h * per) * kThreads + threadIdx.x;
+            id[y] = at + y < groups && n < a.ids_count ? __ldg(from + h * a.ids_head_stride + n) : -1;
         }
     }
     __device__ __forceinline__ int list_heads(int tile) const {
@@ -240,7 +240,7 @@ struct Warp {
     // The first ids of a tile that comes next, into registers.
     __device__ __forceinline__ void read_ids(const Request& r, int head, int tile) {
         ids = lists(r, head, tile);
-        read_places(ids, threadIdx.x, list_heads(tile), early);
+        read_groups(ids, 0, list_heads(tile) * (staged_pitch(a.ids_count) / kThreads), early);
     }
     int early[4];
 
@@ -289,38 +289,38 @@ struct Warp {
     // the whole CTA.
     __device__ __forceinline__ void stage_ids(int* list, int* table, int heads) const {
         constexpr int kFree = -1;  // (16-bit places would do, but their atomics are ten times as slow)
-        const int pitch = staged_pitch(a.ids_count), all = heads * pitch;
-        for (int x = threadIdx.x; x < kTable; x += kThreads) table[x] = kFree;
-        int id[4] = {early[0], early[1], early[2], early[3]};
-        for (int x0 = threadIdx.x; x0 < all; x0 += kThreads * 4) {
-            if (x0 != threadIdx.x) read_places(ids, x0, heads, id);
+        const int pitch = staged_pitch(a.ids_count), per = pitch / kThreads, groups = heads * per;
+        for (int x = threadIdx.x; x < kTable / 4; x += kThreads) reinterpret_cast<int4*>(table)[x] = make_int4(kFree, kFree, kFree, kFree);
+        int id4[4] = {early[0], early[1], early[2], early[3]};
+        for (int at = 0; at < groups; at += 4) {
+            if (at > 0) read_groups(ids, at, groups, id4);
 #pragma unroll
             for (int y = 0; y < 4; ++y)
-                if (x0 + y * kThreads < all) list[x0 + y * kThreads] = counts(id[y]) ? id[y] : -1;
+                if (at + y < groups) list[(at + y) * kThreads + threadIdx.x] = counts(id4[y]) ? id4[y] : -1;
         }
         __syncthreads();
         const auto first_place = [&](int id, int h) {
-            return ((static_cast<uint32_t>(id) + static_cast<uint32_t>(h) * 0x9E3779B9u) * 2654435761u) >> 21;  // of 2048
+            return ((static_cast<uint32_t>(id) + static_cast<uint32_t>(h) * 0x9E3779B9u) * 2654435761u) >> 19;  // of 8192
         };
-        const auto same = [&](int x, int id, int h) { return list[x] == id && x / pitch == h; };
-        for (int x = threadIdx.x; x < all; x += kThreads) {
-            const int id = list[x], h = x / pitch;
+        const auto same = [&](int x, int id, int h) { return list[x] == id && static_cast<uint32_t>(x - h * pitch) < static_cast<uint32_t>(pitch); };
+        for (int at = 0; at < groups; ++at) {
+            const int x = at * kThreads + threadIdx.x, id = list[x], h = at / per;
             if (id < 0) continue;
-            for (uint32_t at = first_place(id, h);; at = (at + 1) % kTable) {
-                int old = atomicCAS(table + at, kFree, x);
+            for (uint32_t place = first_place(id, h);; place = (place + 1) % kTable) {
+                const int old = atomicCAS(table + place, kFree, x);
                 if (old == kFree) break;
                 if (!same(old, id, h)) continue;  // another id's place
-                atomicMin(table + at, x);  // the same id's
+                atomicMin(table + place, x);
                 break;
             }
         }
         __syncthreads();
-        for (int x = threadIdx.x; x < all; x += kThreads) {
-            const int id = list[x], h = x / pitch;
+        for (int at = 0; at < groups; ++at) {
+            const int x = at * kThreads + threadIdx.x, id = list[x], h = at / per;
             if (id < 0) continue;
-            uint32_t at = first_place(id, h);
-            while (!same(table[at], id, h)) at = (at + 1) % kTable;
-            if (table[at] != x) list[x] = -1;  // no place that the table holds
+            uint32_t place = first_place(id, h);
+            while (!same(table[place], id, h)) place = (place + 1) % kTable;
+            if (table[place] != x) list[x] = -1;  // no place that the table holds
         }
         __syncthreads();
     }
@@ -507,7 +507,7 @@ struct Warp {
 
 template <typename T, int kDim, bool kIds>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(const AttentionParams a) {
-    using S = Smem<kDim>;
+    using S = Smem<kDim, kIds>;
     extern __shared__ __align__(128) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     char* ws = static_cast<char*>(a.workspace);
@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
 
 template <typename T, int kDim, bool kIds>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
-    constexpr int bytes = kIds ? Smem<kDim>::kBytesIds : Smem<kDim>::kBytes;
+    constexpr int bytes = Smem<kDim, kIds>::kBytes;
     static_assert((bytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
     a.base_align = kChunk;
     a.tile_rows = tile_rows(a);
