@@ -12,6 +12,9 @@ GENCODE := -gencode arch=compute_100a,code=$(ARCH)
 NVFLAGS := -std=c++17 -O3 $(GENCODE) -lineinfo -Xptxas -v $(EXTRA_NVFLAGS)
 CSRC    := flashgann_b200/csrc
 LIB     := flashgann_b200/libflashgann.so
+TORCH_OPS := flashgann_b200/_torch_ops.so
+PYTHON  ?= python3
+CUDA_HOME ?= /usr/local/cuda
 BIN_DIR := bin
 
 KERNEL_SRC := $(CSRC)/fg_search.cu $(CSRC)/fg_search_warp.cu $(CSRC)/fg_shard_merge.cu $(CSRC)/fg_kv.cu \
@@ -25,7 +28,16 @@ OBJS       := $(patsubst $(CSRC)/%.cu,$(OBJ_DIR)/%.o,$(KERNEL_SRC))
 
 all: lib gpu_flashgann
 
-lib: $(LIB)
+lib: $(LIB) $(TORCH_OPS)
+
+# the torch binding of the cache and attention calls (flashgann_b200/attention.py)
+TORCH_FLAGS = $(shell $(PYTHON) -c "import os, sysconfig, torch; t = os.path.dirname(torch.__file__); \
+    print('-I%s/include -I%s/include/torch/csrc/api/include -I%s -I%s/include -D_GLIBCXX_USE_CXX11_ABI=%d -L%s/lib -Wl,-rpath,%s/lib' % \
+          (t, t, sysconfig.get_paths()['include'], '$(CUDA_HOME)', torch._C._GLIBCXX_USE_CXX11_ABI, t, t))")
+
+$(TORCH_OPS): $(CSRC)/fg_torch.cpp include/flashgann.h $(LIB)
+	$(CXX) -std=c++17 -O2 -fPIC -shared $< -o $@ $(TORCH_FLAGS) -lc10 -ltorch_cpu -ltorch_python -lc10_cuda \
+	    -L$(dir $(LIB)) -lflashgann -Wl,-rpath,'$$ORIGIN'
 
 $(OBJ_DIR)/%.o: $(CSRC)/%.cu $(HEADERS) | $(OBJ_DIR)
 	$(NVCC) $(NVFLAGS) -Xcompiler -fPIC -c -o $@ $< 2> $(OBJ_DIR)/$*.ptxas.log || (cat $(OBJ_DIR)/$*.ptxas.log; exit 1)
@@ -54,4 +66,4 @@ oracle:
 	$(MAKE) -C oracle
 
 clean:
-	rm -f $(LIB) $(BIN_DIR)/gpu_flashgann $(CSRC)/ptxas.log $(OBJS) $(OBJ_DIR)/*.ptxas.log
+	rm -f $(LIB) $(TORCH_OPS) $(BIN_DIR)/gpu_flashgann $(CSRC)/ptxas.log $(OBJS) $(OBJ_DIR)/*.ptxas.log
