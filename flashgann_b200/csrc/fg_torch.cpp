@@ -34,12 +34,14 @@ void check(int rc, const char* call) {
     if (rc != FG_OK) raise(rc, std::string(call) + ": " + fg_status_string(rc) + " (" + fg_last_error() + ")");
 }
 
-void need(bool ok, const std::string& message) {
-    if (!ok) raise(FG_ERR_ARG, message);
-}
+// a macro: the message is put together only where it is raised
+#define FG_NEED(ok, message)                      \
+    do {                                          \
+        if (!(ok)) raise(FG_ERR_ARG, (message));  \
+    } while (0)
 
 int32_t i32(int64_t x, const char* name) {
-    need(x >= INT32_MIN && x <= INT32_MAX, std::string(name) + " " + std::to_string(x) + " is out of range");
+    FG_NEED(x >= INT32_MIN && x <= INT32_MAX, std::string(name) + " " + std::to_string(x) + " is out of range");
     return static_cast<int32_t>(x);
 }
 
@@ -56,7 +58,7 @@ class On {
 public:
     // stream: a handle, or -1 for the current one
     On(const at::Tensor& like, int64_t stream) {
-        need(like.is_cuda(), "expected a CUDA tensor");
+        FG_NEED(like.is_cuda(), "expected a CUDA tensor");
         index_ = like.device().index();
         device_.emplace(index_);
         stream_ = c10::cuda::getCurrentCUDAStream(index_);
@@ -68,7 +70,7 @@ public:
     }
     template <typename... Tensors>
     void uses(const at::Tensor& t, const Tensors&... more) {
-        need(t.is_cuda() && t.device().index() == index_, "a tensor is on " + t.device().str() + ", not on device " + std::to_string(index_));
+        FG_NEED(t.is_cuda() && t.device().index() == index_, "a tensor is on " + t.device().str() + ", not on device " + std::to_string(index_));
         if (other_) t.record_stream(stream_->unwrap());
         if constexpr (sizeof...(more) > 0) uses(more...);
     }
@@ -82,24 +84,24 @@ private:
 };
 
 at::Tensor ints(const at::Tensor& t, int64_t dims, const char* name, at::ScalarType type = at::kInt) {
-    need(t.scalar_type() == type && t.dim() == dims,
-         std::string(name) + " must be " + at::toString(type) + " with " + std::to_string(dims) + " dimension(s), not " + shape(t));
+    FG_NEED(t.scalar_type() == type && t.dim() == dims,
+            std::string(name) + " must be " + at::toString(type) + " with " + std::to_string(dims) + " dimension(s), not " + shape(t));
     return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous();
 }
 
 // [tokens, heads, dim] with a contiguous last axis and 16-byte aligned rows (a copy where it is not)
 at::Tensor rows(const at::Tensor& t, const char* name) {
-    need(t.dim() == 3, std::string(name) + " must be [tokens, heads, dim], not " + shape(t));
+    FG_NEED(t.dim() == 3, std::string(name) + " must be [tokens, heads, dim], not " + shape(t));
     if ((t.stride(2) != 1 && t.size(2) > 1) || (t.stride(0) | t.stride(1)) % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16)
         return t.clone(at::MemoryFormat::Contiguous);
     return t;
 }
 
 fg_kv_cache cache(const at::Tensor& k, const at::Tensor& v) {
-    need(k.dim() == 4 && v.sizes() == k.sizes(), "caches must be [pages, page_size, heads, dim] alike, not " + shape(k) + " and " + shape(v));
-    need((k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16) && v.scalar_type() == k.scalar_type(),
-         "caches must both be float16 or bfloat16, not " + shape(k) + " and " + shape(v));
-    need(k.strides() == v.strides() && k.stride(3) == 1, "caches must have the same strides and a contiguous last axis");
+    FG_NEED(k.dim() == 4 && v.sizes() == k.sizes(), "caches must be [pages, page_size, heads, dim] alike, not " + shape(k) + " and " + shape(v));
+    FG_NEED((k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16) && v.scalar_type() == k.scalar_type(),
+            "caches must both be float16 or bfloat16, not " + shape(k) + " and " + shape(v));
+    FG_NEED(k.strides() == v.strides() && k.stride(3) == 1, "caches must have the same strides and a contiguous last axis");
     fg_kv_cache c{};
     c.k = k.data_ptr();
     c.v = v.data_ptr();
@@ -124,11 +126,11 @@ Six kv_plan(at::Tensor ctx_len, at::Tensor new_len, const at::Tensor& table, at:
     ctx_len = ints(ctx_len, 1, "ctx_len");
     new_len = ints(new_len, 1, "new_len");
     free_pages = ints(free_pages, 1, "free_pages");
-    const int64_t R = ctx_len.size(0), T = tokens > 0 ? tokens : 0;
-    need(new_len.size(0) == R, "ctx_len and new_len differ in length");
-    need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == R && (table.size(1) <= 1 || table.stride(1) == 1),
-         "block_table must be int32 [" + std::to_string(R) + ", width] with contiguous rows");
-    need(!free_head || (free_head->scalar_type() == at::kInt && free_head->numel() == 1), "free_head must be int32 [1]");
+    const int64_t R = ctx_len.size(0), T = i32(tokens, "tokens") > 0 ? tokens : 0;
+    FG_NEED(new_len.size(0) == R, "ctx_len and new_len differ in length");
+    FG_NEED(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == R && (table.size(1) <= 1 || table.stride(1) == 1),
+            "block_table must be int32 [" + std::to_string(R) + ", width] with contiguous rows");
+    FG_NEED(!free_head || (free_head->scalar_type() == at::kInt && free_head->numel() == 1), "free_head must be int32 [1]");
     const at::Tensor slot = at::empty({T}, ctx_len.options().dtype(at::kLong));
     const at::Tensor all = at::empty({3 * R + 2 + T}, ctx_len.options());
     int32_t* p = all.data_ptr<int32_t>();
@@ -149,9 +151,9 @@ void kv_append(const at::Tensor& k_cache, const at::Tensor& v_cache, at::Tensor 
     slot = ints(slot, 1, "slot", at::kLong);
     const int64_t T = slot.size(0);
     for (const at::Tensor* t : {&k, &v})
-        need(t->scalar_type() == k_cache.scalar_type() && t->dim() == 3 && t->size(0) == T && t->size(1) == c.heads && t->size(2) == c.dim,
-             "k and v must be " + std::string(at::toString(k_cache.scalar_type())) + " [" + std::to_string(T) + ", " + std::to_string(c.heads) +
-                 ", " + std::to_string(c.dim) + "], not " + shape(*t));
+        FG_NEED(t->scalar_type() == k_cache.scalar_type() && t->dim() == 3 && t->size(0) == T && t->size(1) == c.heads && t->size(2) == c.dim,
+                "k and v must be " + std::string(at::toString(k_cache.scalar_type())) + " [" + std::to_string(T) + ", " + std::to_string(c.heads) +
+                    ", " + std::to_string(c.dim) + "], not " + shape(*t));
     k = rows(k, "k");
     v = rows(v, "v");
     check(fg_kv_append_device(&c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slot.data_ptr<int64_t>(),
@@ -171,20 +173,20 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const 
     const fg_kv_cache c = cache(k_cache, v_cache);
     q = rows(q, "q");
     const int64_t T = q.size(0), heads = q.size(1), dim = q.size(2);
-    need(q.scalar_type() == k_cache.scalar_type() && dim == c.dim,
-         "q must be " + std::string(at::toString(k_cache.scalar_type())) + " [tokens, heads, " + std::to_string(c.dim) + "], not " + shape(q));
+    FG_NEED(q.scalar_type() == k_cache.scalar_type() && dim == c.dim,
+            "q must be " + std::string(at::toString(k_cache.scalar_type())) + " [tokens, heads, " + std::to_string(c.dim) + "], not " + shape(q));
     table = ints(table, 2, "block_table");
     query_start = ints(query_start, 1, "query_start");
     kv_len = ints(kv_len, 1, "kv_len");
     const int64_t R = kv_len.size(0);
-    need(query_start.size(0) == R + 1 && table.size(0) == R,
-         std::to_string(R) + " lengths need " + std::to_string(R + 1) + " query_start entries and " + std::to_string(R) + " table rows, not " +
-             std::to_string(query_start.size(0)) + " and " + std::to_string(table.size(0)));
+    FG_NEED(query_start.size(0) == R + 1 && table.size(0) == R,
+            std::to_string(R) + " lengths need " + std::to_string(R + 1) + " query_start entries and " + std::to_string(R) + " table rows, not " +
+                std::to_string(query_start.size(0)) + " and " + std::to_string(table.size(0)));
     at::Tensor out;
     if (out_or_none) {
         out = *out_or_none;
-        need(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1,
-             "out must be like q, " + shape(q) + ", with a contiguous last axis");
+        FG_NEED(out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.stride(2) == 1,
+                "out must be like q, " + shape(q) + ", with a contiguous last axis");
     } else {
         out = at::empty({T, heads, dim}, q.options());
     }
@@ -192,8 +194,8 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const 
     if (return_lse) lse = at::empty({T, heads}, q.options().dtype(at::kFloat));
     fg_attention x{};
     if (ids) {
-        need(ids->scalar_type() == at::kInt && ids->dim() == 3 && ids->size(0) == T && ids->size(1) == heads,
-             "ids must be int32 [" + std::to_string(T) + ", " + std::to_string(heads) + ", count], not " + shape(*ids));
+        FG_NEED(ids->scalar_type() == at::kInt && ids->dim() == 3 && ids->size(0) == T && ids->size(1) == heads,
+                "ids must be int32 [" + std::to_string(T) + ", " + std::to_string(heads) + ", count], not " + shape(*ids));
         if (ids->stride(2) != 1 && ids->size(2) > 1) ids = ids->contiguous();
         x.ids = ids->data_ptr<int32_t>();
         x.ids_token_stride = ids->stride(0);
