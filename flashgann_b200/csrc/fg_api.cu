@@ -843,6 +843,11 @@ int check_rows(const void* p, int64_t token_stride, int64_t head_stride, const c
     return FG_OK;
 }
 
+// whether rows of `dim` elements that are written may overlap along an axis of `count` rows
+bool overlaps(int64_t stride, int64_t count, int32_t dim) {
+    return count > 1 && stride < dim;
+}
+
 int sm_count(int* sms) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -915,6 +920,8 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     if (x->tokens == 0 || x->requests == 0) return FG_OK;
     if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, "q"))) return rc;
     if ((rc = check_rows(x->out, x->out_token_stride, x->out_head_stride, "out"))) return rc;
+    if (overlaps(x->out_token_stride, x->tokens, c->dim) || overlaps(x->out_head_stride, x->heads, c->dim))
+        return fail(FG_ERR_ARG, "rows of out overlap");
     if (!x->query_start || !x->kv_len || (!x->block_table && x->table_width > 0) || (retrieved && !x->ids && x->ids_count))
         return fail(FG_ERR_ARG, "null buffer");
     if (x->table_stride < 0) return fail(FG_ERR_ARG, "negative table stride");
@@ -1024,6 +1031,9 @@ int fg_kv_append_device(const fg_kv_cache* cache, const void* d_k, int64_t k_tok
     if ((rc = check_rows(d_k, k_token_stride, k_head_stride, "k"))) return rc;
     if ((rc = check_rows(d_v, v_token_stride, v_head_stride, "v"))) return rc;
     if (!d_slot) return fail(FG_ERR_ARG, "null slots");
+    if (overlaps(cache->page_stride, cache->pages, cache->dim) || overlaps(cache->token_stride, cache->page_size, cache->dim) ||
+        overlaps(cache->head_stride, cache->heads, cache->dim))
+        return fail(FG_ERR_ARG, "rows of the cache overlap");
     fg::AppendArgs a;
     a.k_cache = cache->k;
     a.v_cache = cache->v;

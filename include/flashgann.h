@@ -252,8 +252,9 @@ int fg_shard_merge_device(const uint32_t* d_ids, const float* d_dists, const uin
  *
  * All calls run on the calling thread's current device and are asynchronous
  * on `stream` (a cudaStream_t, NULL = default stream); they allocate nothing,
- * keep nothing and may be captured in a CUDA graph.  Buffers are device
- * memory and must not overlap.  Lengths, tables, slots and ids are read on
+ * keep nothing and may be captured in a CUDA graph (make a first call of each
+ * kind before a capture: it loads the kernels).  Buffers are device memory and
+ * must not overlap; strides that make the rows of an output overlap are refused.  Lengths, tables, slots and ids are read on
  * the device: values that address nothing (negative or too large pages,
  * slots, ids) are skipped, never followed. */
 

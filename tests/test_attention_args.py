@@ -124,3 +124,16 @@ def test_struct_sizes():
     """The ctypes mirrors have the C structs' layout (no padding is assumed)."""
     assert ctypes.sizeof(_capi.KVCacheArgs) == 64 and _capi.KVCacheArgs.pages.offset == 40
     assert ctypes.sizeof(_capi.AttentionArgs) == 168 and _capi.AttentionArgs.tokens.offset == 128
+
+
+@pytest.mark.parametrize("kw", [dict(out_token_stride=0), dict(out_head_stride=0), dict(out_head_stride=56)])
+def test_overlapping_outputs_are_refused(kw):
+    _refused("fg_paged_attention_device", _cache(), _args(**kw), "rows of out overlap")
+    _refused("fg_retrieved_attention_device", _cache(), _args(**kw), "rows of out overlap")
+
+
+@pytest.mark.parametrize("kw", [dict(page_stride=0), dict(token_stride=0), dict(head_stride=0), dict(head_stride=32)])
+def test_append_to_overlapping_rows_is_refused(kw):
+    L = fg.lib()
+    assert L.fg_kv_append_device(_cache(**kw), PTR, 128, 64, PTR, 128, 64, PTR, 3, None) == fg.FG_ERR_ARG
+    assert "rows of the cache overlap" in L.fg_last_error().decode()
