@@ -50,12 +50,20 @@ int tile_rows(const AttentionParams& a) { return a.ids_count > 0 ? std::min(kRow
 
 // Whether tiles are split over CTAs (a.ctas: SMs).  The host knows how many
 // chunks no tile has more of (from the table's width, or from the window, the
-// first tokens and the ids) and about how many tiles there are.  Not split:
-// no partials, no second kernel (4 us on the host), and every tile's ids are
-// read once; but the CTAs are as unevenly filled as the tiles fall.  Measured,
-// whole / split, us: 2 tiles of 37 chunks 10.3 / 8.2 and 15.7 / 19.5 with the
-// host's part; 8 of 57 18.5 / 10.2; 160 of 46 with ids 29 / 32; 296 of 57 30 / 34;
-// 320 of 46 with ids 56 / 45; 512 of them 62 / 65.
+// first tokens and the ids) and about how many tiles there are.  Not split: no
+// partials, no second kernel, and every tile's ids are read once; but the CTAs
+// are as unevenly filled as the tiles fall.  So tiles longer than 64 chunks are
+// always split, and shorter ones by how the CTAs (296) would be filled.
+// Measured, us a call, whole / split, 4 heads of 128:
+//   an eighth of the CTAs or less: 1 tile of 15 chunks 8.2 / 9.5, of 21
+//     10.3 / 9.4, of 40 14.5 / 9.5; 32 of 21 10.4 / 10.8, of 27 12.3 / 10.9;
+//     with ids 32 tiles of 12 12.7 / 14.4, of 24 16.4 / 16.1, of 36 20.5 / 16.4
+//   up to 80 % of them: 96 of 33 14.4 / 15.2, of 40 16.4 / 15.4; 160 of 33
+//     17.6 / 18.5, of 40 20.3 / 18.9; with ids, whose table every part makes
+//     again, 96 of 60 28.7 / 31.9, 160 of 36 22.6 / 26.7
+//   a last round below 80 %: 320 of 15 18.5 / 18.5, of 21 22.6 / 20.5, of 40
+//     34.7 / 28.8; with ids 320 of 12 26.5 / 26.3, of 24 33.7 / 30.8
+//   fuller: 296 of 40 21.5 / 22.6, 512 of 40 41.5 / 42.9, with ids 47.3 / 51.5
 bool attention_rows_splits(const AttentionParams& a) {
     int64_t keys = static_cast<int64_t>(a.table_width) * a.page_size;
     if (a.window >= 0) keys = std::min<int64_t>(keys, static_cast<int64_t>(a.window) + kRows + a.sinks);
@@ -68,8 +76,9 @@ bool attention_rows_splits(const AttentionParams& a) {
     }
     const int64_t ctas = static_cast<int64_t>(a.ctas) * kCtasPerSm;
     if (chunks > 64) return true;
-    if (tiles <= ctas) return chunks > 40 && tiles * 3 < ctas;
-    return chunks > 24 && tiles * 10 < (tiles + ctas - 1) / ctas * ctas * 8;
+    if (tiles * 8 <= ctas) return chunks > 20;
+    if (tiles * 10 >= (tiles + ctas - 1) / ctas * ctas * 8) return false;
+    return tiles <= ctas ? chunks > 36 && a.ids_count == 0 : chunks > 18;
 }
 
 namespace attn {
