@@ -26,6 +26,12 @@
 // heads' lists once, drop the ids that do not count (out of range, in the window,
 // repeated) and leave the rest in shared memory, see stage_ids.
 //
+// Measured (device time, 32 or 64 query heads on 8, dim 128, bf16): 64 ragged
+// decodes, 1.1 GB of keys and values, 176 to 179 us, 6.1 to 6.25 TB/s; one of
+// 131K keys at most, 82 us; one of a few hundred keys of dim 64 7.6 us.  With 64 requests x 100 ids
+// 57.5 us for 175 MB: there 8 warps per SM, as many as their registers allow,
+// do not cover the latency of short tiles.
+//
 // Tiles that are short whatever the lengths are (a narrow table, or a window and
 // a few ids) are not split where that leaves the CTAs evenly filled, see
 // attention_rows_splits.

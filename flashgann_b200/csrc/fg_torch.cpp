@@ -4,9 +4,9 @@
 // The other calls of the library are bound by ctypes.  These are made once for
 // each layer of a decode step, where filling the argument structs and making
 // the outputs in Python took 12 of 16 us and the kernel's launch 3; here it is
-// the same checks and allocations in C++ (a decode of one short request: 16 us
-// to 10.6, of which 10 are the kernel's).  No work beside that: every call
-// ends in the C ABI (include/flashgann.h).
+// the same checks and allocations in C++ (a call of one kernel: 6.9 us on the
+// host).  No work beside that: every call ends in
+// the C ABI (include/flashgann.h).
 #include <cmath>
 #include <cstdint>
 #include <optional>
