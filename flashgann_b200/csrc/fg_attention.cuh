@@ -57,6 +57,12 @@ __host__ __device__ inline size_t workspace_records_bytes(int ctas) {
 // one partial: rows x dim sums, then rows maxima and rows sums
 __host__ __device__ inline size_t partial_floats(int rows, int dim) { return static_cast<size_t>(rows) * (dim + 2); }
 
+// Shared memory that locate takes at its start: the block's warp sums and one
+// sum for each request.  A launch of more requests than its kernel's other
+// uses have room for asks for this much instead.
+constexpr int kMaxRequests = 16384;
+__host__ __device__ constexpr int locate_bytes(int requests) { return (64 + requests) * static_cast<int>(sizeof(int)); }
+
 // One request as every kernel reads it, clamped to the buffers the launch was given.
 struct Request {
     int start, rows, kv_len;  // first query token, new tokens, keys
@@ -176,7 +182,7 @@ __device__ __forceinline__ int64_t share(int64_t total, int c, int ctas) {
     return each * c + rest * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);  // both below 2^16
 }
 
-// Called by all kThreads threads; scratch holds requests + 64 ints.  kLanes
+// Called by all kThreads threads; scratch holds locate_bytes(requests).  kLanes
 // threads count the tiles of a request: 1 where requests are short, 8 where
 // they have many tiles.
 template <int kRows, Layout kLayout, int kChunk, int kThreads, int kLanes>

@@ -694,8 +694,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
 
 template <typename T, int kDim, bool kIds>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
-    constexpr int bytes = Smem<kDim, kIds>::kBytes;
-    static_assert((bytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
+    using S = Smem<kDim, kIds>;
+    static_assert((S::kBytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
+    constexpr int most = std::max(S::kBytes, locate_bytes(kMaxRequests));
+    static_assert(most <= 227 * 1024, "a CTA's shared memory");
+    const int bytes = std::max(S::kBytes, locate_bytes(a.requests));
     a.base_align = kChunk;
     a.tile_rows = tile_rows(a);
     const bool split = attention_rows_splits(a);
@@ -703,7 +706,7 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     a.unit_shift = split ? 2 : 24;  // a unit: one chunk for each warp, or a tile
     a.tile_units = split ? 2 : 0;   // a tile's start and end take about as long as two chunks of each warp
     static SmemOnce once;
-    cudaError_t e = once.set(reinterpret_cast<const void*>(attention_rows_kernel<T, kDim, kIds>), bytes);
+    cudaError_t e = once.set(reinterpret_cast<const void*>(attention_rows_kernel<T, kDim, kIds>), most);
     if (e != cudaSuccess) return e;
     attention_rows_kernel<T, kDim, kIds><<<a.ctas, kThreads, bytes, stream>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess || !split) return e;
@@ -731,7 +734,7 @@ size_t attention_rows_workspace(const AttentionParams& a, int sms, int dim) {
     const int ctas = sms * kCtasPerSm;
     return attn::workspace_records_bytes(ctas) + 2 * static_cast<size_t>(ctas) * attn::partial_floats(kRows, dim) * sizeof(float);
 }
-int attention_max_requests() { return 16384; }
+int attention_max_requests() { return attn::kMaxRequests; }
 int attention_max_ids() { return kMaxIds; }
 
 cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream) {

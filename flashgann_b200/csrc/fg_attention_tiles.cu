@@ -961,6 +961,7 @@ bool encode(CUtensorMap* map, const AttentionParams& a, const void* data, const 
 template <typename T, int kDim>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = Smem<kDim>::kBytes;
+    static_assert(bytes >= locate_bytes(kMaxRequests), "the scan over the requests fits the tiles' room");
     static SmemOnce once;
     cudaError_t e = once.set(reinterpret_cast<const void*>(attention_tiles_kernel<T, kDim>), bytes);
     if (e != cudaSuccess) return e;

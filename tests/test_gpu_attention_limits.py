@@ -1,0 +1,88 @@
+"""The cache and attention operators on the GPU at the ends of what they promise: batches of thousands of requests,
+sums that pass 32 bits, scores far apart in 16-bit weights.  References are the definitions in 64 bits; tolerances
+are those of test_gpu_attention.py, and stated at the test where they differ."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from tests.test_gpu_attention import _cuda, _dt, _run, U
+
+pytestmark = pytest.mark.gpu
+
+
+def _batch(rng, requests, *, heads, kv_heads, dim, page, new, ctx):
+    """Requests with up to ctx tokens in the cache and up to new more each, a third of them without any; all pages are
+    drawn from a small cache, so that requests share them (as prefixes do)."""
+    pages = 97
+    c = rng.integers(0, ctx + 1, requests)
+    n = rng.integers(1, new + 1, requests) * (rng.random(requests) < 2 / 3)
+    n[rng.integers(0, requests)] = 1
+    start = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    width = -(-(ctx + new) // page)
+
+    def draw(*shape):  # multiples of 1/32 up to +-4: exact in both types
+        return np.clip(np.round(rng.standard_normal(shape) * 32) / 32, -3.96875, 3.96875).astype(np.float32)
+
+    return dict(q=draw(int(start[-1]), heads, dim), k=draw(pages, page, kv_heads, dim), v=draw(pages, page, kv_heads, dim),
+                table=rng.integers(0, pages, (requests, width)).astype(np.int32), start=start,
+                kv_len=(c + n).astype(np.int32))
+
+
+def _ref64(x, *, window=-1, sinks=0, ids=None, at=4096):
+    """(out, lse) of every row in 64 bits on the GPU, `at` rows at a time."""
+    import torch
+    q, k, v, table = (_cuda(x[n]) for n in ("q", "k", "v", "table"))
+    start, kv_len = _cuda(x["start"]).long(), _cuda(x["kv_len"]).long()
+    T, heads, dim = q.shape
+    page, H = k.shape[1], k.shape[2]
+    t = torch.arange(T, device="cuda")
+    r = torch.searchsorted(start[1:].contiguous(), t, right=True)
+    p = kv_len[r] - start[r + 1] + t
+    j = torch.arange(int(kv_len.max()), device="cuda")
+    outs, lses = [], []
+    for lo in range(0, T, at):
+        rr, pp = r[lo:lo + at], p[lo:lo + at, None]
+        pg = table[rr[:, None], (j // page)[None, :]].long()
+        see = j[None] <= pp
+        if window >= 0:
+            see = see & ((pp - j[None] < window) | (j[None] < sinks))
+        see = see[:, None].expand(-1, heads, -1)
+        if ids is not None:
+            got = _cuda(ids[lo:lo + at]).long()
+            mark = torch.zeros((*got.shape[:2], len(j) + 1), dtype=torch.bool, device="cuda")
+            mark.scatter_(2, torch.where((got < 0) | (got > pp[:, None]), len(j), got), True)
+            see = see | mark[..., :-1]
+        kk = k[pg, j % page].double().repeat_interleave(heads // H, 2)
+        s = torch.einsum("thd,tjhd->thj", q[lo:lo + at].double(), kk) * dim ** -0.5
+        s = s.masked_fill(~see, -np.inf)
+        vv = v[pg, j % page].double().repeat_interleave(heads // H, 2)
+        outs.append(torch.einsum("thj,tjhd->thd", torch.softmax(s, -1).nan_to_num(0.0), vv))
+        lses.append(torch.logsumexp(s, -1))
+    return torch.cat(outs), torch.cat(lses)
+
+
+def _close(got, want, dtype, vmax=4.0):
+    import torch
+    (out, lse), (o, l) = got, want
+    assert torch.equal(torch.isneginf(lse.double()), torch.isneginf(l))
+    fine = torch.isfinite(l)
+    assert torch.isfinite(out.float()).all()
+    assert ((out.double() - o).abs() <= (2 * U[dtype] + 2e-4) * vmax).all(), float((out.double() - o).abs().max())
+    assert ((lse.double() - l)[fine].abs() <= 2e-4).all()
+
+
+# ---- many requests: the scan over their lengths ----
+
+@pytest.mark.parametrize("requests,dim,dtype", [(12224, 64, "bf16"), (12225, 64, "fp16"), (16384, 64, "bf16"),
+                                                (16384, 96, "fp16"), (16384, 128, "bf16")])
+def test_as_many_requests_as_there_may_be(requests, dim, dtype):
+    """The sums over 16384 requests take 64 KB of shared memory, more than the keys of the smallest head size do."""
+    rng = np.random.default_rng(requests + dim)
+    x = _batch(rng, requests, heads=2, kv_heads=1, dim=dim, page=16, new=1, ctx=30)
+    _close(_run(x, dtype), _ref64(x), dtype)
+    ids = rng.integers(-1, 40, (x["q"].shape[0], 2, 6)).astype(np.int32)
+    _close(_run(x, dtype, ids=ids, window=3, sinks=1), _ref64(x, ids=ids, window=3, sinks=1), dtype)
+    # the kernel of many rows, for the same requests
+    _close(_run(x, dtype, max_new=1000, window=9), _ref64(x, window=9), dtype)
