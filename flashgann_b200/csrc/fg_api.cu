@@ -871,6 +871,30 @@ bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
     return !retrieved && many_rows(c, x) && x->scale > 0.f && c->page_size >= 8 && !expanded;
 }
 
+// Counts, mask and scale: everything that the choice of a kernel and the size of its workspace are computed from.
+int check_counts(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
+    if (x->tokens < 0 || x->requests < 0 || x->table_width < 0 || x->max_new < 0)
+        return fail(FG_ERR_ARG, "bad attention shape tokens=%d requests=%d table_width=%d max_new=%d", x->tokens,
+                    x->requests, x->table_width, x->max_new);
+    if (x->heads < 1 || x->heads % c->heads)
+        return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", x->heads, c->heads);
+    if (x->heads / c->heads > 256) return fail(FG_ERR_UNSUPPORTED, "%d query heads for each kv head", x->heads / c->heads);
+    if (static_cast<int64_t>(x->tokens) * (x->heads / c->heads) > INT32_MAX - 512)
+        return fail(FG_ERR_UNSUPPORTED, "%d tokens of %d heads for each kv head", x->tokens, x->heads / c->heads);
+    if (x->requests > fg::attention_max_requests())
+        return fail(FG_ERR_UNSUPPORTED, "%d requests, at most %d", x->requests, fg::attention_max_requests());
+    if (x->window < -1 || x->sinks < 0) return fail(FG_ERR_ARG, "bad mask window=%d sinks=%d", x->window, x->sinks);
+    if (!(std::fabs(x->scale) <= FLT_MAX)) return fail(FG_ERR_ARG, "scale is not finite");
+    if (retrieved) {
+        if (x->window < 0) return fail(FG_ERR_ARG, "retrieved attention needs a window >= 0");
+        if (x->ids_count < 0 || x->ids_token_stride < 0 || x->ids_head_stride < 0)
+            return fail(FG_ERR_ARG, "bad ids: count %d, or a negative stride", x->ids_count);
+        if (x->ids_count > fg::attention_max_ids())
+            return fail(FG_ERR_UNSUPPORTED, "%d ids for each row, at most %d", x->ids_count, fg::attention_max_ids());
+    }
+    return FG_OK;
+}
+
 int workspace_bytes(const fg_kv_cache* c, const fg_attention* x, bool retrieved, uint64_t* bytes) {
     int sms = 0;
     const int rc = sm_count(&sms);
@@ -898,25 +922,7 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     int rc = check_cache(c);
     if (rc) return rc;
     if (!x) return fail(FG_ERR_ARG, "null arguments");
-    if (x->tokens < 0 || x->requests < 0 || x->table_width < 0 || x->max_new < 0)
-        return fail(FG_ERR_ARG, "bad attention shape tokens=%d requests=%d table_width=%d max_new=%d", x->tokens,
-                    x->requests, x->table_width, x->max_new);
-    if (x->heads < 1 || x->heads % c->heads)
-        return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", x->heads, c->heads);
-    if (x->heads / c->heads > 256) return fail(FG_ERR_UNSUPPORTED, "%d query heads for each kv head", x->heads / c->heads);
-    if (static_cast<int64_t>(x->tokens) * (x->heads / c->heads) > INT32_MAX - 512)
-        return fail(FG_ERR_UNSUPPORTED, "%d tokens of %d heads for each kv head", x->tokens, x->heads / c->heads);
-    if (x->requests > fg::attention_max_requests())
-        return fail(FG_ERR_UNSUPPORTED, "%d requests, at most %d", x->requests, fg::attention_max_requests());
-    if (x->window < -1 || x->sinks < 0) return fail(FG_ERR_ARG, "bad mask window=%d sinks=%d", x->window, x->sinks);
-    if (!(std::fabs(x->scale) <= FLT_MAX)) return fail(FG_ERR_ARG, "scale is not finite");
-    if (retrieved) {
-        if (x->window < 0) return fail(FG_ERR_ARG, "retrieved attention needs a window >= 0");
-        if (x->ids_count < 0 || x->ids_token_stride < 0 || x->ids_head_stride < 0)
-            return fail(FG_ERR_ARG, "bad ids: count %d, or a negative stride", x->ids_count);
-        if (x->ids_count > fg::attention_max_ids())
-            return fail(FG_ERR_UNSUPPORTED, "%d ids for each row, at most %d", x->ids_count, fg::attention_max_ids());
-    }
+    if ((rc = check_counts(c, x, retrieved))) return rc;
     if (x->tokens == 0 || x->requests == 0) return FG_OK;
     if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, "q"))) return rc;
     if ((rc = check_rows(x->out, x->out_token_stride, x->out_head_stride, "out"))) return rc;
@@ -1061,8 +1067,7 @@ int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* a
     int rc = check_cache(cache);
     if (rc) return rc;
     if (!args || !bytes) return fail(FG_ERR_ARG, "null argument");
-    if (args->heads < 1 || args->heads % cache->heads)
-        return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", args->heads, cache->heads);
+    if ((rc = check_counts(cache, args, retrieved != 0))) return rc;
     return workspace_bytes(cache, args, retrieved != 0, bytes);
 }
 

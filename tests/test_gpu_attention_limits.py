@@ -86,3 +86,12 @@ def test_as_many_requests_as_there_may_be(requests, dim, dtype):
     _close(_run(x, dtype, ids=ids, window=3, sinks=1), _ref64(x, ids=ids, window=3, sinks=1), dtype)
     # the kernel of many rows, for the same requests
     _close(_run(x, dtype, max_new=1000, window=9), _ref64(x, window=9), dtype)
+
+
+def test_too_many_ids_are_refused():
+    import flashgann_b200 as fg
+    rng = np.random.default_rng(0)
+    x = _batch(rng, 2, heads=2, kv_heads=1, dim=64, page=16, new=1, ctx=30)
+    for count in (1025, 2000):
+        with pytest.raises(fg.FlashGANNError, match=f"{count} ids"):
+            _run(x, "fp16", ids=np.zeros((x["q"].shape[0], 2, count), np.int32), window=3)
