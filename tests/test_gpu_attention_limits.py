@@ -95,3 +95,32 @@ def test_too_many_ids_are_refused():
     for count in (1025, 2000):
         with pytest.raises(fg.FlashGANNError, match=f"{count} ids"):
             _run(x, "fp16", ids=np.zeros((x["q"].shape[0], 2, count), np.int32), window=3)
+
+
+@pytest.mark.parametrize("requests", [4, 5, 32, 33, 64, 65, 128, 129, 257, 513, 2000])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype", [(6, 2, 96, 8, "fp16"), (4, 4, 64, 16, "bf16"), (8, 1, 128, 32, "bf16")])
+def test_batches_around_the_scans_steps(requests, heads, kv_heads, dim, page, dtype):
+    """One warp scans up to 32 requests (4 in the kernel of many rows), the block 128 (64) at a time: sizes at and past
+    each of these, requests without tokens among them, in both kernels and with ids."""
+    rng = np.random.default_rng(requests * heads)
+    x = _batch(rng, requests, heads=heads, kv_heads=kv_heads, dim=dim, page=page, new=3, ctx=70)
+    for window, sinks in [(-1, 0), (20, 3)]:
+        want = _ref64(x, window=window, sinks=sinks)
+        for max_new in (1, 1000):
+            _close(_run(x, dtype, window=window, sinks=sinks, max_new=max_new), want, dtype)
+    ids = rng.integers(-1, 90, (x["q"].shape[0], heads, 9)).astype(np.int32)
+    _close(_run(x, dtype, ids=ids, window=5, sinks=2), _ref64(x, ids=ids, window=5, sinks=2), dtype)
+
+
+@pytest.mark.parametrize("requests", [7, 65, 150])
+def test_batches_of_chunks_and_long_contexts(requests):
+    """Requests of up to 200 rows and contexts that are split over CTAs, beside short ones."""
+    rng = np.random.default_rng(requests)
+    x = _batch(rng, requests, heads=4, kv_heads=2, dim=64, page=16, new=50, ctx=20)
+    long = rng.integers(0, requests, 2)
+    x["kv_len"][long] += 900
+    x["table"] = rng.integers(0, x["k"].shape[0], (requests, 70)).astype(np.int32)
+    for window, sinks in [(-1, 0), (300, 20)]:
+        want = _ref64(x, window=window, sinks=sinks, at=256)
+        for max_new in (1, 1000):
+            _close(_run(x, "fp16", window=window, sinks=sinks, max_new=max_new), want, "fp16")
