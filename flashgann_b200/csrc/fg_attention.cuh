@@ -328,6 +328,7 @@ template <>
 struct Half2<__half> {
     static constexpr uint32_t kExpMask = 0x7C00u;
     static constexpr uint32_t kFormat = 0;  // as an operand of tcgen05.mma
+    static constexpr bool kNarrow = true;   // ends at 2^-24 and 65504: weights are given room below, see the kernels
     __device__ static __forceinline__ uint32_t pack(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);
@@ -339,6 +340,7 @@ template <>
 struct Half2<__nv_bfloat16> {
     static constexpr uint32_t kExpMask = 0x7F80u;
     static constexpr uint32_t kFormat = 1;
+    static constexpr bool kNarrow = false;
     __device__ static __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&h);

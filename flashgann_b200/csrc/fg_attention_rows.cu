@@ -182,6 +182,10 @@ template <typename T, int kDim, bool kIds>
 struct Warp {
     using S = Smem<kDim, kIds>;
     static constexpr int kPieces = kDim / 8;              // 16-byte pieces of a row
+    // A float16 weight below 2^-25 would be zero in the product while the sum l counts it: many keys far below the
+    // maximum would be lost.  Weights and o are 2^15 times as large there, exactly, until the warps join, so that those
+    // down to 2^-29 keep their relative precision and those down to 2^-40 count.
+    static constexpr float kLift = Half2<T>::kNarrow ? 32768.f : 1.f;
 
     const AttentionParams& a;
     const int lane;
@@ -504,8 +508,8 @@ struct Warp {
             l[x] += (e0 + e1) + (e2 + e3);  // this lane's columns; joined over the 4 lanes of a row at the end
             // weights go to the product in the cache's 16-bit type, as the matrix pipe takes them: at most 1, relative
             // rounding 2^-8 (bf16) or 2^-11, in size that of the result's own rounding; the sum l keeps 32 bits
-            pa[x] = Half2<T>::pack(e0, e1);
-            pa[x + 2] = Half2<T>::pack(e2, e3);
+            pa[x] = Half2<T>::pack(e0 * kLift, e1 * kLift);
+            pa[x + 2] = Half2<T>::pack(e2 * kLift, e3 * kLift);
         }
         // keys (lane & 15), dims 8 * (lane >= 16)
         const int vrow = lane & 15, vpiece = lane >> 4;
@@ -620,6 +624,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             w.l[x] += __shfl_xor_sync(0xFFFFFFFFu, w.l[x], 2);
         }
         __syncthreads();
+        constexpr float kUnlift = 1.f / Warp<T, kDim, kIds>::kLift;
         constexpr int kSumPitch = kDim + 4;
         float* sums = reinterpret_cast<float*>(smem);                       // [warp][row][kSumPitch]
         float* stat = sums + kWarps * kRows * kSumPitch;                    // [warp][row][2]
@@ -630,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             float* dst = sums + (warp * kRows + row) * kSumPitch + (lane & 3) * 2;
 #pragma unroll
             for (int n = 0; n < kDim / 8; ++n)
-                *reinterpret_cast<float2*>(dst + n * 8) = make_float2(w.o[n][2 * x], w.o[n][2 * x + 1]);
+                *reinterpret_cast<float2*>(dst + n * 8) = make_float2(w.o[n][2 * x] * kUnlift, w.o[n][2 * x + 1] * kUnlift);
             if ((lane & 3) == 0) {
                 stat[(warp * kRows + row) * 2] = w.m[x];
                 stat[(warp * kRows + row) * 2 + 1] = w.l[x];

@@ -31,10 +31,15 @@
 // 1112 TFLOP/s on the device.  A block takes 3650 cycles, of which the tensor
 // pipe is busy for 2048: each half waits for its own weights.
 //
-// The running maximum that the weights are relative to is raised only when it
-// grows by more than 2^8: then O and the sum are scaled, which costs a round
-// trip of O through registers.  Weights up to 2^8 keep their relative
-// precision in both 16-bit types, and the 32-bit sums have room.
+// The base that the weights are relative to is raised only when the running
+// maximum is more than 2^8 above what it was then: O and the sum are scaled,
+// which costs a round trip of O through registers.  Weights up to 2^8 keep
+// their relative precision in both 16-bit types, and the 32-bit sums have room.
+// float16 ends at 2^-24: a weight below 2^-25 would be zero in the product
+// while the sum counts it, and many keys far below the maximum would be lost.
+// Its base is 2^7 below the maximum, so that weights reach 2^15 and those of
+// 2^-32 of the maximum still count.  It costs nothing: sums, partials and lse
+// are relative to the base in any case.
 //
 // Every wait is bounded: one that runs out marks the CTA, all roles leave
 // their loops, and the rows of the tiles in work get NaN.
@@ -53,6 +58,8 @@ constexpr int kThreads = 512;
 constexpr int kSlots = 5;    // see Loader::block; K and V tiles in the ring: two blocks and a half
 constexpr int kTileBlocks = 3;  // a tile costs about as much as that many blocks beside its own (1 to 4 measured)
 constexpr float kRaise = 8.f;
+template <typename T>
+constexpr float kLift = Half2<T>::kNarrow ? 7.f : 0.f;  // log2 of a float16 weight at the maximum
 
 template <int kDim>
 struct Smem {
@@ -544,8 +551,10 @@ struct Softmax {
             poison = sh->nonfinite[f % kSlots] == 1 + f;
         }
         const float mx = row_max(s);
-        if (__any_sync(0xFFFFFFFFu, !(mx <= m + kRaise) && m == m)) {  // also where mx is NaN: so becomes the row, once
-            const float mn = max3(m, mx, mx);
+        // where the base's own rounding is no longer small beside that room, nothing above the maximum is let pass
+        const float room = kLift<T> + (kLift<T> == 0.f || fabsf(m) < 0x1p20f ? kRaise : 0.f);
+        if (__any_sync(0xFFFFFFFFu, !(mx <= m + room) && m == m)) {  // also where mx is NaN: so becomes the row, once
+            const float mn = max3(m, mx - kLift<T>, mx - kLift<T>);
             if (u != w.u0) {  // the segment's first products write O, all others add to it
                 const float f = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
                 l *= f;

@@ -344,7 +344,8 @@ int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* a
  * exponentials; a row that sees nothing (or only scores of -inf) gets 0 and
  * -inf.  K and V of keys that a row does not see do not touch it, whatever
  * they hold.  Sums are kept in 32 bits; the weights of the second product are
- * rounded to the cache's type.  Results are the same on every run.  Rows past
+ * rounded to the cache's type (those of float16 scaled so that weights of 2^-32
+ * of the largest still count).  Results are the same on every run.  Rows past
  * query_start[requests] are not written.  At most 16384 requests, heads /
  * cache->heads <= 256. */
 int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream);

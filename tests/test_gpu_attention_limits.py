@@ -124,3 +124,37 @@ def test_batches_of_chunks_and_long_contexts(requests):
         want = _ref64(x, window=window, sinks=sinks, at=256)
         for max_new in (1, 1000):
             _close(_run(x, "fp16", window=window, sinks=sinks, max_new=max_new), want, "fp16")
+
+
+# ---- weights in 16 bits ----
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("depth", [12.0, 17.5, 20.0])
+@pytest.mark.parametrize("kernel", ["rows", "tiles"])
+def test_many_keys_far_below_the_maximum(kernel, depth, dtype):
+    """Four keys with a score of `depth` before half a million with a score of 0: e^-17.5 is below half of float16's
+    least number, but all of them together are 0.3 % of the sum, and the output is that share of their value.  One
+    tile to a CTA, so that each warp (each row) meets a maximum first and the tail after it.  Beside the usual
+    tolerances: a lane's running sum of about 1 takes up to 8192 addends, each rounded to 2^-24."""
+    import torch
+    import flashgann_b200 as fg
+    n, page, dim = 1 << 19, 64, 64
+    requests, heads, new = (37, 8, 1) if kernel == "rows" else (37, 4, 20)  # 296 or 148 tiles
+    dt = _dt(dtype)
+    k, v = (torch.zeros((2, page, heads, dim), dtype=dt, device="cuda") for _ in range(2))
+    k[0, ::16, :, 0] = 1.0                  # the first page: every 16th key
+    v[..., :32] = 1.0                       # half of the columns hold the tail's value and nothing of the four keys'
+    v[0, ::16, :, :32] = 0.0
+    v[0, ::16, :, 32:] = 1.0                # the others the reverse
+    q = torch.zeros((requests * new, heads, dim), dtype=dt, device="cuda")
+    q[..., 0] = 1.0
+    table = torch.ones((requests, n // page), dtype=torch.int32, device="cuda")
+    table[:, 0] = 0
+    start = torch.arange(0, requests * new + 1, new, dtype=torch.int32, device="cuda")
+    kv_len = torch.full((requests,), n, dtype=torch.int32, device="cuda")
+    out, lse = fg.paged_attention(q, k, v, table, start, kv_len, new, scale=depth, return_lse=True)
+    tail = (torch.arange(n - new, n, device="cuda").double() + 1 - 4).repeat(requests)[:, None, None] * np.exp(-depth)
+    want = torch.cat([(tail / (4 + tail)).expand(-1, heads, 32), (4 / (4 + tail)).expand(-1, heads, 32)], 2)
+    tol = 2 * U[dtype] + 2e-4
+    assert ((out.double() - want).abs() <= tol).all(), float((out.double() - want).abs().max())
+    assert ((lse.double() - (depth + torch.log(4 + tail[..., 0]))).abs() <= 2e-4 + 8192 * 2.0 ** -24).all()
