@@ -860,15 +860,29 @@ int sm_count(int* sms) {
 // would read the keys once for each 16 rows, and the tiles kernel takes them
 // 256 at a time.  That one folds the scale into its maxima, so it needs a
 // positive one; its copies are whole groups of 8 rows of a page, and take no
-// axis of stride 0 (an expanded tensor).
+// axis of stride 0 (an expanded tensor); its sums of work are 32 bits.
 bool many_rows(const fg_kv_cache* c, const fg_attention* x) {
     return static_cast<int64_t>(x->max_new) * (x->heads / c->heads) > 16;
+}
+fg::AttentionParams counts(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
+    fg::AttentionParams a;
+    a.table_width = x->table_width;
+    a.page_size = c->page_size;
+    a.window = x->window;
+    a.sinks = x->sinks;
+    a.group = x->heads / c->heads;
+    a.ids_count = retrieved ? x->ids_count : 0;
+    a.requests = x->requests;
+    a.tokens = x->tokens;
+    a.kv_heads = c->heads;
+    return a;
 }
 bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
     const bool expanded = (c->token_stride == 0 && c->page_size > 1) || (c->head_stride == 0 && c->heads > 1) ||
                           (c->page_stride == 0 && c->pages > 1) || (x->q_token_stride == 0 && x->tokens > 1) ||
                           (x->q_head_stride == 0 && x->heads > 1);
-    return !retrieved && many_rows(c, x) && x->scale > 0.f && c->page_size >= 8 && !expanded;
+    return !retrieved && many_rows(c, x) && x->scale > 0.f && c->page_size >= 8 && !expanded &&
+           fg::attention_tiles_counts(counts(c, x, retrieved));
 }
 
 // Counts, mask and scale: everything that the choice of a kernel and the size of its workspace are computed from.
@@ -903,16 +917,7 @@ int workspace_bytes(const fg_kv_cache* c, const fg_attention* x, bool retrieved,
         *bytes = fg::attention_tiles_workspace(sms, c->dim);
         return FG_OK;
     }
-    fg::AttentionParams a;  // what decides whether tiles are split
-    a.table_width = x->table_width;
-    a.page_size = c->page_size;
-    a.window = x->window;
-    a.sinks = x->sinks;
-    a.group = x->heads / c->heads;
-    a.ids_count = retrieved ? x->ids_count : 0;
-    a.requests = x->requests;
-    a.tokens = x->tokens;
-    a.kv_heads = c->heads;
+    fg::AttentionParams a = counts(c, x, retrieved);  // what decides whether tiles are split
     a.ctas = sms;
     *bytes = fg::attention_rows_workspace(a, sms, c->dim);
     return FG_OK;

@@ -61,7 +61,8 @@ __host__ __device__ inline size_t partial_floats(int rows, int dim) { return sta
 // sum for each request.  A launch of more requests than its kernel's other
 // uses have room for asks for this much instead.
 constexpr int kMaxRequests = 16384;
-__host__ __device__ constexpr int locate_bytes(int requests) { return (64 + requests) * static_cast<int>(sizeof(int)); }
+template <typename Sum>
+__host__ __device__ constexpr int locate_bytes(int requests) { return (64 + requests) * static_cast<int>(sizeof(Sum)); }
 
 // One request as every kernel reads it, clamped to the buffers the launch was given.
 struct Request {
@@ -171,8 +172,8 @@ struct Place {
 };
 
 // a / b, without a 64-bit division where 32 bits will do
-__device__ __forceinline__ int64_t divide(int64_t a, uint32_t b) {
-    if ((a >> 32) == 0) return static_cast<uint32_t>(a) / b;
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
     return a / b;
 }
 // total * c / ctas
@@ -182,15 +183,18 @@ __device__ __forceinline__ int64_t share(int64_t total, int c, int ctas) {
     return each * c + rest * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);  // both below 2^16
 }
 
-// Called by all kThreads threads; scratch holds locate_bytes(requests).  kLanes
+// Called by all kThreads threads; scratch holds locate_bytes(requests).  Sum
+// holds the units of a kv head: 64 bits where thousands of requests may share a
+// context of millions of keys or a prompt may have 2^19 tiles, 32 where the host
+// keeps such calls away.  kLanes
 // threads count the tiles of a request: 1 where requests are short, 8 where
 // they have many tiles.
-template <int kRows, Layout kLayout, int kChunk, int kThreads, int kLanes>
-__device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, int cta, int ctas) {
-    int* pre = scratch + 64;  // inclusive prefix of the requests' units
+template <int kRows, Layout kLayout, int kChunk, int kThreads, int kLanes, typename Sum>
+__device__ __forceinline__ Place locate(const AttentionParams& a, Sum* scratch, int cta, int ctas) {
+    Sum* pre = scratch + 64;  // inclusive prefix of the requests' units
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kWarps = kThreads / 32;
-    int carry = 0, few = 0;
+    Sum carry = 0, few = 0;
     if (a.requests <= 32 / kLanes) {  // every warp on its own, without a barrier
         if (lane / kLanes < a.requests) {
             const Request r = load_request(a, lane / kLanes);
@@ -199,14 +203,14 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
         }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(0xFFFFFFFFu, few, d);
+            const Sum v = __shfl_up_sync(0xFFFFFFFFu, few, d);
             if (lane >= d) few += v;
         }
         carry = __shfl_sync(0xFFFFFFFFu, few, 31);
     } else {
         for (int b0 = 0; b0 < a.requests; b0 += kThreads / kLanes) {
             const int b = b0 + tid / kLanes;
-            int s = 0;
+            Sum s = 0;
             if (b < a.requests) {
                 const Request r = load_request(a, b);
                 const int n = Tiles<kRows, kLayout>::count(a, r);
@@ -214,14 +218,14 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
             }
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const int v = __shfl_up_sync(0xFFFFFFFFu, s, d);
+                const Sum v = __shfl_up_sync(0xFFFFFFFFu, s, d);
                 if (lane >= d) s += v;
             }
             if (lane == 31) scratch[warp] = s;
             __syncthreads();
-            int before = carry, sum = 0;
+            Sum before = carry, sum = 0;
             for (int w = 0; w < kWarps; ++w) {
-                const int v = scratch[w];
+                const Sum v = scratch[w];
                 if (w < warp) before += v;
                 sum += v;
             }
@@ -240,12 +244,12 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
     }
     x.unit = share(x.total, cta, x.ctas);
     x.end = share(x.total, cta + 1, x.ctas);
-    x.head = static_cast<int>(divide(x.unit, static_cast<uint32_t>(per_head)));
-    int rest = static_cast<int>(x.unit - x.head * per_head);
+    x.head = static_cast<int>(divide(x.unit, per_head));
+    Sum rest = static_cast<Sum>(x.unit - x.head * per_head);  // units before the range, of this head
     int lo = 0, hi = a.requests - 1;  // first request whose inclusive prefix exceeds rest
     if (a.requests <= 32 / kLanes) {
         lo = (__ffs(__ballot_sync(0xFFFFFFFFu, few > rest)) - 1) / kLanes;
-        const int before = __shfl_sync(0xFFFFFFFFu, few, max(lo * kLanes - 1, 0));
+        const Sum before = __shfl_sync(0xFFFFFFFFu, few, max(lo * kLanes - 1, 0));
         if (lo > 0) rest -= before;
     } else {
         while (lo < hi) {
@@ -260,6 +264,7 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
     // the tile that holds unit `rest` of the request, 32 tiles at a time, in every warp
     const int tiles = Tiles<kRows, kLayout>::count(a, r);
     int t = 0;
+    bool found = false;
     for (int t0 = 0; t0 < tiles; t0 += 32) {
         const int mine = t0 + lane;
         const int u = mine < tiles ? tile_keys<kRows, kLayout, kChunk>(a, r, mine).units : 0;
@@ -274,13 +279,14 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, 
             const int first = __ffs(past) - 1;
             t = t0 + first;
             rest -= __shfl_sync(0xFFFFFFFFu, s - u, first);
+            found = true;
             break;
         }
         t = min(t0 + 32, tiles) - 1;
         rest -= __shfl_sync(0xFFFFFFFFu, s, 31);
     }
     x.tile = t;
-    x.offset = rest;
+    x.offset = found && rest > 0 ? static_cast<int>(rest) : 0;  // always found, unless query_start is not ascending and sums wrapped
     return x;
 }
 
@@ -291,7 +297,8 @@ __device__ __forceinline__ TileRecord tile_record(const AttentionParams& a, cons
     if (c == 0 || x.unit >= x.end || x.offset <= a.tile_units) return rec;
     const int64_t before = share(x.total, c - 1, x.ctas);  // where the CTA before starts
     if (before > first + a.tile_units) return rec;      // an earlier CTA's range starts inside the tile too
-    const int end = static_cast<int>((last * x.ctas - 1) / x.total);  // the CTA whose range holds the tile's last unit
+    // the CTA whose range holds the tile's last unit
+    const int end = static_cast<int>(min((last * x.ctas - 1) / x.total, static_cast<int64_t>(x.ctas - 1)));
     rec.parts = end - c + 2;
     rec.before = 2 * (c - 1) + (before >= first ? 0 : 1);  // its second segment unless its range starts with this tile
     rec.head = x.head;

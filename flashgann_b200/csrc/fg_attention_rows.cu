@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     char* ws = static_cast<char*>(a.workspace);
 
     asm volatile("griddepcontrol.launch_dependents;");
-    const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kThreads, 1, int64_t>(a, reinterpret_cast<int64_t*>(smem), blockIdx.x, a.ctas);
     __syncthreads();  // the rings overlay the scan
     if (pl.unit >= pl.end) {
         if (threadIdx.x == 0 && ws) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
@@ -701,9 +701,9 @@ template <typename T, int kDim, bool kIds>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     using S = Smem<kDim, kIds>;
     static_assert((S::kBytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
-    constexpr int most = std::max(S::kBytes, locate_bytes(kMaxRequests));
+    constexpr int most = std::max(S::kBytes, locate_bytes<int64_t>(kMaxRequests));
     static_assert(most <= 227 * 1024, "a CTA's shared memory");
-    const int bytes = std::max(S::kBytes, locate_bytes(a.requests));
+    const int bytes = std::max(S::kBytes, locate_bytes<int64_t>(a.requests));
     a.base_align = kChunk;
     a.tile_rows = tile_rows(a);
     const bool split = attention_rows_splits(a);

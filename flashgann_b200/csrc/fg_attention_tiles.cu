@@ -43,6 +43,8 @@
 //
 // Every wait is bounded: one that runs out marks the CTA, all roles leave
 // their loops, and the rows of the tiles in work get NaN.
+#include <algorithm>
+
 #include <cuda.h>
 
 #include "fg_attention.cuh"
@@ -712,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                        const __grid_constant__ CUtensorMap v_map, const int box_shift) {
     using S = Smem<kDim>;
-    extern __shared__ char dynamic[];
+    extern __shared__ __align__(16) char dynamic[];
     __shared__ Shared shared;
     Shared* sh = &shared;
     const uint32_t raw = smem_addr(dynamic);
@@ -721,7 +723,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     char* ws = static_cast<char*>(a.workspace);
 
     asm volatile("griddepcontrol.launch_dependents;");
-    const Place pl = locate<kRows, kTokens, kBlock, kThreads, 8>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, kTokens, kBlock, kThreads, 8, int>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
     if (pl.unit >= pl.end) {
         if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
         return;
@@ -970,7 +972,7 @@ bool encode(CUtensorMap* map, const AttentionParams& a, const void* data, const 
 template <typename T, int kDim>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = Smem<kDim>::kBytes;
-    static_assert(bytes >= locate_bytes(kMaxRequests), "the scan over the requests fits the tiles' room");
+    static_assert(bytes >= locate_bytes<int>(kMaxRequests), "the scan over the requests fits the tiles' room");
     static SmemOnce once;
     cudaError_t e = once.set(reinterpret_cast<const void*>(attention_tiles_kernel<T, kDim>), bytes);
     if (e != cudaSuccess) return e;
@@ -1004,6 +1006,15 @@ cudaError_t by_dim(const AttentionParams& a, cudaStream_t s) {
 
 }  // namespace
 }  // namespace attn
+
+// Whether the kernel's 32-bit sums of blocks hold a call: 2^31 blocks would take it ten seconds, but the table's width
+// and the counts do not exclude them.  (64-bit sums cost every call: 2048 tokens on 8192 280.5 us for 277.2, 24 chunks
+// under a window 139 for 134.)
+bool attention_tiles_counts(const AttentionParams& a) {
+    const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.table_width) * a.page_size, INT32_MAX);
+    const int64_t tiles = static_cast<int64_t>(a.tokens) / (attn::kRows / a.group) + a.requests;
+    return tiles * (keys / attn::kBlock + 4 + attn::kTileBlocks) <= INT32_MAX;
+}
 
 size_t attention_tiles_workspace(int sms, int dim) {
     const int ctas = sms;

@@ -147,6 +147,7 @@ int attention_max_ids();
 bool attention_rows_splits(const AttentionParams& a);
 size_t attention_rows_workspace(const AttentionParams& a, int sms, int dim);  // 0 where nothing is split
 cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream);
+bool attention_tiles_counts(const AttentionParams& a);
 size_t attention_tiles_workspace(int sms, int dim);
 cudaError_t launch_attention_tiles(const AttentionParams& a, cudaStream_t stream);
 

@@ -158,3 +158,48 @@ def test_many_keys_far_below_the_maximum(kernel, depth, dtype):
     tol = 2 * U[dtype] + 2e-4
     assert ((out.double() - want).abs() <= tol).all(), float((out.double() - want).abs().max())
     assert ((lse.double() - (depth + torch.log(4 + tail[..., 0]))).abs() <= 2e-4 + 8192 * 2.0 ** -24).all()
+
+
+# ---- sums of work past 32 bits ----
+
+def test_more_than_2_to_the_31_units_of_work():
+    """4096 requests of 35 million keys each, 2.2e9 units of 64 keys for a kv head; all but the first page of a request
+    are missing, so that little is read.  (Eight seconds: every chunk is walked.)"""
+    import torch
+    import flashgann_b200 as fg
+    requests, page, dim, n = 4096, 4096, 64, 35_000_000
+    g = torch.Generator(device="cuda").manual_seed(9)
+    k, v, q = ((torch.randn(s, generator=g, device="cuda").clamp(-3.9, 3.9) * 32).round().div(32).half()
+               for s in ((1, page, 1, dim), (1, page, 1, dim), (requests, 1, dim)))
+    table = torch.full((1, -(-n // page)), -1, dtype=torch.int32, device="cuda")
+    table[0, 0] = 0
+    start = torch.arange(requests + 1, dtype=torch.int32, device="cuda")
+    kv_len = torch.full((requests,), n, dtype=torch.int32, device="cuda")
+    out = torch.full((requests, 1, dim), 7.0, dtype=torch.float16, device="cuda")
+    _, lse = fg.paged_attention(q, k, v, table.expand(requests, -1), start, kv_len, 1, out=out, return_lse=True)
+    s = q[:, 0].double() @ k[0, :, 0].double().T * dim ** -0.5
+    _close((out, lse), (torch.softmax(s, -1)[:, None] @ v[0, :, 0].double(), torch.logsumexp(s, -1)[:, None]), "fp16")
+
+
+def test_calls_of_2_to_the_31_blocks_leave_the_kernel_of_many_rows():
+    """Its sums of blocks are 32 bits: where the counts do not exclude more, the other kernel takes the call, as the
+    size of the workspace shows."""
+    import ctypes
+    import flashgann_b200 as fg
+    from tests.test_attention_args import _args, _cache
+
+    def need(**kw):
+        n = ctypes.c_uint64()
+        kw = dict(dict(window=-1, heads=2, requests=16384, tokens=16384, table_width=1 << 20), **kw)
+        assert fg.lib().fg_attention_workspace_bytes(_cache(page_size=16), _args(**kw), 0, ctypes.byref(n)) == fg.FG_OK
+        return n.value
+
+    few = need(max_new=1)
+    assert need(max_new=1000, table_width=1 << 19) != few   # 16384 requests of 2^23 keys: 1.1e9 blocks
+    assert need(max_new=1000) == few                        # twice as many
+    # all positions that there are, for 100 and for 128 requests
+    assert need(max_new=1000, table_width=1 << 30, requests=100, tokens=100) != few
+    assert need(max_new=1000, table_width=1 << 30, requests=128, tokens=128) == few
+    # one request, of 2^13 and of 2^14 tiles
+    assert need(max_new=1000, tokens=1 << 21, requests=1) != few
+    assert need(max_new=1000, tokens=1 << 22, requests=1) == few
