@@ -41,8 +41,11 @@
 // 2^-32 of the maximum still count.  It costs nothing: sums, partials and lse
 // are relative to the base in any case.
 //
-// Every wait is bounded: one that runs out marks the CTA, all roles leave
-// their loops, and the rows of the tiles in work get NaN.
+// Every wait is bounded: one that runs out marks the CTA, which ends the other
+// roles' waits too.  Nothing is loaded or issued from then on, and the warps that
+// did leave once their copies and products have ended; the softmax warps walk on
+// to the end of the CTA's range without waiting and write NaN for all of its rows
+// that were not stored before.
 #include <algorithm>
 
 #include <cuda.h>
@@ -86,7 +89,6 @@ struct Shared {
     int missing[4];         // 1 + number of the block that has keys in range without a page
     uint32_t boxes[4];      // of block n % 4: bit i, copy i found its page
     int nonfinite[kSlots];  // 1 + number of the ring item whose V tile infinities or NaN were taken out of
-    int scratch[64];
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -114,27 +116,45 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, int parity) {
 __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
 }
-// false: the wait ran out
-__device__ __forceinline__ bool bar_wait(uint64_t* b, int parity, Shared* sh) {
+__device__ __forceinline__ volatile int* stalled(Shared* sh) { return &sh->stalled; }
+// For the softmax warps.  A lane whose wait runs out, or that finds that
+// another's did, is late and goes on without waiting any more: no vote, and the
+// warp's lanes stay together.
+__device__ __forceinline__ void bar_wait(const AttentionParams& a, uint64_t* b, int parity, Shared* sh, bool* late) {
+    if (*late) return;
     for (int i = 0; !bar_try(b, parity); ++i)
-        if (i == (1 << 22)) {
-            *reinterpret_cast<volatile int*>(&sh->stalled) = 1;
+        if (i >= a.wait_tries || *stalled(sh)) {
+            *stalled(sh) = 1;
+            *late = true;
+            return;
+        }
+}
+// For the issuing warp.  false in all lanes: the wait ran out, or another's did.
+__device__ __forceinline__ bool bar_wait_all(const AttentionParams& a, uint64_t* b, int parity, Shared* sh) {
+    for (int i = 0; !__all_sync(0xFFFFFFFFu, bar_try(b, parity)); ++i)
+        if (__any_sync(0xFFFFFFFFu, i >= a.wait_tries || *stalled(sh))) {
+            *stalled(sh) = 1;
             return false;
         }
     return true;
 }
 // For waits that nothing hurries: leaves the issue slots to the other warps.
-// They may last as long as a tile (a V tile to be looked through comes after
-// all others: 16 ms in a context of a million keys), the limit is seconds.
-__device__ __forceinline__ bool bar_wait_idle(uint64_t* b, int parity, Shared* sh) {
-    for (int i = 0; !bar_try(b, parity); ++i) {
-        if (i == (1 << 26)) {
-            *reinterpret_cast<volatile int*>(&sh->stalled) = 1;
+// They may last as long as a tile (a V tile to be looked through comes after all
+// others: 16 ms in a context of a million keys), the limit is seconds.
+__device__ __forceinline__ bool bar_wait_idle(const AttentionParams& a, uint64_t* b, int parity, Shared* sh) {
+    for (int i = 0; !__all_sync(0xFFFFFFFFu, bar_try(b, parity)); ++i) {
+        if (__any_sync(0xFFFFFFFFu, i >= a.wait_tries * 16 || *stalled(sh))) {
+            *stalled(sh) = 1;
             return false;
         }
         __nanosleep(50);
     }
     return true;
+}
+// Before a warp leaves: what it started itself, and what ends by itself.
+__device__ __forceinline__ void bar_wait_own(uint64_t* b, int parity) {
+    for (int i = 0; i < (1 << 22) && !bar_try(b, parity); ++i) {
+    }
 }
 
 // ---- tcgen05 ----
@@ -319,6 +339,8 @@ struct Loader {
     const int box, panel;  // this lane's copy
     const int half;
     const CUtensorMap* const map;
+    uint32_t raws = 0;    // bit s: parity of the number of copies that sh->raw[s] told of
+    uint32_t flight = 0;  // the last copies, a byte each: 0x80, 0x40 raw, 0x20 parity, slot
 
     __device__ __forceinline__ Loader(const AttentionParams& args, Shared* s, uint32_t ring_addr, int shift, int h, const CUtensorMap* m)
         : a(args), sh(s), ring(ring_addr), lane(threadIdx.x & 31), box_shift(shift), box((threadIdx.x & 31) / S::kPanels),
@@ -342,8 +364,12 @@ struct Loader {
         const int f = 2 * n + half, slot = f % kSlots;
         // the slot's last content: V of block n - 3 (for K), K of block n - 2 (for V)
         const int e = half == 1 && before ? n - 2 : n - 3;
-        if (e >= 0 && !bar_wait_idle(&sh->used[e & 3], (e >> 2) & 1, sh)) return false;
-        uint64_t* bar = half == 1 && checked ? &sh->raw[slot] : &sh->full[slot];
+        if (e >= 0 && !bar_wait_idle(a, &sh->used[e & 3], (e >> 2) & 1, sh)) return false;
+        const bool to_raw = half == 1 && checked;
+        uint64_t* bar = to_raw ? &sh->raw[slot] : &sh->full[slot];
+        const uint32_t parity = (to_raw ? raws >> slot : f / kSlots) & 1;
+        if (to_raw) raws ^= 1u << slot;
+        flight = flight << 8 | 0x80u | (to_raw ? 0x40u : 0u) | parity << 5 | slot;
         if (lane == 0) {
             if (half == 0 && found != wanted) {
                 uint32_t bits = 0;
@@ -351,12 +377,20 @@ struct Loader {
                 sh->boxes[n & 3] = bits;
                 sh->missing[n & 3] = 1 + n;
             }
-            if (bar != &sh->raw[slot]) bar_arrive3(bar);
+            if (!to_raw) bar_arrive3(bar);
             bar_expect(bar, S::kTile);
         }
         __syncwarp();
         if (mine) load_box(ring + slot * S::kTile + panel * S::kPanelRows + (box << box_shift) * 128, map, bar, panel * 64, j & (a.page_size - 1), w.head, pg);
         return true;
+    }
+    // The copies that may be under way: K of the last two blocks, V of the last three (block() waits for the use of those
+    // before).  They are done when all went well.
+    __device__ __forceinline__ void finish() const {
+        for (int i = 0; i < 2 + half; ++i) {
+            const uint32_t code = flight >> (8 * i);
+            if (code & 0x80u) bar_wait_own(code & 0x40u ? &sh->raw[code & 7u] : &sh->full[code & 7u], (code >> 5) & 1);
+        }
     }
 };
 
@@ -381,7 +415,7 @@ struct Helper {
     // in the ring.
     __device__ __forceinline__ bool clear_masked(const Walk& w, int j0, int limit, int f) {
         const int slot = f % kSlots;
-        if (!bar_wait_idle(&sh->raw[slot], (looked >> slot) & 1, sh)) return false;
+        if (!bar_wait_idle(a, &sh->raw[slot], (looked >> slot) & 1, sh)) return false;
         looked ^= 1u << slot;
         const uint32_t base = ring + slot * S::kTile;
         const int p = tid & 15;
@@ -470,6 +504,7 @@ struct Softmax {
     const uint32_t score, output;  // TMEM addresses of this warp's lanes
     const int row;        // of the tile
     float m, l;           // base of the weights, their sum
+    bool late = false;    // see bar_wait
     int done = 0;         // blocks of this half so far, over all tiles
     int settled = 0;      // of them, those whose products pv_done tells of: a segment's last, and with a V tile looked through
     const int box_shift;
@@ -514,10 +549,10 @@ struct Softmax {
         if ((threadIdx.x & 31) == 0) bar_arrive(&sh->p_full[half][part]);
     }
 
-    // block u of the walk's tile, number n in the CTA; false: stalled
-    __device__ __forceinline__ bool block(const Walk& w, int u, int n, int p, const Span& mine) {
+    // block u of the walk's tile, number n in the CTA
+    __device__ __forceinline__ void block(const Walk& w, int u, int n, int p, const Span& mine) {
         // the scores are there, and with them the products of the block before have reached O
-        if (!bar_wait(&sh->s_full[half], done & 1, sh)) return false;
+        bar_wait(a, &sh->s_full[half], done & 1, sh, &late);
         tmem_fence_after();
         float s[kBlock];
 #pragma unroll
@@ -549,7 +584,7 @@ struct Softmax {
         }
         if (checked) {  // the V tile was looked through
             const int f = 2 * n + 1;
-            if (!bar_wait(&sh->full[f % kSlots], (f / kSlots) & 1, sh)) return false;
+            bar_wait(a, &sh->full[f % kSlots], (f / kSlots) & 1, sh, &late);
             poison = sh->nonfinite[f % kSlots] == 1 + f;
         }
         const float mx = row_max(s);
@@ -585,13 +620,12 @@ struct Softmax {
         ++done;
         if (checked || u + 1 == w.u1) ++settled;
         if (poison) {
-            if (!bar_wait(&sh->pv_done[half], (settled - 1) & 1, sh)) return false;
+            bar_wait(a, &sh->pv_done[half], (settled - 1) & 1, sh, &late);
             tmem_fence_after();
             add_nonfinite(w, u, n, p);
             tmem_store_wait();
             tmem_fence_before();
         }
-        return true;
     }
 
     // Infinities and NaN that the loader took out of V, for the rows that see them.
@@ -643,9 +677,11 @@ struct Softmax {
     }
 
     // The segment's end: this thread's row of O to the output or, for part of a tile, to the workspace.
-    __device__ __forceinline__ bool store(const Walk& w, bool ok) {
-        if (ok) ok = bar_wait(&sh->pv_done[half], (settled - 1) & 1, sh);
+    __device__ __forceinline__ void store(const Walk& w) {
+        bar_wait(a, &sh->pv_done[half], (settled - 1) & 1, sh, &late);
         tmem_fence_after();
+        // after another warp of the half was late, products may have been issued before this one's weights were there
+        const bool ok = !__any_sync(0xFFFFFFFFu, late || *stalled(sh));
         int i = 0, g = 0;
         const bool valid = Tiles<kRows, kTokens>::row(a, w.req, w.tile, row, &i, &g);
         const int64_t token = w.req.start + i;
@@ -705,7 +741,6 @@ struct Softmax {
             part[kRows * kDim + kRows + row] = ok ? l : NAN;
         }
         tmem_fence_before();
-        return ok;
     }
 };
 
@@ -765,7 +800,6 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         Softmax<T, kDim> sm(a, sh, tmem, box_shift);
         int n = 0;
-        bool ok = true;
         do {
             if (sm.half * kHalf >= w.rows) {  // nothing in this half
                 n += w.u1 - w.u0;
@@ -780,9 +814,9 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
             const Span mine = w.seen(from, to);
             sm.m = -INFINITY;
             sm.l = 0.f;
-            for (int u = w.u0; ok && u < w.u1; ++u, ++n) ok = sm.block(w, u, n, p, mine);
-            ok = sm.store(w, ok);
-        } while (w.next() && ok);
+            for (int u = w.u0; u < w.u1; ++u, ++n) sm.block(w, u, n, p, mine);
+            sm.store(w);
+        } while (w.next());
     } else if (warp < 12) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         Helper<T, kDim> hp(a, sh, ring);
@@ -837,12 +871,12 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                     }
                 }
             } at{0, 0};  // the next tile to be used
-            const auto filled = [&](const Turn& t) { return bar_wait(&sh->full[t.slot], t.parity, sh); };
+            const auto filled = [&](const Turn& t) { return bar_wait_all(a, &sh->full[t.slot], t.parity, sh); };
             int n = 0, segment = 0, done[2] = {0, 0};
             bool ok = true;
             do {
                 const int halves = w.rows > kHalf ? 2 : 1, blocks = w.u1 - w.u0;
-                ok = bar_wait(&sh->q_full, segment & 1, sh) && filled(at);
+                ok = bar_wait_all(a, &sh->q_full, segment & 1, sh) && filled(at);
                 if (!ok) break;
                 scores(0, at.slot);
                 if (halves == 2) scores(1, at.slot);
@@ -857,13 +891,13 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                 for (int b = 0; ok && b < blocks; ++b, ++n) {
                     const bool more = b + 1 < blocks;
                     const auto turn = [&](int h) {
-                        ok = bar_wait(&sh->p_full[h][0], done[h] & 1, sh);
+                        ok = bar_wait_all(a, &sh->p_full[h][0], done[h] & 1, sh);
                         if (!ok) return;
                         tmem_fence_after();
                         output(h, v.slot, 0, b > 0);
                         // the block before, told late: a commit takes its time, and here the tensor cores have work
                         if (h == 0 && b > 0) commit(&sh->used[(n - 1) & 3]);
-                        ok = bar_wait(&sh->p_full[h][1], done[h] & 1, sh);
+                        ok = bar_wait_all(a, &sh->p_full[h][1], done[h] & 1, sh);
                         if (!ok) return;
                         tmem_fence_after();
                         output(h, v.slot, 1, true);
@@ -892,21 +926,22 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
             } while (ok && w.next());
             // all products end before the block does, also after a stall
             commit(&sh->drain);
-            for (int i = 0; i < (1 << 22) && !bar_try(&sh->drain, 0); ++i) {
-            }
+            bar_wait_own(&sh->drain, 0);
         } else if (warp == 15) {
             int segment = 0;
             bool ok = true;
             do {
-                ok = bar_wait_idle(&sh->q_empty, (segment & 1) ^ 1, sh);
-                if (ok && lane == 0) {
+                ok = bar_wait_idle(a, &sh->q_empty, (segment & 1) ^ 1, sh);
+                if (!ok) break;
+                if (lane == 0) {
                     const int rows = Tiles<kRows, kTokens>::per(a) * a.group;
                     bar_expect(&sh->q_full, S::kPanels * rows * 128);
                     for (int i = 0; i < S::kPanels; ++i) load_box(q + i * S::kQPanel, &q_map, &sh->q_full, i * 64, w.head * a.group, w.token, 0);
                 }
                 __syncwarp();
                 ++segment;
-            } while (ok && w.next());
+            } while (w.next());
+            if (segment > 0) bar_wait_own(&sh->q_full, (segment - 1) & 1);
         } else {
             Loader<kDim> ld(a, sh, ring, box_shift, warp - 13, warp == 13 ? &k_map : &v_map);
             int n = 0;
@@ -921,16 +956,15 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
                         next_j0 = w.block(u + 1, &next_limit);
                         next_pg = ld.page(w, next_j0, next_limit);
                     }
-                    ok = ld.block(w, u, j0, limit, pg, n, (firsts >> 1) & 1);
+                    if (warp == 13 && n >= a.lost_block) ok = false;
+                    else ok = ld.block(w, u, j0, limit, pg, n, (firsts >> 1) & 1);
                     firsts = firsts << 1 | (u == w.u0);
                     j0 = next_j0;
                     limit = next_limit;
                     pg = next_pg;
                 }
             } while (ok && w.next());
-            // after a stall: time for the copies under way to end before the block does
-            if (!ok)
-                for (int i = 0; i < (1 << 14); ++i) bar_try(&sh->drain, 0);
+            ld.finish();
         }
         __syncwarp();
     }
@@ -939,6 +973,8 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     tmem_fence_after();
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
+
+std::atomic<int> g_wait_tries{1 << 22}, g_lost_block{INT32_MAX};
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -983,6 +1019,8 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     a.base_align = 1 << box_shift;
     a.unit_shift = 0;
     a.tile_units = kTileBlocks;
+    a.wait_tries = g_wait_tries.load(std::memory_order_relaxed);
+    a.lost_block = g_lost_block.load(std::memory_order_relaxed);
     const int64_t cache_size[3] = {a.page_size, a.kv_heads, a.pages}, cache_stride[3] = {a.token_stride, a.head_stride, a.page_stride};
     const int64_t q_size[3] = {a.heads, a.tokens, 1}, q_stride[3] = {a.q_head_stride, a.q_token_stride, 0};
     CUtensorMap q_map, k_map, v_map;
@@ -1014,6 +1052,11 @@ bool attention_tiles_counts(const AttentionParams& a) {
     const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.table_width) * a.page_size, INT32_MAX);
     const int64_t tiles = static_cast<int64_t>(a.tokens) / (attn::kRows / a.group) + a.requests;
     return tiles * (keys / attn::kBlock + 4 + attn::kTileBlocks) <= INT32_MAX;
+}
+
+void set_attention_waits(int lost_block, int tries) {
+    attn::g_lost_block.store(lost_block, std::memory_order_relaxed);
+    attn::g_wait_tries.store(tries, std::memory_order_relaxed);
 }
 
 size_t attention_tiles_workspace(int sms, int dim) {

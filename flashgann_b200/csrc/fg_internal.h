@@ -141,6 +141,8 @@ struct AttentionParams {
     int unit_shift = 0;     // log2 of the key chunks in a unit of work
     int tile_units = 0;     // what a tile costs beside its chunks, in units
     int tile_rows = 16;     // retrieved form: heads to a tile
+    // kernel of many rows: how often a wait inside a CTA looks again before it gives up; block whose K tile never comes
+    int wait_tries = 0, lost_block = 0;
 };
 int attention_max_requests();
 int attention_max_ids();
@@ -148,6 +150,7 @@ bool attention_rows_splits(const AttentionParams& a);
 size_t attention_rows_workspace(const AttentionParams& a, int sms, int dim);  // 0 where nothing is split
 cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream);
 bool attention_tiles_counts(const AttentionParams& a);
+void set_attention_waits(int lost_block, int tries);  // none and 2^22 unless a test sets them
 size_t attention_tiles_workspace(int sms, int dim);
 cudaError_t launch_attention_tiles(const AttentionParams& a, cudaStream_t stream);
 

@@ -203,3 +203,33 @@ def test_calls_of_2_to_the_31_blocks_leave_the_kernel_of_many_rows():
     # one request, of 2^13 and of 2^14 tiles
     assert need(max_new=1000, tokens=1 << 21, requests=1) != few
     assert need(max_new=1000, tokens=1 << 22, requests=1) == few
+
+
+# ---- waits inside the kernel of many rows ----
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("fp16", 64)])
+def test_a_wait_that_runs_out_shows_in_every_row_it_leaves(dtype, dim):
+    """K tiles from some block of each CTA on are never loaded (a flag that nothing sets): the waits for them run out
+    and the CTAs give up.  Their rows are NaN, whole tiles and parts that are joined alike, and no row keeps what the
+    output held before.  The next call is not touched by it."""
+    import torch
+    import flashgann_b200 as fg
+    rng = np.random.default_rng(dim)
+    for requests, new, ctx, window, sinks in [(1, 300, 6000, -1, 0), (40, 70, 300, -1, 0), (40, 70, 300, 90, 9)]:
+        x = _batch(rng, requests, heads=4, kv_heads=2, dim=dim, page=16, new=new, ctx=ctx)
+        want, want_lse = _ref64(x, window=window, sinks=sinks, at=128)
+        shares = []
+        for first in (0, 1, 2, 3, 5, 9, 1000):
+            out = torch.full(want.shape, 7.0, dtype=_dt(dtype), device="cuda")
+            fg.lib().fg_test_attention_lose_blocks(first)
+            try:
+                _, lse = _run(x, dtype, window=window, sinks=sinks, max_new=1000, out=out)
+                torch.cuda.synchronize()
+            finally:
+                fg.lib().fg_test_attention_lose_blocks(-1)
+            lost = torch.isnan(lse)
+            shares.append(float(lost.float().mean()))
+            assert torch.equal(lost[..., None].expand_as(out), torch.isnan(out))
+            _close((out[~lost][:, None], lse[~lost][:, None]), (want[~lost][:, None], want_lse[~lost][:, None]), dtype)
+        assert shares[0] == 1.0 and shares[-1] == 0.0 and sorted(shares, reverse=True) == shares
+        _close(_run(x, dtype, window=window, sinks=sinks, max_new=1000), (want, want_lse), dtype)
