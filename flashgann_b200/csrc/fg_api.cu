@@ -1,6 +1,7 @@
 // fg_api.cu -- the C ABI (include/flashgann.h): index residency, search
 // launches, and the host helpers of the reference CLI.
 #include <algorithm>
+#include <array>
 #include <cfloat>
 #include <chrono>
 #include <cmath>
@@ -843,9 +844,21 @@ int check_rows(const void* p, int64_t token_stride, int64_t head_stride, const c
     return FG_OK;
 }
 
-// whether rows of `dim` elements that are written may overlap along an axis of `count` rows
-bool overlaps(int64_t stride, int64_t count, int32_t dim) {
-    return count > 1 && stride < dim;
+// Whether rows of `dim` elements that are written may overlap.  Axes (stride, entries) nest where each one's stride
+// passes what the axes with smaller strides cover together; other layouts count as overlapping.
+struct Axis {
+    int64_t stride = 0, count = 0;
+};
+bool overlaps(std::array<Axis, 3> axis, int64_t dim) {
+    std::sort(axis.begin(), axis.end(), [](const Axis& x, const Axis& y) { return x.stride < y.stride; });
+    int64_t covered = dim;
+    for (const Axis& x : axis) {
+        if (x.count <= 1) continue;
+        if (x.stride < covered) return true;
+        int64_t more;
+        if (__builtin_mul_overflow(x.count - 1, x.stride, &more) || __builtin_add_overflow(covered, more, &covered)) return true;
+    }
+    return false;
 }
 
 int sm_count(int* sms) {
@@ -931,7 +944,7 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     if (x->tokens == 0 || x->requests == 0) return FG_OK;
     if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, "q"))) return rc;
     if ((rc = check_rows(x->out, x->out_token_stride, x->out_head_stride, "out"))) return rc;
-    if (overlaps(x->out_token_stride, x->tokens, c->dim) || overlaps(x->out_head_stride, x->heads, c->dim))
+    if (overlaps({{{x->out_token_stride, x->tokens}, {x->out_head_stride, x->heads}}}, c->dim))
         return fail(FG_ERR_ARG, "rows of out overlap");
     if (!x->query_start || !x->kv_len || (!x->block_table && x->table_width > 0) || (retrieved && !x->ids && x->ids_count))
         return fail(FG_ERR_ARG, "null buffer");
@@ -1008,6 +1021,7 @@ int fg_kv_plan_device(const int32_t* d_ctx_len, const int32_t* d_new_len, int32_
     if (!d_ctx_len || !d_new_len || !d_query_start || !d_kv_len || !d_free_head_out || !d_refused ||
         (free_count && !d_free_pages) || (table_width && !d_block_table) || (tokens && (!d_position || !d_slot)))
         return fail(FG_ERR_ARG, "null buffer");
+    if (overlaps({{{table_stride, requests}}}, table_width)) return fail(FG_ERR_ARG, "rows of the block table overlap");
     if (d_free_head == d_free_head_out) return fail(FG_ERR_ARG, "free_head and free_head_out are the same buffer");
     fg::PlanArgs a;
     a.ctx_len = d_ctx_len;
@@ -1041,10 +1055,9 @@ int fg_kv_append_device(const fg_kv_cache* cache, const void* d_k, int64_t k_tok
     if (tokens == 0) return FG_OK;
     if ((rc = check_rows(d_k, k_token_stride, k_head_stride, "k"))) return rc;
     if ((rc = check_rows(d_v, v_token_stride, v_head_stride, "v"))) return rc;
-    if (!d_slot) return fail(FG_ERR_ARG, "null slots");
-    if (overlaps(cache->page_stride, cache->pages, cache->dim) || overlaps(cache->token_stride, cache->page_size, cache->dim) ||
-        overlaps(cache->head_stride, cache->heads, cache->dim))
+    if (overlaps({{{cache->page_stride, cache->pages}, {cache->token_stride, cache->page_size}, {cache->head_stride, cache->heads}}}, cache->dim))
         return fail(FG_ERR_ARG, "rows of the cache overlap");
+    if (!d_slot) return fail(FG_ERR_ARG, "null slots");
     fg::AppendArgs a;
     a.k_cache = cache->k;
     a.v_cache = cache->v;

@@ -254,9 +254,11 @@ int fg_shard_merge_device(const uint32_t* d_ids, const float* d_dists, const uin
  * on `stream` (a cudaStream_t, NULL = default stream); they allocate nothing,
  * keep nothing and may be captured in a CUDA graph (make a first call of each
  * kind before a capture: it loads the kernels).  Buffers are device memory and
- * must not overlap; strides that make the rows of an output overlap are refused.  Lengths, tables, slots and ids are read on
- * the device: values that address nothing (negative or too large pages,
- * slots, ids) are skipped, never followed. */
+ * must not overlap, nor rows of one that is written (an output, the cache of an
+ * append, a plan's block table): strides by which an axis does not pass what the
+ * axes with smaller strides cover are refused.  Lengths, tables, slots and ids
+ * are read on the device: values that address nothing (negative or too large
+ * pages, slots, ids) are skipped, never followed. */
 
 /* Element types of queries, caches and outputs. */
 #define FG_DTYPE_F16 0

@@ -8,7 +8,7 @@ import ctypes
 import pytest
 
 import flashgann_b200 as fg
-from tests.test_attention_args import ARGS, IDS, _args, _cache
+from tests.test_attention_args import ARGS, IDS, PTR, _args, _cache
 
 # those that say something about counts, the mask or the scale; the rest are buffers and strides
 COUNTS = [(kw, word) for kw, word in ARGS if set(kw) & {"tokens", "requests", "heads", "window", "sinks", "scale"}]
@@ -27,3 +27,53 @@ def test_workspace_bytes_refuses_what_the_call_refuses(retrieved, kw, word):
     assert rc in (fg.FG_ERR_ARG, fg.FG_ERR_UNSUPPORTED), rc
     assert word in L.fg_last_error().decode(), L.fg_last_error().decode()
     assert need.value == 7
+
+
+# ---- rows that are written must not overlap ----
+
+# tokens 3, heads 4, dim 64: (token stride, head stride)
+@pytest.mark.parametrize("strides,fine", [
+    ((256, 64), True), ((64, 192), True), ((64, 64), False), ((248, 64), False), ((64, 184), False), ((64, 128), False),
+    ((1024, 72), True), ((72, 1024), True), ((128, 256), False), ((0, 64), False), ((1 << 62, 1 << 62), False)])
+def test_outputs_whose_axes_do_not_nest_are_refused(strides, fine):
+    L = fg.lib()
+    for call in ("fg_paged_attention_device", "fg_retrieved_attention_device"):
+        # a layout that is fine goes on to the next refusal
+        rc = getattr(L, call)(_cache(), _args(out_token_stride=strides[0], out_head_stride=strides[1], kv_len=None), None)
+        assert rc == fg.FG_ERR_ARG
+        assert ("null buffer" if fine else "rows of out overlap") in L.fg_last_error().decode()
+
+
+@pytest.mark.parametrize("tokens,heads,strides,fine", [(1, 4, (0, 64), True), (3, 1, (64, 0), True), (1, 4, (64, 64), True)])
+def test_axes_of_one_entry_have_any_stride(tokens, heads, strides, fine):
+    L = fg.lib()
+    cache = _cache(heads=1, token_stride=64, page_stride=1024)
+    assert L.fg_paged_attention_device(cache, _args(tokens=tokens, heads=heads, out_token_stride=strides[0],
+                                                    out_head_stride=strides[1], kv_len=None), None) == fg.FG_ERR_ARG
+    assert "null buffer" in L.fg_last_error().decode()
+
+
+# pages 4, page size 16, heads 2, dim 64: (page, token, head)
+@pytest.mark.parametrize("strides", [(64, 64, 64), (2048, 128, 128), (2048, 64, 512), (1024, 128, 64), (2040, 128, 64),
+                                     (64, 128, 2048), (4096, 256, 256), (64, 512, 128)])
+def test_append_to_caches_whose_axes_do_not_nest_is_refused(strides):
+    L = fg.lib()
+    cache = _cache(page_stride=strides[0], token_stride=strides[1], head_stride=strides[2])
+    assert L.fg_kv_append_device(cache, PTR, 128, 64, PTR, 128, 64, PTR, 3, None) == fg.FG_ERR_ARG
+    assert "rows of the cache overlap" in L.fg_last_error().decode()
+
+
+@pytest.mark.parametrize("strides", [(2048, 128, 64), (2048, 64, 1024), (64, 512, 256), (8192, 128, 64), (128, 512, 8192)])
+def test_append_takes_caches_in_any_order_of_axes(strides):
+    L = fg.lib()
+    cache = _cache(page_stride=strides[0], token_stride=strides[1], head_stride=strides[2])
+    assert L.fg_kv_append_device(cache, PTR, 128, 64, PTR, 128, 64, None, 3, None) == fg.FG_ERR_ARG
+    assert "null slots" in L.fg_last_error().decode()
+
+
+@pytest.mark.parametrize("requests,stride,fine", [(2, 0, False), (2, 3, False), (2, 4, True), (1, 0, True), (5, 1, False)])
+def test_plan_refuses_overlapping_table_rows(requests, stride, fine):
+    L = fg.lib()
+    rc = L.fg_kv_plan_device(PTR, PTR, requests, PTR, 5, PTR, 16, PTR, 4, stride, 3, PTR, PTR, PTR, PTR, PTR, PTR, None)
+    assert rc == fg.FG_ERR_ARG  # free_head and free_head_out are the same buffer: the next refusal
+    assert ("same buffer" if fine else "rows of the block table overlap") in L.fg_last_error().decode()

@@ -233,3 +233,23 @@ def test_a_wait_that_runs_out_shows_in_every_row_it_leaves(dtype, dim):
             _close((out[~lost][:, None], lse[~lost][:, None]), (want[~lost][:, None], want_lse[~lost][:, None]), dtype)
         assert shares[0] == 1.0 and shares[-1] == 0.0 and sorted(shares, reverse=True) == shares
         _close(_run(x, dtype, window=window, sinks=sinks, max_new=1000), (want, want_lse), dtype)
+
+
+# ---- rows that are written must not overlap ----
+
+def test_overlapping_tensors_are_refused():
+    import torch
+    import flashgann_b200 as fg
+    x = _batch(np.random.default_rng(1), 3, heads=2, kv_heads=1, dim=64, page=16, new=2, ctx=30)
+    T = x["q"].shape[0]
+    flat = torch.full((T * 3 * 64,), 7.0, dtype=torch.float16, device="cuda")
+    for strides in [(64, 64, 1), (64, 128, 1), (0, 64, 1), (96, 64, 1)]:
+        with pytest.raises(fg.FlashGANNError, match="rows of out overlap"):
+            _run(x, "fp16", out=flat.as_strided((T, 2, 64), strides))
+    assert (flat == 7).all()
+    by_head = flat.as_strided((T, 2, 64), (64, T * 64, 1))  # any order of axes that nest
+    _close(_run(x, "fp16", out=by_head), _ref64(x), "fp16")
+    assert (flat[T * 2 * 64:] == 7).all()
+    ints = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(fg.FlashGANNError, match="rows of the block table overlap"):
+        fg.kv_plan(ints, ints + 1, ints[None, :1].expand(2, 4).contiguous()[:1].expand(2, 4), ints, tokens=2, page_size=16)
