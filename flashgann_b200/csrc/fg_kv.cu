@@ -40,7 +40,7 @@ __device__ __forceinline__ Need page_need(const PlanArgs& a, int64_t ctx, int64_
     Need n;
     n.had = (ctx + round) >> a.page_shift;
     const int64_t will = (ctx + add + round) >> a.page_shift;
-    n.wide = will > a.table_width;
+    n.wide = will > a.table_width || ctx + add > INT32_MAX;  // lengths and positions are 32 bits
     n.pages = n.wide ? 0 : will - n.had;
     return n;
 }
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(const PlanArgs a)
         const bool refused = n.wide || (n.pages > 0 && pe > room);
         if (!refused && n.pages > 0) last = pe;  // the admitted ones are a prefix of those that need pages
         a.query_start[b + 1] = static_cast<int32_t>(min(te, static_cast<int64_t>(INT32_MAX)));
-        a.kv_len[b] = refused ? 0 : static_cast<int32_t>(min(ctx + add, static_cast<int64_t>(INT32_MAX)));
+        a.kv_len[b] = refused ? 0 : static_cast<int32_t>(ctx + add);
         a.refused[b] = refused;
     }
     if (writes && last) atomicMax(&taken, static_cast<unsigned long long>(last));

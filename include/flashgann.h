@@ -288,8 +288,8 @@ typedef struct fg_kv_cache {
  * the last request's; d_free_head_out[1], the first page not taken (not
  * d_free_head itself, which other CTAs may still be reading);
  * d_refused[requests], 1 for a request that got nothing because its length
- * passes the table's width, or because it needs pages that are no longer
- * there after the requests before it (one that needs none goes on): its kv_len
+ * passes the table's width or 2^31 - 1, or because it needs pages that are no
+ * longer there after the requests before it (one that needs none goes on): its kv_len
  * is 0, its positions and slots -1, its table row as it was.
  * At most 8192 requests. */
 int fg_kv_plan_device(const int32_t* d_ctx_len, const int32_t* d_new_len, int32_t requests,

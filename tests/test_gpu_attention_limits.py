@@ -253,3 +253,21 @@ def test_overlapping_tensors_are_refused():
     ints = torch.zeros(2, dtype=torch.int32, device="cuda")
     with pytest.raises(fg.FlashGANNError, match="rows of the block table overlap"):
         fg.kv_plan(ints, ints + 1, ints[None, :1].expand(2, 4).contiguous()[:1].expand(2, 4), ints, tokens=2, page_size=16)
+
+
+# ---- plan ----
+
+def test_plan_refuses_lengths_past_31_bits():
+    """Lengths and positions are 32 bits: a request that would pass them gets nothing, whatever its table holds."""
+    import flashgann_b200 as fg
+    top = 2 ** 31 - 1
+    ctx, new = [top, top - 2, top, top - 1], [0, 2, 1, 5]
+    table = np.arange(12, dtype=np.int32).reshape(4, 3)  # three pages of 2^30 rows each
+    got = _cuda(table)
+    p = fg.kv_plan(_cuda(np.array(ctx, np.int32)), _cuda(np.array(new, np.int32)), got, _cuda(np.array([40], np.int32)),
+                   tokens=8, page_size=2 ** 30)
+    assert p.refused.tolist() == [0, 0, 1, 1] and p.kv_len.tolist() == [top, top, 0, 0]
+    assert p.query_start.tolist() == [0, 0, 2, 3, 8] and p.free_head.tolist() == [0]
+    assert p.position.tolist() == [top - 2, top - 1] + [-1] * 6
+    assert p.slot.tolist() == [(4 << 30) + 2 ** 30 - 3, (4 << 30) + 2 ** 30 - 2] + [-1] * 6
+    assert np.array_equal(got.cpu().numpy(), table)
