@@ -25,7 +25,6 @@
 // atomics, no waiting between CTAs, and the same bits on every run.
 #pragma once
 
-#include <atomic>
 #include <cfloat>
 #include <cstdint>
 
@@ -354,21 +353,6 @@ struct Half2<__nv_bfloat16> {
     }
     __device__ static __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
     __device__ static __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
-};
-
-// A kernel's shared memory limit, raised on a device's first launch of it.
-struct SmemOnce {
-    std::atomic<uint64_t> devices{0};
-    cudaError_t set(const void* kernel, int bytes) {
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess) return e;
-        const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
-        if (devices.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e == cudaSuccess) devices.fetch_or(bit, std::memory_order_relaxed);
-        return e;
-    }
 };
 
 // Joins the partials of every tile that two or more CTAs of the main kernel

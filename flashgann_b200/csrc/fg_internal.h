@@ -3,6 +3,7 @@
 // include/flashgann.h.
 #pragma once
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
@@ -79,6 +80,22 @@ cudaError_t launch_shard_merge(const uint32_t* ids, const float* dists, const ui
                                int k, int K, uint32_t* out_ids, float* out_dists, cudaStream_t stream);
 
 // ---- key/value cache and attention (fg_kv.cu, fg_attention_rows.cu, fg_attention_tiles.cu) ----
+
+// A kernel's shared memory limit, raised on a device's first launch of it to the most that any launch takes: threads may
+// launch at the same time.
+struct SmemOnce {
+    std::atomic<uint64_t> devices{0};
+    cudaError_t set(const void* kernel, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+        if (devices.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) devices.fetch_or(bit, std::memory_order_relaxed);
+        return e;
+    }
+};
 
 struct PlanArgs {
     const int32_t* ctx_len = nullptr;

@@ -180,12 +180,15 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendA
 
 }  // namespace
 
-int kv_plan_max_requests() { return 8192; }  // 20 bytes of each in one CTA's shared memory
+constexpr int kPlanRequests = 8192;
+constexpr int kPlanBytes = 2 * sizeof(int64_t) + sizeof(int32_t);  // of a request, in one CTA's shared memory
+int kv_plan_max_requests() { return kPlanRequests; }
 
 cudaError_t launch_kv_plan(const PlanArgs& a, cudaStream_t stream) {
-    const size_t smem = static_cast<size_t>(a.requests) * (2 * sizeof(int64_t) + sizeof(int32_t));
+    const size_t smem = static_cast<size_t>(a.requests) * kPlanBytes;
     if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        static SmemOnce once;
+        const cudaError_t e = once.set(reinterpret_cast<const void*>(kv_plan_kernel), kPlanRequests * kPlanBytes);
         if (e != cudaSuccess) return e;
     }
     const int64_t pages = std::min<int64_t>(a.free_count, static_cast<int64_t>(a.requests) * a.table_width);

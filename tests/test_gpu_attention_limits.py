@@ -271,3 +271,31 @@ def test_plan_refuses_lengths_past_31_bits():
     assert p.position.tolist() == [top - 2, top - 1] + [-1] * 6
     assert p.slot.tolist() == [(4 << 30) + 2 ** 30 - 3, (4 << 30) + 2 ** 30 - 2] + [-1] * 6
     assert np.array_equal(got.cpu().numpy(), table)
+
+
+def test_plans_of_many_requests_from_threads():
+    """Plans above 2048 requests need more shared memory than a kernel gets unasked; calls of different sizes from
+    threads at the same time all get theirs."""
+    import threading
+    import torch
+    import flashgann_b200 as fg
+    L, bad = fg.lib(), []
+
+    def plans(requests):
+        z = torch.zeros(6 * requests + 64, dtype=torch.int32, device="cuda")
+        p, stream = z.data_ptr(), torch.cuda.Stream()
+        at = [p + 4 * requests * i for i in range(6)]
+        for _ in range(3000):
+            rc = L.fg_kv_plan_device(at[0], at[1], requests, None, 0, None, 16, None, 0, 0, 0, at[2], at[3] + 16, None, None,
+                                     at[4] + 32, at[5] + 48, stream.cuda_stream)
+            if rc != fg.FG_OK:
+                bad.append((requests, L.fg_last_error().decode()))
+                break
+        stream.synchronize()
+
+    threads = [threading.Thread(target=plans, args=(n,)) for n in (2100, 8192, 4000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
