@@ -898,6 +898,8 @@ bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
            fg::attention_tiles_counts(counts(c, x, retrieved));
 }
 
+constexpr double kLog2e = 1.4426950408889634;  // exponents are base 2 in the kernels
+
 // Counts, mask and scale: everything that the choice of a kernel and the size of its workspace are computed from.
 int check_counts(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
     if (x->tokens < 0 || x->requests < 0 || x->table_width < 0 || x->max_new < 0)
@@ -911,7 +913,7 @@ int check_counts(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
     if (x->requests > fg::attention_max_requests())
         return fail(FG_ERR_UNSUPPORTED, "%d requests, at most %d", x->requests, fg::attention_max_requests());
     if (x->window < -1 || x->sinks < 0) return fail(FG_ERR_ARG, "bad mask window=%d sinks=%d", x->window, x->sinks);
-    if (!(std::fabs(x->scale) <= FLT_MAX)) return fail(FG_ERR_ARG, "scale is not finite");
+    if (!(std::fabs(x->scale * kLog2e) <= FLT_MAX)) return fail(FG_ERR_ARG, "scale %g is not finite, or not once log2(e) is folded in", x->scale);
     if (retrieved) {
         if (x->window < 0) return fail(FG_ERR_ARG, "retrieved attention needs a window >= 0");
         if (x->ids_count < 0 || x->ids_token_stride < 0 || x->ids_head_stride < 0)
@@ -989,7 +991,7 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     a.group_mul = static_cast<uint32_t>(((1ull << a.group_shift) + a.group - 1) / a.group);
     a.window = x->window;
     a.sinks = x->sinks;
-    a.scale_log2 = static_cast<float>(x->scale * 1.4426950408889634);
+    a.scale_log2 = static_cast<float>(x->scale * kLog2e);
     if (retrieved && x->ids_count > 0) {
         a.ids = x->ids;
         a.ids_count = x->ids_count;

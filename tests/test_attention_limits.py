@@ -77,3 +77,10 @@ def test_plan_refuses_overlapping_table_rows(requests, stride, fine):
     rc = L.fg_kv_plan_device(PTR, PTR, requests, PTR, 5, PTR, 16, PTR, 4, stride, 3, PTR, PTR, PTR, PTR, PTR, PTR, None)
     assert rc == fg.FG_ERR_ARG  # free_head and free_head_out are the same buffer: the next refusal
     assert ("same buffer" if fine else "rows of the block table overlap") in L.fg_last_error().decode()
+
+
+@pytest.mark.parametrize("scale,fine", [(2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False)])
+def test_scales_that_overflow_with_log2e_are_refused(scale, fine):
+    L = fg.lib()
+    assert L.fg_paged_attention_device(_cache(), _args(scale=scale, kv_len=None), None) == fg.FG_ERR_ARG
+    assert ("null buffer" if fine else "scale") in L.fg_last_error().decode()
