@@ -7,7 +7,9 @@ a slot, ``kv_append`` writes the new keys and values there, and then either
 tokens) or ``retrieved_attention`` (window, first tokens and the ids that a
 search returned for each query head) reads them.  All four take torch CUDA
 tensors, run in libflashgann.so (include/flashgann.h has the exact rules) on
-``stream`` (default: torch's current stream) and wait for nothing.
+``stream`` (default: torch's current stream) and wait for nothing.  They are
+for serving and have no backward pass: where torch records gradients, a tensor
+that requires one is refused (call them under ``torch.no_grad()``).
 """
 
 from __future__ import annotations

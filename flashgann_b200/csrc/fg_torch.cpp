@@ -15,6 +15,7 @@
 #include <vector>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -83,6 +84,17 @@ private:
     std::optional<c10::cuda::CUDAStreamGuard> other_;
 };
 
+// The calls have no backward pass: a gradient that would be lost is refused.
+template <typename... Tensors>
+void no_gradient(const char* names, const Tensors&... t) {
+    FG_NEED(!c10::GradMode::is_enabled() || !(... || t.requires_grad()),
+            std::string("one of ") + names + " requires a gradient, and this call computes none: call it under torch.no_grad()");
+}
+// What a call writes in place, for autograd's count of a tensor's versions.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor ints(const at::Tensor& t, int64_t dims, const char* name, at::ScalarType type = at::kInt) {
     FG_NEED(t.scalar_type() == type && t.dim() == dims,
             std::string(name) + " must be " + at::toString(type) + " with " + std::to_string(dims) + " dimension(s), not " + shape(t));
@@ -140,6 +152,7 @@ Six kv_plan(at::Tensor ctx_len, at::Tensor new_len, const at::Tensor& table, at:
                             i32(tokens, "tokens"), p, p + R + 1, p + 3 * R + 2, slot.data_ptr<int64_t>(), p + 2 * R + 1, p + 2 * R + 2,
                             on.stream()),
           "fg_kv_plan_device");
+    written(table);
     const std::vector<at::Tensor> v = all.split_with_sizes({R + 1, R, 1, R, T});
     return {v[0], v[1], v[4], slot, v[2], v[3]};
 }
@@ -147,6 +160,7 @@ Six kv_plan(at::Tensor ctx_len, at::Tensor new_len, const at::Tensor& table, at:
 void kv_append(const at::Tensor& k_cache, const at::Tensor& v_cache, at::Tensor k, at::Tensor v, at::Tensor slot, int64_t stream) {
     On on(k_cache, stream);
     on.uses(k_cache, v_cache, k, v, slot);
+    no_gradient("k_cache, v_cache, k and v", k_cache, v_cache, k, v);
     const fg_kv_cache c = cache(k_cache, v_cache);
     slot = ints(slot, 1, "slot", at::kLong);
     const int64_t T = slot.size(0);
@@ -159,6 +173,8 @@ void kv_append(const at::Tensor& k_cache, const at::Tensor& v_cache, at::Tensor 
     check(fg_kv_append_device(&c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), slot.data_ptr<int64_t>(),
                               i32(T, "tokens"), on.stream()),
           "fg_kv_append_device");
+    written(k_cache);
+    written(v_cache);
 }
 
 std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const at::Tensor& k_cache, const at::Tensor& v_cache, at::Tensor table,
@@ -170,6 +186,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const 
     on.uses(q, k_cache, v_cache, table, query_start, kv_len);
     if (ids) on.uses(*ids);
     if (out_or_none) on.uses(*out_or_none);
+    no_gradient("q, k_cache, v_cache and out", q, k_cache, v_cache, out_or_none ? *out_or_none : q);
     const fg_kv_cache c = cache(k_cache, v_cache);
     q = rows(q, "q");
     const int64_t T = q.size(0), heads = q.size(1), dim = q.size(2);
@@ -231,6 +248,7 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const 
     }
     if (ids) check(fg_retrieved_attention_device(&c, &x, on.stream()), "fg_retrieved_attention_device");
     else check(fg_paged_attention_device(&c, &x, on.stream()), "fg_paged_attention_device");
+    if (out_or_none) written(out);
     return {out, lse};
 }
 

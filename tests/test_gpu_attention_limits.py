@@ -299,3 +299,49 @@ def test_plans_of_many_requests_from_threads():
     for t in threads:
         t.join()
     assert not bad, bad
+
+
+# ---- gradients and versions ----
+
+def test_gradients_are_refused_and_writes_are_counted():
+    """No call has a backward pass: under grad mode a tensor that requires a gradient is refused, and what a call
+    writes in place gets a new version, so that autograd notices."""
+    import torch
+    import flashgann_b200 as fg
+    x = _batch(np.random.default_rng(2), 3, heads=2, kv_heads=1, dim=64, page=16, new=2, ctx=30)
+    dt = torch.float16
+    q, k, v = (_cuda(x[n], dt) for n in ("q", "k", "v"))
+    rest = (_cuda(x["table"]), _cuda(x["start"]), _cuda(x["kv_len"]))
+    T = q.shape[0]
+    new, slot = torch.zeros((T, 1, 64), dtype=dt, device="cuda"), torch.arange(T, device="cuda")
+    ids = torch.zeros((T, 2, 4), dtype=torch.int32, device="cuda")
+    calls = {
+        "paged": lambda q, k, v, n, out: fg.paged_attention(q, k, v, *rest, 2, out=out),
+        "retrieved": lambda q, k, v, n, out: fg.retrieved_attention(q, k, v, *rest, ids, window=3, out=out),
+        "append": lambda q, k, v, n, out: fg.kv_append(k, v, n, n, slot)}
+    for name, call in calls.items():
+        for i, t in enumerate((q, k, v, new, torch.empty_like(q))):
+            args = [q, k.clone(), v.clone(), new, None]
+            args[i] = t.clone().requires_grad_()
+            if (name == "append") == (i in (0, 4)) and i not in (1, 2):
+                call(*args)  # not an argument of this call
+                continue
+            with pytest.raises(fg.FlashGANNError, match="requires a gradient"):
+                call(*args)
+            with torch.no_grad():
+                call(*args)
+            with torch.inference_mode():
+                call(*args)
+    versions = [t._version for t in (q, k, v, new)]
+    fg.kv_append(k, v, new, new, slot)
+    out = torch.empty_like(q)
+    before = out._version
+    fg.paged_attention(q, k, v, *rest, 2, out=out)
+    assert out._version == before + 1
+    assert [t._version for t in (q, k, v, new)] == [versions[0], versions[1] + 1, versions[2] + 1, versions[3]]
+    one, table = torch.ones(3, dtype=torch.int32, device="cuda"), rest[0].clone()
+    fg.kv_plan(one, one, table, one, tokens=3, page_size=16)
+    assert table._version == 1
+    with torch.inference_mode():
+        kk = k.clone()
+        fg.kv_append(kk, kk.clone(), new, new, slot)
