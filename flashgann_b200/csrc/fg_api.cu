@@ -813,6 +813,9 @@ int fg_shard_merge_device(const uint32_t* d_ids, const float* d_dists, const uin
 
 namespace {
 
+// An axis of one entry may have any stride: nothing is ever added for it.
+int64_t used_stride(int64_t stride, int64_t count) { return count > 1 ? stride : 0; }
+
 int check_cache(const fg_kv_cache* c) {
     if (!c || !c->k || !c->v) return fail(FG_ERR_ARG, "null cache");
     if (c->dtype != FG_DTYPE_F16 && c->dtype != FG_DTYPE_BF16) return fail(FG_ERR_ARG, "unknown cache dtype %d", c->dtype);
@@ -823,9 +826,10 @@ int check_cache(const fg_kv_cache* c) {
         return fail(FG_ERR_UNSUPPORTED, "page size %d is not a power of two", c->page_size);
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
         return fail(FG_ERR_ARG, "cache is not 16-byte aligned");
-    if ((c->page_stride | c->token_stride | c->head_stride) & 7)
-        return fail(FG_ERR_ARG, "cache strides are not multiples of 16 bytes");
-    if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0) return fail(FG_ERR_ARG, "negative cache stride");
+    const int64_t page = used_stride(c->page_stride, c->pages), token = used_stride(c->token_stride, c->page_size),
+                  head = used_stride(c->head_stride, c->heads);
+    if ((page | token | head) & 7) return fail(FG_ERR_ARG, "cache strides are not multiples of 16 bytes");
+    if (page < 0 || token < 0 || head < 0) return fail(FG_ERR_ARG, "negative cache stride");
     return FG_OK;
 }
 
@@ -836,7 +840,9 @@ int log2_of(int32_t x) {
 }
 
 // Rows [tokens, heads, dim] given by a pointer and two strides.
-int check_rows(const void* p, int64_t token_stride, int64_t head_stride, const char* what) {
+int check_rows(const void* p, int64_t token_stride, int64_t head_stride, int32_t tokens, int32_t heads, const char* what) {
+    token_stride = used_stride(token_stride, tokens);
+    head_stride = used_stride(head_stride, heads);
     if (!p) return fail(FG_ERR_ARG, "null %s", what);
     if (reinterpret_cast<uintptr_t>(p) & 15) return fail(FG_ERR_ARG, "%s is not 16-byte aligned", what);
     if ((token_stride | head_stride) & 7) return fail(FG_ERR_ARG, "strides of %s are not multiples of 16 bytes", what);
@@ -944,8 +950,8 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     if (!x) return fail(FG_ERR_ARG, "null arguments");
     if ((rc = check_counts(c, x, retrieved))) return rc;
     if (x->tokens == 0 || x->requests == 0) return FG_OK;
-    if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, "q"))) return rc;
-    if ((rc = check_rows(x->out, x->out_token_stride, x->out_head_stride, "out"))) return rc;
+    if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, x->tokens, x->heads, "q"))) return rc;
+    if ((rc = check_rows(x->out, x->out_token_stride, x->out_head_stride, x->tokens, x->heads, "out"))) return rc;
     if (overlaps({{{x->out_token_stride, x->tokens}, {x->out_head_stride, x->heads}}}, c->dim))
         return fail(FG_ERR_ARG, "rows of out overlap");
     if (!x->query_start || !x->kv_len || (!x->block_table && x->table_width > 0) || (retrieved && !x->ids && x->ids_count))
@@ -1055,8 +1061,8 @@ int fg_kv_append_device(const fg_kv_cache* cache, const void* d_k, int64_t k_tok
     if (rc) return rc;
     if (tokens < 0) return fail(FG_ERR_ARG, "bad token count %d", tokens);
     if (tokens == 0) return FG_OK;
-    if ((rc = check_rows(d_k, k_token_stride, k_head_stride, "k"))) return rc;
-    if ((rc = check_rows(d_v, v_token_stride, v_head_stride, "v"))) return rc;
+    if ((rc = check_rows(d_k, k_token_stride, k_head_stride, tokens, cache->heads, "k"))) return rc;
+    if ((rc = check_rows(d_v, v_token_stride, v_head_stride, tokens, cache->heads, "v"))) return rc;
     if (overlaps({{{cache->page_stride, cache->pages}, {cache->token_stride, cache->page_size}, {cache->head_stride, cache->heads}}}, cache->dim))
         return fail(FG_ERR_ARG, "rows of the cache overlap");
     if (!d_slot) return fail(FG_ERR_ARG, "null slots");

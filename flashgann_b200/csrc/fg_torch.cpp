@@ -104,7 +104,8 @@ at::Tensor ints(const at::Tensor& t, int64_t dims, const char* name, at::ScalarT
 // [tokens, heads, dim] with a contiguous last axis and 16-byte aligned rows (a copy where it is not)
 at::Tensor rows(const at::Tensor& t, const char* name) {
     FG_NEED(t.dim() == 3, std::string(name) + " must be [tokens, heads, dim], not " + shape(t));
-    if ((t.stride(2) != 1 && t.size(2) > 1) || (t.stride(0) | t.stride(1)) % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16)
+    const int64_t strides = (t.size(0) > 1 ? t.stride(0) : 0) | (t.size(1) > 1 ? t.stride(1) : 0);
+    if ((t.stride(2) != 1 && t.size(2) > 1) || strides % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16)
         return t.clone(at::MemoryFormat::Contiguous);
     return t;
 }
@@ -113,7 +114,9 @@ fg_kv_cache cache(const at::Tensor& k, const at::Tensor& v) {
     FG_NEED(k.dim() == 4 && v.sizes() == k.sizes(), "caches must be [pages, page_size, heads, dim] alike, not " + shape(k) + " and " + shape(v));
     FG_NEED((k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16) && v.scalar_type() == k.scalar_type(),
             "caches must both be float16 or bfloat16, not " + shape(k) + " and " + shape(v));
-    FG_NEED(k.strides() == v.strides() && k.stride(3) == 1, "caches must have the same strides and a contiguous last axis");
+    for (int64_t i = 0; i < 3; ++i)  // torch leaves the stride of an axis of one entry open
+        FG_NEED(k.stride(i) == v.stride(i) || k.size(i) == 1, "caches must have the same strides");
+    FG_NEED(k.stride(3) == 1 && v.stride(3) == 1, "caches must have a contiguous last axis");
     fg_kv_cache c{};
     c.k = k.data_ptr();
     c.v = v.data_ptr();

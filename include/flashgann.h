@@ -268,8 +268,9 @@ int fg_shard_merge_device(const uint32_t* d_ids, const float* d_dists, const uin
  * page_size], row j % page_size.  Row (page, t, head) of K starts at element
  * page * page_stride + t * token_stride + head * head_stride of k, and of V
  * likewise of v: any order of the axes, and slices of a larger buffer.
- * k, v and the strides in bytes must be multiples of 16; page_size a power of
- * two; dim 64, 96 or 128, contiguous. */
+ * k, v and the strides in bytes must be multiples of 16 (that of an axis of one
+ * entry, here and in all rows, is not looked at); page_size a power of two; dim
+ * 64, 96 or 128, contiguous. */
 typedef struct fg_kv_cache {
     void* k;
     void* v;

@@ -84,3 +84,18 @@ def test_scales_that_overflow_with_log2e_are_refused(scale, fine):
     L = fg.lib()
     assert L.fg_paged_attention_device(_cache(), _args(scale=scale, kv_len=None), None) == fg.FG_ERR_ARG
     assert ("null buffer" if fine else "scale") in L.fg_last_error().decode()
+
+
+@pytest.mark.parametrize("cache,args", [
+    (dict(pages=1, page_stride=-3), dict()), (dict(heads=1, head_stride=5, token_stride=64), dict()),
+    (dict(page_size=1, token_stride=-9), dict()),
+    (dict(), dict(tokens=1, q_token_stride=-1, out_token_stride=3)),
+    (dict(heads=1), dict(heads=1, q_head_stride=7, out_head_stride=-7))])
+def test_strides_of_axes_of_one_entry_are_not_looked_at(cache, args):
+    L = fg.lib()
+    for call in ("fg_paged_attention_device", "fg_retrieved_attention_device"):
+        assert getattr(L, call)(_cache(**cache), _args(kv_len=None, **args), None) == fg.FG_ERR_ARG
+        assert "null buffer" in L.fg_last_error().decode()
+    rows = (PTR, 1, 64, PTR, 3, 64, None, 1) if not cache.get("heads") else (PTR, 8, 3, PTR, 8, -1, None, 3)
+    assert L.fg_kv_append_device(_cache(**cache), *rows, None) == fg.FG_ERR_ARG
+    assert "null slots" in L.fg_last_error().decode()

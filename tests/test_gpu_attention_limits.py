@@ -345,3 +345,37 @@ def test_gradients_are_refused_and_writes_are_counted():
     with torch.inference_mode():
         kk = k.clone()
         fg.kv_append(kk, kk.clone(), new, new, slot)
+
+
+# ---- axes of one entry ----
+
+@pytest.mark.parametrize("new", [1, 30])
+def test_axes_of_one_entry_have_any_stride(new):
+    """One kv head, K with the pages' rows outside and V with the heads outside: the same layout, other strides of the
+    axis of one entry; and one token, one page, one head with strides that no tensor core would take."""
+    import torch
+    import flashgann_b200 as fg
+    dt = torch.float16
+    x = _batch(np.random.default_rng(new), 3, heads=2, kv_heads=1, dim=64, page=16, new=new, ctx=30)
+    q, k, v = (_cuda(x[n], dt) for n in ("q", "k", "v"))
+    rest = (_cuda(x["table"]), _cuda(x["start"]), _cuda(x["kv_len"]))
+    by_head = v.transpose(1, 2).contiguous().transpose(1, 2).as_strided(v.shape, (1024, 64, 1024, 1))
+    odd = v.as_strided(v.shape, (1024, 64, 3, 1))
+    for vv in (v, by_head, odd):
+        for kk in (k, k.as_strided(k.shape, (1024, 64, 5, 1))):
+            _close(fg.paged_attention(q, kk, vv, *rest, new, return_lse=True), _ref64(x), "fp16")
+    T = q.shape[0]
+    a, b = k.clone(), by_head.clone(memory_format=torch.preserve_format)
+    slot = torch.randperm(k.shape[0] * 16, device="cuda")[:T]
+    fg.kv_append(a, b.as_strided(b.shape, (1024, 64, 7, 1)), q[:, :1], q[:, 1:], slot)
+    assert torch.equal(a.view(-1, 64)[slot], q[:, 0]) and torch.equal(b.reshape(-1, 64)[slot], q[:, 1])
+    one = _batch(np.random.default_rng(7), 1, heads=1, kv_heads=1, dim=64, page=64, new=1, ctx=30)
+    q, k, v = (_cuda(one[n], dt) for n in ("q", "k", "v"))
+    one["table"][:] = 0
+    one["k"], one["v"] = one["k"][:1], one["v"][:1]
+    rest = (_cuda(one["table"]), _cuda(one["start"]), _cuda(one["kv_len"]))
+    out = torch.zeros(100, dtype=dt, device="cuda").as_strided((1, 1, 64), (5, 3, 1))
+    k, v = (t[:1].as_strided((1, 64, 1, 64), (9, 64, 11, 1)) for t in (k, v))
+    for max_new in (1, 100):
+        _, lse = fg.paged_attention(q.as_strided(q.shape, (3, 1, 1)), k, v, *rest, max_new, out=out, return_lse=True)
+        _close((out, lse), _ref64(one), "fp16")
