@@ -1,7 +1,8 @@
 # FlashGANN-B200 build.
 #
 #   make gpu_flashgann [EXTRA_NVFLAGS="-DINTERNAL_TOPK=1024"]   -> bin/gpu_flashgann (+ the library)
-#   make lib                                                  -> flashgann_b200/libflashgann.so
+#   make lib                                                  -> flashgann_b200/libflashgann.so, and where $(PYTHON) has a
+#                                                                torch with CUDA its binding flashgann_b200/_torch_ops.so
 #   make oracle                                               -> oracle/liboracle.so (test infrastructure)
 #
 # Same knobs as the reference Makefile (ARCH, EXTRA_NVFLAGS); this build
@@ -24,11 +25,18 @@ ATTN_HEADERS := $(CSRC)/fg_attention.cuh
 OBJ_DIR    := flashgann_b200/_build
 OBJS       := $(patsubst $(CSRC)/%.cu,$(OBJ_DIR)/%.o,$(KERNEL_SRC))
 
-.PHONY: all lib gpu_flashgann oracle clean
+# the library itself needs no torch: without one its binding is left out
+HAS_TORCH := $(shell $(PYTHON) -c "import importlib.util as u, os; s = u.find_spec('torch'); \
+    print('yes' if s and os.path.exists(os.path.join(os.path.dirname(s.origin), 'lib', 'libc10_cuda.so')) else '')" 2>/dev/null)
+
+.PHONY: all lib gpu_flashgann oracle clean no_torch
 
 all: lib gpu_flashgann
 
-lib: $(LIB) $(TORCH_OPS)
+lib: $(LIB) $(if $(HAS_TORCH),$(TORCH_OPS),no_torch)
+
+no_torch:
+	@echo "$(PYTHON) has no torch with CUDA: $(TORCH_OPS), which only flashgann_b200/attention.py needs, is not built"
 
 # the torch binding of the cache and attention calls (flashgann_b200/attention.py)
 TORCH_FLAGS = $(shell $(PYTHON) -c "import os, sysconfig, torch; t = os.path.dirname(torch.__file__); \
