@@ -32,7 +32,7 @@ __all__ = [
     "QuantizationGraph", "FlashGANNError", "QueryStats", "lib", "load_fvecs", "load_ivecs", "compute_recall",
     "append_run_stats_to_csv", "infer_metric_from_dataset_path", "effective_sort_beam_size", "METRIC_L2",
     "METRIC_IP",
-    "search_multi", "KVPlan", "kv_plan", "kv_append", "paged_attention", "retrieved_attention",
+    "search_multi",
 ]
 
 
@@ -308,7 +308,8 @@ def infer_metric_from_dataset_path(path: str) -> int:
     return int(lib().fg_infer_metric_from_path(os.fsencode(path)))
 
 
-# flashgann_b200.attention needs torch, which the search's host-buffer calls do not: loaded on first use
+# flashgann_b200.attention needs torch, which the search's host-buffer calls do not: loaded on first use, and not in
+# __all__, so that a star import does without it
 _ATTENTION = ("KVPlan", "kv_append", "kv_plan", "paged_attention", "retrieved_attention")
 
 
