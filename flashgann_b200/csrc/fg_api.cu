@@ -1097,10 +1097,10 @@ int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* a
     return workspace_bytes(cache, args, retrieved != 0, bytes);
 }
 
-// For tests only: in every CTA of the kernel of many rows, K tiles from this block on never come, and the waits for them
-// run out soon (NaN in the rows that were not stored before).  Below 0: as usual.
-extern "C" __attribute__((visibility("default"))) void fg_test_attention_lose_blocks(int32_t first) {
-    fg::set_attention_waits(first < 0 ? INT32_MAX : first, first < 0 ? 1 << 22 : 4);
+// For tests only: in every CTA of the kernel of many rows, K tiles from block `first` on never come, and the waits for
+// them run out after so many tries (NaN in the rows that were not stored before).  Below 0: as usual.
+extern "C" __attribute__((visibility("default"))) void fg_test_attention_lose_blocks(int32_t first, int32_t tries) {
+    fg::set_attention_waits(first, tries);
 }
 
 int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {

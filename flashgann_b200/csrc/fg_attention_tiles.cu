@@ -116,6 +116,9 @@ __device__ __forceinline__ bool bar_try(uint64_t* b, int parity) {
 __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
 }
+// A try that finds nothing takes 4 us (measured), so that the usual limit is a
+// second; a wait between two blocks lasts microseconds.
+constexpr int kWaitTries = 1 << 18;
 __device__ __forceinline__ volatile int* stalled(Shared* sh) { return &sh->stalled; }
 // For the softmax warps.  A lane whose wait runs out, or that finds that
 // another's did, is late and goes on without waiting any more: no vote, and the
@@ -140,10 +143,11 @@ __device__ __forceinline__ bool bar_wait_all(const AttentionParams& a, uint64_t*
 }
 // For waits that nothing hurries: leaves the issue slots to the other warps.
 // They may last as long as a tile (a V tile to be looked through comes after all
-// others: 16 ms in a context of a million keys), the limit is seconds.
+// others: 16 ms in a context of a million keys); where one does not end, one of
+// the other kind does not either, which runs out first.
 __device__ __forceinline__ bool bar_wait_idle(const AttentionParams& a, uint64_t* b, int parity, Shared* sh) {
     for (int i = 0; !__all_sync(0xFFFFFFFFu, bar_try(b, parity)); ++i) {
-        if (__any_sync(0xFFFFFFFFu, i >= a.wait_tries * 16 || *stalled(sh))) {
+        if (__any_sync(0xFFFFFFFFu, i >= a.wait_tries * 256 || *stalled(sh))) {
             *stalled(sh) = 1;
             return false;
         }
@@ -153,7 +157,7 @@ __device__ __forceinline__ bool bar_wait_idle(const AttentionParams& a, uint64_t
 }
 // Before a warp leaves: what it started itself, and what ends by itself.
 __device__ __forceinline__ void bar_wait_own(uint64_t* b, int parity) {
-    for (int i = 0; i < (1 << 22) && !bar_try(b, parity); ++i) {
+    for (int i = 0; i < kWaitTries && !bar_try(b, parity); ++i) {
     }
 }
 
@@ -974,7 +978,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-std::atomic<int> g_wait_tries{1 << 22}, g_lost_block{INT32_MAX};
+std::atomic<int> g_wait_tries{kWaitTries}, g_lost_block{INT32_MAX};
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -1055,8 +1059,8 @@ bool attention_tiles_counts(const AttentionParams& a) {
 }
 
 void set_attention_waits(int lost_block, int tries) {
-    attn::g_lost_block.store(lost_block, std::memory_order_relaxed);
-    attn::g_wait_tries.store(tries, std::memory_order_relaxed);
+    attn::g_lost_block.store(lost_block < 0 ? INT32_MAX : lost_block, std::memory_order_relaxed);
+    attn::g_wait_tries.store(tries < 0 ? attn::kWaitTries : tries, std::memory_order_relaxed);
 }
 
 size_t attention_tiles_workspace(int sms, int dim) {

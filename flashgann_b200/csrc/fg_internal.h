@@ -167,7 +167,7 @@ bool attention_rows_splits(const AttentionParams& a);
 size_t attention_rows_workspace(const AttentionParams& a, int sms, int dim);  // 0 where nothing is split
 cudaError_t launch_attention_rows(const AttentionParams& a, cudaStream_t stream);
 bool attention_tiles_counts(const AttentionParams& a);
-void set_attention_waits(int lost_block, int tries);  // none and 2^22 unless a test sets them
+void set_attention_waits(int lost_block, int tries);  // for tests; below 0: none, and a limit of a second
 size_t attention_tiles_workspace(int sms, int dim);
 cudaError_t launch_attention_tiles(const AttentionParams& a, cudaStream_t stream);
 

@@ -221,12 +221,12 @@ def test_a_wait_that_runs_out_shows_in_every_row_it_leaves(dtype, dim):
         shares = []
         for first in (0, 1, 2, 3, 5, 9, 1000):
             out = torch.full(want.shape, 7.0, dtype=_dt(dtype), device="cuda")
-            fg.lib().fg_test_attention_lose_blocks(first)
+            fg.lib().fg_test_attention_lose_blocks(first, 4)
             try:
                 _, lse = _run(x, dtype, window=window, sinks=sinks, max_new=1000, out=out)
                 torch.cuda.synchronize()
             finally:
-                fg.lib().fg_test_attention_lose_blocks(-1)
+                fg.lib().fg_test_attention_lose_blocks(-1, -1)
             lost = torch.isnan(lse)
             shares.append(float(lost.float().mean()))
             assert torch.equal(lost[..., None].expand_as(out), torch.isnan(out))
@@ -379,3 +379,24 @@ def test_axes_of_one_entry_have_any_stride(new):
     for max_new in (1, 100):
         _, lse = fg.paged_attention(q.as_strided(q.shape, (3, 1, 1)), k, v, *rest, max_new, out=out, return_lse=True)
         _close((out, lse), _ref64(one), "fp16")
+
+
+def test_waits_run_out_within_seconds():
+    """With the limit that all calls have: a copy that never comes costs about a second, not the GPU."""
+    import time
+    import torch
+    import flashgann_b200 as fg
+    x = _batch(np.random.default_rng(3), 2, heads=4, kv_heads=2, dim=64, page=16, new=70, ctx=900)
+    _run(x, "bf16", max_new=1000)
+    torch.cuda.synchronize()
+    fg.lib().fg_test_attention_lose_blocks(0, -1)
+    try:
+        t = time.monotonic()
+        out, lse = _run(x, "bf16", max_new=1000)
+        torch.cuda.synchronize()
+        t = time.monotonic() - t
+    finally:
+        fg.lib().fg_test_attention_lose_blocks(-1, -1)
+    assert 0.2 < t < 5, t
+    assert torch.isnan(out).all() and torch.isnan(lse).all()
+    _close(_run(x, "bf16", max_new=1000), _ref64(x), "bf16")
