@@ -796,6 +796,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sh->tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // locate's sums lie where the copies go
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
