@@ -78,7 +78,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     a token sees, itself included (None or -1: all); sinks: first tokens that
     stay visible.  scale: default dim ** -0.5.  Returns out [T, heads, dim],
     with return_lse also the rows' log-sum-exp float32 [T, heads]; a row that
-    sees nothing is 0 and -inf."""
+    sees nothing is 0 and -inf.  Sums are 32 bits, the weights of the product
+    with V are rounded to the cache's type."""
     out, lse = _torch_ops.attention(q, k_cache, v_cache, block_table, query_start, kv_len, max_new, None,
                                     -1 if window is None else window, sinks, scale, out, return_lse, _handle(stream))
     return (out, lse) if return_lse else out

@@ -27,9 +27,9 @@
 // repeated) and leave the rest in shared memory, see stage_ids.
 //
 // Measured (device time, 32 or 64 query heads on 8, dim 128, bf16): 64 ragged
-// decodes, 1.1 GB of keys and values, 176 to 179 us, 6.1 to 6.25 TB/s; one of
-// 131K keys at most, 82 us; one of a few hundred keys of dim 64 7.6 us.  With 64 requests x 100 ids
-// 57.5 us for 175 MB: there 8 warps per SM, as many as their registers allow,
+// decodes, 1.1 GB of keys and values, 174 to 180 us, 6.1 to 6.3 TB/s; one of
+// 131K keys at most, 80 to 83 us; one of a few hundred keys of dim 64 7.6 to 8.3
+// us.  With 64 requests x 100 ids 57 to 58 us for 175 MB: there 8 warps per SM, as many as their registers allow,
 // do not cover the latency of short tiles.
 //
 // Tiles that are short whatever the lengths are (a narrow table, or a window and
@@ -302,7 +302,7 @@ struct Warp {
 
     // Reads the lists of the tile's heads into shared memory, with -1 in the
     // place of ids that do not count.  Of equal ids in a list the first stays: a
-    // hash table (open addressing, half full at most) holds for each id of each
+    // hash table (open addressing, an eighth full at most) holds for each id of each
     // head the least of its places in the lists; an id whose place is another's
     // goes.  The result does not depend on the order of the atomics.  Called by
     // the whole CTA.

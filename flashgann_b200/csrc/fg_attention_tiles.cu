@@ -27,8 +27,8 @@
 // was slower: the special-function units are not what is short, issue slots and
 // latencies are.)
 //
-// Measured: 2048 tokens on 8192 keys, 32 heads on 8, dim 128, bf16: 278 us,
-// 1112 TFLOP/s on the device.  A block takes 3650 cycles, of which the tensor
+// Measured: 2048 tokens on 8192 keys, 32 heads on 8, dim 128, bf16: 276 to 281
+// us, 1100 to 1120 TFLOP/s on the device.  A block takes 3650 cycles, of which the tensor
 // pipe is busy for 2048: each half waits for its own weights.
 //
 // The base that the weights are relative to is raised only when the running
