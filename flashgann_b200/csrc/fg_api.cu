@@ -879,7 +879,8 @@ int sm_count(int* sms) {
 // would read the keys once for each 16 rows, and the tiles kernel takes them
 // 256 at a time.  That one folds the scale into its maxima, so it needs a
 // positive one; its copies are whole groups of 8 rows of a page, and take no
-// axis of stride 0 (an expanded tensor); its sums of work are 32 bits.
+// axis of stride 0 (an expanded tensor); its unit of work is a block of keys, of
+// which it counts fewer than 2^31.
 bool many_rows(const fg_kv_cache* c, const fg_attention* x) {
     return static_cast<int64_t>(x->max_new) * (x->heads / c->heads) > 16;
 }

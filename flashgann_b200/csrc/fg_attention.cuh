@@ -60,8 +60,7 @@ __host__ __device__ inline size_t partial_floats(int rows, int dim) { return sta
 // sum for each request.  A launch of more requests than its kernel's other
 // uses have room for asks for this much instead.
 constexpr int kMaxRequests = 16384;
-template <typename Sum>
-__host__ __device__ constexpr int locate_bytes(int requests) { return (64 + requests) * static_cast<int>(sizeof(Sum)); }
+__host__ __device__ constexpr int locate_bytes(int requests) { return (64 + requests) * static_cast<int>(sizeof(int)); }
 
 // One request as every kernel reads it, clamped to the buffers the launch was given.
 struct Request {
@@ -171,8 +170,8 @@ struct Place {
 };
 
 // a / b, without a 64-bit division where 32 bits will do
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+__device__ __forceinline__ int64_t divide(int64_t a, uint32_t b) {
+    if ((a >> 32) == 0) return static_cast<uint32_t>(a) / b;
     return a / b;
 }
 // total * c / ctas
@@ -182,18 +181,18 @@ __device__ __forceinline__ int64_t share(int64_t total, int c, int ctas) {
     return each * c + rest * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas);  // both below 2^16
 }
 
-// Called by all kThreads threads; scratch holds locate_bytes(requests).  Sum
-// holds the units of a kv head: 64 bits where thousands of requests may share a
-// context of millions of keys or a prompt may have 2^19 tiles, 32 where the host
-// keeps such calls away.  kLanes
+// Called by all kThreads threads; scratch holds locate_bytes(requests).  The
+// units of a kv head are summed in 32 bits: the host sees to it, from the counts
+// and the table's width, that there are fewer than 2^31 (64-bit sums cost every
+// call 0.2 to 0.3 us, and 1 % in the kernel of many rows).  kLanes
 // threads count the tiles of a request: 1 where requests are short, 8 where
 // they have many tiles.
-template <int kRows, Layout kLayout, int kChunk, int kThreads, int kLanes, typename Sum>
-__device__ __forceinline__ Place locate(const AttentionParams& a, Sum* scratch, int cta, int ctas) {
-    Sum* pre = scratch + 64;  // inclusive prefix of the requests' units
+template <int kRows, Layout kLayout, int kChunk, int kThreads, int kLanes>
+__device__ __forceinline__ Place locate(const AttentionParams& a, int* scratch, int cta, int ctas) {
+    int* pre = scratch + 64;  // inclusive prefix of the requests' units
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int kWarps = kThreads / 32;
-    Sum carry = 0, few = 0;
+    int carry = 0, few = 0;
     if (a.requests <= 32 / kLanes) {  // every warp on its own, without a barrier
         if (lane / kLanes < a.requests) {
             const Request r = load_request(a, lane / kLanes);
@@ -202,14 +201,14 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, Sum* scratch, 
         }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const Sum v = __shfl_up_sync(0xFFFFFFFFu, few, d);
+            const int v = __shfl_up_sync(0xFFFFFFFFu, few, d);
             if (lane >= d) few += v;
         }
         carry = __shfl_sync(0xFFFFFFFFu, few, 31);
     } else {
         for (int b0 = 0; b0 < a.requests; b0 += kThreads / kLanes) {
             const int b = b0 + tid / kLanes;
-            Sum s = 0;
+            int s = 0;
             if (b < a.requests) {
                 const Request r = load_request(a, b);
                 const int n = Tiles<kRows, kLayout>::count(a, r);
@@ -217,14 +216,14 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, Sum* scratch, 
             }
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const Sum v = __shfl_up_sync(0xFFFFFFFFu, s, d);
+                const int v = __shfl_up_sync(0xFFFFFFFFu, s, d);
                 if (lane >= d) s += v;
             }
             if (lane == 31) scratch[warp] = s;
             __syncthreads();
-            Sum before = carry, sum = 0;
+            int before = carry, sum = 0;
             for (int w = 0; w < kWarps; ++w) {
-                const Sum v = scratch[w];
+                const int v = scratch[w];
                 if (w < warp) before += v;
                 sum += v;
             }
@@ -243,12 +242,12 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, Sum* scratch, 
     }
     x.unit = share(x.total, cta, x.ctas);
     x.end = share(x.total, cta + 1, x.ctas);
-    x.head = static_cast<int>(divide(x.unit, per_head));
-    Sum rest = static_cast<Sum>(x.unit - x.head * per_head);  // units before the range, of this head
+    x.head = static_cast<int>(divide(x.unit, static_cast<uint32_t>(per_head)));
+    int rest = static_cast<int>(x.unit - x.head * per_head);  // units before the range, of this head
     int lo = 0, hi = a.requests - 1;  // first request whose inclusive prefix exceeds rest
     if (a.requests <= 32 / kLanes) {
-        lo = (__ffs(__ballot_sync(0xFFFFFFFFu, few > rest)) - 1) / kLanes;
-        const Sum before = __shfl_sync(0xFFFFFFFFu, few, max(lo * kLanes - 1, 0));
+        lo = max(0, __ffs(__ballot_sync(0xFFFFFFFFu, few > rest)) - 1) / kLanes;  // none only where sums wrapped, see below
+        const int before = __shfl_sync(0xFFFFFFFFu, few, max(lo * kLanes - 1, 0));
         if (lo > 0) rest -= before;
     } else {
         while (lo < hi) {
@@ -285,7 +284,7 @@ __device__ __forceinline__ Place locate(const AttentionParams& a, Sum* scratch, 
         rest -= __shfl_sync(0xFFFFFFFFu, s, 31);
     }
     x.tile = t;
-    x.offset = found && rest > 0 ? static_cast<int>(rest) : 0;  // always found, unless query_start is not ascending and sums wrapped
+    x.offset = found && rest > 0 ? rest : 0;  // always found, unless query_start is not ascending and sums wrapped
     return x;
 }
 

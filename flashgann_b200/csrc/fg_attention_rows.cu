@@ -91,6 +91,7 @@ namespace attn {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kTileUnits = 2;  // a tile's start and end take about as long as two chunks of each warp
 constexpr int kThreads = kWarps * 32;
 static_assert(kThreads == 128, "lists of ids lie in groups of 128");
 constexpr int kTable = 8192;     // places of the hash table over them: with 2048 or 4096 staging takes twice or 1.3 times as long
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     char* ws = static_cast<char*>(a.workspace);
 
     asm volatile("griddepcontrol.launch_dependents;");
-    const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kThreads, 1, int64_t>(a, reinterpret_cast<int64_t*>(smem), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
     __syncthreads();  // the rings overlay the scan
     if (pl.unit >= pl.end) {
         if (threadIdx.x == 0 && ws) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
@@ -697,19 +698,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
     }
 }
 
+// log2 of the chunks in a unit where tiles are split: one for each warp, more only where the table's width and the counts
+// do not exclude 2^31 units of a kv head (thousands of requests that share a context of millions of keys, a prompt of 2^19
+// tiles).
+int unit_shift(const AttentionParams& a) {
+    const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.table_width) * a.page_size, INT32_MAX);
+    const int64_t heads = a.ids_count > 0 ? std::min(a.group, a.tile_rows) : 0;
+    const int64_t chunks = keys / kChunk + 4 + heads * ((a.ids_count + kChunk - 1) / kChunk);
+    const int64_t tiles = a.ids_count > 0 ? static_cast<int64_t>(a.tokens) * ((a.group + a.tile_rows - 1) / a.tile_rows)
+                                          : static_cast<int64_t>(a.tokens) * a.group / kRows + a.requests;
+    int shift = 2;
+    while (shift < 24 && tiles * ((chunks >> shift) + 1 + kTileUnits) > INT32_MAX) ++shift;
+    return shift;
+}
+
 template <typename T, int kDim, bool kIds>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     using S = Smem<kDim, kIds>;
     static_assert((S::kBytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
-    constexpr int most = std::max(S::kBytes, locate_bytes<int64_t>(kMaxRequests));
+    constexpr int most = std::max(S::kBytes, locate_bytes(kMaxRequests));
     static_assert(most <= 227 * 1024, "a CTA's shared memory");
-    const int bytes = std::max(S::kBytes, locate_bytes<int64_t>(a.requests));
+    const int bytes = std::max(S::kBytes, locate_bytes(a.requests));
     a.base_align = kChunk;
     a.tile_rows = tile_rows(a);
     const bool split = attention_rows_splits(a);
     a.ctas *= kCtasPerSm;
-    a.unit_shift = split ? 2 : 24;  // a unit: one chunk for each warp, or a tile
-    a.tile_units = split ? 2 : 0;   // a tile's start and end take about as long as two chunks of each warp
+    a.unit_shift = split ? unit_shift(a) : 24;  // a unit: one chunk for each warp (or more, see there), or a tile
+    a.tile_units = split ? kTileUnits : 0;
     static SmemOnce once;
     cudaError_t e = once.set(reinterpret_cast<const void*>(attention_rows_kernel<T, kDim, kIds>), most);
     if (e != cudaSuccess) return e;

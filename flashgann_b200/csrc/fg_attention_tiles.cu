@@ -762,7 +762,7 @@ attention_tiles_kernel(const AttentionParams a, const __grid_constant__ CUtensor
     char* ws = static_cast<char*>(a.workspace);
 
     asm volatile("griddepcontrol.launch_dependents;");
-    const Place pl = locate<kRows, kTokens, kBlock, kThreads, 8, int>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, kTokens, kBlock, kThreads, 8>(a, reinterpret_cast<int*>(dynamic), blockIdx.x, a.ctas);
     if (pl.unit >= pl.end) {
         if (threadIdx.x == 0) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
         return;
@@ -1013,7 +1013,7 @@ bool encode(CUtensorMap* map, const AttentionParams& a, const void* data, const 
 template <typename T, int kDim>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     constexpr int bytes = Smem<kDim>::kBytes;
-    static_assert(bytes >= locate_bytes<int>(kMaxRequests), "the scan over the requests fits the tiles' room");
+    static_assert(bytes >= locate_bytes(kMaxRequests), "the scan over the requests fits the tiles' room");
     static SmemOnce once;
     cudaError_t e = once.set(reinterpret_cast<const void*>(attention_tiles_kernel<T, kDim>), bytes);
     if (e != cudaSuccess) return e;
@@ -1050,9 +1050,8 @@ cudaError_t by_dim(const AttentionParams& a, cudaStream_t s) {
 }  // namespace
 }  // namespace attn
 
-// Whether the kernel's 32-bit sums of blocks hold a call: 2^31 blocks would take it ten seconds, but the table's width
-// and the counts do not exclude them.  (64-bit sums cost every call: 2048 tokens on 8192 280.5 us for 277.2, 24 chunks
-// under a window 139 for 134.)
+// Whether the 32-bit sums of blocks hold a call: 2^31 blocks would take the kernel ten seconds, but the table's width and
+// the counts do not exclude them.
 bool attention_tiles_counts(const AttentionParams& a) {
     const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.table_width) * a.page_size, INT32_MAX);
     const int64_t tiles = static_cast<int64_t>(a.tokens) / (attn::kRows / a.group) + a.requests;
