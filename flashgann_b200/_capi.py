@@ -69,6 +69,24 @@ class AttentionArgs(ctypes.Structure):
                 ("ids_count", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
+class KVSummaryArgs(ctypes.Structure):
+    """fg_kv_summary"""
+    _fields_ = [("bounds", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("bounds_page_stride", ctypes.c_int64),
+                ("bounds_head_stride", ctypes.c_int64), ("scale_page_stride", ctypes.c_int64),
+                ("scale_head_stride", ctypes.c_int64), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("dim", ctypes.c_int32)]
+
+
+class BlockSelectionArgs(ctypes.Structure):
+    """fg_block_selection"""
+    _fields_ = [("q", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("query_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("blocks", ctypes.c_void_p), ("blocks_token_stride", ctypes.c_int64),
+                ("blocks_head_stride", ctypes.c_int64), ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("requests", ctypes.c_int32), ("table_width", ctypes.c_int32), ("window", ctypes.c_int32),
+                ("sinks", ctypes.c_int32), ("count", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
 # (name, restype, argtypes) for every entry point of include/flashgann.h
 _vp = ctypes.c_void_p
 _u64 = ctypes.c_uint64
@@ -106,6 +124,10 @@ SIGNATURES = [
     ("fg_paged_attention_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs), _vp]),
     ("fg_retrieved_attention_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs),
                                                      _vp]),
+    ("fg_kv_summarize_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(KVSummaryArgs), _vp, _i32,
+                                              _i64, _vp, _vp, _i32, _i32, _vp]),
+    ("fg_select_blocks_device", ctypes.c_int, [ctypes.POINTER(KVSummaryArgs), ctypes.POINTER(BlockSelectionArgs),
+                                               _vp]),
     ("fg_effective_sort_beam_size", _u32, [_u32]),
     ("fg_entry_point_centroid", _u32, [_vp, _u64, _u64, _u64, _i32]),
     ("fg_compute_recall", ctypes.c_float, [_vp, _vp, _u64, _i32, _i32]),

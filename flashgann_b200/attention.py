@@ -97,3 +97,31 @@ def retrieved_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     out, lse = _torch_ops.attention(q, k_cache, v_cache, block_table, query_start, kv_len, 1, ids, window, sinks, scale,
                                     out, return_lse, _handle(stream))
     return (out, lse) if return_lse else out
+
+
+def kv_summarize(k_cache: torch.Tensor, bounds: torch.Tensor, scale: torch.Tensor, block_table: torch.Tensor,
+                 query_start: torch.Tensor, kv_len: torch.Tensor, *, tokens: int, stream=None) -> None:
+    """Summaries of the pages that hold the step's new tokens, for
+    ``select_blocks`` (fg_kv_summarize_device); after ``kv_append``.
+
+    bounds int8 [pages, kv_heads, 2, dim], scale float32 [pages, kv_heads]:
+    least and largest value of each element over a page's keys, in whole
+    multiples of scale; made once beside the caches and updated in place.
+    query_start, kv_len: as from ``kv_plan`` (new pages only; a query_start of
+    the running sums of kv_len gives all pages, as after ``kv_evict``); tokens:
+    at least query_start's last entry."""
+    _torch_ops.kv_summarize(k_cache, bounds, scale, block_table, query_start, kv_len, tokens, _handle(stream))
+
+
+def select_blocks(q: torch.Tensor, bounds: torch.Tensor, scale: torch.Tensor, block_table: torch.Tensor,
+                  query_start: torch.Tensor, kv_len: torch.Tensor, count: int, *, page_size: int, window: int,
+                  sinks: int = 0, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """For each new token and kv head the ``count`` pages (numbers of blocks of
+    page_size positions) whose bound on the token's scores is highest, among
+    those with keys that window and first tokens do not show: int32 [T,
+    kv_heads, count], ascending, then -1 (fg_select_blocks_device).
+
+    q [T, heads, dim]; bounds and scale from ``kv_summarize``.  The heads of a
+    group choose together, by the largest of their bounds."""
+    return _torch_ops.select_blocks(q, bounds, scale, block_table, query_start, kv_len, count, page_size, window, sinks,
+                                    out, _handle(stream))

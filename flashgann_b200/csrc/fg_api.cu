@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include "fg_config.h"
+#include "fg_cache.h"
 #include "fg_internal.h"
 
 struct fg_index {
@@ -816,15 +817,15 @@ namespace {
 // An axis of one entry may have any stride: nothing is ever added for it.
 int64_t used_stride(int64_t stride, int64_t count) { return count > 1 ? stride : 0; }
 
-int check_cache(const fg_kv_cache* c) {
-    if (!c || !c->k || !c->v) return fail(FG_ERR_ARG, "null cache");
+int check_cache(const fg_kv_cache* c, bool keys_only = false) {
+    if (!c || !c->k || (!c->v && !keys_only)) return fail(FG_ERR_ARG, "null cache");
     if (c->dtype != FG_DTYPE_F16 && c->dtype != FG_DTYPE_BF16) return fail(FG_ERR_ARG, "unknown cache dtype %d", c->dtype);
     if (c->dim != 64 && c->dim != 96 && c->dim != 128)
         return fail(FG_ERR_UNSUPPORTED, "head dim %d is not 64, 96 or 128", c->dim);
     if (c->pages < 1 || c->heads < 1) return fail(FG_ERR_ARG, "bad cache shape pages=%d heads=%d", c->pages, c->heads);
     if (c->page_size < 1 || (c->page_size & (c->page_size - 1)))
         return fail(FG_ERR_UNSUPPORTED, "page size %d is not a power of two", c->page_size);
-    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
+    if ((reinterpret_cast<uintptr_t>(c->k) | (keys_only ? 0 : reinterpret_cast<uintptr_t>(c->v))) & 15)
         return fail(FG_ERR_ARG, "cache is not 16-byte aligned");
     const int64_t page = used_stride(c->page_stride, c->pages), token = used_stride(c->token_stride, c->page_size),
                   head = used_stride(c->head_stride, c->heads);
@@ -1112,6 +1113,142 @@ int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args
 int fg_retrieved_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {
     g_err.clear();
     return attention(cache, args, true, stream);
+}
+
+// ---- attention over chosen pages ----
+
+namespace {
+
+int check_summary(const fg_kv_summary* s) {
+    if (!s || !s->bounds || !s->scale) return fail(FG_ERR_ARG, "null summary");
+    if (s->dim != 64 && s->dim != 96 && s->dim != 128)
+        return fail(FG_ERR_UNSUPPORTED, "head dim %d is not 64, 96 or 128", s->dim);
+    if (s->pages < 1 || s->heads < 1) return fail(FG_ERR_ARG, "bad summary shape pages=%d heads=%d", s->pages, s->heads);
+    if (s->page_size < 1 || (s->page_size & (s->page_size - 1)))
+        return fail(FG_ERR_UNSUPPORTED, "page size %d is not a power of two", s->page_size);
+    if (reinterpret_cast<uintptr_t>(s->bounds) & 15) return fail(FG_ERR_ARG, "bounds are not 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(s->scale) & 3) return fail(FG_ERR_ARG, "scale is not aligned");
+    const int64_t page = used_stride(s->bounds_page_stride, s->pages), head = used_stride(s->bounds_head_stride, s->heads);
+    if ((page | head) & 15) return fail(FG_ERR_ARG, "strides of bounds are not multiples of 16 bytes");
+    if (page < 0 || head < 0 || used_stride(s->scale_page_stride, s->pages) < 0 || used_stride(s->scale_head_stride, s->heads) < 0)
+        return fail(FG_ERR_ARG, "negative stride of the summary");
+    return FG_OK;
+}
+
+fg::Summary summary_of(const fg_kv_summary* s) {
+    fg::Summary x;
+    x.bounds = s->bounds;
+    x.scale = s->scale;
+    x.bounds_page_stride = s->bounds_page_stride;
+    x.bounds_head_stride = s->bounds_head_stride;
+    x.scale_page_stride = s->scale_page_stride;
+    x.scale_head_stride = s->scale_head_stride;
+    return x;
+}
+
+fg::PagedRows paged_rows(const fg_kv_cache* c) {
+    fg::PagedRows x;
+    x.k = c->k;
+    x.page_stride = c->page_stride;
+    x.token_stride = c->token_stride;
+    x.head_stride = c->head_stride;
+    x.pages = c->pages;
+    x.page_shift = log2_of(c->page_size);
+    x.heads = c->heads;
+    x.dim = c->dim;
+    x.dtype = c->dtype;
+    return x;
+}
+
+// Counts and buffers that say where the requests are.
+int check_requests(const int32_t* table, int32_t width, int64_t stride, const int32_t* query_start, const int32_t* kv_len,
+                   int32_t requests, int32_t tokens) {
+    if (tokens < 0 || requests < 0 || width < 0)
+        return fail(FG_ERR_ARG, "bad shape tokens=%d requests=%d table_width=%d", tokens, requests, width);
+    if (requests == 0 || tokens == 0) return FG_OK;
+    if (!query_start || !kv_len || (!table && width > 0)) return fail(FG_ERR_ARG, "null buffer");
+    if (stride < 0) return fail(FG_ERR_ARG, "negative table stride");
+    return FG_OK;
+}
+
+fg::Requests requests_of(const int32_t* table, int32_t width, int64_t stride, const int32_t* query_start, const int32_t* kv_len,
+                         int32_t requests, int32_t tokens) {
+    fg::Requests r;
+    r.block_table = table;
+    r.table_stride = stride;
+    r.table_width = width;
+    r.query_start = query_start;
+    r.kv_len = kv_len;
+    r.requests = requests;
+    r.tokens = tokens;
+    return r;
+}
+
+}  // namespace
+
+int fg_kv_summarize_device(const fg_kv_cache* cache, const fg_kv_summary* summary, const int32_t* d_block_table, int32_t table_width,
+                           int64_t table_stride, const int32_t* d_query_start, const int32_t* d_kv_len, int32_t requests, int32_t tokens,
+                           void* stream) {
+    int rc = check_cache(cache, true);
+    if (rc || (rc = check_summary(summary))) return rc;
+    if (summary->pages != cache->pages || summary->page_size != cache->page_size || summary->heads != cache->heads || summary->dim != cache->dim)
+        return fail(FG_ERR_ARG, "the summary is not of this cache's shape");
+    if ((rc = check_requests(d_block_table, table_width, table_stride, d_query_start, d_kv_len, requests, tokens))) return rc;
+    if (overlaps({{{summary->bounds_page_stride, summary->pages}, {summary->bounds_head_stride, summary->heads}}}, 2 * summary->dim) ||
+        overlaps({{{summary->scale_page_stride, summary->pages}, {summary->scale_head_stride, summary->heads}}}, 1))
+        return fail(FG_ERR_ARG, "rows of the summary overlap");
+    if (requests == 0 || tokens == 0) return FG_OK;
+    if (((tokens >> log2_of(cache->page_size)) + 2 * static_cast<int64_t>(requests)) * cache->heads > INT32_MAX)
+        return fail(FG_ERR_UNSUPPORTED, "%d tokens of %d requests, %d heads", tokens, requests, cache->heads);
+    fg::SummarizeArgs a;
+    a.cache = paged_rows(cache);
+    a.summary = summary_of(summary);
+    a.req = requests_of(d_block_table, table_width, table_stride, d_query_start, d_kv_len, requests, tokens);
+    const cudaError_t e = fg::launch_kv_summarize(a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FG_OK : cuda_fail(e, "summary launch");
+}
+
+int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selection* x, void* stream) {
+    int rc = check_summary(summary);
+    if (rc) return rc;
+    if (!x) return fail(FG_ERR_ARG, "null arguments");
+    if (x->dtype != FG_DTYPE_F16 && x->dtype != FG_DTYPE_BF16) return fail(FG_ERR_ARG, "unknown query dtype %d", x->dtype);
+    if ((rc = check_requests(x->block_table, x->table_width, x->table_stride, x->query_start, x->kv_len, x->requests, x->tokens))) return rc;
+    if (x->heads < 1 || x->heads % summary->heads)
+        return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", x->heads, summary->heads);
+    if (x->heads / summary->heads > 256) return fail(FG_ERR_UNSUPPORTED, "%d query heads for each kv head", x->heads / summary->heads);
+    if (x->window < 0 || x->sinks < 0) return fail(FG_ERR_ARG, "bad mask window=%d sinks=%d", x->window, x->sinks);
+    if (x->count < 0) return fail(FG_ERR_ARG, "bad count %d", x->count);
+    if (x->table_width > fg::select_max_width())
+        return fail(FG_ERR_UNSUPPORTED, "table_width %d, at most %d", x->table_width, fg::select_max_width());
+    if (static_cast<int64_t>(x->tokens) * summary->heads > INT32_MAX / 8)
+        return fail(FG_ERR_UNSUPPORTED, "%d tokens of %d kv heads", x->tokens, summary->heads);
+    if (x->tokens == 0 || x->requests == 0 || x->count == 0) return FG_OK;
+    if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, x->tokens, x->heads, "q"))) return rc;
+    if (!x->blocks) return fail(FG_ERR_ARG, "null blocks");
+    if (overlaps({{{x->blocks_token_stride, x->tokens}, {x->blocks_head_stride, summary->heads}}}, x->count))
+        return fail(FG_ERR_ARG, "rows of blocks overlap");
+    fg::SelectArgs a;
+    a.summary = summary_of(summary);
+    a.req = requests_of(x->block_table, x->table_width, x->table_stride, x->query_start, x->kv_len, x->requests, x->tokens);
+    a.q = x->q;
+    a.q_token_stride = x->q_token_stride;
+    a.q_head_stride = x->q_head_stride;
+    a.blocks = x->blocks;
+    a.blocks_token_stride = x->blocks_token_stride;
+    a.blocks_head_stride = x->blocks_head_stride;
+    a.pages = summary->pages;
+    a.page_shift = log2_of(summary->page_size);
+    a.kv_heads = summary->heads;
+    a.group = x->heads / summary->heads;
+    a.dim = summary->dim;
+    a.dtype = x->dtype;
+    a.window = x->window;
+    a.sinks = x->sinks;
+    a.count = x->count;
+    if ((rc = sm_count(&a.sms))) return rc;
+    const cudaError_t e = fg::launch_select_blocks(a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FG_OK : cuda_fail(e, "selection launch");
 }
 
 uint32_t fg_effective_sort_beam_size(uint32_t beam) { return fg::effective_sort_beam(beam); }

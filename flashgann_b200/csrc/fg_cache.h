@@ -1,0 +1,54 @@
+// fg_cache.h -- arguments and launchers of the kernels that choose what a step
+// reads from the cache: page summaries, block selection, key weights, eviction.
+#pragma once
+
+#include <cstdint>
+
+#include <cuda_runtime.h>
+
+namespace fg {
+
+// K of a paged cache, or of both halves; strides in elements.
+struct PagedRows {
+    const void* k = nullptr;
+    int64_t page_stride = 0, token_stride = 0, head_stride = 0;
+    int pages = 0, page_shift = 0, heads = 0, dim = 0, dtype = 0;
+};
+
+struct Requests {
+    const int32_t* block_table = nullptr;
+    int64_t table_stride = 0;
+    const int32_t* query_start = nullptr;
+    const int32_t* kv_len = nullptr;
+    int table_width = 0, requests = 0, tokens = 0;
+};
+
+// int8 [pages, heads, 2, dim] (lower bounds, upper bounds) and float [pages, heads]; strides in elements
+struct Summary {
+    int8_t* bounds = nullptr;
+    float* scale = nullptr;
+    int64_t bounds_page_stride = 0, bounds_head_stride = 0, scale_page_stride = 0, scale_head_stride = 0;
+};
+
+struct SummarizeArgs {
+    PagedRows cache;
+    Summary summary;
+    Requests req;
+};
+cudaError_t launch_kv_summarize(const SummarizeArgs& a, cudaStream_t stream);
+
+struct SelectArgs {
+    Summary summary;
+    Requests req;
+    const void* q = nullptr;
+    int64_t q_token_stride = 0, q_head_stride = 0;
+    int32_t* blocks = nullptr;  // [tokens, kv_heads, count]
+    int64_t blocks_token_stride = 0, blocks_head_stride = 0;
+    int pages = 0, page_shift = 0, kv_heads = 0, group = 0, dim = 0, dtype = 0;
+    int window = 0, sinks = 0, count = 0;
+    int sms = 0;
+};
+int select_max_width();
+cudaError_t launch_select_blocks(const SelectArgs& a, cudaStream_t stream);
+
+}  // namespace fg

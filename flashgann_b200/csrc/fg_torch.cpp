@@ -110,7 +110,7 @@ at::Tensor rows(const at::Tensor& t, const char* name) {
     return t;
 }
 
-fg_kv_cache cache(const at::Tensor& k, const at::Tensor& v) {
+fg_kv_cache cache(const at::Tensor& k, const at::Tensor& v) {  // (k, k) where only the keys are read
     FG_NEED(k.dim() == 4 && v.sizes() == k.sizes(), "caches must be [pages, page_size, heads, dim] alike, not " + shape(k) + " and " + shape(v));
     FG_NEED((k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16) && v.scalar_type() == k.scalar_type(),
             "caches must both be float16 or bfloat16, not " + shape(k) + " and " + shape(v));
@@ -180,6 +180,17 @@ void kv_append(const at::Tensor& k_cache, const at::Tensor& v_cache, at::Tensor 
     written(v_cache);
 }
 
+// The lengths that say where a batch's requests are, checked against one another.
+void requests(at::Tensor& table, at::Tensor& query_start, at::Tensor& kv_len) {
+    table = ints(table, 2, "block_table");
+    query_start = ints(query_start, 1, "query_start");
+    kv_len = ints(kv_len, 1, "kv_len");
+    const int64_t R = kv_len.size(0);
+    FG_NEED(query_start.size(0) == R + 1 && table.size(0) == R,
+            std::to_string(R) + " lengths need " + std::to_string(R + 1) + " query_start entries and " + std::to_string(R) + " table rows, not " +
+                std::to_string(query_start.size(0)) + " and " + std::to_string(table.size(0)));
+}
+
 std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const at::Tensor& k_cache, const at::Tensor& v_cache, at::Tensor table,
                                                             at::Tensor query_start, at::Tensor kv_len, int64_t max_new,
                                                             std::optional<at::Tensor> ids, int64_t window, int64_t sinks,
@@ -195,13 +206,8 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const 
     const int64_t T = q.size(0), heads = q.size(1), dim = q.size(2);
     FG_NEED(q.scalar_type() == k_cache.scalar_type() && dim == c.dim,
             "q must be " + std::string(at::toString(k_cache.scalar_type())) + " [tokens, heads, " + std::to_string(c.dim) + "], not " + shape(q));
-    table = ints(table, 2, "block_table");
-    query_start = ints(query_start, 1, "query_start");
-    kv_len = ints(kv_len, 1, "kv_len");
+    requests(table, query_start, kv_len);
     const int64_t R = kv_len.size(0);
-    FG_NEED(query_start.size(0) == R + 1 && table.size(0) == R,
-            std::to_string(R) + " lengths need " + std::to_string(R + 1) + " query_start entries and " + std::to_string(R) + " table rows, not " +
-                std::to_string(query_start.size(0)) + " and " + std::to_string(table.size(0)));
     at::Tensor out;
     if (out_or_none) {
         out = *out_or_none;
@@ -255,10 +261,96 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const 
     return {out, lse};
 }
 
+fg_kv_summary summary(const at::Tensor& bounds, const at::Tensor& scale, int64_t page_size) {
+    FG_NEED(bounds.scalar_type() == at::kChar && bounds.dim() == 4 && bounds.size(2) == 2,
+            "bounds must be int8 [pages, heads, 2, dim], not " + shape(bounds));
+    FG_NEED(bounds.stride(3) == 1 && bounds.stride(2) == bounds.size(3), "bounds must have contiguous last two axes");
+    FG_NEED(scale.scalar_type() == at::kFloat && scale.dim() == 2 && scale.size(0) == bounds.size(0) && scale.size(1) == bounds.size(1),
+            "scale must be float32 [" + std::to_string(bounds.size(0)) + ", " + std::to_string(bounds.size(1)) + "], not " + shape(scale));
+    fg_kv_summary s{};
+    s.bounds = bounds.data_ptr<int8_t>();
+    s.scale = scale.data_ptr<float>();
+    s.bounds_page_stride = bounds.stride(0);
+    s.bounds_head_stride = bounds.stride(1);
+    s.scale_page_stride = scale.stride(0);
+    s.scale_head_stride = scale.stride(1);
+    s.pages = i32(bounds.size(0), "pages");
+    s.page_size = i32(page_size, "page size");
+    s.heads = i32(bounds.size(1), "heads");
+    s.dim = i32(bounds.size(3), "dim");
+    return s;
+}
+
+void kv_summarize(const at::Tensor& k_cache, const at::Tensor& bounds, const at::Tensor& scale, at::Tensor table, at::Tensor query_start,
+                  at::Tensor kv_len, int64_t tokens, int64_t stream) {
+    On on(k_cache, stream);
+    on.uses(k_cache, bounds, scale, table, query_start, kv_len);
+    no_gradient("k_cache and scale", k_cache, scale);
+    const fg_kv_cache c = cache(k_cache, k_cache);
+    const fg_kv_summary s = summary(bounds, scale, c.page_size);
+    requests(table, query_start, kv_len);
+    check(fg_kv_summarize_device(&c, &s, table.data_ptr<int32_t>(), i32(table.size(1), "table width"), table.stride(0),
+                                 query_start.data_ptr<int32_t>(), kv_len.data_ptr<int32_t>(), i32(kv_len.size(0), "requests"),
+                                 i32(tokens, "tokens"), on.stream()),
+          "fg_kv_summarize_device");
+    written(bounds);
+    written(scale);
+}
+
+at::Tensor select_blocks(at::Tensor q, const at::Tensor& bounds, const at::Tensor& scale, at::Tensor table, at::Tensor query_start,
+                         at::Tensor kv_len, int64_t count, int64_t page_size, int64_t window, int64_t sinks,
+                         const std::optional<at::Tensor>& out_or_none, int64_t stream) {
+    On on(q, stream);
+    on.uses(q, bounds, scale, table, query_start, kv_len);
+    if (out_or_none) on.uses(*out_or_none);
+    no_gradient("q and scale", q, scale);
+    const fg_kv_summary s = summary(bounds, scale, page_size);
+    q = rows(q, "q");
+    FG_NEED((q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16) && q.size(2) == s.dim,
+            "q must be float16 or bfloat16 [tokens, heads, " + std::to_string(s.dim) + "], not " + shape(q));
+    requests(table, query_start, kv_len);
+    const int64_t T = q.size(0);
+    FG_NEED(count >= 0, "count " + std::to_string(count) + " is negative");
+    at::Tensor out;
+    if (out_or_none) {
+        out = *out_or_none;
+        FG_NEED(out.scalar_type() == at::kInt && out.dim() == 3 && out.size(0) == T && out.size(1) == s.heads && out.size(2) == count &&
+                    (out.stride(2) == 1 || count <= 1),
+                "out must be int32 [" + std::to_string(T) + ", " + std::to_string(s.heads) + ", " + std::to_string(count) +
+                    "] with a contiguous last axis, not " + shape(out));
+    } else {
+        out = at::empty({T, s.heads, count}, q.options().dtype(at::kInt));
+    }
+    fg_block_selection x{};
+    x.q = q.data_ptr();
+    x.q_token_stride = q.stride(0);
+    x.q_head_stride = q.stride(1);
+    x.block_table = table.data_ptr<int32_t>();
+    x.table_stride = table.stride(0);
+    x.query_start = query_start.data_ptr<int32_t>();
+    x.kv_len = kv_len.data_ptr<int32_t>();
+    x.blocks = out.data_ptr<int32_t>();
+    x.blocks_token_stride = out.stride(0);
+    x.blocks_head_stride = out.stride(1);
+    x.tokens = i32(T, "tokens");
+    x.heads = i32(q.size(1), "heads");
+    x.requests = i32(kv_len.size(0), "requests");
+    x.table_width = i32(table.size(1), "table width");
+    x.window = i32(window, "window");
+    x.sinks = i32(sinks, "sinks");
+    x.count = i32(count, "count");
+    x.dtype = q.scalar_type() == at::kHalf ? FG_DTYPE_F16 : FG_DTYPE_BF16;
+    check(fg_select_blocks_device(&s, &x, on.stream()), "fg_select_blocks_device");
+    if (out_or_none) written(out);
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_ops, m) {
     m.def("kv_plan", &kv_plan);
     m.def("kv_append", &kv_append);
     m.def("attention", &attention);
+    m.def("kv_summarize", &kv_summarize);
+    m.def("select_blocks", &select_blocks);
 }

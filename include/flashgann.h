@@ -361,6 +361,70 @@ int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args
  * than a search finds). */
 int fg_retrieved_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream);
 
+/* ---- attention over chosen pages ----
+ *
+ * For contexts that no index was built over: each page's keys are summed up in
+ * 8 bits, a query's bound on its scores with them is computed for every page,
+ * and the attention reads the window, the first tokens and the pages of the
+ * highest bounds.  The same rules as above hold (device, stream, buffers,
+ * capture). */
+
+/* Summaries of a cache's pages, for each kv head: bounds[page, head, 0, d] and
+ * [page, head, 1, d] are the least and the largest value of the page's keys in
+ * element d, rounded down and up to whole multiples (-127 to 127) of
+ * scale[page, head], which is the largest magnitude times the 32-bit number
+ * nearest 1 / 127.  scale is inf (and the bounds 0) where a key is not finite.  The last two axes are contiguous;
+ * bounds and its strides are multiples of 16 bytes. */
+typedef struct fg_kv_summary {
+    int8_t* bounds;
+    float* scale;
+    int64_t bounds_page_stride, bounds_head_stride; /* bytes */
+    int64_t scale_page_stride, scale_head_stride;   /* elements */
+    int32_t pages, page_size, heads, dim;
+} fg_kv_summary;
+
+/* Writes the summaries of the pages that hold the new tokens of each request,
+ * positions kv_len[b] - new_b to kv_len[b] - 1 (new_b = query_start[b + 1] -
+ * query_start[b]; a query_start made from kv_len itself gives all pages), from
+ * the keys before kv_len[b] alone, whatever lies behind them.  After the append
+ * of the step; with a cache whose v may be NULL.  tokens: the most that
+ * query_start[requests] can be.  Pages of one call must differ. */
+int fg_kv_summarize_device(const fg_kv_cache* cache, const fg_kv_summary* summary, const int32_t* d_block_table,
+                           int32_t table_width, int64_t table_stride, const int32_t* d_query_start,
+                           const int32_t* d_kv_len, int32_t requests, int32_t tokens, void* stream);
+
+/* Arguments of the selection. */
+typedef struct fg_block_selection {
+    const void* q;                         /* [tokens, heads, dim] of `dtype` */
+    int64_t q_token_stride, q_head_stride; /* elements, multiples of 16 bytes */
+    const int32_t* block_table;            /* [requests, table_width] */
+    int64_t table_stride;
+    const int32_t* query_start;            /* [requests + 1] */
+    const int32_t* kv_len;                 /* [requests], new tokens included */
+    int32_t* blocks;                       /* [tokens, kv_heads, count] */
+    int64_t blocks_token_stride, blocks_head_stride;
+    int32_t tokens, heads, requests, table_width;
+    int32_t window, sinks, count, dtype;
+} fg_block_selection;
+
+/* For the new token at position p (as in fg_paged_attention_device) and each kv
+ * head, the `count` blocks of the highest score, ascending, then -1.  Block x of
+ * a request is its positions [x * page_size, (x + 1) * page_size), the page
+ * block_table[x].  Blocks with a key that window and first tokens do not show
+ * (a position >= sinks and <= p - window) are chosen from; those without a page
+ * in the cache are not.  The score is in the 8-bit arithmetic of the summary:
+ * with top the largest |q_d| of a query head, Q_d = q_d * 127 / top rounded to
+ * the nearest whole number and t = top times the 32-bit number nearest 1 / 127,
+ *   score = max over the kv head's query heads of
+ *           (sum_d Q_d * bounds[Q_d < 0 ? 0 : 1][d]) * t, times scale,
+ * the products after the sum in 32 bits (a bound of q.k, so for attention with a
+ * positive scale); a query head with a value that is not finite counts as 0, a
+ * page of scale inf has the score inf.  Of equal scores the lowest block comes
+ * first.  The same bits on every run.  The last axis of blocks is contiguous.
+ * Rows past query_start[requests] are not written.  Needs a window >= 0,
+ * heads / summary->heads <= 256, a table_width of at most 262144. */
+int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selection* args, void* stream);
+
 /* ---- host helpers of the reference CLI ---- */
 
 /* include/utils.cuh:119-127 */
