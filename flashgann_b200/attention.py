@@ -81,7 +81,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     sees nothing is 0 and -inf.  Sums are 32 bits, the weights of the product
     with V are rounded to the cache's type."""
     out, lse = _torch_ops.attention(q, k_cache, v_cache, block_table, query_start, kv_len, max_new, None,
-                                    -1 if window is None else window, sinks, scale, out, return_lse, _handle(stream))
+                                    False, -1 if window is None else window, sinks, scale, out, return_lse, _handle(stream))
     return (out, lse) if return_lse else out
 
 
@@ -94,8 +94,8 @@ def retrieved_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     of the request's context, in any order, as a search over its keys returns
     them (uint32 ids as int32 bits; negative, repeated, already visible and
     future ones count nothing)."""
-    out, lse = _torch_ops.attention(q, k_cache, v_cache, block_table, query_start, kv_len, 1, ids, window, sinks, scale,
-                                    out, return_lse, _handle(stream))
+    out, lse = _torch_ops.attention(q, k_cache, v_cache, block_table, query_start, kv_len, 1, ids, False, window, sinks,
+                                    scale, out, return_lse, _handle(stream))
     return (out, lse) if return_lse else out
 
 
@@ -125,3 +125,17 @@ def select_blocks(q: torch.Tensor, bounds: torch.Tensor, scale: torch.Tensor, bl
     group choose together, by the largest of their bounds."""
     return _torch_ops.select_blocks(q, bounds, scale, block_table, query_start, kv_len, count, page_size, window, sinks,
                                     out, _handle(stream))
+
+
+def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    query_start: torch.Tensor, kv_len: torch.Tensor, blocks: torch.Tensor, *, window: int,
+                    sinks: int = 0, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    return_lse: bool = False, stream=None):
+    """paged_attention over the window, the first tokens and chosen blocks
+    (fg_block_attention_device): blocks int32 [T, kv_heads, count], as
+    ``select_blocks`` returns them or any others (block x: positions x *
+    page_size to (x + 1) * page_size - 1; negative, repeated and future ones
+    and positions that are visible already count nothing)."""
+    out, lse = _torch_ops.attention(q, k_cache, v_cache, block_table, query_start, kv_len, 1, blocks, True, window,
+                                    sinks, scale, out, return_lse, _handle(stream))
+    return (out, lse) if return_lse else out

@@ -885,31 +885,34 @@ int sm_count(int* sms) {
 bool many_rows(const fg_kv_cache* c, const fg_attention* x) {
     return static_cast<int64_t>(x->max_new) * (x->heads / c->heads) > 16;
 }
-fg::AttentionParams counts(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
+// What an attention call's rows see beside the mask.
+enum Form { kMask = 0, kIds = 1, kBlocks = 2 };
+fg::AttentionParams counts(const fg_kv_cache* c, const fg_attention* x, Form form) {
     fg::AttentionParams a;
     a.table_width = x->table_width;
     a.page_size = c->page_size;
     a.window = x->window;
     a.sinks = x->sinks;
     a.group = x->heads / c->heads;
-    a.ids_count = retrieved ? x->ids_count : 0;
+    a.ids_count = form != kMask ? x->ids_count : 0;
+    a.chosen = form == kBlocks && a.ids_count > 0;
     a.requests = x->requests;
     a.tokens = x->tokens;
     a.kv_heads = c->heads;
     return a;
 }
-bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
+bool takes_tiles(const fg_kv_cache* c, const fg_attention* x, Form form) {
     const bool expanded = (c->token_stride == 0 && c->page_size > 1) || (c->head_stride == 0 && c->heads > 1) ||
                           (c->page_stride == 0 && c->pages > 1) || (x->q_token_stride == 0 && x->tokens > 1) ||
                           (x->q_head_stride == 0 && x->heads > 1);
-    return !retrieved && many_rows(c, x) && x->scale > 0.f && c->page_size >= 8 && !expanded &&
-           fg::attention_tiles_counts(counts(c, x, retrieved));
+    return form == kMask && many_rows(c, x) && x->scale > 0.f && c->page_size >= 8 && !expanded &&
+           fg::attention_tiles_counts(counts(c, x, form));
 }
 
 constexpr double kLog2e = 1.4426950408889634;  // exponents are base 2 in the kernels
 
 // Counts, mask and scale: everything that the choice of a kernel and the size of its workspace are computed from.
-int check_counts(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
+int check_counts(const fg_kv_cache* c, const fg_attention* x, Form form) {
     if (x->tokens < 0 || x->requests < 0 || x->table_width < 0 || x->max_new < 0)
         return fail(FG_ERR_ARG, "bad attention shape tokens=%d requests=%d table_width=%d max_new=%d", x->tokens,
                     x->requests, x->table_width, x->max_new);
@@ -922,45 +925,45 @@ int check_counts(const fg_kv_cache* c, const fg_attention* x, bool retrieved) {
         return fail(FG_ERR_UNSUPPORTED, "%d requests, at most %d", x->requests, fg::attention_max_requests());
     if (x->window < -1 || x->sinks < 0) return fail(FG_ERR_ARG, "bad mask window=%d sinks=%d", x->window, x->sinks);
     if (!(std::fabs(x->scale * kLog2e) <= FLT_MAX)) return fail(FG_ERR_ARG, "scale %g is not finite, or not once log2(e) is folded in", x->scale);
-    if (retrieved) {
-        if (x->window < 0) return fail(FG_ERR_ARG, "retrieved attention needs a window >= 0");
+    if (form != kMask) {
+        if (x->window < 0) return fail(FG_ERR_ARG, "%s attention needs a window >= 0", form == kIds ? "retrieved" : "block");
         if (x->ids_count < 0 || x->ids_token_stride < 0 || x->ids_head_stride < 0)
-            return fail(FG_ERR_ARG, "bad ids: count %d, or a negative stride", x->ids_count);
+            return fail(FG_ERR_ARG, "bad %s: count %d, or a negative stride", form == kIds ? "ids" : "blocks", x->ids_count);
         if (x->ids_count > fg::attention_max_ids())
-            return fail(FG_ERR_UNSUPPORTED, "%d ids for each row, at most %d", x->ids_count, fg::attention_max_ids());
+            return fail(FG_ERR_UNSUPPORTED, "%d %s for each row, at most %d", x->ids_count, form == kIds ? "ids" : "blocks", fg::attention_max_ids());
     }
     return FG_OK;
 }
 
-int workspace_bytes(const fg_kv_cache* c, const fg_attention* x, bool retrieved, uint64_t* bytes) {
+int workspace_bytes(const fg_kv_cache* c, const fg_attention* x, Form form, uint64_t* bytes) {
     int sms = 0;
     const int rc = sm_count(&sms);
     if (rc) return rc;
-    if (takes_tiles(c, x, retrieved)) {
+    if (takes_tiles(c, x, form)) {
         *bytes = fg::attention_tiles_workspace(sms, c->dim);
         return FG_OK;
     }
-    fg::AttentionParams a = counts(c, x, retrieved);  // what decides whether tiles are split
+    fg::AttentionParams a = counts(c, x, form);  // what decides whether tiles are split
     a.ctas = sms;
     *bytes = fg::attention_rows_workspace(a, sms, c->dim);
     return FG_OK;
 }
 
-int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void* stream) {
+int attention(const fg_kv_cache* c, const fg_attention* x, Form form, void* stream) {
     int rc = check_cache(c);
     if (rc) return rc;
     if (!x) return fail(FG_ERR_ARG, "null arguments");
-    if ((rc = check_counts(c, x, retrieved))) return rc;
+    if ((rc = check_counts(c, x, form))) return rc;
     if (x->tokens == 0 || x->requests == 0) return FG_OK;
     if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, x->tokens, x->heads, "q"))) return rc;
     if ((rc = check_rows(x->out, x->out_token_stride, x->out_head_stride, x->tokens, x->heads, "out"))) return rc;
     if (overlaps({{{x->out_token_stride, x->tokens}, {x->out_head_stride, x->heads}}}, c->dim))
         return fail(FG_ERR_ARG, "rows of out overlap");
-    if (!x->query_start || !x->kv_len || (!x->block_table && x->table_width > 0) || (retrieved && !x->ids && x->ids_count))
+    if (!x->query_start || !x->kv_len || (!x->block_table && x->table_width > 0) || (form != kMask && !x->ids && x->ids_count))
         return fail(FG_ERR_ARG, "null buffer");
     if (x->table_stride < 0) return fail(FG_ERR_ARG, "negative table stride");
     uint64_t need = 0;
-    if ((rc = workspace_bytes(c, x, retrieved, &need))) return rc;
+    if ((rc = workspace_bytes(c, x, form, &need))) return rc;
     if (need && (!x->workspace || (reinterpret_cast<uintptr_t>(x->workspace) & 255)))
         return fail(FG_ERR_ARG, "workspace is null or not 256-byte aligned");
     if (x->workspace_bytes < need)
@@ -1000,15 +1003,16 @@ int attention(const fg_kv_cache* c, const fg_attention* x, bool retrieved, void*
     a.window = x->window;
     a.sinks = x->sinks;
     a.scale_log2 = static_cast<float>(x->scale * kLog2e);
-    if (retrieved && x->ids_count > 0) {
+    if (form != kMask && x->ids_count > 0) {
         a.ids = x->ids;
+        a.chosen = form == kBlocks;
         a.ids_count = x->ids_count;
         a.ids_token_stride = x->ids_token_stride;
         a.ids_head_stride = x->ids_head_stride;
     }
     a.workspace = need ? x->workspace : nullptr;
     if ((rc = sm_count(&a.ctas))) return rc;
-    const cudaError_t e = takes_tiles(c, x, retrieved) ? fg::launch_attention_tiles(a, static_cast<cudaStream_t>(stream))
+    const cudaError_t e = takes_tiles(c, x, form) ? fg::launch_attention_tiles(a, static_cast<cudaStream_t>(stream))
                                                        : fg::launch_attention_rows(a, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? FG_OK : cuda_fail(e, "attention launch");
 }
@@ -1095,8 +1099,9 @@ int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* a
     int rc = check_cache(cache);
     if (rc) return rc;
     if (!args || !bytes) return fail(FG_ERR_ARG, "null argument");
-    if ((rc = check_counts(cache, args, retrieved != 0))) return rc;
-    return workspace_bytes(cache, args, retrieved != 0, bytes);
+    const Form form = retrieved == kBlocks ? kBlocks : retrieved ? kIds : kMask;
+    if ((rc = check_counts(cache, args, form))) return rc;
+    return workspace_bytes(cache, args, form, bytes);
 }
 
 // For tests only: in every CTA of the kernel of many rows, K tiles from block `first` on never come, and the waits for
@@ -1107,12 +1112,17 @@ extern "C" __attribute__((visibility("default"))) void fg_test_attention_lose_bl
 
 int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {
     g_err.clear();
-    return attention(cache, args, false, stream);
+    return attention(cache, args, kMask, stream);
 }
 
 int fg_retrieved_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {
     g_err.clear();
-    return attention(cache, args, true, stream);
+    return attention(cache, args, kIds, stream);
+}
+
+int fg_block_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {
+    g_err.clear();
+    return attention(cache, args, kBlocks, stream);
 }
 
 // ---- attention over chosen pages ----
@@ -1189,6 +1199,7 @@ fg::Requests requests_of(const int32_t* table, int32_t width, int64_t stride, co
 int fg_kv_summarize_device(const fg_kv_cache* cache, const fg_kv_summary* summary, const int32_t* d_block_table, int32_t table_width,
                            int64_t table_stride, const int32_t* d_query_start, const int32_t* d_kv_len, int32_t requests, int32_t tokens,
                            void* stream) {
+    g_err.clear();
     int rc = check_cache(cache, true);
     if (rc || (rc = check_summary(summary))) return rc;
     if (summary->pages != cache->pages || summary->page_size != cache->page_size || summary->heads != cache->heads || summary->dim != cache->dim)
@@ -1209,6 +1220,7 @@ int fg_kv_summarize_device(const fg_kv_cache* cache, const fg_kv_summary* summar
 }
 
 int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selection* x, void* stream) {
+    g_err.clear();
     int rc = check_summary(summary);
     if (rc) return rc;
     if (!x) return fail(FG_ERR_ARG, "null arguments");

@@ -5,7 +5,8 @@
 // Mathematics.  Query row (token i of a request, head h) stands at position
 // p = kv_len - new + i and sees the keys
 //     V(p) = { j : 0 <= j <= p, and (no window, or p - j < window, or j < sinks) }
-// plus, for the retrieved form, those of its head's ids that are in [0, p].
+// plus, for the retrieved form, those of its head's ids that are in [0, p], and
+// for the form of chosen pages the keys j <= p of its kv head's blocks.
 // With s_j = scale * q.k_j it returns o = sum_j e^(s_j) v_j / sum_j e^(s_j)
 // and lse = log sum_j e^(s_j) over j in V(p); 0 and -inf where V(p) is empty.
 // All kernels walk the keys once with a running maximum m, sum l and
@@ -96,21 +97,23 @@ __device__ __forceinline__ int div_group(const AttentionParams& a, int n) {
 //   kPacked  kRows consecutive (token, head of the group) pairs of a request
 //   kTokens  the group's heads of as many tokens as fit kRows rows
 //   kToken   one token, tile_rows heads of the group (what each head retrieved is its own)
-enum Layout { kPacked, kTokens, kToken };
+//   kChosen  the same, of which all rows see the token's chosen pages
+enum Layout { kPacked, kTokens, kToken, kChosen };
 
 template <int kRows, Layout kLayout>
 struct Tiles {
+    static constexpr bool kOne = kLayout == kToken || kLayout == kChosen;
     // tokens of a tile, or tiles of a token
     __device__ static __forceinline__ int per(const AttentionParams& a) {
         return kLayout == kTokens ? div_group(a, kRows) : (a.group + a.tile_rows - 1) / a.tile_rows;
     }
     __device__ static __forceinline__ int count(const AttentionParams& a, const Request& r) {
-        if (kLayout == kToken) return r.rows * per(a);
+        if (kOne) return r.rows * per(a);
         if (kLayout == kTokens) return (r.rows + per(a) - 1) / per(a);
         return (r.rows * a.group + kRows - 1) / kRows;
     }
     __device__ static __forceinline__ void tokens(const AttentionParams& a, const Request& r, int t, int* i0, int* i1) {
-        if (kLayout == kToken) {
+        if (kOne) {
             *i0 = *i1 = t / per(a);
         } else if (kLayout == kTokens) {
             *i0 = t * per(a);
@@ -122,7 +125,7 @@ struct Tiles {
     }
     // row -> (token of the request, head of the group); false past the tile's end
     __device__ static __forceinline__ bool row(const AttentionParams& a, const Request& r, int t, int row, int* i, int* g) {
-        if (kLayout == kToken) {
+        if (kOne) {
             const int n = per(a);
             *i = t / n;
             *g = (t - *i * n) * a.tile_rows + row;
@@ -154,6 +157,11 @@ __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Re
     if (kLayout == kToken && a.ids_count > 0 && k.lo > 0) {
         const int heads = min(a.tile_rows, a.group - (t % Tiles<kRows, kLayout>::per(a)) * a.tile_rows);
         k.id_chunks = heads * ((a.ids_count + kChunk - 1) / kChunk);
+    }
+    if (kLayout == kChosen && k.lo > a.sinks) {
+        // no more blocks can count than hold a key between the first tokens and the window
+        const int blocks = min(a.ids_count, ((k.lo - 1) >> a.page_shift) - (a.sinks >> a.page_shift) + 1);
+        k.id_chunks = static_cast<int>(((static_cast<int64_t>(blocks) << a.page_shift) + kChunk - 1) / kChunk);
     }
     k.chunks = k.sink_chunks + k.near_chunks + k.id_chunks;
     // a tile that sees nothing still writes its rows

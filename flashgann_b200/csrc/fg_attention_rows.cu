@@ -1,5 +1,5 @@
 // fg_attention_rows.cu -- attention of few query rows over the paged cache:
-// decode steps, a few drafted tokens, and the retrieved form.
+// decode steps, a few drafted tokens, the retrieved form and that of chosen pages.
 //
 // A tile is 16 query rows of one kv head (the heads that share it, times the
 // request's tokens), the height of one m16n8k16 product.  With so few rows a
@@ -26,6 +26,11 @@
 // heads' lists once, drop the ids that do not count (out of range, in the window,
 // repeated) and leave the rest in shared memory, see stage_ids.
 //
+// Chosen pages are contiguous runs of keys that all rows of a tile see (a tile is
+// one token's heads, whose kv head the list belongs to).  The list is brought to
+// shared memory without the blocks that do not count, see stage_blocks; key n of
+// its chunks is row n % page_size of block n / page_size.
+//
 // Measured (device time, 32 or 64 query heads on 8, dim 128, bf16): 64 ragged
 // decodes, 1.1 GB of keys and values, 174 to 180 us, 6.1 to 6.3 TB/s; one of
 // 131K keys at most, 80 to 83 us; one of a few hundred keys of dim 64 7.6 to 8.3
@@ -51,7 +56,7 @@ constexpr int kMaxIds = 1024;  // ids of a tile's heads, in shared memory
 __host__ __device__ __forceinline__ int staged_pitch(int count) { return (count + 127) & ~127; }
 
 // Heads to a tile: with ids as many as have room for theirs.
-int tile_rows(const AttentionParams& a) { return a.ids_count > 0 ? std::min(kRows, kMaxIds / staged_pitch(a.ids_count)) : kRows; }
+int tile_rows(const AttentionParams& a) { return a.ids_count > 0 && !a.chosen ? std::min(kRows, kMaxIds / staged_pitch(a.ids_count)) : kRows; }
 }  // namespace
 
 // Whether tiles are split over CTAs (a.ctas: SMs).  The host knows how many
@@ -77,14 +82,15 @@ bool attention_rows_splits(const AttentionParams& a) {
     int64_t tiles = static_cast<int64_t>(a.requests) * a.kv_heads;
     if (a.ids_count > 0) {
         const int rows = tile_rows(a);
-        chunks += static_cast<int64_t>(std::min(a.group, rows)) * ((a.ids_count + kChunk - 1) / kChunk);
+        if (a.chosen) chunks += std::min(static_cast<int64_t>(a.ids_count), static_cast<int64_t>(a.table_width)) * a.page_size / kChunk + 1;
+        else chunks += static_cast<int64_t>(std::min(a.group, rows)) * ((a.ids_count + kChunk - 1) / kChunk);
         tiles = static_cast<int64_t>(a.tokens) * a.kv_heads * ((a.group + rows - 1) / rows);
     }
     const int64_t ctas = static_cast<int64_t>(a.ctas) * kCtasPerSm;
     if (chunks > 64) return true;
     if (tiles * 8 <= ctas) return chunks > 20;
     if (tiles * 10 >= (tiles + ctas - 1) / ctas * ctas * 8) return false;
-    return tiles <= ctas ? chunks > 36 && a.ids_count == 0 : chunks > 18;
+    return tiles <= ctas ? chunks > 36 && (a.ids_count == 0 || a.chosen) : chunks > 18;
 }
 
 namespace attn {
@@ -94,10 +100,13 @@ constexpr int kWarps = 4;
 constexpr int kTileUnits = 2;  // a tile's start and end take about as long as two chunks of each warp
 constexpr int kThreads = kWarps * 32;
 static_assert(kThreads == 128, "lists of ids lie in groups of 128");
+constexpr int kBlockTable = 2048;  // the same for one list of blocks: half full at most
 constexpr int kTable = 8192;     // places of the hash table over them: with 2048 or 4096 staging takes twice or 1.3 times as long
 
-template <int kDim, bool kIds>
+// What a kernel's tiles see: kPacked, the mask alone; kToken, retrieved ids too; kChosen, chosen pages too.
+template <int kDim, Layout kForm>
 struct Smem {
+    static constexpr bool kIds = kForm == kToken;
     // ldmatrix reads 8 rows without bank conflicts: rows of 128 or 256 bytes with their 16-byte pieces exchanged by the
     // row's number, rows of 192 bytes padded to an odd multiple of 16
     static constexpr bool kExchange = kDim % 64 == 0;
@@ -109,8 +118,8 @@ struct Smem {
     static constexpr int kStages = kIds ? 2 : 3;  // of the ring; with ids the third one's room is the table's (3 % for decodes)
     static constexpr int kRing = kStages * 2 * kTile;  // K and V of each stage
     static constexpr int kWarpBytes = kRing;
-    static constexpr int kIdsAt = kWarps * kWarpBytes;  // retrieved form: the tile's ids and the table
-    static constexpr int kBytes = kIdsAt + (kIds ? kMaxIds * 4 + kTable * 4 : 0);
+    static constexpr int kIdsAt = kWarps * kWarpBytes;  // retrieved form: the tile's ids and the table; blocks likewise
+    static constexpr int kBytes = kIdsAt + (kIds ? kMaxIds * 4 + kTable * 4 : kForm == kChosen ? (kMaxIds + kBlockTable) * 4 : 0);
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -179,9 +188,11 @@ struct Chunk {
     __device__ __forceinline__ bool has(int col) const { return (ok[col >> 3] >> ((col & 7) * 4)) & 1u; }
 };
 
-template <typename T, int kDim, bool kIds>
+template <typename T, int kDim, Layout kForm>
 struct Warp {
-    using S = Smem<kDim, kIds>;
+    using S = Smem<kDim, kForm>;
+    static constexpr bool kIds = kForm == kToken;
+    static constexpr bool kOne = kForm != kPacked;        // the tile's rows are of one token
     static constexpr int kPieces = kDim / 8;              // 16-byte pieces of a row
     // A float16 weight below 2^-25 would be zero in the product while the sum l counts it: many keys far below the
     // maximum would be lost.  Weights and o are 2^15 times as large there, exactly, until the warps join, so that those
@@ -200,6 +211,7 @@ struct Warp {
     int prow[2];       // positions of this lane's two rows (-1: no row)
     const int32_t* ids;  // the tile's lists of retrieved ids
     const int* staged;   // those of all its rows that count, in shared memory
+    int staged_count;    // chosen pages: how many
     // running state
     uint32_t q[kDim / 16][4];
     float o[kDim / 8][4];
@@ -213,13 +225,13 @@ struct Warp {
         table = a.block_table + request * a.table_stride;
         head_off = head * a.head_stride;
         int i0, i1;
-        Tiles<kRows, kIds ? kToken : kPacked>::tokens(a, req, tile, &i0, &i1);
+        Tiles<kRows, kForm>::tokens(a, req, tile, &i0, &i1);
         p0 = req.kv_len - req.rows + i0;
         p1 = req.kv_len - req.rows + i1;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             int i, g;
-            const bool ok = Tiles<kRows, kIds ? kToken : kPacked>::row(a, req, tile, (lane >> 2) + 8 * x, &i, &g);
+            const bool ok = Tiles<kRows, kForm>::row(a, req, tile, (lane >> 2) + 8 * x, &i, &g);
             prow[x] = ok ? req.kv_len - req.rows + i : -1;
             const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(req.start + i) * a.q_token_stride +
                            static_cast<int64_t>(head * a.group + g) * a.q_head_stride + (lane & 3) * 2;
@@ -242,8 +254,9 @@ struct Warp {
     // The lists of a tile's heads.
     __device__ __forceinline__ const int32_t* lists(const Request& r, int head, int tile) const {
         int i, g;
-        Tiles<kRows, kIds ? kToken : kPacked>::row(a, r, tile, 0, &i, &g);
-        return a.ids + static_cast<int64_t>(r.start + i) * a.ids_token_stride + static_cast<int64_t>(head * a.group + g) * a.ids_head_stride;
+        Tiles<kRows, kForm>::row(a, r, tile, 0, &i, &g);
+        return a.ids + static_cast<int64_t>(r.start + i) * a.ids_token_stride +
+               static_cast<int64_t>(kForm == kChosen ? head : head * a.group + g) * a.ids_head_stride;
     }
     // The lists lie in shared memory in groups of kThreads places, each of one head; group `at` and the three after it.
     __device__ __forceinline__ void read_groups(const int32_t* from, int at, int groups, int (&id)[4]) const {
@@ -255,6 +268,7 @@ struct Warp {
         }
     }
     __device__ __forceinline__ int list_heads(int tile) const {
+        if (kForm == kChosen) return 1;
         return min(a.tile_rows, a.group - (tile % Tiles<kRows, kToken>::per(a)) * a.tile_rows);
     }
     // The first ids of a tile that comes next, into registers.
@@ -291,6 +305,14 @@ struct Warp {
             const int* list = staged + f.row * staged_pitch(a.ids_count);
             f.j[0] = list[n];
             f.j[1] = list[n + 8];
+        } else if (kForm == kChosen) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int n = (c - keys.sink_chunks - keys.near_chunks) * kChunk + x + 8 * y, at = n >> a.page_shift;
+                if (at >= staged_count) continue;
+                const int j = (staged[at] << a.page_shift) + (n & (a.page_size - 1));
+                if (j >= a.sinks && j < keys.lo) f.j[y] = j;  // the others the mask has, or they are in the future
+            }
         }
 #pragma unroll
         for (int y = 0; y < 2; ++y)
@@ -345,6 +367,94 @@ struct Warp {
         __syncthreads();
     }
 
+    // Reads the tile's list of blocks into shared memory, without those that hold no key between the first tokens and the
+    // window, and of equal ones without all but the first.  A list as the selection leaves it, ascending and then negative,
+    // has no equal ones; any other goes through a hash table as in stage_ids.  Called by the whole CTA.
+    __device__ __forceinline__ void stage_blocks(int* list, int* hash) {
+        constexpr int kFree = -1;
+        const int groups = staged_pitch(a.ids_count) / kThreads, warp = threadIdx.x >> 5;
+        const int first = a.sinks >> a.page_shift, last = keys.lo > a.sinks ? (keys.lo - 1) >> a.page_shift : -1;
+        int id[kMaxIds / kThreads];
+        uint32_t here = 0;  // bit y: id[y] counts
+        bool sorted = true;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) id[y] = early[y];
+        if (groups > 4) {
+            int more[4];
+            read_groups(ids, 4, groups, more);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) id[4 + y] = more[y];
+        } else {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) id[4 + y] = -1;
+        }
+#pragma unroll
+        for (int y = 0; y < kMaxIds / kThreads; ++y)
+            if (y < groups) {
+                list[y * kThreads + threadIdx.x] = id[y];
+                if (id[y] >= first && id[y] <= last) here |= 1u << y;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int y = 0; y < kMaxIds / kThreads; ++y) {
+            const int x = y * kThreads + threadIdx.x;
+            if (y < groups && x > 0 && id[y] >= 0) {
+                const int before = list[x - 1];
+                sorted = sorted && before >= 0 && before < id[y];
+            }
+        }
+        if (!__syncthreads_and(sorted)) {
+            for (int x = threadIdx.x; x < kBlockTable / 4; x += kThreads) reinterpret_cast<int4*>(hash)[x] = make_int4(kFree, kFree, kFree, kFree);
+            __syncthreads();
+            const auto first_place = [](int b) { return (static_cast<uint32_t>(b) * 2654435761u) >> 21; };  // of 2048
+#pragma unroll
+            for (int y = 0; y < kMaxIds / kThreads; ++y) {
+                if (!((here >> y) & 1)) continue;
+                const int x = y * kThreads + threadIdx.x;
+                for (uint32_t place = first_place(id[y]);; place = (place + 1) % kBlockTable) {
+                    const int old = atomicCAS(hash + place, kFree, x);
+                    if (old == kFree) break;
+                    if (list[old] != id[y]) continue;  // another block's place
+                    atomicMin(hash + place, x);
+                    break;
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int y = 0; y < kMaxIds / kThreads; ++y) {
+                if (!((here >> y) & 1)) continue;
+                uint32_t place = first_place(id[y]);
+                while (list[hash[place]] != id[y]) place = (place + 1) % kBlockTable;
+                if (hash[place] != y * kThreads + static_cast<int>(threadIdx.x)) here &= ~(1u << y);
+            }
+            __syncthreads();
+        }
+        // those that count move together, in order
+        int* counts = hash;  // of each group and warp
+#pragma unroll
+        for (int y = 0; y < kMaxIds / kThreads; ++y) {
+            const uint32_t b = __ballot_sync(0xFFFFFFFFu, (here >> y) & 1);
+            if (lane == 0) counts[y * kWarps + warp] = __popc(b);
+        }
+        __syncthreads();
+        int at = 0;
+#pragma unroll
+        for (int y = 0; y < kMaxIds / kThreads; ++y) {
+            const uint32_t b = __ballot_sync(0xFFFFFFFFu, (here >> y) & 1);
+            int before = 0, all = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const int n = counts[y * kWarps + w];
+                if (w < warp) before += n;
+                all += n;
+            }
+            if ((here >> y) & 1) list[at + before + __popc(b & ((1u << lane) - 1))] = id[y];
+            at += all;
+        }
+        staged_count = at;
+        __syncthreads();
+    }
+
     // Starts the copies of a chunk into stage s.
     __device__ __forceinline__ Chunk load(const Found& f, int s) const {
         Chunk ch;
@@ -370,7 +480,7 @@ struct Warp {
 
     __device__ __forceinline__ bool sees(const Chunk& ch, int x, int col) const {
         if (!ch.has(col)) return false;
-        if (kIds) return ch.row < 0 || (lane >> 2) + 8 * x == ch.row;  // one token: what is loaded is visible
+        if (kOne) return ch.row < 0 || (lane >> 2) + 8 * x == ch.row;  // one token: what is loaded is visible
         const int j = ch.key + col, p = prow[x];
         return j <= p && (a.window < 0 || p - j < a.window || j < a.sinks);
     }
@@ -445,7 +555,7 @@ struct Warp {
 
     // Rows of the tile differ in what they see, and a sum is not finite.
     __device__ __forceinline__ bool tainted() const {
-        if (!kIds && p0 == p1) return false;
+        if (kForm == kChosen || (!kIds && p0 == p1)) return false;
         float t = 0.f;
 #pragma unroll
         for (int n = 0; n < kDim / 8; ++n)
@@ -469,7 +579,7 @@ struct Warp {
             mma<T>(sc[1], q[k], b[2], b[3]);
         }
         const bool whole = (ch.ok[0] & ch.ok[1]) == 0xFFFFFFFFu && ch.row < 0 &&
-                           (kIds || p0 == p1 || (ch.key + kChunk - 1 <= p0 && (a.window < 0 || p1 - ch.key < a.window ||
+                           (kOne || p0 == p1 || (ch.key + kChunk - 1 <= p0 && (a.window < 0 || p1 - ch.key < a.window ||
                                                                               ch.key + kChunk - 1 < a.sinks)));
         bool poison = false;
 #pragma unroll
@@ -525,35 +635,36 @@ struct Warp {
     }
 };
 
-template <typename T, int kDim, bool kIds>
+template <typename T, int kDim, Layout kForm>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(const AttentionParams a) {
-    using S = Smem<kDim, kIds>;
+    using S = Smem<kDim, kForm>;
+    constexpr bool kLists = kForm != kPacked;
     extern __shared__ __align__(128) char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     char* ws = static_cast<char*>(a.workspace);
 
     asm volatile("griddepcontrol.launch_dependents;");
-    const Place pl = locate<kRows, kIds ? kToken : kPacked, kChunk, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
+    const Place pl = locate<kRows, kForm, kChunk, kThreads, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
     __syncthreads();  // the rings overlay the scan
     if (pl.unit >= pl.end) {
         if (threadIdx.x == 0 && ws) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = TileRecord{};
         return;
     }
 
-    Warp<T, kDim, kIds> w(a, smem_addr(smem) + warp * S::kWarpBytes);
+    Warp<T, kDim, kForm> w(a, smem_addr(smem) + warp * S::kWarpBytes);
     int head = pl.head, request = pl.request, tile = pl.tile;
     int64_t unit = pl.unit, tile_first = pl.unit - pl.offset;
     w.req = load_request(a, request);
-    w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk>(a, w.req, tile);
+    w.keys = tile_keys<kRows, kForm, kChunk>(a, w.req, tile);
     if (threadIdx.x == 0 && ws) reinterpret_cast<TileRecord*>(ws)[blockIdx.x] = tile_record(a, pl, blockIdx.x, w.req, w.keys.units);
-    if (kIds) w.read_ids(w.req, head, tile);
+    if (kLists) w.read_ids(w.req, head, tile);
     bool first_segment = true;
     while (true) {
         const int64_t tile_last = tile_first + w.keys.units;
         const int u0 = max(0, static_cast<int>(unit - tile_first) - a.tile_units);
         const int u1 = static_cast<int>(min(tile_last, pl.end) - tile_first) - a.tile_units;
         if (u1 <= 0) break;  // the range ends before the tile's first chunk
-        const int c1 = min(u1 << a.unit_shift, w.keys.chunks);
+        int c1 = min(u1 << a.unit_shift, w.keys.chunks);
         w.begin(head, request, tile);
         const int window_end = w.keys.sink_chunks + w.keys.near_chunks;  // chunks from here on need the tile's ids
         const int c0 = u0 << a.unit_shift;
@@ -574,12 +685,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
                     }
             };
             int ready = S::kStages;
-            if (kIds && !w.safe && c1 > window_end) {
+            if (kLists && !w.safe && c1 > window_end) {
                 // those of the first chunks that need no ids, so that their copies are under way while the ids are read
                 ready = max(0, min(ready, (window_end - c0) / kWarps));
                 begin_stages(0, ready);
                 int* list = reinterpret_cast<int*>(smem + S::kIdsAt);
-                w.stage_ids(list, list + kMaxIds, w.list_heads(tile));
+                if constexpr (kForm == kChosen) {
+                    w.stage_blocks(list, list + kMaxIds);
+                    c1 = min(c1, max(window_end, window_end + static_cast<int>(((static_cast<int64_t>(w.staged_count) << a.page_shift) + kChunk - 1) / kChunk)));
+                } else {
+                    w.stage_ids(list, list + kMaxIds, w.list_heads(tile));
+                }
                 w.staged = list;
                 begin_stages(ready, S::kStages);
             } else {
@@ -615,8 +731,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         // the next tile's request and ids are read beside the join
         Request next_req = w.req;
         int next_head = head, next_request = request, next_number = tile;
-        const bool more = pl.end - tile_last > a.tile_units && next_tile<kRows, kIds ? kToken : kPacked>(a, &next_req, &next_head, &next_request, &next_number);
-        if (kIds && more) w.read_ids(next_req, next_head, next_number);
+        const bool more = pl.end - tile_last > a.tile_units && next_tile<kRows, kForm>(a, &next_req, &next_head, &next_request, &next_number);
+        if (kLists && more) w.read_ids(next_req, next_head, next_number);
 
         // join the warps: rows of (m, l) and sums, over the rings
 #pragma unroll
@@ -625,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             w.l[x] += __shfl_xor_sync(0xFFFFFFFFu, w.l[x], 2);
         }
         __syncthreads();
-        constexpr float kUnlift = 1.f / Warp<T, kDim, kIds>::kLift;
+        constexpr float kUnlift = 1.f / Warp<T, kDim, kForm>::kLift;
         constexpr int kSumPitch = kDim + 4;
         float* sums = reinterpret_cast<float*>(smem);                       // [warp][row][kSumPitch]
         float* stat = sums + kWarps * kRows * kSumPitch;                    // [warp][row][2]
@@ -669,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
             }
             if (whole_tile) {
                 int i, g;
-                if (Tiles<kRows, kIds ? kToken : kPacked>::row(a, w.req, tile, row, &i, &g)) {
+                if (Tiles<kRows, kForm>::row(a, w.req, tile, row, &i, &g)) {
                     const float inv = ll == 0.f ? 1.f : 1.f / ll;
                     const int64_t token = w.req.start + i;
                     const int h = head * a.group + g;
@@ -692,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
         head = next_head;
         request = next_request;
         tile = next_number;
-        w.keys = tile_keys<kRows, kIds ? kToken : kPacked, kChunk>(a, w.req, tile);
+        w.keys = tile_keys<kRows, kForm, kChunk>(a, w.req, tile);
         first_segment = false;
         __syncthreads();  // the join's reads end before the next tile's copies
     }
@@ -704,7 +820,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rows_kernel(co
 int unit_shift(const AttentionParams& a) {
     const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.table_width) * a.page_size, INT32_MAX);
     const int64_t heads = a.ids_count > 0 ? std::min(a.group, a.tile_rows) : 0;
-    const int64_t chunks = keys / kChunk + 4 + heads * ((a.ids_count + kChunk - 1) / kChunk);
+    // the blocks of a list that count lie in the context
+    const int64_t listed = a.chosen ? keys / kChunk + 1 : heads * ((a.ids_count + kChunk - 1) / kChunk);
+    const int64_t chunks = keys / kChunk + 4 + listed;
     const int64_t tiles = a.ids_count > 0 ? static_cast<int64_t>(a.tokens) * ((a.group + a.tile_rows - 1) / a.tile_rows)
                                           : static_cast<int64_t>(a.tokens) * a.group / kRows + a.requests;
     int shift = 2;
@@ -712,9 +830,9 @@ int unit_shift(const AttentionParams& a) {
     return shift;
 }
 
-template <typename T, int kDim, bool kIds>
+template <typename T, int kDim, Layout kForm>
 cudaError_t launch(AttentionParams a, cudaStream_t stream) {
-    using S = Smem<kDim, kIds>;
+    using S = Smem<kDim, kForm>;
     static_assert((S::kBytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
     constexpr int most = std::max(S::kBytes, locate_bytes(kMaxRequests));
     static_assert(most <= 227 * 1024, "a CTA's shared memory");
@@ -726,16 +844,17 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     a.unit_shift = split ? unit_shift(a) : 24;  // a unit: one chunk for each warp (or more, see there), or a tile
     a.tile_units = split ? kTileUnits : 0;
     static SmemOnce once;
-    cudaError_t e = once.set(reinterpret_cast<const void*>(attention_rows_kernel<T, kDim, kIds>), most);
+    cudaError_t e = once.set(reinterpret_cast<const void*>(attention_rows_kernel<T, kDim, kForm>), most);
     if (e != cudaSuccess) return e;
-    attention_rows_kernel<T, kDim, kIds><<<a.ctas, kThreads, bytes, stream>>>(a);
+    attention_rows_kernel<T, kDim, kForm><<<a.ctas, kThreads, bytes, stream>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess || !split) return e;
-    return launch_combine<T, kRows, kDim, kIds ? kToken : kPacked, 1>(a, stream);
+    return launch_combine<T, kRows, kDim, kForm, 1>(a, stream);
 }
 
 template <typename T, int kDim>
 cudaError_t by_ids(const AttentionParams& a, cudaStream_t s) {
-    return a.ids ? launch<T, kDim, true>(a, s) : launch<T, kDim, false>(a, s);
+    if (a.chosen) return launch<T, kDim, kChosen>(a, s);
+    return a.ids ? launch<T, kDim, kToken>(a, s) : launch<T, kDim, kPacked>(a, s);
 }
 template <typename T>
 cudaError_t by_dim(const AttentionParams& a, cudaStream_t s) {

@@ -151,6 +151,7 @@ struct AttentionParams {
     float scale_log2 = 0.f;  // scale * log2(e): all exponents are base 2
     const int32_t* ids = nullptr;
     int ids_count = 0;
+    bool chosen = false;  // ids are blocks of page_size keys, one list for each kv head
     int64_t ids_token_stride = 0, ids_head_stride = 0;
     void* workspace = nullptr;
     int ctas = 0;           // CTAs that share the work (to the launchers: SMs)

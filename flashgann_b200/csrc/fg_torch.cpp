@@ -193,7 +193,7 @@ void requests(at::Tensor& table, at::Tensor& query_start, at::Tensor& kv_len) {
 
 std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const at::Tensor& k_cache, const at::Tensor& v_cache, at::Tensor table,
                                                             at::Tensor query_start, at::Tensor kv_len, int64_t max_new,
-                                                            std::optional<at::Tensor> ids, int64_t window, int64_t sinks,
+                                                            std::optional<at::Tensor> ids, bool blocks, int64_t window, int64_t sinks,
                                                             std::optional<double> scale, const std::optional<at::Tensor>& out_or_none,
                                                             bool return_lse, int64_t stream) {
     On on(q, stream);
@@ -220,8 +220,10 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const 
     if (return_lse) lse = at::empty({T, heads}, q.options().dtype(at::kFloat));
     fg_attention x{};
     if (ids) {
-        FG_NEED(ids->scalar_type() == at::kInt && ids->dim() == 3 && ids->size(0) == T && ids->size(1) == heads,
-                "ids must be int32 [" + std::to_string(T) + ", " + std::to_string(heads) + ", count], not " + shape(*ids));
+        const int64_t lists = blocks ? c.heads : heads;
+        FG_NEED(ids->scalar_type() == at::kInt && ids->dim() == 3 && ids->size(0) == T && ids->size(1) == lists,
+                std::string(blocks ? "blocks" : "ids") + " must be int32 [" + std::to_string(T) + ", " + std::to_string(lists) + ", count], not " +
+                    shape(*ids));
         if (ids->stride(2) != 1 && ids->size(2) > 1) ids = ids->contiguous();
         x.ids = ids->data_ptr<int32_t>();
         x.ids_token_stride = ids->stride(0);
@@ -248,14 +250,15 @@ std::tuple<at::Tensor, std::optional<at::Tensor>> attention(at::Tensor q, const 
     x.sinks = i32(sinks, "sinks");
     x.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(dim)));
     uint64_t bytes = 0;
-    check(fg_attention_workspace_bytes(&c, &x, ids.has_value(), &bytes), "fg_attention_workspace_bytes");
+    check(fg_attention_workspace_bytes(&c, &x, !ids ? 0 : blocks ? 2 : 1, &bytes), "fg_attention_workspace_bytes");
     at::Tensor work;
     if (bytes) {
         work = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
         x.workspace = work.data_ptr();
         x.workspace_bytes = bytes;
     }
-    if (ids) check(fg_retrieved_attention_device(&c, &x, on.stream()), "fg_retrieved_attention_device");
+    if (ids && blocks) check(fg_block_attention_device(&c, &x, on.stream()), "fg_block_attention_device");
+    else if (ids) check(fg_retrieved_attention_device(&c, &x, on.stream()), "fg_retrieved_attention_device");
     else check(fg_paged_attention_device(&c, &x, on.stream()), "fg_paged_attention_device");
     if (out_or_none) written(out);
     return {out, lse};

@@ -318,7 +318,8 @@ typedef struct fg_attention {
     int64_t table_stride;
     const int32_t* query_start;                 /* [requests + 1] */
     const int32_t* kv_len;                      /* [requests], new tokens included */
-    const int32_t* ids;                         /* fg_retrieved_attention_device: [tokens, heads, ids_count] */
+    const int32_t* ids;                         /* fg_retrieved_attention_device: [tokens, heads, ids_count]
+                                                 * fg_block_attention_device: blocks [tokens, kv heads, ids_count] */
     int64_t ids_token_stride, ids_head_stride;
     void* workspace;                            /* fg_attention_workspace_bytes, 256-byte aligned; contents do not matter;
                                                  * NULL where 0 bytes are needed */
@@ -333,7 +334,8 @@ typedef struct fg_attention {
 
 /* Bytes of workspace that a call needs on the current device, for partial
  * results of rows whose keys are split over CTAs (0: none, where no row can
- * have many keys).  retrieved: 1 for fg_retrieved_attention_device.  Depends
+ * have many keys).  retrieved: 1 for fg_retrieved_attention_device, 2 for
+ * fg_block_attention_device.  Depends
  * on args' counts (tokens, heads, requests, table_width, max_new, window,
  * sinks, ids_count), the scale's sign and which strides are 0 only. */
 int fg_attention_workspace_bytes(const fg_kv_cache* cache, const fg_attention* args, int32_t retrieved,
@@ -424,6 +426,15 @@ typedef struct fg_block_selection {
  * Rows past query_start[requests] are not written.  Needs a window >= 0,
  * heads / summary->heads <= 256, a table_width of at most 262144. */
 int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selection* args, void* stream);
+
+/* fg_paged_attention_device over window, first tokens and chosen blocks: row
+ * (token, head) also sees the positions j <= p of the blocks of page_size
+ * positions in ids[token, head's kv head, :].  The visible keys are a set:
+ * blocks in any order, a block that repeats counts once, as do its positions
+ * that window and first tokens show already; negative blocks and those past the
+ * context count nothing.  Needs a window >= 0; at most 1024 blocks for each kv
+ * head. */
+int fg_block_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream);
 
 /* ---- host helpers of the reference CLI ---- */
 

@@ -69,3 +69,12 @@ def select_ref(q, bounds, scale, table, query_start, kv_len, count, page, window
                 got = sorted(cand[x] for x in order)
                 out[t, h] = got + [-1] * (count - len(got))
     return out
+
+
+def block_ids(blocks, page, heads, width):
+    """The positions of blocks [T, kv_heads, count] as ids [T, heads, count * page], -1 where there are none."""
+    T, kv_heads, count = blocks.shape
+    ok = (blocks >= 0) & (blocks < width)  # past the table: past the context
+    ids = np.where(ok, blocks, 0).astype(np.int64)[..., None] * page + np.arange(page)
+    ids = np.where(ok[..., None], ids, -1).reshape(T, kv_heads, count * page)
+    return np.repeat(ids, heads // kv_heads, 1)
