@@ -20,7 +20,7 @@ BIN_DIR := bin
 
 KERNEL_SRC := $(CSRC)/fg_search.cu $(CSRC)/fg_search_warp.cu $(CSRC)/fg_shard_merge.cu $(CSRC)/fg_kv.cu \
               $(CSRC)/fg_attention_rows.cu $(CSRC)/fg_attention_tiles.cu $(CSRC)/fg_blocks.cu \
-              $(CSRC)/fg_api.cu
+              $(CSRC)/fg_key_weights.cu $(CSRC)/fg_evict.cu $(CSRC)/fg_api.cu
 HEADERS    := $(CSRC)/fg_config.h $(CSRC)/fg_internal.h $(CSRC)/fg_device.cuh include/flashgann.h
 ATTN_HEADERS := $(CSRC)/fg_attention.cuh
 OBJ_DIR    := flashgann_b200/_build
@@ -54,9 +54,9 @@ $(OBJ_DIR)/%.o: $(CSRC)/%.cu $(HEADERS) | $(OBJ_DIR)
 $(OBJ_DIR):
 	mkdir -p $(OBJ_DIR)
 
-$(OBJ_DIR)/fg_attention_rows.o $(OBJ_DIR)/fg_attention_tiles.o: $(ATTN_HEADERS)
-$(OBJ_DIR)/fg_blocks.o: $(CSRC)/fg_cache.h $(CSRC)/fg_topk.cuh
-$(OBJ_DIR)/fg_api.o: $(CSRC)/fg_cache.h
+$(OBJ_DIR)/fg_attention_rows.o $(OBJ_DIR)/fg_attention_tiles.o $(OBJ_DIR)/fg_key_weights.o: $(ATTN_HEADERS)
+$(OBJ_DIR)/fg_blocks.o $(OBJ_DIR)/fg_evict.o: $(CSRC)/fg_topk.cuh
+$(OBJ_DIR)/fg_blocks.o $(OBJ_DIR)/fg_evict.o $(OBJ_DIR)/fg_key_weights.o $(OBJ_DIR)/fg_api.o: $(CSRC)/fg_cache.h
 
 $(LIB): $(OBJS)
 	$(NVCC) $(GENCODE) -shared -o $@ $(OBJS)

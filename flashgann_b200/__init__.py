@@ -310,8 +310,8 @@ def infer_metric_from_dataset_path(path: str) -> int:
 
 # flashgann_b200.attention needs torch, which the search's host-buffer calls do not: loaded on first use, and not in
 # __all__, so that a star import does without it
-_ATTENTION = ("KVPlan", "block_attention", "kv_append", "kv_plan", "kv_summarize", "paged_attention",
-              "retrieved_attention", "select_blocks")
+_ATTENTION = ("KVEviction", "KVPlan", "attention_weights", "block_attention", "kv_append", "kv_evict", "kv_plan",
+              "kv_summarize", "paged_attention", "retrieved_attention", "select_blocks")
 
 
 def __getattr__(name: str):

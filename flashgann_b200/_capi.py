@@ -129,6 +129,10 @@ SIGNATURES = [
     ("fg_select_blocks_device", ctypes.c_int, [ctypes.POINTER(KVSummaryArgs), ctypes.POINTER(BlockSelectionArgs),
                                                _vp]),
     ("fg_block_attention_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs), _vp]),
+    ("fg_attention_weights_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs), _vp,
+                                                   _i64, _i64, _vp, _vp]),
+    ("fg_kv_evict_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), _vp, _i64, _i64, _vp, _i32, _i64, _vp, _i32,
+                                          _i32, _i32, _i32, _vp, _vp, _vp]),
     ("fg_effective_sort_beam_size", _u32, [_u32]),
     ("fg_entry_point_centroid", _u32, [_vp, _u64, _u64, _u64, _i32]),
     ("fg_compute_recall", ctypes.c_float, [_vp, _vp, _u64, _i32, _i32]),

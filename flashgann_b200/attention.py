@@ -39,6 +39,12 @@ class KVPlan(NamedTuple):
     refused: torch.Tensor      # int32 [R]: 1 where the pages did not suffice
 
 
+class KVEviction(NamedTuple):
+    """What kv_evict returns; R requests."""
+    kv_len: torch.Tensor  # int32 [R]: tokens that stayed
+    kept: torch.Tensor    # int32 [R, kv_heads, budget]: where each was before, ascending (-1 past the length)
+
+
 def _handle(stream) -> int:
     return -1 if stream is None else getattr(stream, "cuda_stream", stream) or 0
 
@@ -139,3 +145,35 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     out, lse = _torch_ops.attention(q, k_cache, v_cache, block_table, query_start, kv_len, 1, blocks, True, window,
                                     sinks, scale, out, return_lse, _handle(stream))
     return (out, lse) if return_lse else out
+
+
+def attention_weights(q: torch.Tensor, k_cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor,
+                      query_start: torch.Tensor, kv_len: torch.Tensor, lse: torch.Tensor, *,
+                      window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None,
+                      held: Optional[torch.Tensor] = None, stream=None) -> None:
+    """Adds to weights float32 [pages, kv_heads, page_size] the attention that
+    the step's rows paid to each key of their requests
+    (fg_attention_weights_device); after ``paged_attention(...,
+    return_lse=True)`` with the same arguments, whose lse float32 [T, heads]
+    this takes.
+
+    Weights of positions from held[b] on (int32 [R]; default: of the new tokens)
+    start at 0.  For a prompt the last tokens may do: their rows of q and lse,
+    a query_start that counts them alone, and held of 0."""
+    _torch_ops.attention_weights(q, k_cache, weights, block_table, query_start, kv_len, lse, held,
+                                 -1 if window is None else window, sinks, scale, _handle(stream))
+
+
+def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor,
+             kv_len: torch.Tensor, budget: int, *, recent: int = 0, sinks: int = 0, stream=None) -> KVEviction:
+    """Cuts requests of more than ``budget`` tokens down to it, in place
+    (fg_kv_evict_device): each kv head keeps the first ``sinks`` tokens, the
+    last ``recent`` and the heaviest of those between, by weights float32
+    [pages, kv_heads, page_size] from ``attention_weights``; keys, values and
+    weights of those move to the first positions, in order.
+
+    Table entries from ceil(budget / page_size) on of such requests are free
+    afterwards; kv_len of the result is the next step's ctx_len.  Page
+    summaries are made anew with ``kv_summarize`` over all pages."""
+    return KVEviction(*_torch_ops.kv_evict(k_cache, v_cache, weights, block_table, kv_len, budget, recent, sinks,
+                                           _handle(stream)))

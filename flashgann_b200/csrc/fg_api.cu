@@ -949,26 +949,8 @@ int workspace_bytes(const fg_kv_cache* c, const fg_attention* x, Form form, uint
     return FG_OK;
 }
 
-int attention(const fg_kv_cache* c, const fg_attention* x, Form form, void* stream) {
-    int rc = check_cache(c);
-    if (rc) return rc;
-    if (!x) return fail(FG_ERR_ARG, "null arguments");
-    if ((rc = check_counts(c, x, form))) return rc;
-    if (x->tokens == 0 || x->requests == 0) return FG_OK;
-    if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, x->tokens, x->heads, "q"))) return rc;
-    if ((rc = check_rows(x->out, x->out_token_stride, x->out_head_stride, x->tokens, x->heads, "out"))) return rc;
-    if (overlaps({{{x->out_token_stride, x->tokens}, {x->out_head_stride, x->heads}}}, c->dim))
-        return fail(FG_ERR_ARG, "rows of out overlap");
-    if (!x->query_start || !x->kv_len || (!x->block_table && x->table_width > 0) || (form != kMask && !x->ids && x->ids_count))
-        return fail(FG_ERR_ARG, "null buffer");
-    if (x->table_stride < 0) return fail(FG_ERR_ARG, "negative table stride");
-    uint64_t need = 0;
-    if ((rc = workspace_bytes(c, x, form, &need))) return rc;
-    if (need && (!x->workspace || (reinterpret_cast<uintptr_t>(x->workspace) & 255)))
-        return fail(FG_ERR_ARG, "workspace is null or not 256-byte aligned");
-    if (x->workspace_bytes < need)
-        return fail(FG_ERR_ARG, "workspace of %llu bytes, %llu needed", (unsigned long long)x->workspace_bytes,
-                    (unsigned long long)need);
+// What a kernel is told of the cache, the queries, the requests and the mask.
+fg::AttentionParams params(const fg_kv_cache* c, const fg_attention* x) {
     fg::AttentionParams a;
     a.k_cache = c->k;
     a.v_cache = c->v;
@@ -1003,6 +985,30 @@ int attention(const fg_kv_cache* c, const fg_attention* x, Form form, void* stre
     a.window = x->window;
     a.sinks = x->sinks;
     a.scale_log2 = static_cast<float>(x->scale * kLog2e);
+    return a;
+}
+
+int attention(const fg_kv_cache* c, const fg_attention* x, Form form, void* stream) {
+    int rc = check_cache(c);
+    if (rc) return rc;
+    if (!x) return fail(FG_ERR_ARG, "null arguments");
+    if ((rc = check_counts(c, x, form))) return rc;
+    if (x->tokens == 0 || x->requests == 0) return FG_OK;
+    if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, x->tokens, x->heads, "q"))) return rc;
+    if ((rc = check_rows(x->out, x->out_token_stride, x->out_head_stride, x->tokens, x->heads, "out"))) return rc;
+    if (overlaps({{{x->out_token_stride, x->tokens}, {x->out_head_stride, x->heads}}}, c->dim))
+        return fail(FG_ERR_ARG, "rows of out overlap");
+    if (!x->query_start || !x->kv_len || (!x->block_table && x->table_width > 0) || (form != kMask && !x->ids && x->ids_count))
+        return fail(FG_ERR_ARG, "null buffer");
+    if (x->table_stride < 0) return fail(FG_ERR_ARG, "negative table stride");
+    uint64_t need = 0;
+    if ((rc = workspace_bytes(c, x, form, &need))) return rc;
+    if (need && (!x->workspace || (reinterpret_cast<uintptr_t>(x->workspace) & 255)))
+        return fail(FG_ERR_ARG, "workspace is null or not 256-byte aligned");
+    if (x->workspace_bytes < need)
+        return fail(FG_ERR_ARG, "workspace of %llu bytes, %llu needed", (unsigned long long)x->workspace_bytes,
+                    (unsigned long long)need);
+    fg::AttentionParams a = params(c, x);
     if (form != kMask && x->ids_count > 0) {
         a.ids = x->ids;
         a.chosen = form == kBlocks;
@@ -1261,6 +1267,89 @@ int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selecti
     if ((rc = sm_count(&a.sms))) return rc;
     const cudaError_t e = fg::launch_select_blocks(a, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? FG_OK : cuda_fail(e, "selection launch");
+}
+
+// ---- eviction by attention weight ----
+
+namespace {
+
+int check_weights(const fg_kv_cache* c, const float* w, int64_t page_stride, int64_t head_stride) {
+    if (!w) return fail(FG_ERR_ARG, "null weights");
+    if (reinterpret_cast<uintptr_t>(w) & 3) return fail(FG_ERR_ARG, "weights are not aligned");
+    if (used_stride(page_stride, c->pages) < 0 || used_stride(head_stride, c->heads) < 0)
+        return fail(FG_ERR_ARG, "negative stride of the weights");
+    if (overlaps({{{page_stride, c->pages}, {head_stride, c->heads}}}, c->page_size)) return fail(FG_ERR_ARG, "rows of the weights overlap");
+    return FG_OK;
+}
+
+fg::KeyWeights key_weights(float* w, int64_t page_stride, int64_t head_stride) {
+    fg::KeyWeights x;
+    x.w = w;
+    x.page_stride = page_stride;
+    x.head_stride = head_stride;
+    return x;
+}
+
+}  // namespace
+
+int fg_attention_weights_device(const fg_kv_cache* cache, const fg_attention* x, float* d_weights, int64_t weights_page_stride,
+                                int64_t weights_head_stride, const int32_t* d_held, void* stream) {
+    g_err.clear();
+    int rc = check_cache(cache, true);
+    if (rc) return rc;
+    if (!x) return fail(FG_ERR_ARG, "null arguments");
+    if ((rc = check_counts(cache, x, kMask))) return rc;
+    if ((rc = check_weights(cache, d_weights, weights_page_stride, weights_head_stride))) return rc;
+    if (x->tokens == 0 || x->requests == 0) return FG_OK;
+    if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, x->tokens, x->heads, "q"))) return rc;
+    if (!x->lse) return fail(FG_ERR_ARG, "null lse");
+    if ((rc = check_requests(x->block_table, x->table_width, x->table_stride, x->query_start, x->kv_len, x->requests, x->tokens))) return rc;
+    fg::AttentionParams a = params(cache, x);
+    fg::WeightsArgs w;
+    w.weights = key_weights(d_weights, weights_page_stride, weights_head_stride);
+    w.lse = x->lse;
+    w.held = d_held;
+    w.scale = x->scale;
+    if ((rc = sm_count(&a.ctas))) return rc;
+    const cudaError_t e = fg::launch_attention_weights(a, w, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FG_OK : cuda_fail(e, "key weights launch");
+}
+
+int fg_kv_evict_device(const fg_kv_cache* cache, float* d_weights, int64_t weights_page_stride, int64_t weights_head_stride,
+                       const int32_t* d_block_table, int32_t table_width, int64_t table_stride, const int32_t* d_kv_len, int32_t requests,
+                       int32_t budget, int32_t recent, int32_t sinks, int32_t* d_kv_len_out, int32_t* d_kept, void* stream) {
+    g_err.clear();
+    int rc = check_cache(cache);
+    if (rc) return rc;
+    if (requests < 0 || table_width < 0) return fail(FG_ERR_ARG, "bad shape requests=%d table_width=%d", requests, table_width);
+    if (budget < 1 || recent < 0 || sinks < 0 || static_cast<int64_t>(recent) + sinks > budget)
+        return fail(FG_ERR_ARG, "bad budget %d with recent=%d sinks=%d", budget, recent, sinks);
+    if ((rc = check_weights(cache, d_weights, weights_page_stride, weights_head_stride))) return rc;
+    if (overlaps({{{cache->page_stride, cache->pages}, {cache->token_stride, cache->page_size}, {cache->head_stride, cache->heads}}}, cache->dim))
+        return fail(FG_ERR_ARG, "rows of the cache overlap");
+    if (requests == 0) return FG_OK;
+    if (!d_kv_len || !d_kv_len_out || !d_kept || (!d_block_table && table_width > 0)) return fail(FG_ERR_ARG, "null buffer");
+    if (d_kv_len_out == d_kv_len) return fail(FG_ERR_ARG, "kv_len and its output are the same buffer");
+    if (table_stride < 0) return fail(FG_ERR_ARG, "negative table stride");
+    if (static_cast<int64_t>(requests) * cache->heads > INT32_MAX / 8)
+        return fail(FG_ERR_UNSUPPORTED, "%d requests of %d heads", requests, cache->heads);
+    fg::EvictArgs a;
+    a.cache = paged_rows(cache);
+    a.v = cache->v;
+    a.weights = key_weights(d_weights, weights_page_stride, weights_head_stride);
+    a.block_table = d_block_table;
+    a.table_stride = table_stride;
+    a.kv_len = d_kv_len;
+    a.table_width = table_width;
+    a.requests = requests;
+    a.budget = budget;
+    a.recent = recent;
+    a.sinks = sinks;
+    a.kv_len_out = d_kv_len_out;
+    a.kept = d_kept;
+    if ((rc = sm_count(&a.sms))) return rc;
+    const cudaError_t e = fg::launch_kv_evict(a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? FG_OK : cuda_fail(e, "eviction launch");
 }
 
 uint32_t fg_effective_sort_beam_size(uint32_t beam) { return fg::effective_sort_beam(beam); }

@@ -66,6 +66,7 @@ __host__ __device__ constexpr int locate_bytes(int requests) { return (64 + requ
 // One request as every kernel reads it, clamped to the buffers the launch was given.
 struct Request {
     int start, rows, kv_len;  // first query token, new tokens, keys
+    int index;                // its number
 };
 
 __device__ __forceinline__ Request load_request(const AttentionParams& a, int b) {
@@ -74,6 +75,7 @@ __device__ __forceinline__ Request load_request(const AttentionParams& a, int b)
     r.start = s;
     r.rows = max(0, e - s);
     r.kv_len = max(0, a.kv_len[b]);
+    r.index = b;
     return r;
 }
 
@@ -98,7 +100,8 @@ __device__ __forceinline__ int div_group(const AttentionParams& a, int n) {
 //   kTokens  the group's heads of as many tokens as fit kRows rows
 //   kToken   one token, tile_rows heads of the group (what each head retrieved is its own)
 //   kChosen  the same, of which all rows see the token's chosen pages
-enum Layout { kPacked, kTokens, kToken, kChosen };
+//   kWhole   all rows of the request; the keys that any of them sees, and those that have no weight yet
+enum Layout { kPacked, kTokens, kToken, kChosen, kWhole };
 
 template <int kRows, Layout kLayout>
 struct Tiles {
@@ -109,12 +112,16 @@ struct Tiles {
     }
     __device__ static __forceinline__ int count(const AttentionParams& a, const Request& r) {
         if (kOne) return r.rows * per(a);
+        if (kLayout == kWhole) return r.rows > 0;
         if (kLayout == kTokens) return (r.rows + per(a) - 1) / per(a);
         return (r.rows * a.group + kRows - 1) / kRows;
     }
     __device__ static __forceinline__ void tokens(const AttentionParams& a, const Request& r, int t, int* i0, int* i1) {
         if (kOne) {
             *i0 = *i1 = t / per(a);
+        } else if (kLayout == kWhole) {
+            *i0 = 0;
+            *i1 = r.rows - 1;
         } else if (kLayout == kTokens) {
             *i0 = t * per(a);
             *i1 = min(r.rows, *i0 + per(a)) - 1;
@@ -139,6 +146,10 @@ struct Tiles {
     }
 };
 
+// kWhole: what a chunk of keys costs, in units.  Products and exponentials of 64 rows take about as long as the chunk's
+// way from memory.
+__device__ __forceinline__ int whole_cost(const AttentionParams& a, const Request& r) { return 1 + ((r.rows * a.group) >> 6); }
+
 template <int kRows, Layout kLayout, int kChunk>
 __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Request& r, int t) {
     TileKeys k;
@@ -149,6 +160,7 @@ __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Re
     const int64_t room = min(static_cast<int64_t>(a.table_width) * a.page_size, static_cast<int64_t>(INT32_MAX - 1023));
     k.hi = p1 < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(p1) + 1, room));
     k.lo = (a.window < 0 || p0 < a.window) ? 0 : min(p0 - a.window + 1, k.hi);
+    if (kLayout == kWhole) k.lo = min(k.lo, a.held ? max(0, a.held[r.index]) : max(0, p0));
     k.base = k.lo & -a.base_align;
     k.sink_hi = min(a.sinks, k.base);
     k.sink_chunks = (k.sink_hi + kChunk - 1) / kChunk;
@@ -166,6 +178,7 @@ __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Re
     k.chunks = k.sink_chunks + k.near_chunks + k.id_chunks;
     // a tile that sees nothing still writes its rows
     k.units = a.tile_units + max(1, (k.chunks + (1 << a.unit_shift) - 1) >> a.unit_shift);
+    if (kLayout == kWhole) k.units = max(1, (k.chunks + (1 << a.unit_shift) - 1) >> a.unit_shift) * whole_cost(a, r);
     return k;
 }
 
@@ -381,7 +394,7 @@ __global__ void __launch_bounds__(256) attention_combine_kernel(const AttentionP
     const auto partial = [&](int x) { return partials + (x == 0 ? rec.before : 2 * (c - 1 + x)) * kPartial; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane * 4;
     const int row = ((blockIdx.x % kBlocks) * 8 + warp) * kJoin;
-    const Request r = {rec.start, rec.rows, 0};
+    const Request r = {rec.start, rec.rows, 0, 0};
     int i[kJoin], g[kJoin];
     bool valid[kJoin];
     float m[kJoin], ref[kJoin], l[kJoin];

@@ -51,4 +51,35 @@ struct SelectArgs {
 int select_max_width();
 cudaError_t launch_select_blocks(const SelectArgs& a, cudaStream_t stream);
 
+struct AttentionParams;
+
+// float [pages, heads, page_size], the last axis contiguous; strides in elements
+struct KeyWeights {
+    float* w = nullptr;
+    int64_t page_stride = 0, head_stride = 0;
+};
+
+struct WeightsArgs {
+    KeyWeights weights;
+    const float* lse = nullptr;     // [tokens, heads]
+    const int32_t* held = nullptr;  // [requests], optional
+    float scale = 0.f;
+};
+cudaError_t launch_attention_weights(const AttentionParams& a, const WeightsArgs& w, cudaStream_t stream);
+
+struct EvictArgs {
+    PagedRows cache;
+    void* v = nullptr;
+    KeyWeights weights;
+    const int32_t* block_table = nullptr;
+    int64_t table_stride = 0;
+    const int32_t* kv_len = nullptr;
+    int table_width = 0, requests = 0;
+    int budget = 0, recent = 0, sinks = 0;
+    int32_t* kv_len_out = nullptr;
+    int32_t* kept = nullptr;  // [requests, heads, budget]
+    int sms = 0;
+};
+cudaError_t launch_kv_evict(const EvictArgs& a, cudaStream_t stream);
+
 }  // namespace fg

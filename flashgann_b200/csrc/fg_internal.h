@@ -159,6 +159,7 @@ struct AttentionParams {
     int unit_shift = 0;     // log2 of the key chunks in a unit of work
     int tile_units = 0;     // what a tile costs beside its chunks, in units
     int tile_rows = 16;     // retrieved form: heads to a tile
+    const int32_t* held = nullptr;  // key weights: positions of each request that have one already (optional)
     // kernel of many rows: how often a wait inside a CTA looks again before it gives up; block whose K tile never comes
     int wait_tries = 0, lost_block = 0;
 };

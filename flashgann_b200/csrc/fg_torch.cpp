@@ -348,6 +348,82 @@ at::Tensor select_blocks(at::Tensor q, const at::Tensor& bounds, const at::Tenso
     return out;
 }
 
+// float32 [pages, heads, page_size] beside a cache
+void check_weights(const at::Tensor& weights, const fg_kv_cache& c) {
+    FG_NEED(weights.scalar_type() == at::kFloat && weights.dim() == 3 && weights.size(0) == c.pages && weights.size(1) == c.heads &&
+                weights.size(2) == c.page_size && (weights.stride(2) == 1 || c.page_size == 1),
+            "weights must be float32 [" + std::to_string(c.pages) + ", " + std::to_string(c.heads) + ", " + std::to_string(c.page_size) +
+                "] with a contiguous last axis, not " + shape(weights));
+}
+
+void attention_weights(at::Tensor q, const at::Tensor& k_cache, const at::Tensor& weights, at::Tensor table, at::Tensor query_start,
+                       at::Tensor kv_len, at::Tensor lse, std::optional<at::Tensor> held, int64_t window, int64_t sinks,
+                       std::optional<double> scale, int64_t stream) {
+    On on(q, stream);
+    on.uses(q, k_cache, weights, table, query_start, kv_len, lse);
+    if (held) on.uses(*held);
+    no_gradient("q, k_cache, weights and lse", q, k_cache, weights, lse);
+    const fg_kv_cache c = cache(k_cache, k_cache);
+    check_weights(weights, c);
+    q = rows(q, "q");
+    const int64_t T = q.size(0), heads = q.size(1), dim = q.size(2);
+    FG_NEED(q.scalar_type() == k_cache.scalar_type() && dim == c.dim,
+            "q must be " + std::string(at::toString(k_cache.scalar_type())) + " [tokens, heads, " + std::to_string(c.dim) + "], not " + shape(q));
+    FG_NEED(lse.scalar_type() == at::kFloat && lse.dim() == 2 && lse.size(0) == T && lse.size(1) == heads,
+            "lse must be float32 [" + std::to_string(T) + ", " + std::to_string(heads) + "], not " + shape(lse));
+    lse = lse.contiguous();
+    requests(table, query_start, kv_len);
+    if (held) {
+        held = ints(*held, 1, "held");
+        FG_NEED(held->size(0) == kv_len.size(0), "held and kv_len differ in length");
+    }
+    fg_attention x{};
+    x.q = q.data_ptr();
+    x.q_token_stride = q.stride(0);
+    x.q_head_stride = q.stride(1);
+    x.lse = lse.data_ptr<float>();
+    x.block_table = table.data_ptr<int32_t>();
+    x.table_stride = table.stride(0);
+    x.query_start = query_start.data_ptr<int32_t>();
+    x.kv_len = kv_len.data_ptr<int32_t>();
+    x.tokens = i32(T, "tokens");
+    x.heads = i32(heads, "heads");
+    x.requests = i32(kv_len.size(0), "requests");
+    x.table_width = i32(table.size(1), "table width");
+    x.window = i32(window, "window");
+    x.sinks = i32(sinks, "sinks");
+    x.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(dim)));
+    check(fg_attention_weights_device(&c, &x, weights.data_ptr<float>(), weights.stride(0), weights.stride(1),
+                                      held ? held->data_ptr<int32_t>() : nullptr, on.stream()),
+          "fg_attention_weights_device");
+    written(weights);
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_evict(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& weights, at::Tensor table,
+                                            at::Tensor kv_len, int64_t budget, int64_t recent, int64_t sinks, int64_t stream) {
+    On on(k_cache, stream);
+    on.uses(k_cache, v_cache, weights, table, kv_len);
+    no_gradient("k_cache, v_cache and weights", k_cache, v_cache, weights);
+    const fg_kv_cache c = cache(k_cache, v_cache);
+    check_weights(weights, c);
+    table = ints(table, 2, "block_table");
+    kv_len = ints(kv_len, 1, "kv_len");
+    const int64_t R = kv_len.size(0);
+    FG_NEED(table.size(0) == R, std::to_string(R) + " lengths need as many table rows, not " + std::to_string(table.size(0)));
+    FG_NEED(budget >= 1, "budget " + std::to_string(budget) + " is not positive");
+    const at::Tensor len = at::empty({R}, kv_len.options());
+    const at::Tensor kept = at::empty({R, c.heads, i32(budget, "budget")}, kv_len.options());
+    check(fg_kv_evict_device(&c, weights.data_ptr<float>(), weights.stride(0), weights.stride(1), table.data_ptr<int32_t>(),
+                             i32(table.size(1), "table width"), table.stride(0), kv_len.data_ptr<int32_t>(), i32(R, "requests"),
+                             i32(budget, "budget"), i32(recent, "recent"), i32(sinks, "sinks"), len.data_ptr<int32_t>(),
+                             kept.data_ptr<int32_t>(), on.stream()),
+          "fg_kv_evict_device");
+    written(k_cache);
+    written(v_cache);
+    written(weights);
+    return {len, kept};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_ops, m) {
@@ -356,4 +432,6 @@ PYBIND11_MODULE(_torch_ops, m) {
     m.def("attention", &attention);
     m.def("kv_summarize", &kv_summarize);
     m.def("select_blocks", &select_blocks);
+    m.def("attention_weights", &attention_weights);
+    m.def("kv_evict", &kv_evict);
 }

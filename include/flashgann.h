@@ -436,6 +436,46 @@ int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selecti
  * head. */
 int fg_block_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream);
 
+/* ---- eviction by attention weight ----
+ *
+ * The other way to bound what a step reads: keep the cache short.  Each key's
+ * attention weight is summed up over the steps, and where a request has passed
+ * its budget each kv head drops its lightest keys.  The same rules as above
+ * hold. */
+
+/* Adds to d_weights (float [pages, heads, page_size], strides in elements, the
+ * last axis contiguous; beside the cache, one for each layer) the weights that
+ * the step's rows gave to each key: for position j of a request and each kv head
+ *   weight = (j < held ? weight : 0) + sum of exp(scale * q.k_j - lse)
+ * over its new tokens' rows of the kv head's query heads that see j (mask as in
+ * fg_paged_attention_device).  args: q, lse (here read: [tokens, heads], as the
+ * step's attention left it), block_table, query_start, kv_len, window, sinks,
+ * scale and the counts; out, ids, workspace and max_new are not looked at.
+ * d_held [requests]: tokens whose weights are there already (NULL: those before
+ * the new ones); weights from there to kv_len[b] start at 0, whatever was there.
+ * Rows whose lse is not finite add nothing.  Sums are 32 bits, in the order of
+ * the rows: the same bits on every run.  Only the last tokens of a prompt may be
+ * given: query_start counts them alone.  The cache's v may be NULL. */
+int fg_attention_weights_device(const fg_kv_cache* cache, const fg_attention* args, float* d_weights,
+                                int64_t weights_page_stride, int64_t weights_head_stride, const int32_t* d_held,
+                                void* stream);
+
+/* For each request of more than `budget` positions and each kv head: the first
+ * `sinks`, the last `recent` and, of those between, the budget - sinks - recent
+ * of the largest weights stay (of equal weights the lowest position; NaN counts
+ * as -inf, positions without a page are lighter still) and move, in ascending
+ * order, to positions 0 to budget - 1: rows of K and V and their weights, in
+ * place.  d_kv_len_out[requests] = min(kv_len, budget) (not d_kv_len itself);
+ * d_kept [requests, heads, budget]: the position that each was at, -1 past the
+ * request's length.  Requests within the budget stay as they are.  Pages of
+ * block_table from ceil(budget / page_size) on are free afterwards (where all
+ * layers that share the table are done); pages that two requests share must not
+ * be evicted from.  sinks + recent <= budget, budget >= 1. */
+int fg_kv_evict_device(const fg_kv_cache* cache, float* d_weights, int64_t weights_page_stride,
+                       int64_t weights_head_stride, const int32_t* d_block_table, int32_t table_width,
+                       int64_t table_stride, const int32_t* d_kv_len, int32_t requests, int32_t budget, int32_t recent,
+                       int32_t sinks, int32_t* d_kv_len_out, int32_t* d_kept, void* stream);
+
 /* ---- host helpers of the reference CLI ---- */
 
 /* include/utils.cuh:119-127 */
