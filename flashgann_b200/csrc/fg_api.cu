@@ -1116,6 +1116,11 @@ extern "C" __attribute__((visibility("default"))) void fg_test_attention_lose_bl
     fg::set_attention_waits(first, tries);
 }
 
+// Likewise of the key weights' kernel: products of a CTA's tile are not issued from block `first` on (NaN in its keys).
+extern "C" __attribute__((visibility("default"))) void fg_test_key_weights_lose_blocks(int32_t first, int32_t tries) {
+    fg::set_key_weights_waits(first, tries);
+}
+
 int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {
     g_err.clear();
     return attention(cache, args, kMask, stream);

@@ -146,9 +146,9 @@ struct Tiles {
     }
 };
 
-// kWhole: what a chunk of keys costs, in units.  Products and exponentials of 64 rows take about as long as the chunk's
-// way from memory.
-__device__ __forceinline__ int whole_cost(const AttentionParams& a, const Request& r) { return 1 + ((r.rows * a.group) >> 6); }
+// kWhole: what a chunk of keys costs, in units.  The exponentials of 175 rows take as long as the chunk's way from memory.
+constexpr int kWholeRows = 7;
+__device__ __forceinline__ int whole_cost(const AttentionParams& a, const Request& r) { return 1 + ((r.rows * a.group) >> kWholeRows); }
 
 template <int kRows, Layout kLayout, int kChunk>
 __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Request& r, int t) {

@@ -65,6 +65,7 @@ struct WeightsArgs {
     const int32_t* held = nullptr;  // [requests], optional
     float scale = 0.f;
 };
+void set_key_weights_waits(int lost_block, int tries);  // for tests; below 0: none, and a limit of a second
 cudaError_t launch_attention_weights(const AttentionParams& a, const WeightsArgs& w, cudaStream_t stream);
 
 struct EvictArgs {
