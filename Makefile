@@ -54,8 +54,8 @@ $(OBJ_DIR)/%.o: $(CSRC)/%.cu $(HEADERS) | $(OBJ_DIR)
 $(OBJ_DIR):
 	mkdir -p $(OBJ_DIR)
 
-$(OBJ_DIR)/fg_attention_rows.o $(OBJ_DIR)/fg_attention_tiles.o $(OBJ_DIR)/fg_key_weights.o: $(ATTN_HEADERS)
-$(OBJ_DIR)/fg_attention_tiles.o $(OBJ_DIR)/fg_key_weights.o: $(CSRC)/fg_tcgen05.cuh
+$(OBJ_DIR)/fg_attention_rows.o $(OBJ_DIR)/fg_attention_tiles.o $(OBJ_DIR)/fg_key_weights.o $(OBJ_DIR)/fg_blocks.o: $(ATTN_HEADERS)
+$(OBJ_DIR)/fg_attention_tiles.o $(OBJ_DIR)/fg_key_weights.o $(OBJ_DIR)/fg_blocks.o: $(CSRC)/fg_tcgen05.cuh
 $(OBJ_DIR)/fg_blocks.o $(OBJ_DIR)/fg_evict.o: $(CSRC)/fg_topk.cuh
 $(OBJ_DIR)/fg_blocks.o $(OBJ_DIR)/fg_evict.o $(OBJ_DIR)/fg_key_weights.o $(OBJ_DIR)/fg_api.o: $(CSRC)/fg_cache.h
 

@@ -82,7 +82,8 @@ class BlockSelectionArgs(ctypes.Structure):
     _fields_ = [("q", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
                 ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("query_start", ctypes.c_void_p),
                 ("kv_len", ctypes.c_void_p), ("blocks", ctypes.c_void_p), ("blocks_token_stride", ctypes.c_int64),
-                ("blocks_head_stride", ctypes.c_int64), ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("blocks_head_stride", ctypes.c_int64), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64), ("tokens", ctypes.c_int32), ("heads", ctypes.c_int32),
                 ("requests", ctypes.c_int32), ("table_width", ctypes.c_int32), ("window", ctypes.c_int32),
                 ("sinks", ctypes.c_int32), ("count", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
@@ -126,6 +127,8 @@ SIGNATURES = [
                                                      _vp]),
     ("fg_kv_summarize_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(KVSummaryArgs), _vp, _i32,
                                               _i64, _vp, _vp, _i32, _i32, _vp]),
+    ("fg_select_blocks_workspace_bytes", ctypes.c_int, [ctypes.POINTER(KVSummaryArgs),
+                                                        ctypes.POINTER(BlockSelectionArgs), ctypes.POINTER(_u64)]),
     ("fg_select_blocks_device", ctypes.c_int, [ctypes.POINTER(KVSummaryArgs), ctypes.POINTER(BlockSelectionArgs),
                                                _vp]),
     ("fg_block_attention_device", ctypes.c_int, [ctypes.POINTER(KVCacheArgs), ctypes.POINTER(AttentionArgs), _vp]),

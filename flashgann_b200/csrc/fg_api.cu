@@ -1230,27 +1230,51 @@ int fg_kv_summarize_device(const fg_kv_cache* cache, const fg_kv_summary* summar
     return e == cudaSuccess ? FG_OK : cuda_fail(e, "summary launch");
 }
 
-int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selection* x, void* stream) {
-    g_err.clear();
-    int rc = check_summary(summary);
+namespace {
+
+int check_selection(const fg_kv_summary* summary, const fg_block_selection* x) {
+    const int rc = check_summary(summary);
     if (rc) return rc;
     if (!x) return fail(FG_ERR_ARG, "null arguments");
     if (x->dtype != FG_DTYPE_F16 && x->dtype != FG_DTYPE_BF16) return fail(FG_ERR_ARG, "unknown query dtype %d", x->dtype);
-    if ((rc = check_requests(x->block_table, x->table_width, x->table_stride, x->query_start, x->kv_len, x->requests, x->tokens))) return rc;
+    if (x->tokens < 0 || x->requests < 0 || x->table_width < 0)
+        return fail(FG_ERR_ARG, "bad shape tokens=%d requests=%d table_width=%d", x->tokens, x->requests, x->table_width);
     if (x->heads < 1 || x->heads % summary->heads)
         return fail(FG_ERR_ARG, "%d query heads do not divide over %d kv heads", x->heads, summary->heads);
     if (x->heads / summary->heads > 256) return fail(FG_ERR_UNSUPPORTED, "%d query heads for each kv head", x->heads / summary->heads);
     if (x->window < 0 || x->sinks < 0) return fail(FG_ERR_ARG, "bad mask window=%d sinks=%d", x->window, x->sinks);
     if (x->count < 0) return fail(FG_ERR_ARG, "bad count %d", x->count);
-    if (x->table_width > fg::select_max_width())
-        return fail(FG_ERR_UNSUPPORTED, "table_width %d, at most %d", x->table_width, fg::select_max_width());
-    if (static_cast<int64_t>(x->tokens) * summary->heads > INT32_MAX / 8)
-        return fail(FG_ERR_UNSUPPORTED, "%d tokens of %d kv heads", x->tokens, summary->heads);
+    if (!fg::select_counts(x->tokens, summary->heads, x->table_width))
+        return fail(FG_ERR_UNSUPPORTED, "%d tokens of %d kv heads and %d blocks", x->tokens, summary->heads, x->table_width);
+    return FG_OK;
+}
+
+}  // namespace
+
+int fg_select_blocks_workspace_bytes(const fg_kv_summary* summary, const fg_block_selection* args, uint64_t* bytes) {
+    g_err.clear();
+    const int rc = check_selection(summary, args);
+    if (rc) return rc;
+    if (!bytes) return fail(FG_ERR_ARG, "null argument");
+    *bytes = fg::select_workspace(args->tokens, summary->heads, args->table_width);
+    return FG_OK;
+}
+
+int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selection* x, void* stream) {
+    g_err.clear();
+    int rc = check_selection(summary, x);
+    if (rc) return rc;
+    if ((rc = check_requests(x->block_table, x->table_width, x->table_stride, x->query_start, x->kv_len, x->requests, x->tokens))) return rc;
     if (x->tokens == 0 || x->requests == 0 || x->count == 0) return FG_OK;
     if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, x->tokens, x->heads, "q"))) return rc;
     if (!x->blocks) return fail(FG_ERR_ARG, "null blocks");
     if (overlaps({{{x->blocks_token_stride, x->tokens}, {x->blocks_head_stride, summary->heads}}}, x->count))
         return fail(FG_ERR_ARG, "rows of blocks overlap");
+    const uint64_t need = fg::select_workspace(x->tokens, summary->heads, x->table_width);
+    if (need && (!x->workspace || (reinterpret_cast<uintptr_t>(x->workspace) & 15)))
+        return fail(FG_ERR_ARG, "workspace is null or not 16-byte aligned");
+    if (x->workspace_bytes < need)
+        return fail(FG_ERR_ARG, "workspace of %llu bytes, %llu needed", (unsigned long long)x->workspace_bytes, (unsigned long long)need);
     fg::SelectArgs a;
     a.summary = summary_of(summary);
     a.req = requests_of(x->block_table, x->table_width, x->table_stride, x->query_start, x->kv_len, x->requests, x->tokens);
@@ -1269,6 +1293,7 @@ int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selecti
     a.window = x->window;
     a.sinks = x->sinks;
     a.count = x->count;
+    a.scores = need ? static_cast<uint32_t*>(x->workspace) : nullptr;
     if ((rc = sm_count(&a.sms))) return rc;
     const cudaError_t e = fg::launch_select_blocks(a, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? FG_OK : cuda_fail(e, "selection launch");

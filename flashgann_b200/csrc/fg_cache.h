@@ -46,9 +46,11 @@ struct SelectArgs {
     int64_t blocks_token_stride = 0, blocks_head_stride = 0;
     int pages = 0, page_shift = 0, kv_heads = 0, group = 0, dim = 0, dtype = 0;
     int window = 0, sinks = 0, count = 0;
+    uint32_t* scores = nullptr;  // workspace
     int sms = 0;
 };
-int select_max_width();
+bool select_counts(int tokens, int kv_heads, int table_width);  // whether a launch can have so many CTAs
+size_t select_workspace(int tokens, int kv_heads, int table_width);  // 0 where the scores stay in shared memory
 cudaError_t launch_select_blocks(const SelectArgs& a, cudaStream_t stream);
 
 struct AttentionParams;

@@ -27,21 +27,18 @@
 namespace fg {
 namespace {
 
-using topk::kThreads;
-
+constexpr int kThreads = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxSmem = 100 * 1024;  // two CTAs to an SM
 constexpr int kLoads = 8;             // 16-byte pieces of a thread under way
 
-template <int kDim>
+template <int kDim, typename Ctas>
 __global__ void __launch_bounds__(kThreads) kv_evict_kernel(const EvictArgs a, int room) {
-    namespace cg = cooperative_groups;
-    const cg::cluster_group cluster = cg::this_cluster();
     extern __shared__ __align__(16) char smem[];
     topk::Shared& s = *reinterpret_cast<topk::Shared*>(smem);
     uint32_t* near = reinterpret_cast<uint32_t*>(smem + sizeof(topk::Shared));  // [room]
     const int tid = threadIdx.x;
-    const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const int ranks = Ctas::ranks(), rank = Ctas::rank();
     const int row = static_cast<int>(blockIdx.x) / ranks;
     const int b = row / a.cache.heads, head = row - b * a.cache.heads;
     const int shift = a.cache.page_shift, in_page = (1 << shift) - 1;
@@ -70,15 +67,24 @@ __global__ void __launch_bounds__(kThreads) kv_evict_kernel(const EvictArgs a, i
         const float w = *weight_at(page, j);
         return topk::order_key(w == w ? w : -INFINITY);
     };
-    for (int i = tid; i < min(m, room); i += kThreads) near[i] = read(i);
+    topk::clear<kThreads>(s);
+    uint32_t least = 0xFFFFFFFFu, most = 0;
+    for (int i = tid; i < m; i += kThreads) {
+        const uint32_t key = read(i);
+        least = min(least, key);
+        most = max(most, key);
+        if (i < room) near[i] = key;
+    }
     __syncthreads();
-    const auto keys = [&](int i) { return i < room ? near[i] : read(i); };
-    const topk::Threshold thr = topk::threshold(cluster, s, m, a.budget - a.recent - a.sinks, keys);
-    topk::emit(cluster, s, m, thr, keys, [&](int place, int i) { kept[a.sinks + place] = a.sinks + c0 + i; });
+    topk::range(s, least, most);
+    Ctas::sync();
+    const auto keys = topk::read_keys<kThreads>([&](int i) { return i < room ? near[i] : read(i); });
+    const topk::Threshold thr = topk::threshold<kThreads, Ctas>(s, m, a.budget - a.recent - a.sinks, keys);
+    topk::emit<kThreads, Ctas>(s, m, thr, keys, [&](int place, int i) { kept[a.sinks + place] = a.sinks + c0 + i; });
     for (int x = rank * kThreads + tid; x < a.sinks; x += ranks * kThreads) kept[x] = x;
     for (int x = rank * kThreads + tid; x < a.recent; x += ranks * kThreads) kept[a.budget - a.recent + x] = len - a.recent + x;
     __threadfence();
-    cluster.sync();  // the whole list is there, and no weight is read as a key any more
+    Ctas::sync();  // the whole list is there, and no weight is read as a key any more
 
     // a thread has one 16-byte piece of K or V of several rows
     constexpr int kPieces = 2 * kDim / 8, kTogether = kThreads / kPieces;
@@ -111,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) kv_evict_kernel(const EvictArgs a, i
             to[x] = piece_at(there, i);
             if (piece == 0) w[x] = *weight_at(here, from[x]);
         }
-        cluster.sync();
+        Ctas::sync();
 #pragma unroll
         for (int x = 0; x < kLoads; ++x) {
             if (!to[x]) continue;
@@ -127,16 +133,24 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.requests) * a.cache.heads;
     const int64_t most = std::min<int64_t>(static_cast<int64_t>(a.table_width) << a.cache.page_shift, INT32_MAX);
     int ranks = 1;
-    while (ranks < kMaxCluster && rows * ranks < a.sms) ranks *= 2;
+    while (ranks < kMaxCluster && rows * ranks < a.sms && most > 2048 * ranks) ranks *= 2;
     constexpr int kRoom = (kMaxSmem - static_cast<int>(sizeof(topk::Shared))) / 4;
     const int room = static_cast<int>(std::min<int64_t>((most + ranks - 1) / ranks, kRoom));
+    const int bytes = static_cast<int>(sizeof(topk::Shared)) + room * 4;
+    if (ranks == 1) {
+        static SmemOnce once;
+        const cudaError_t e = once.set(reinterpret_cast<const void*>(kv_evict_kernel<kDim, topk::One>), kMaxSmem);
+        if (e != cudaSuccess) return e;
+        kv_evict_kernel<kDim, topk::One><<<static_cast<unsigned>(rows), kThreads, bytes, stream>>>(a, room);
+        return cudaGetLastError();
+    }
     static SmemOnce once;
-    const cudaError_t e = once.set(reinterpret_cast<const void*>(kv_evict_kernel<kDim>), kMaxSmem);
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kv_evict_kernel<kDim, topk::Cluster>), kMaxSmem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows * ranks));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = sizeof(topk::Shared) + static_cast<size_t>(room) * 4;
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -144,7 +158,7 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kv_evict_kernel<kDim>, a, room);
+    return cudaLaunchKernelEx(&cfg, kv_evict_kernel<kDim, topk::Cluster>, a, room);
 }
 
 }  // namespace

@@ -98,6 +98,17 @@ __device__ __forceinline__ void mma_smem(uint32_t d, uint32_t a, uint32_t b, uin
         "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(kOperandHigh)
         : "memory");
 }
+// 8-bit integers, sums of 32 bits
+__host__ __device__ constexpr uint32_t instruction_s8(int n) {  // 128 rows, n columns
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_smem_s8(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(add), "r"(kOperandHigh)
+        : "memory");
+}
 __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"

@@ -343,6 +343,14 @@ at::Tensor select_blocks(at::Tensor q, const at::Tensor& bounds, const at::Tenso
     x.sinks = i32(sinks, "sinks");
     x.count = i32(count, "count");
     x.dtype = q.scalar_type() == at::kHalf ? FG_DTYPE_F16 : FG_DTYPE_BF16;
+    uint64_t bytes = 0;
+    check(fg_select_blocks_workspace_bytes(&s, &x, &bytes), "fg_select_blocks_workspace_bytes");
+    at::Tensor work;
+    if (bytes) {
+        work = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+        x.workspace = work.data_ptr();
+        x.workspace_bytes = bytes;
+    }
     check(fg_select_blocks_device(&s, &x, on.stream()), "fg_select_blocks_device");
     if (out_or_none) written(out);
     return out;

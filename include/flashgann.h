@@ -405,9 +405,17 @@ typedef struct fg_block_selection {
     const int32_t* kv_len;                 /* [requests], new tokens included */
     int32_t* blocks;                       /* [tokens, kv_heads, count] */
     int64_t blocks_token_stride, blocks_head_stride;
+    void* workspace;                       /* fg_select_blocks_workspace_bytes, 16-byte aligned; contents do not matter;
+                                            * NULL where 0 bytes are needed */
+    uint64_t workspace_bytes;
     int32_t tokens, heads, requests, table_width;
     int32_t window, sinks, count, dtype;
 } fg_block_selection;
+
+/* Bytes of workspace that a selection needs, for the scores of long contexts
+ * (0 where table_width is small).  Depends on tokens, table_width and
+ * summary->heads only. */
+int fg_select_blocks_workspace_bytes(const fg_kv_summary* summary, const fg_block_selection* args, uint64_t* bytes);
 
 /* For the new token at position p (as in fg_paged_attention_device) and each kv
  * head, the `count` blocks of the highest score, ascending, then -1.  Block x of
@@ -423,8 +431,8 @@ typedef struct fg_block_selection {
  * positive scale); a query head with a value that is not finite counts as 0, a
  * page of scale inf has the score inf.  Of equal scores the lowest block comes
  * first.  The same bits on every run.  The last axis of blocks is contiguous.
- * Rows past query_start[requests] are not written.  Needs a window >= 0,
- * heads / summary->heads <= 256, a table_width of at most 262144. */
+ * Rows past query_start[requests] are not written.  Needs a window >= 0 and
+ * heads / summary->heads <= 256. */
 int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selection* args, void* stream);
 
 /* fg_paged_attention_device over window, first tokens and chosen blocks: row

@@ -79,11 +79,30 @@ def test_summarize_refuses_overlapping_summaries(kw):
     (dict(table_width=-1), "table_width=-1"), (dict(block_table=None), "null buffer"), (dict(table_stride=-1), "stride"),
     (dict(dtype=5), "dtype"), (dict(heads=5), "5 query heads"), (dict(heads=0), "0 query heads"),
     (dict(heads=2 * 257), "257 query heads"), (dict(window=-1), "window=-1"), (dict(sinks=-1), "sinks=-1"),
-    (dict(count=-1), "count -1"), (dict(table_width=262145), "table_width 262145"), (dict(tokens=2 ** 30), "tokens"),
+    (dict(count=-1), "count -1"), (dict(table_width=257), "workspace is null"),
+    (dict(table_width=257, workspace=PTR + 8, workspace_bytes=1 << 20), "16-byte aligned"),
+    (dict(table_width=257, workspace=PTR, workspace_bytes=3 * 2 * 257 * 4 - 1), "6168 needed"),
+    (dict(table_width=2 ** 31 - 1, tokens=100), "blocks"), (dict(tokens=2 ** 30), "tokens"),
     (dict(q=None), "null q"), (dict(q=PTR + 8), "q is not"), (dict(q_head_stride=4), "strides of q"),
     (dict(blocks=None), "null blocks"), (dict(blocks_head_stride=9), "overlap"), (dict(blocks_token_stride=0), "overlap")])
 def test_selection_refusals(kw, word):
     _refused(fg.lib().fg_select_blocks_device(_summary(), _selection(**kw), None), word)
+
+
+@pytest.mark.parametrize("kw,word", [(dict(requests=-1), "requests=-1"), (dict(heads=5), "5 query heads"),
+                                     (dict(window=-1), "window=-1"), (dict(count=-1), "count -1"), (dict(dtype=5), "dtype"),
+                                     (dict(tokens=2 ** 30), "tokens"), (dict(table_width=-1), "table_width=-1")])
+def test_workspace_bytes_refuses_what_the_call_refuses(kw, word):
+    need = ctypes.c_uint64(7)
+    _refused(fg.lib().fg_select_blocks_workspace_bytes(_summary(), _selection(**kw), ctypes.byref(need)), word)
+    assert need.value == 7
+
+
+@pytest.mark.parametrize("width,need", [(4, 0), (256, 0), (257, 3 * 2 * 257 * 4), (10 ** 6, 3 * 2 * 10 ** 6 * 4)])
+def test_workspace_bytes(width, need):
+    got = ctypes.c_uint64(7)
+    assert fg.lib().fg_select_blocks_workspace_bytes(_summary(), _selection(table_width=width), ctypes.byref(got)) == fg.FG_OK
+    assert got.value == need
 
 
 def test_empty_calls_and_null_structs():
@@ -100,7 +119,7 @@ def test_empty_calls_and_null_structs():
 
 def test_struct_sizes():
     assert ctypes.sizeof(_capi.KVSummaryArgs) == 64 and _capi.KVSummaryArgs.pages.offset == 48
-    assert ctypes.sizeof(_capi.BlockSelectionArgs) == 112 and _capi.BlockSelectionArgs.tokens.offset == 80
+    assert ctypes.sizeof(_capi.BlockSelectionArgs) == 128 and _capi.BlockSelectionArgs.tokens.offset == 96
 
 
 def test_python_wrappers_refuse_host_tensors():

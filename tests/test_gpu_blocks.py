@@ -127,6 +127,9 @@ SELECTIONS = [
     ([3, 2000, 0, 60], [0, 2, 4, 1], 5, 1, 96, 1, "bf16"),
     ([40000], [1], 2, 1, 64, 8, "fp16"),
     ([200] * 90, [1] * 90, 16, 8, 64, 4, "bf16"),       # many rows: a CTA to each
+    ([290] * 40, [1] * 40, 12, 4, 96, 1, "fp16"),       # the same, more than 256 pages
+    ([2300, 100] * 10, [1] * 20, 128, 8, 128, 8, "bf16"),
+    ([280] * 80, [1] * 80, 40, 2, 64, 1, "bf16"),       # many rows of many heads
 ]
 
 
@@ -140,6 +143,34 @@ def test_selection(case, mask):
         got = _select(x, s, count, *mask, dtype)
         assert np.array_equal(got.cpu().numpy(), _select_ref(x, want, count, *mask)), count
     assert _select(x, s, 0, *mask, dtype).shape == (sum(new), kv_heads, 0)
+
+
+def test_selection_of_more_pages_than_shared_memory_holds():
+    x = make(np.random.default_rng(9), ctx=[61000], new=[1], heads=2, kv_heads=1, dim=64, page=1)
+    s, want = _summaries(x)
+    for count, mask in [(5, (10, 3)), (1000, (0, 0)), (60000, (100, 0)), (61001, (0, 0))]:
+        got = _select(x, s, count, *mask)
+        assert np.array_equal(got.cpu().numpy(), _select_ref(x, want, count, *mask)), count
+
+
+def test_selection_of_many_tokens():
+    """Tokens of many requests, some without: the rows of each are found."""
+    rng = np.random.default_rng(10)
+    new = rng.integers(0, 4, 300).tolist()
+    for page in (1, 16):  # one kernel and two
+        x = make(rng, ctx=rng.integers(0, 300, 300).tolist(), new=new, heads=4, kv_heads=2, dim=64, page=page)
+        s, want = _summaries(x)
+        got = _select(x, s, 5, 8, 2)
+        assert np.array_equal(got.cpu().numpy(), _select_ref(x, want, 5, 8, 2))
+
+
+@pytest.mark.parametrize("kv_heads,heads", [(16, 16), (48, 96), (2, 512), (3, 120)])
+def test_selection_of_many_heads(kv_heads, heads):
+    """More query heads than one CTA keeps."""
+    x = make(np.random.default_rng(kv_heads), ctx=[700], new=[2], heads=heads, kv_heads=kv_heads, dim=128, page=2)
+    s, want = _summaries(x)
+    got = _select(x, s, 9, 20, 2)
+    assert np.array_equal(got.cpu().numpy(), _select_ref(x, want, 9, 20, 2))
 
 
 def test_selection_of_equal_scores():
