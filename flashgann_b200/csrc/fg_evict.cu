@@ -6,13 +6,18 @@
 // -inf).  In ascending order they move to positions 0 .. budget - 1: rows of K and
 // V and the weights, in place.
 //
-// A cluster of CTAs has one request and kv head.  Its weights are read once, as
-// keys of fg_topk.cuh (those beyond shared memory's room are read again), the kept
-// positions go to the result, and then the cluster moves the rows, chunk by chunk
-// of consecutive places: all of its CTAs load the chunk's rows into registers, the
-// cluster waits, and they store them.  Place i is filled from kept[i] >= i, and the
-// sources of later chunks lie behind the chunk, so the next chunk's loads need not
-// wait for the stores.
+// A CTA, or a cluster where there are few, has one request and kv head.  Its
+// weights are read once, as keys of fg_topk.cuh (those beyond shared memory's room
+// are read again), the kept positions go to the result, and then the rows move,
+// kChunk consecutive places for each CTA at a time: K and V rows come by 16-byte
+// cp.async into a ring of kStages chunks, and when all CTAs have a chunk they store
+// it.  Place i is filled from kept[i] >= i, and the sources of later chunks lie
+// behind the chunk, so loads may run ahead of stores as far as they like.  Where
+// rows come from and go to is looked up three chunks before, a step to each, by a
+// thread to a row, which moves the row's weight too.
+//
+// What bounds it: the weights' way and, of the rows that move, there and back.
+// 32 requests of 900 to 8000 positions to 1024, 8 kv heads of 128: see kStages.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -29,11 +34,24 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxSmem = 100 * 1024;  // two CTAs to an SM
-constexpr int kLoads = 8;             // 16-byte pieces of a thread under way
+constexpr int kMaxSmem = 110 * 1024;  // two CTAs to an SM
+constexpr int kChunk = 64;            // rows
+constexpr int kStages = 3;            // of chunks (registers instead, a chunk after the other: 93 us)
+
+template <int kDim>
+struct Ring {
+    static constexpr int kRow = 4 * kDim;  // bytes of K and V
+    static constexpr int kBytes = kStages * kChunk * kRow;
+};
+// Where the rows of chunks begin, from and to (elements of the cache's halves; from below 0: it stays), and their weights.
+struct Moves {
+    int64_t from[kStages + 1][kChunk], to[kStages + 1][kChunk];
+    float w[kStages + 1][kChunk];
+    float* w_to[kStages + 1][kChunk];
+};
 
 template <int kDim, typename Ctas>
-__global__ void __launch_bounds__(kThreads) kv_evict_kernel(const EvictArgs a, int room) {
+__global__ void __launch_bounds__(kThreads, 2) kv_evict_kernel(const EvictArgs a, int room) {
     extern __shared__ __align__(16) char smem[];
     topk::Shared& s = *reinterpret_cast<topk::Shared*>(smem);
     uint32_t* near = reinterpret_cast<uint32_t*>(smem + sizeof(topk::Shared));  // [room]
@@ -69,6 +87,7 @@ __global__ void __launch_bounds__(kThreads) kv_evict_kernel(const EvictArgs a, i
     };
     topk::clear<kThreads>(s);
     uint32_t least = 0xFFFFFFFFu, most = 0;
+#pragma unroll 8
     for (int i = tid; i < m; i += kThreads) {
         const uint32_t key = read(i);
         least = min(least, key);
@@ -86,45 +105,82 @@ __global__ void __launch_bounds__(kThreads) kv_evict_kernel(const EvictArgs a, i
     __threadfence();
     Ctas::sync();  // the whole list is there, and no weight is read as a key any more
 
+    // the ring and the moves lie where the keys were
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    Moves& mv = *reinterpret_cast<Moves*>(smem + Ring<kDim>::kBytes);
     // a thread has one 16-byte piece of K or V of several rows
-    constexpr int kPieces = 2 * kDim / 8, kTogether = kThreads / kPieces;
-    const int piece = tid % kPieces, slot = tid / kPieces;
+    constexpr int kPieces = 2 * kDim / 8, kTogether = kThreads / kPieces, kEach = (kChunk + kTogether - 1) / kTogether;
+    const int piece = tid % kPieces, slot = tid < kTogether * kPieces ? tid / kPieces : kChunk;
     const bool values = piece >= kPieces / 2;
-    char* base = static_cast<char*>(values ? a.v : const_cast<void*>(a.cache.k));
-    const int64_t off = head * a.cache.head_stride + (values ? piece - kPieces / 2 : piece) * 8;
-    const auto piece_at = [&](int page, int j) {
-        return reinterpret_cast<uint4*>(base + 2 * (page * a.cache.page_stride + (j & in_page) * a.cache.token_stride + off));
+    char* base = static_cast<char*>(values ? a.v : const_cast<void*>(a.cache.k)) +
+                 2 * (head * a.cache.head_stride + (values ? piece - kPieces / 2 : piece) * 8);
+    const int first = a.sinks, chunks = (a.budget - first + ranks * kChunk - 1) / (ranks * kChunk);
+    const auto place = [&](int c) { return first + (c * ranks + rank) * kChunk + tid; };  // of this thread's row of chunk c
+
+    // a row's way: the position it is at (two chunks before its loads), both pages (one before), its offsets and weight
+    int from2 = -1, from1 = -1, here1 = -1, there1 = -1;
+    const auto step = [&](int c) {  // offsets of chunk c, pages of c + 1, positions of c + 2
+        if (tid >= kChunk) return;
+        int64_t from = -1, to = 0;
+        float w = 0.f;
+        float* w_to = nullptr;
+        if (from1 >= 0 && here1 >= 0 && there1 >= 0) {
+            const int i = place(c);
+            from = here1 * a.cache.page_stride + (from1 & in_page) * a.cache.token_stride;
+            to = there1 * a.cache.page_stride + (i & in_page) * a.cache.token_stride;
+            w = *weight_at(here1, from1);
+            w_to = weight_at(there1, i);
+        }
+        const int at = c & kStages;  // c % (kStages + 1)
+        mv.from[at][tid] = from;
+        mv.to[at][tid] = to;
+        mv.w[at][tid] = w;
+        mv.w_to[at][tid] = w_to;
+        from1 = from2;
+        const int i1 = place(c + 1), i2 = place(c + 2);
+        if (from1 == i1) from1 = -1;  // in place already
+        here1 = from1 >= 0 ? page_of(from1) : -1;
+        there1 = from1 >= 0 ? page_of(i1) : -1;
+        from2 = c + 2 < chunks && i2 < a.budget ? __ldcg(kept + i2) : -1;
     };
-    for (int i0 = a.sinks; i0 < a.budget; i0 += ranks * kLoads * kTogether) {
-        uint4 v[kLoads];
-        float w[kLoads];
-        uint4* to[kLoads];
-        int from[kLoads];
+    static_assert((kStages & (kStages + 1)) == 0, "c & kStages");
+    const auto load = [&](int c) {
+        if (c < chunks)
 #pragma unroll
-        for (int x = 0; x < kLoads; ++x) {
-            const int i = i0 + (rank * kLoads + x) * kTogether + slot;
-            from[x] = slot < kTogether && i < a.budget ? __ldcg(kept + i) : i;
-            if (from[x] == i) from[x] = -1;  // in place already, or none
-        }
+            for (int x = 0; x < kEach; ++x) {
+                const int row = slot + x * kTogether;
+                if (row >= kChunk) continue;
+                const int64_t at = mv.from[c & kStages][row];
+                if (at >= 0)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring + (c % kStages * kChunk + row) * Ring<kDim>::kRow + piece * 16),
+                                 "l"(base + 2 * at)
+                                 : "memory");
+            }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    __syncthreads();  // the keys are done with
+    step(-2);
+    step(-1);
+    for (int c = 0; c < kStages; ++c) step(c);
+    __syncthreads();
+    for (int c = 0; c < kStages - 1; ++c) load(c);
+    for (int c = 0; c < chunks; ++c) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        Ctas::sync();  // all have the chunk; the one before is stored
+        load(c + kStages - 1);
 #pragma unroll
-        for (int x = 0; x < kLoads; ++x) {
-            const int i = i0 + (rank * kLoads + x) * kTogether + slot;
-            to[x] = nullptr;
-            if (from[x] < 0) continue;
-            const int here = page_of(from[x]), there = page_of(i);
-            if (here < 0 || there < 0) continue;
-            v[x] = *piece_at(here, from[x]);
-            to[x] = piece_at(there, i);
-            if (piece == 0) w[x] = *weight_at(here, from[x]);
+        for (int x = 0; x < kEach; ++x) {
+            const int row = slot + x * kTogether;
+            if (row >= kChunk || mv.from[c & kStages][row] < 0) continue;
+            uint4 v;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(ring + (c % kStages * kChunk + row) * Ring<kDim>::kRow + piece * 16)
+                         : "memory");
+            *reinterpret_cast<uint4*>(base + 2 * mv.to[c & kStages][row]) = v;
         }
-        Ctas::sync();
-#pragma unroll
-        for (int x = 0; x < kLoads; ++x) {
-            if (!to[x]) continue;
-            const int i = i0 + (rank * kLoads + x) * kTogether + slot;
-            *to[x] = v[x];
-            if (piece == 0) *weight_at(page_of(i), i) = w[x];
-        }
+        if (tid < kChunk && mv.w_to[c & kStages][tid]) *mv.w_to[c & kStages][tid] = mv.w[c & kStages][tid];
+        step(c + kStages);  // where chunk c - 1 was
     }
 }
 
@@ -136,7 +192,8 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream) {
     while (ranks < kMaxCluster && rows * ranks < a.sms && most > 2048 * ranks) ranks *= 2;
     constexpr int kRoom = (kMaxSmem - static_cast<int>(sizeof(topk::Shared))) / 4;
     const int room = static_cast<int>(std::min<int64_t>((most + ranks - 1) / ranks, kRoom));
-    const int bytes = static_cast<int>(sizeof(topk::Shared)) + room * 4;
+    static_assert(Ring<128>::kBytes + sizeof(Moves) <= kMaxSmem && (kMaxSmem + 1024) * 2 <= 228 * 1024, "two CTAs to an SM");
+    const int bytes = std::max(static_cast<int>(sizeof(topk::Shared)) + room * 4, Ring<kDim>::kBytes + static_cast<int>(sizeof(Moves)));
     if (ranks == 1) {
         static SmemOnce once;
         const cudaError_t e = once.set(reinterpret_cast<const void*>(kv_evict_kernel<kDim, topk::One>), kMaxSmem);

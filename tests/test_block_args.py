@@ -82,7 +82,7 @@ def test_summarize_refuses_overlapping_summaries(kw):
     (dict(count=-1), "count -1"), (dict(table_width=257), "workspace is null"),
     (dict(table_width=257, workspace=PTR + 8, workspace_bytes=1 << 20), "16-byte aligned"),
     (dict(table_width=257, workspace=PTR, workspace_bytes=3 * 2 * 257 * 4 - 1), "6168 needed"),
-    (dict(table_width=2 ** 31 - 1, tokens=100), "blocks"), (dict(tokens=2 ** 30), "tokens"),
+    (dict(table_width=2 ** 31 - 1, tokens=1000), "blocks"), (dict(tokens=2 ** 30), "tokens"),
     (dict(q=None), "null q"), (dict(q=PTR + 8), "q is not"), (dict(q_head_stride=4), "strides of q"),
     (dict(blocks=None), "null blocks"), (dict(blocks_head_stride=9), "overlap"), (dict(blocks_token_stride=0), "overlap")])
 def test_selection_refusals(kw, word):
