@@ -146,9 +146,8 @@ struct Tiles {
     }
 };
 
-// kWhole: what a chunk of keys costs, in units.  The exponentials of 175 rows take as long as the chunk's way from memory.
-constexpr int kWholeRows = 7;
-__device__ __forceinline__ int whole_cost(const AttentionParams& a, const Request& r) { return 1 + ((r.rows * a.group) >> kWholeRows); }
+// kWhole: what a chunk of keys costs, in units: how often it is gone through, tile_rows rows at a time.
+__device__ __forceinline__ int whole_cost(const AttentionParams& a, const Request& r) { return max(1, (r.rows * a.group + a.tile_rows - 1) / a.tile_rows); }
 
 template <int kRows, Layout kLayout, int kChunk>
 __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Request& r, int t) {

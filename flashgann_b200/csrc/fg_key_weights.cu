@@ -36,8 +36,8 @@ constexpr int kRows = 16;    // not looked at: a tile is a request
 constexpr int kBlock = 128;  // keys
 constexpr int kThreads = 128;
 constexpr int kCtasPerSm = 2;
-constexpr int kFew = 32;     // up to so many rows' queries lie behind the whole ring,
-constexpr int kMany = 128;   // more, up to so many at a time, in its last places
+constexpr int kFew = 16;     // rows at a time where there are few
+constexpr int kMany = 128;   // and where there are many
 constexpr int kColumns = 2 * kMany;  // of TMEM: two blocks' scores
 constexpr int kTries = 1 << 18;      // a try that finds nothing takes 4 us: a second
 
@@ -46,12 +46,10 @@ struct Ring {
     static constexpr int kPanels = (kDim + 63) / 64;  // 64 columns (128 bytes) each
     static constexpr int kPanel = kBlock * 128;
     static constexpr int kTile = kPanels * kPanel;
-    static constexpr int kStages = kDim == 64 ? 6 : 3;
-    static constexpr int kStagesMany = kDim == 64 ? 4 : 2;
+    static constexpr int kStages = kDim == 64 ? 4 : 2;
     static constexpr int kLook = kStages + 1;         // blocks whose rows are known
-    static constexpr int kQueriesFew = kStages * kTile, kQueriesMany = kStagesMany * kTile;
-    static constexpr int kBytes = kQueriesFew + kPanels * kFew * 128;
-    static_assert(kBytes - kQueriesMany >= kPanels * kMany * 128, "the queries' room");
+    static constexpr int kQueries = kStages * kTile;
+    static constexpr int kBytes = kQueries + kPanels * kMany * 128;
 };
 
 template <int kDim>
@@ -73,15 +71,6 @@ template <int N>
 __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// until all but the last n groups have arrived
-__device__ __forceinline__ void copy_wait_but(int n) {
-    if (n >= 4) copy_wait<4>();
-    else if (n == 3) copy_wait<3>();
-    else if (n == 2) copy_wait<2>();
-    else if (n == 1) copy_wait<1>();
-    else copy_wait<0>();
-}
-
 struct Limits {
     int tries, lost;  // of waits; block from which on no products are issued (none: INT32_MAX)
 };
@@ -133,9 +122,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
         const auto first_key = [&](int c) { return c < keys.sink_chunks ? c * kBlock : keys.base + (c - keys.sink_chunks) * kBlock; };
         for (int g0 = 0; c0 < c1 && g0 < rows; g0 += kMany) {
             const int n = min(rows - g0, kMany), columns = n <= 16 ? 16 : (n + 31) & ~31;
-            const int stages = rows <= kFew ? R::kStages : R::kStagesMany;
-            const uint32_t queries = tiles + (rows <= kFew ? R::kQueriesFew : R::kQueriesMany);
-            const int panel = (rows <= kFew ? kFew : kMany) * 128;  // of the queries
+            constexpr int stages = R::kStages, panel = kMany * 128;  // of the queries
+            const uint32_t queries = tiles + R::kQueries;
             // the page of this thread's key of block c, which all look up for one another
             const auto find = [&](int c) {
                 if (c >= c1) return -1;
@@ -266,7 +254,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
             };
             int at = 0;
             for (int c = c0; c < c1; ++c) {
-                copy_wait_but(c == c0 ? stages - 1 : stages - 2);
+                if (c == c0) copy_wait<stages - 1>();
+                else copy_wait<stages - 2>();
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 tmem_fence_before();
                 late = __syncthreads_or(late);
@@ -302,33 +291,324 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kColumns) : "memory");
 }
 
+// ---- few rows ----
+
+// The blocks of a CTA's range, one after the other; a tile of more than kFew rows is gone through once for each kFew.  A
+// segment is the blocks of one tile and such rows.
+struct Walk {
+    const AttentionParams& a;
+    Request r;
+    TileKeys keys;
+    int head, request, tile, c, c0, c1, g0, rows;
+    int64_t tile_first, end;
+    bool more;  // there is a block
+    bool opens; // and it is the first of its segment
+    __device__ __forceinline__ Walk(const AttentionParams& args, const Place& pl)
+        : a(args), head(pl.head), request(pl.request), tile(pl.tile), tile_first(pl.unit - pl.offset), end(pl.end), more(true) {
+        r = load_request(a, request);
+        set(pl.unit);
+    }
+    __device__ __forceinline__ void set(int64_t unit) {
+        while (true) {
+            keys = tile_keys<kRows, kWhole, kBlock>(a, r, 0);
+            rows = r.rows * a.group;
+            const int cost = whole_cost(a, r);
+            const int64_t tile_last = tile_first + keys.units;
+            // a block belongs to the CTA whose range holds its first unit
+            const auto block_at = [&](int64_t u) {
+                return static_cast<int>(min(((u - tile_first + cost - 1) / cost) << a.unit_shift, static_cast<int64_t>(keys.chunks)));
+            };
+            c = c0 = block_at(unit);
+            c1 = block_at(min(tile_last, end));
+            g0 = 0;
+            opens = true;
+            if (c0 < c1) return;
+            if (tile_last >= end || !next_tile<kRows, kWhole>(a, &r, &head, &request, &tile)) break;
+            unit = tile_first = tile_last;
+        }
+        more = false;
+    }
+    __device__ __forceinline__ void next() {
+        opens = false;
+        if (++c < c1) return;
+        opens = true;
+        c = c0;
+        g0 += kFew;
+        if (g0 < rows) return;
+        const int64_t tile_last = tile_first + keys.units;
+        if (tile_last >= end || !next_tile<kRows, kWhole>(a, &r, &head, &request, &tile)) {
+            more = false;
+            return;
+        }
+        tile_first = tile_last;
+        set(tile_last);
+    }
+    __device__ __forceinline__ int first() const { return c < keys.sink_chunks ? c * kBlock : keys.base + (c - keys.sink_chunks) * kBlock; }
+    // page of key x of the block, or -1
+    __device__ __forceinline__ int page(int x) const {
+        if (!more) return -1;
+        const int j = first() + x, at = j >> a.page_shift;
+        if (!(c < keys.sink_chunks ? j < keys.sink_hi : j < keys.hi && (j >= keys.lo || j < a.sinks)) || at >= a.table_width) return -1;
+        const int page = __ldg(a.block_table + request * a.table_stride + at);
+        return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages) ? page : -1;
+    }
+};
+
+template <int kDim>
+struct FewRing {
+    static constexpr int kPanels = Ring<kDim>::kPanels, kPanel = Ring<kDim>::kPanel, kTile = Ring<kDim>::kTile;
+    static constexpr int kStages = kDim == 64 ? 5 : 3;
+    static constexpr int kQuery = kPanels * kFew * 128;  // of a segment; a multiple of 1024
+    static constexpr int kBytes = kStages * (kTile + kQuery);  // as many segments as blocks may be in work
+};
+template <int kDim>
+struct FewShared {
+    static constexpr int kStages = FewRing<kDim>::kStages;
+    // of the segments that are told of: those in the ring, the one before and the one behind it
+    alignas(16) float lse[kStages + 2][kFew];  // inf where a row adds nothing,
+    alignas(16) int p[kStages + 2][kFew];      // and their positions; -1 there
+    // of the block that is brought next and the one behind it; in elements
+    int64_t row[2][kBlock];     // where a key's row begins; -1: it is not there
+    int64_t query[2][kFew];     // and a query's, where the block is the first of its segment
+    int opens[2];
+    uint64_t done[2];
+    uint64_t drain;
+    uint32_t tmem;
+};
+
+// As the kernel of many rows, with kFew rows at a time and without a pause between tiles: half of the warps bring blocks and
+// their tiles' queries kStages - 1 blocks ahead, over the ends of tiles, the other half have a key's scores to a thread.  Between
+// two barriers one block's products run, the scores of the one before are read, and its place is filled again.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(2 * kBlock, kCtasPerSm) attention_weights_few_kernel(const AttentionParams a, const WeightsArgs w, const Limits limits) {
+    using R = FewRing<kDim>;
+    extern __shared__ char smem[];
+    const Place pl = locate<kRows, kWhole, kBlock, 2 * kBlock, 1>(a, reinterpret_cast<int*>(smem), blockIdx.x, a.ctas);
+    if (pl.unit >= pl.end) return;
+    const bool loads = threadIdx.x >= kBlock;
+    const int tid = threadIdx.x % kBlock, warp = tid >> 5;  // of its half
+    __syncthreads();  // what follows overlays the scan
+    const uint32_t tiles = (smem_addr(smem) + 1023) & ~1023u, queries = tiles + R::kStages * R::kTile;  // on 1024 bytes
+    FewShared<kDim>& sh = *reinterpret_cast<FewShared<kDim>*>(smem + (tiles - smem_addr(smem)) + R::kBytes);
+    if (threadIdx.x == 0) {
+        bar_init(&sh.done[0], 1);
+        bar_init(&sh.done[1], 1);
+        bar_init(&sh.drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x < 32) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&sh.tmem)), "n"(2 * kFew) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = sh.tmem;
+    bool late = false;  // a wait ran out
+    const auto wait = [&](int block) {  // for its products
+        if (late) return;
+        for (int i = 0; !bar_try(&sh.done[block & 1], (block >> 1) & 1); ++i)
+            if (i >= limits.tries) {
+                late = true;
+                break;
+            }
+    };
+    Walk at(a, pl);
+    if (loads) {
+        using Sh = FewShared<kDim>;
+        // A block is told of, a key to a thread, one round before it is brought, 16 bytes (of each 128) of 8 keys to a thread;
+        // its page is read another round before.
+        const uint32_t to = tiles + (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);
+        const T* from = static_cast<const T*>(a.k_cache) + (tid & 7) * 8;
+        int page = at.page(tid), segment = -1, told = 0, brought = 0, stage = 0, q_slot = -1;
+        const auto tell = [&] {
+            if (!at.more) return;
+            sh.row[told & 1][tid] =
+                page < 0 ? -1 : page * a.page_stride + ((at.first() + tid) & (a.page_size - 1)) * a.token_stride + at.head * a.head_stride;
+            if (tid == 0) sh.opens[told & 1] = at.opens;
+            if (at.opens && ++segment == Sh::kStages + 2) segment = 0;
+            if (at.opens && tid < kFew) {
+                const int n = at.g0 + min(tid, min(kFew, at.rows - at.g0) - 1), i = div_group(a, n), g = n - i * a.group;  // the last row again past the end
+                const float l = __ldg(w.lse + static_cast<int64_t>(at.r.start + i) * a.heads + at.head * a.group + g);
+                const bool adds = at.g0 + tid < at.rows && isfinite(l);
+                sh.query[told & 1][tid] = static_cast<int64_t>(at.r.start + i) * a.q_token_stride + static_cast<int64_t>(at.head * a.group + g) * a.q_head_stride;
+                sh.lse[segment][tid] = adds ? l : INFINITY;
+                sh.p[segment][tid] = adds ? at.r.kv_len - at.r.rows + i : -1;
+            }
+            ++told;
+            at.next();
+            page = at.page(tid);
+        };
+        const auto bring = [&] {
+            if (brought < told) {
+                if (sh.opens[brought & 1]) {
+                    if (++q_slot == R::kStages) q_slot = 0;
+#pragma unroll
+                    for (int x = tid; x < kFew * (kDim / 8); x += kBlock) {
+                        const int row = x / (kDim / 8), piece = x % (kDim / 8);
+                        copy16(queries + q_slot * R::kQuery + (piece >> 3) * (kFew * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4),
+                               static_cast<const T*>(a.q) + sh.query[brought & 1][row] + piece * 8, !late);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < kBlock / 16; ++x) {
+                    const int64_t row = sh.row[brought & 1][16 * x + (tid >> 3)];
+                    const T* src = from + max(row, static_cast<int64_t>(0));
+#pragma unroll
+                    for (int b = 0; b < R::kPanels; ++b)
+                        if (kDim % 64 == 0 || b == 0 || (tid & 7) < 4) copy16(to + stage * R::kTile + b * R::kPanel + x * 2048, src + b * 64, row >= 0 && !late);
+                }
+                if (++stage == R::kStages) stage = 0;
+                ++brought;
+            }
+            copy_commit();
+        };
+        const auto half_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kBlock) : "memory"); };
+        tell();
+        for (int x = 0; x < R::kStages - 1; ++x) {
+            half_sync();
+            bring();
+            tell();
+        }
+        for (int x = 0; x < brought; ++x) {
+            copy_wait<R::kStages - 2>();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            late = __syncthreads_or(late);
+            if (x > 0) wait(x - 1);
+            bring();  // where block x - 1 was
+            tell();
+        }
+        copy_wait<0>();
+    } else {
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) << 21);  // lanes 32 * warp on
+        int page = at.page(tid), segment = -1;
+        // what is read of the walk after it has gone on: the block whose scores are read next
+        int head = 0, first = 0, here = -1, p0 = 0, p1 = 0, rows = 0;
+        bool all = false, fresh = false;
+        const auto take = [&] {
+            if (at.opens && ++segment == R::kStages + 2) segment = 0;
+            head = at.head;
+            first = at.first();
+            here = page;
+            p0 = at.r.kv_len - at.r.rows;
+            p1 = at.r.kv_len - 1;
+            rows = min(kFew, at.rows - at.g0);
+            const int last = first + kBlock - 1, held = a.held ? max(0, __ldg(a.held + at.request)) : max(0, p0);
+            all = last <= p0 && last < (at.c < at.keys.sink_chunks ? at.keys.sink_hi : at.keys.hi) &&
+                  (a.window < 0 || last < a.sinks || (first >= at.keys.lo && p1 - first < a.window));
+            fresh = at.g0 == 0 && first + tid >= held;
+            at.next();
+            page = at.page(tid);
+        };
+        const auto finish = [&](int block) {
+            wait(block);
+            __syncwarp();
+            tmem_fence_after();
+            float s[kFew], sum[4] = {0.f, 0.f, 0.f, 0.f};
+            tmem_load16(lanes + (block & 1) * kFew, s);
+            tmem_load_wait();
+            const int j = first + tid;
+#pragma unroll
+            for (int x = 0; x < kFew; x += 4)
+                if (x < rows) {
+                    const float4 l4 = *reinterpret_cast<const float4*>(&sh.lse[segment][x]);
+                    const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+                    int p[4] = {0, 0, 0, 0};
+                    if (!all) {
+                        const int4 p4 = *reinterpret_cast<const int4*>(&sh.p[segment][x]);
+                        p[0] = p4.x, p[1] = p4.y, p[2] = p4.z, p[3] = p4.w;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        // the difference first: scores and lse may be large, it is not where the weight counts
+                        const float v = exp2_fast(fmaf(s[x + e], w.scale, -l[e]) * kLog2e);
+                        const bool sees = all ? l[e] < INFINITY : j <= p[e] && (a.window < 0 || p[e] - j < a.window || j < a.sinks);
+                        sum[e] += sees ? v : 0.f;
+                    }
+                }
+            tmem_fence_before();
+            if (here >= 0) {
+                float* to = w.weights.w + head * w.weights.head_stride + here * w.weights.page_stride + (j & (a.page_size - 1));
+                const float add = late ? NAN : (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                // one addition to a key at a time, so that it does not matter when it is done
+                if (fresh) *to = add;
+                else asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(to), "f"(add) : "memory");
+            }
+        };
+        // all of a warp's lanes walk along, so that addresses stay in uniform registers; one issues
+        const bool issues = warp == 0 && elect_one();
+        const uint32_t tm = uniform(tmem), k_low = uniform(operand_low(tiles, 16)), q_low = uniform(operand_low(queries, 16));
+        constexpr uint32_t kDesc = instruction<T>(kFew, false);
+        int stage = 0, q_slot = -1;
+        for (int x = 0; at.more; ++x) {
+            tmem_fence_before();
+            late = __syncthreads_or(late);
+            tmem_fence_after();
+            if (at.opens && ++q_slot == R::kStages) q_slot = 0;
+            if (warp == 0 && !late && x < limits.lost) {
+                const uint32_t kb = uniform(k_low + stage * (R::kTile / 16)), qb = uniform(q_low + q_slot * (R::kQuery / 16)), d = uniform(tm + (x & 1) * kFew);
+                if (issues) {
+#pragma unroll
+                    for (int k = 0; k < kDim / 16; ++k)
+                        mma_smem(d, kb + ((k >> 2) * R::kPanel + (k & 3) * 32) / 16, qb + ((k >> 2) * kFew * 128 + (k & 3) * 32) / 16, kDesc, k > 0);
+                    mma_commit(&sh.done[x & 1]);
+                }
+                __syncwarp();
+            }
+            if (++stage == R::kStages) stage = 0;
+            if (x > 0) finish(x - 1);
+            take();
+            if (!at.more) finish(x);
+        }
+        tmem_fence_before();
+    }
+    // products end before the CTA does, also after a wait that ran out
+    late = __syncthreads_or(late);
+    if (threadIdx.x == 0 && late) {
+        mma_commit(&sh.drain);
+        for (int i = 0; i < kTries && !bar_try(&sh.drain, 0); ++i) {
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(2 * kFew) : "memory");
+}
+
 Limits g_limits = {kTries, INT32_MAX};
 
-template <typename T, int kDim>
+template <typename T, int kDim, bool kFewRows>
 cudaError_t launch(AttentionParams a, const WeightsArgs& w, cudaStream_t stream) {
     a.base_align = kBlock;
     a.tile_units = 0;
+    a.tile_rows = kFewRows ? kFew : kMany;
     a.ctas *= kCtasPerSm;
     a.held = w.held;
     // the units of a kv head are summed in 32 bits
     const int64_t keys = std::min<int64_t>(static_cast<int64_t>(a.table_width) * a.page_size, INT32_MAX);
-    const int64_t costs = a.requests + ((static_cast<int64_t>(a.tokens) * a.group) >> kWholeRows);
+    const int64_t costs = a.requests + static_cast<int64_t>(a.tokens) * a.group / a.tile_rows;
     a.unit_shift = 0;
     while (a.unit_shift < 24 && costs * (((keys / kBlock + 3) >> a.unit_shift) + 1) > INT32_MAX) ++a.unit_shift;
-    constexpr int kBytes = Ring<kDim>::kBytes + 1024 + static_cast<int>(sizeof(Shared<kDim>));
+    constexpr int kBytes = 1024 + (kFewRows ? FewRing<kDim>::kBytes + static_cast<int>(sizeof(FewShared<kDim>))
+                                            : Ring<kDim>::kBytes + static_cast<int>(sizeof(Shared<kDim>)));
     static_assert((kBytes + 1024) * kCtasPerSm <= 228 * 1024, "two CTAs' shared memory");
     constexpr int most = std::max(kBytes, locate_bytes(kMaxRequests));
     const int bytes = std::max(kBytes, locate_bytes(a.requests));
+    const auto kernel = kFewRows ? attention_weights_few_kernel<T, kDim> : attention_weights_kernel<T, kDim>;
     static SmemOnce once;
-    const cudaError_t e = once.set(reinterpret_cast<const void*>(attention_weights_kernel<T, kDim>), most);
+    const cudaError_t e = once.set(reinterpret_cast<const void*>(kernel), most);
     if (e != cudaSuccess) return e;
-    attention_weights_kernel<T, kDim><<<a.ctas, kThreads, bytes, stream>>>(a, w, g_limits);
+    kernel<<<a.ctas, kFewRows ? 2 * kBlock : kThreads, bytes, stream>>>(a, w, g_limits);
     return cudaGetLastError();
+}
+
+// Requests of more than 16 rows on average are gone through 128 rows at a time.
+template <typename T, int kDim>
+cudaError_t by_rows(const AttentionParams& a, const WeightsArgs& w, cudaStream_t s) {
+    return static_cast<int64_t>(a.tokens) * a.group > static_cast<int64_t>(a.requests) * kFew ? launch<T, kDim, false>(a, w, s) : launch<T, kDim, true>(a, w, s);
 }
 
 template <typename T>
 cudaError_t by_dim(const AttentionParams& a, const WeightsArgs& w, cudaStream_t s) {
-    return a.dim == 64 ? launch<T, 64>(a, w, s) : a.dim == 96 ? launch<T, 96>(a, w, s) : launch<T, 128>(a, w, s);
+    return a.dim == 64 ? by_rows<T, 64>(a, w, s) : a.dim == 96 ? by_rows<T, 96>(a, w, s) : by_rows<T, 128>(a, w, s);
 }
 
 }  // namespace
