@@ -71,6 +71,13 @@ template <int N>
 __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// What a block's rows gave to a key.  A request adds to a key once for each group of rows, one after the other, by one thread;
+// an addition by the memory system is not waited for, and counts those of requests that share a page too.
+__device__ __forceinline__ void add_weight(float* to, float x, bool first) {
+    if (first) *to = x;
+    else asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(to), "f"(x) : "memory");
+}
+
 struct Limits {
     int tries, lost;  // of waits; block from which on no products are issued (none: INT32_MAX)
 };
@@ -135,12 +142,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
                 if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) return -1;
                 return page * a.page_stride + ((first_key(c) + tid) & (a.page_size - 1)) * a.token_stride;
             };
-            // its weight; beyond the first rows, with what they gave it
+            // its weight
             const auto weight = [&](int c, int page) -> float* {
                 if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) return nullptr;
                 return w_head + page * w.weights.page_stride + ((first_key(c) + tid) & (a.page_size - 1));
             };
-            const auto so_far = [&](int c, const float* x) { return x && (g0 > 0 || first_key(c) + tid < held) ? *x : 0.f; };
             const auto load = [&](const int64_t* row, uint32_t to) {
                 to += (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);
                 const T* from = k_head + (tid & 7) * 8;
@@ -179,7 +185,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
                 copy_commit();
             }
             float* to = weight(c0, look[0]);
-            float before = so_far(c0, to);
             // in turn: where rows are told (of block c in finish(c)), where those of block c + stages are, its keys' place
             int told = 0, next = stages, stage = 0;
             const auto finish = [&](int c, uint32_t number) {
@@ -202,10 +207,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
 #pragma unroll
                 for (int x = 0; x < R::kLook; ++x) look[x] = look[x + 1];
                 look[R::kLook] = find(c + R::kLook + 1);
-                const float old = before;
                 float* const here = to;
                 to = weight(c + 1, look[0]);
-                before = so_far(c + 1, to);
                 const bool all = last <= p0 && last < (c < keys.sink_chunks ? keys.sink_hi : keys.hi) &&
                                  (a.window < 0 || last < a.sinks || (first >= keys.lo && p1 - first < a.window));
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
                     }
                 }
                 tmem_fence_before();
-                if (here) *here = late ? NAN : old + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                if (here) add_weight(here, late ? NAN : (sum[0] + sum[1]) + (sum[2] + sum[3]), g0 == 0 && j >= held);
             };
             int at = 0;
             for (int c = c0; c < c1; ++c) {
@@ -527,13 +530,9 @@ __global__ void __launch_bounds__(2 * kBlock, kCtasPerSm) attention_weights_few_
                     }
                 }
             tmem_fence_before();
-            if (here >= 0) {
-                float* to = w.weights.w + head * w.weights.head_stride + here * w.weights.page_stride + (j & (a.page_size - 1));
-                const float add = late ? NAN : (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                // one addition to a key at a time, so that it does not matter when it is done
-                if (fresh) *to = add;
-                else asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(to), "f"(add) : "memory");
-            }
+            if (here >= 0)
+                add_weight(w.weights.w + head * w.weights.head_stride + here * w.weights.page_stride + (j & (a.page_size - 1)),
+                           late ? NAN : (sum[0] + sum[1]) + (sum[2] + sum[3]), fresh);
         };
         // all of a warp's lanes walk along, so that addresses stay in uniform registers; one issues
         const bool issues = warp == 0 && elect_one();

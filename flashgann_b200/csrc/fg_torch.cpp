@@ -314,6 +314,7 @@ at::Tensor select_blocks(at::Tensor q, const at::Tensor& bounds, const at::Tenso
     requests(table, query_start, kv_len);
     const int64_t T = q.size(0);
     FG_NEED(count >= 0, "count " + std::to_string(count) + " is negative");
+    i32(count, "count");
     at::Tensor out;
     if (out_or_none) {
         out = *out_or_none;

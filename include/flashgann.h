@@ -462,7 +462,8 @@ int fg_block_attention_device(const fg_kv_cache* cache, const fg_attention* args
  * d_held [requests]: tokens whose weights are there already (NULL: those before
  * the new ones); weights from there to kv_len[b] start at 0, whatever was there.
  * Rows whose lse is not finite add nothing.  Sums are 32 bits, in the order of
- * the rows: the same bits on every run.  Only the last tokens of a prompt may be
+ * the rows: the same bits on every run, but where requests share a page, whose
+ * sums are added to it in any order (of shared pages none may be new).  Only the last tokens of a prompt may be
  * given: query_start counts them alone.  The cache's v may be NULL. */
 int fg_attention_weights_device(const fg_kv_cache* cache, const fg_attention* args, float* d_weights,
                                 int64_t weights_page_stride, int64_t weights_head_stride, const int32_t* d_held,

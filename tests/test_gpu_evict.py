@@ -149,6 +149,26 @@ def test_weights_scales_strides_and_repeats():
     assert (layers[0] == 5).all() and (layers[2] == 5).all()
 
 
+def test_weights_of_shared_pages():
+    """Requests that share a prompt's pages: the pages get what all of them pay."""
+    import torch
+    import flashgann_b200 as fg
+    rng = np.random.default_rng(5)
+    for new in (1, 40):  # both kernels
+        x = make(rng, ctx=[96, 96, 96], new=[new] * 3, heads=4, kv_heads=2, dim=64, page=16)
+        x["table"][1:, :6] = x["table"][0, :6]
+        w = _weights(rng, x)
+        lse = _lse(x)
+        want = w.astype(np.float64)
+        tol = np.zeros_like(want)
+        for b in range(3):  # one request after the other
+            one = dict(table=x["table"][b:b + 1], start=np.array([0, new]), kv_len=x["kv_len"][b:b + 1])
+            rows = slice(b * new, (b + 1) * new)
+            got, t = weights_ref(x["q"][rows], x["k"], one["table"], one["start"], one["kv_len"], lse[rows], want.astype(np.float32))
+            want, tol = got, tol + t + 2.0 ** -23 * np.abs(got)
+        assert (np.abs(_add(x, w, lse, "fp16") - want) <= tol).all()
+
+
 # ---- eviction ----
 
 def _evict(x, w, budget, recent, sinks, dtype="bf16", order="phd"):
