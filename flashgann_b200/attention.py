@@ -1,11 +1,16 @@
 """A paged key/value cache and attention over it, for decoders that find the
-keys of a long context with this package's search.
+keys of a long context with this package's search, or that bound what they read
+of it without one.
 
 The loop of one step: ``kv_plan`` gives each request pages and each new token
 a slot, ``kv_append`` writes the new keys and values there, and then either
 ``paged_attention`` (all of the context, or a sliding window and the first
-tokens) or ``retrieved_attention`` (window, first tokens and the ids that a
-search returned for each query head) reads them.  All four take torch CUDA
+tokens), ``retrieved_attention`` (window, first tokens and the ids that a
+search returned for each query head) or ``block_attention`` (window, first
+tokens and whole pages) reads them.  For the last, ``kv_summarize`` keeps bounds
+of each page's keys and ``select_blocks`` chooses the pages of the highest
+bounds.  To keep the cache short instead, ``attention_weights`` sums up what
+each key was paid and ``kv_evict`` drops the lightest.  All take torch CUDA
 tensors, run in libflashgann.so (include/flashgann.h has the exact rules) on
 ``stream`` (default: torch's current stream) and wait for nothing.  They are
 for serving and have no backward pass: where torch records gradients, a tensor
