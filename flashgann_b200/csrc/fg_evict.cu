@@ -32,7 +32,7 @@
 namespace fg {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxSmem = 110 * 1024;  // two CTAs to an SM
 constexpr int kChunk = 64;            // rows

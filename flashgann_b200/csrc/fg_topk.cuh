@@ -39,7 +39,7 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 constexpr int kList = 32;
 // Bits of a digit: a few thousand keys spread well enough over 256 counts, more want 2048.
 constexpr int kMostBins = 2048;
-__host__ __device__ constexpr int bits_of(int threads) { return threads >= 1024 ? 11 : 8; }
+__host__ __device__ constexpr int bits_of(int threads) { return threads >= 512 ? 11 : 8; }
 
 struct alignas(16) Shared {  // what callers lay behind it is read 16 bytes at a time
     int hist[kMostBins];
