@@ -928,9 +928,9 @@ cudaError_t launch_select(const SelectArgs& a, cudaStream_t stream) {
     const cudaError_t e = scoring.set(reinterpret_cast<const void*>(score_blocks_kernel<T, kDim>), kMaxSmem);
     if (e != cudaSuccess) return e;
     const unsigned parts = (static_cast<unsigned>(a.req.table_width) + kPart - 1) / kPart;
-    // kv heads to a CTA: all, or fewer where there would be less than two CTAs for each SM
+    // kv heads to a CTA: all, or fewer as long as all CTAs run at once, two to an SM
     int each = a.kv_heads;
-    while (each > 1 && static_cast<int64_t>(a.req.tokens) * parts * ((a.kv_heads + each - 1) / each) < 2 * a.sms) each = (each + 1) / 2;
+    while (each > 1 && static_cast<int64_t>(a.req.tokens) * parts * ((a.kv_heads + (each + 1) / 2 - 1) / ((each + 1) / 2)) <= 2 * a.sms) each = (each + 1) / 2;
     const dim3 grid(a.req.tokens * parts, static_cast<unsigned>((a.kv_heads + each - 1) / each));
     score_blocks_kernel<T, kDim><<<grid, kPartThreads, scoring_bytes<kDim>(a.group), stream>>>(a, each);
     const cudaError_t started = cudaGetLastError();

@@ -17,7 +17,8 @@
 // thread to a row, which moves the row's weight too.
 //
 // What bounds it: the weights' way and, of the rows that move, there and back.
-// 32 requests of 900 to 8000 positions to 1024, 8 kv heads of 128: see kStages.
+// 32 requests of 900 to 8000 positions to 1024, 8 kv heads of 128: 59 us, of
+// which the selection takes about 10, for 258 MB.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -36,7 +37,7 @@ constexpr int kThreads = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxSmem = 110 * 1024;  // two CTAs to an SM
 constexpr int kChunk = 64;            // rows
-constexpr int kStages = 3;            // of chunks (registers instead, a chunk after the other: 93 us)
+constexpr int kStages = 3;            // of chunks (registers instead, a chunk after the other: 93 us for 72)
 
 template <int kDim>
 struct Ring {
@@ -189,7 +190,9 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.requests) * a.cache.heads;
     const int64_t most = std::min<int64_t>(static_cast<int64_t>(a.table_width) << a.cache.page_shift, INT32_MAX);
     int ranks = 1;
-    while (ranks < kMaxCluster && rows * ranks < a.sms && most > 2048 * ranks) ranks *= 2;
+    // CTAs to a row: as many as there are SMs for, with 256 positions each; us with 8 kv heads of one request, 1 / 4 or 8:
+    // 576 positions 15.4 / 15.0, 1100 27.2 / 20.6, 2200 43 / 25; of four requests of 1100 27.7 / 20.4 (more CTAs than SMs: 34)
+    while (ranks < kMaxCluster && rows * ranks * 2 <= a.sms && most > 256 * ranks) ranks *= 2;
     constexpr int kRoom = (kMaxSmem - static_cast<int>(sizeof(topk::Shared))) / 4;
     const int room = static_cast<int>(std::min<int64_t>((most + ranks - 1) / ranks, kRoom));
     static_assert(Ring<128>::kBytes + sizeof(Moves) <= kMaxSmem && (kMaxSmem + 1024) * 2 <= 228 * 1024, "two CTAs to an SM");
