@@ -190,9 +190,10 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.requests) * a.cache.heads;
     const int64_t most = std::min<int64_t>(static_cast<int64_t>(a.table_width) << a.cache.page_shift, INT32_MAX);
     int ranks = 1;
-    // CTAs to a row: as many as there are SMs for, with 256 positions each; us with 8 kv heads of one request, 1 / 4 or 8:
-    // 576 positions 15.4 / 15.0, 1100 27.2 / 20.6, 2200 43 / 25; of four requests of 1100 27.7 / 20.4 (more CTAs than SMs: 34)
-    while (ranks < kMaxCluster && rows * ranks * 2 <= a.sms && most > 256 * ranks) ranks *= 2;
+    // CTAs to a row: one for up to 640 positions, else as many as there are SMs for, with 256 positions each.  us with 8 kv
+    // heads of one request, 1 / 4 or 8: 576 positions 15.4 / 15.0 (few moves 14.3 / 16.4), 1100 27.2 / 20.6, 2200 43 / 25; of
+    // four requests of 1100 27.7 / 20.4 (more CTAs than SMs: 34)
+    while (ranks < kMaxCluster && rows * ranks * 2 <= a.sms && most > 640 && most > 256 * ranks) ranks *= 2;
     constexpr int kRoom = (kMaxSmem - static_cast<int>(sizeof(topk::Shared))) / 4;
     const int room = static_cast<int>(std::min<int64_t>((most + ranks - 1) / ranks, kRoom));
     static_assert(Ring<128>::kBytes + sizeof(Moves) <= kMaxSmem && (kMaxSmem + 1024) * 2 <= 228 * 1024, "two CTAs to an SM");
