@@ -841,6 +841,12 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     a.tile_rows = tile_rows(a);
     const bool split = attention_rows_splits(a);
     a.ctas *= kCtasPerSm;
+    if (kForm == kChosen && split) {
+        // Tiles of chosen pages are much the same length: where there are fewer than CTAs, as many CTAs to each, so that few
+        // have two (32 tokens of 85 chunks 40.7 -> 36.7 us, 30 of 76 24.9 -> 23.0, 8 of 85 18.3 -> 18.9).
+        const int64_t tiles = static_cast<int64_t>(a.tokens) * a.kv_heads * ((a.group + a.tile_rows - 1) / a.tile_rows);
+        if (tiles < a.ctas) a.ctas = static_cast<int>(tiles * (a.ctas / tiles));
+    }
     a.unit_shift = split ? unit_shift(a) : 24;  // a unit: one chunk for each warp (or more, see there), or a tile
     a.tile_units = split ? kTileUnits : 0;
     static SmemOnce once;

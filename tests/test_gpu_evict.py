@@ -149,6 +149,33 @@ def test_weights_scales_strides_and_repeats():
     assert (layers[0] == 5).all() and (layers[2] == 5).all()
 
 
+@pytest.mark.parametrize("new", [1, 9])  # the kernels of few and of many rows
+def test_weights_of_tables_for_billions_of_keys(new):
+    """Units of work past 2^31 if every request filled its table: 200 requests of a few tokens, whose rows of the table are
+    one row of 2^27 pages."""
+    import torch
+    import flashgann_b200 as fg
+    rng = np.random.default_rng(6)
+    R, page = 200, 16
+    x = make(rng, ctx=[300], new=[0], heads=2, kv_heads=1, dim=64, page=page)
+    table = torch.full((1, 2 ** 27), -1, dtype=torch.int32, device="cuda")
+    table[0, :x["table"].shape[1]] = _cuda(x["table"][0])
+    lens = rng.integers(new, 300, R).astype(np.int32)
+    q = (rng.integers(-64, 65, (R * new, 2, 64)) / 32).astype(np.float32)
+    lse = (3 + rng.random((R * new, 2))).astype(np.float32)
+    w = torch.zeros((x["k"].shape[0], 1, page), device="cuda")
+    fg.attention_weights(_cuda(q, torch.bfloat16), _cuda(x["k"], torch.bfloat16), w, table.expand(R, -1),
+                         _cuda(np.arange(0, R * new + 1, new, dtype=np.int32)), _cuda(lens), _cuda(lse), held=_cuda(lens))
+    j = np.arange(300)
+    k = x["k"][x["table"][0, j // page], j % page, 0].astype(np.float64)
+    e = np.exp(np.einsum("thd,jd->thj", q.astype(np.float64), k) / 8 - lse[..., None])
+    p = (lens[:, None] - new + np.arange(new)).reshape(-1)
+    want = np.where(j <= p[:, None, None], e, 0).sum((0, 1))
+    got = w[_cuda(x["table"][0, j // page]).long(), 0, _cuda(j % page).long()].double().cpu().numpy()
+    # 2 * R * new terms of up to e^10, each off by (10 + 2) 2^-22 of itself, and as many roundings of the sum
+    assert (np.abs(got - want) <= want * (12 * 2.0 ** -22 + 2 * R * new * 2.0 ** -24)).all()
+
+
 def test_weights_of_shared_pages():
     """Requests that share a prompt's pages: the pages get what all of them pay."""
     import torch
