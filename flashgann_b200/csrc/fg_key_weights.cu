@@ -5,20 +5,21 @@
 //     w[j] = (j < held ? w[j] : 0) + sum over the rows r that see j of e^(scale q_r.k_j - lse_r).
 //
 // A block is 128 keys of one request and kv head.  The tensor cores compute
-// S = K Q^T (tcgen05.mma, 128 keys x up to 128 query rows x dim) into TMEM, where a
-// key is a lane: each of the CTA's 128 threads reads its key's scores and adds up
-// their exponentials by itself.  Every key is one CTA's, which walks all of its
-// rows, 128 at a time: no atomics, and an order that depends on the row alone.
+// S = K Q^T (tcgen05.mma, 128 keys x up to 256 query rows x dim) into TMEM, where a
+// key is a lane: a thread reads its key's scores and adds up their exponentials by
+// itself.  Every key is one CTA's, which walks all of its rows: an order that
+// depends on the row alone.
 //
 // Few rows (a decode step) are bound by the keys' way from memory, 2 * dim bytes
-// each: two CTAs to an SM, whose rings hold up to three blocks each.  Keys come by
+// each: two CTAs to an SM, whose rings hold three blocks each.  Keys come by
 // 16-byte cp.async, which gathers rows of any pages and strides into the 128-byte
-// swizzled layout that tcgen05 reads; pages are looked up a block ahead of the
-// copies.  Many rows (the last tokens of a prompt) are bound by the special-function
-// units, 16 exponentials a clock and SM: the products of the next block run beside
-// them.  (mma.sync does a sixteenth of tcgen05's operations here, 8 clocks for
-// m16n8k16: 256 rows on 8192 keys took 38 us.)  Blocks are split over the CTAs as
-// in fg_attention.cuh.
+// swizzled layout that tcgen05 reads.  64 ragged decodes, 557 MB: 107 us.  Many
+// rows (the last tokens of a prompt) are bound by the special-function units, 16
+// exponentials a clock and SM, and by the way of queries and keys before the first
+// of them: up to 256 rows are gone through at once, by two threads to a key.
+// (mma.sync does a sixteenth of tcgen05's operations here, 8 clocks for m16n8k16:
+// 256 rows on 8192 keys took 38 us; with 128 rows at a time and a thread to a key
+// 20.)  Blocks are split over the CTAs as in fg_attention.cuh.
 //
 // Waits for products are bounded: one that runs out ends the CTA's work, with NaN
 // in the keys that are left.
@@ -34,11 +35,11 @@ namespace {
 
 constexpr int kRows = 16;    // not looked at: a tile is a request
 constexpr int kBlock = 128;  // keys
-constexpr int kThreads = 128;
+constexpr int kThreads = 2 * kBlock;
 constexpr int kCtasPerSm = 2;
 constexpr int kFew = 16;     // rows at a time where there are few
-constexpr int kMany = 128;   // and where there are many
-constexpr int kColumns = 2 * kMany;  // of TMEM: two blocks' scores
+constexpr int kMany = 256;   // and where there are many
+constexpr int kColumns = kMany;      // of TMEM, a block's scores
 constexpr int kTries = 1 << 18;      // a try that finds nothing takes 4 us: a second
 
 template <int kDim>
@@ -46,18 +47,16 @@ struct Ring {
     static constexpr int kPanels = (kDim + 63) / 64;  // 64 columns (128 bytes) each
     static constexpr int kPanel = kBlock * 128;
     static constexpr int kTile = kPanels * kPanel;
-    static constexpr int kStages = kDim == 64 ? 4 : 2;
-    static constexpr int kLook = kStages + 1;         // blocks whose rows are known
-    static constexpr int kQueries = kStages * kTile;
-    static constexpr int kBytes = kQueries + kPanels * kMany * 128;
+    static constexpr int kBytes = kTile + kPanels * kMany * 128;  // a block of keys, the queries
 };
 
 template <int kDim>
 struct Shared {
     alignas(16) float lse[kMany];  // of the rows in work; inf where a row adds nothing,
     alignas(16) int p[kMany];      // and their positions; -1 there
-    int64_t row[Ring<kDim>::kLook][kBlock];  // where a key's row begins, in elements; -1: it is not there
-    uint64_t done[2];              // products of a block
+    int64_t row[2][kBlock];  // where keys' rows begin, in elements, of the block that is loaded next and the one behind it; -1: not there
+    float part[kBlock];      // sums over the second half of the rows
+    uint64_t done;           // products of a block
     uint64_t drain;
     uint32_t tmem;
 };
@@ -93,8 +92,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
     const uint32_t tiles = (smem_addr(smem) + 1023) & ~1023u;  // the ring, on 1024 bytes
     Shared<kDim>& sh = *reinterpret_cast<Shared<kDim>*>(smem + (tiles - smem_addr(smem)) + R::kBytes);
     if (tid == 0) {
-        bar_init(&sh.done[0], 1);
-        bar_init(&sh.done[1], 1);
+        bar_init(&sh.done, 1);
         bar_init(&sh.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -105,12 +103,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = sh.tmem, mine = tmem + (static_cast<uint32_t>(warp) << 21);  // lanes 32 * warp on
+    const uint32_t tmem = sh.tmem, mine = tmem + (static_cast<uint32_t>(warp & 3) << 21);  // lanes 32 * (warp % 4) on
+    const int key = tid % kBlock, half = tid / kBlock;  // two threads to a key, 128 rows each
+    // all of a warp's lanes walk along, so that addresses stay in uniform registers; one issues
+    const bool issues = warp == 0 && elect_one();
+    const uint32_t tm = uniform(tmem), k_low = uniform(operand_low(tiles, 16)), q_low = uniform(operand_low(tiles + R::kTile, 16));
 
     int head = pl.head, request = pl.request, tile = pl.tile;
     int64_t unit = pl.unit, tile_first = pl.unit - pl.offset;
     Request r = load_request(a, request);
-    uint32_t issued = 0;  // blocks in the CTA so far: the number of a block says which scores and barrier are its own
+    uint32_t blocks = 0;  // in the CTA so far
     bool late = false;    // a wait ran out
     while (true) {
         const TileKeys keys = tile_keys<kRows, kWhole, kBlock>(a, r, 0);
@@ -129,41 +131,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
         const auto first_key = [&](int c) { return c < keys.sink_chunks ? c * kBlock : keys.base + (c - keys.sink_chunks) * kBlock; };
         for (int g0 = 0; c0 < c1 && g0 < rows; g0 += kMany) {
             const int n = min(rows - g0, kMany), columns = n <= 16 ? 16 : (n + 31) & ~31;
-            constexpr int stages = R::kStages, panel = kMany * 128;  // of the queries
-            const uint32_t queries = tiles + R::kQueries;
-            // the page of this thread's key of block c, which all look up for one another
+            constexpr int panel = kMany * 128;  // of the queries
+            const uint32_t queries = tiles + R::kTile, desc = uniform(instruction<T>(0, false) | (static_cast<uint32_t>(columns >> 3) << 17));
+            // the page of key `key` of block c, which the first half of the threads look up for all
             const auto find = [&](int c) {
-                if (c >= c1) return -1;
-                const int j = first_key(c) + tid, at = j >> a.page_shift;
-                if (!(c < keys.sink_chunks ? j < keys.sink_hi : j < keys.hi && (j >= keys.lo || j < a.sinks)) || at >= a.table_width) return -1;
-                return __ldg(table + at);
+                const int j = first_key(c) + key, at = j >> a.page_shift;
+                if (half || c >= c1 || !(c < keys.sink_chunks ? j < keys.sink_hi : j < keys.hi && (j >= keys.lo || j < a.sinks)) || at >= a.table_width)
+                    return -1;
+                const int page = __ldg(table + at);
+                return static_cast<uint32_t>(page) < static_cast<uint32_t>(a.pages) ? page : -1;
             };
-            const auto row_of = [&](int c, int page) -> int64_t {
-                if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) return -1;
-                return page * a.page_stride + ((first_key(c) + tid) & (a.page_size - 1)) * a.token_stride;
+            const auto tell = [&](int c, int page) {
+                if (!half) sh.row[c & 1][key] = page < 0 ? -1 : page * a.page_stride + ((first_key(c) + key) & (a.page_size - 1)) * a.token_stride;
             };
-            // its weight
-            const auto weight = [&](int c, int page) -> float* {
-                if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.pages)) return nullptr;
-                return w_head + page * w.weights.page_stride + ((first_key(c) + tid) & (a.page_size - 1));
-            };
-            const auto load = [&](const int64_t* row, uint32_t to) {
-                to += (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);
+            const auto load = [&](int c) {
+                const uint32_t to = tiles + (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);
                 const T* from = k_head + (tid & 7) * 8;
 #pragma unroll
-                for (int x = 0; x < kBlock / 16; ++x) {  // key 16 x + tid / 8
-                    const int64_t at = row[16 * x + (tid >> 3)];
-                    const T* src = from + max(at, static_cast<int64_t>(0));
+                for (int x = 0; x < kBlock / 32; ++x) {  // key 32 x + tid / 8
+                    const int64_t row = sh.row[c & 1][32 * x + (tid >> 3)];
+                    const T* src = from + max(row, static_cast<int64_t>(0));
 #pragma unroll
                     for (int b = 0; b < R::kPanels; ++b)
-                        if (kDim % 64 == 0 || b == 0 || (tid & 7) < 4) copy16(to + b * R::kPanel + x * 2048, src + b * 64, at >= 0);
+                        if (kDim % 64 == 0 || b == 0 || (tid & 7) < 4) copy16(to + b * R::kPanel + x * 4096, src + b * 64, row >= 0);
                 }
             };
             __syncthreads();  // the blocks before are done with
-            // pages of the blocks ahead: looked up kLook blocks before they are read, told kLook - 1 before
-            int look[R::kLook + 1];
-#pragma unroll
-            for (int x = 0; x <= R::kLook; ++x) look[x] = find(c0 + x);
+            int page = find(c0), next = find(c0 + 1);
             for (int x = tid; x < columns * (kDim / 8); x += kThreads) {
                 const int at = x / (kDim / 8), piece = x % (kDim / 8), i = div_group(a, g0 + min(at, n - 1));
                 const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(r.start + i) * a.q_token_stride +
@@ -177,43 +171,46 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
                 sh.lse[x] = adds ? l : INFINITY;
                 sh.p[x] = adds ? p0 + i : -1;
             }
-#pragma unroll
-            for (int x = 0; x < R::kLook; ++x) sh.row[x][tid] = row_of(c0 + x, look[x]);
+            tell(c0, page);
+            tell(c0 + 1, next);
             __syncthreads();
-            for (int x = 0; x < stages; ++x) {
-                if (c0 + x < c1) load(sh.row[x], tiles + x * R::kTile);
-                copy_commit();
-            }
-            float* to = weight(c0, look[0]);
-            // in turn: where rows are told (of block c in finish(c)), where those of block c + stages are, its keys' place
-            int told = 0, next = stages, stage = 0;
-            const auto finish = [&](int c, uint32_t number) {
-                const int first = first_key(c), last = first + kBlock - 1, j = first + tid;
+            load(c0);
+            copy_commit();
+            for (int c = c0; c < c1; ++c) {
+                const int first = first_key(c), last = first + kBlock - 1, j = first + key, here = page;
+                copy_wait<0>();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                tmem_fence_before();
+                late = __syncthreads_or(late);
+                tmem_fence_after();
+                if (warp == 0 && !late && c < limits.lost) {
+                    if (issues) {
+#pragma unroll
+                        for (int k = 0; k < kDim / 16; ++k)
+                            mma_smem(tm, k_low + ((k >> 2) * R::kPanel + (k & 3) * 32) / 16, q_low + ((k >> 2) * panel + (k & 3) * 32) / 16, desc, k > 0);
+                        mma_commit(&sh.done);
+                    }
+                    __syncwarp();
+                }
+                page = next;
+                next = find(c + 2);
                 if (!late)
-                    for (int i = 0; !bar_try(&sh.done[number & 1], (number >> 1) & 1); ++i)
+                    for (int i = 0; !bar_try(&sh.done, blocks & 1); ++i)
                         if (i >= limits.tries) {
                             late = true;
                             break;
                         }
+                ++blocks;
                 __syncwarp();
                 tmem_fence_after();
-                // its keys' place is free
-                if (c + stages < c1 && !late) load(sh.row[next], tiles + stage * R::kTile);
+                // its keys' place is free: the next ones come while its scores are read
+                if (c + 1 < c1 && !late) load(c + 1);
                 copy_commit();
-                sh.row[told][tid] = row_of(c + R::kLook, look[R::kLook]);
-                if (++told == R::kLook) told = 0;
-                if (++next == R::kLook) next = 0;
-                if (++stage == stages) stage = 0;
-#pragma unroll
-                for (int x = 0; x < R::kLook; ++x) look[x] = look[x + 1];
-                look[R::kLook] = find(c + R::kLook + 1);
-                float* const here = to;
-                to = weight(c + 1, look[0]);
+                tell(c + 2, next);
                 const bool all = last <= p0 && last < (c < keys.sink_chunks ? keys.sink_hi : keys.hi) &&
                                  (a.window < 0 || last < a.sinks || (first >= keys.lo && p1 - first < a.window));
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 __syncwarp();
-                const uint32_t scores = mine + (number & 1) * kMany;
                 const auto add = [&](const float* s, int x0, int count, bool check) {
 #pragma unroll
                     for (int x = 0; x < count; x += 4) {
@@ -232,51 +229,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
                         }
                     }
                 };
-                if (columns <= 16) {
-                    float s[16];
-                    tmem_load16(scores, s);
+                // 32 columns at a time, the last ones perhaps of nobody's
+                for (int x0 = half * 128; x0 < min(columns, half * 128 + 128); x0 += 32) {
+                    float s[32];
+                    if (columns == 16) tmem_load16(mine, s);
+                    else tmem_load32(mine + x0, s);
                     tmem_load_wait();
-#pragma unroll
-                    for (int x0 = 0; x0 < 16; x0 += 4)
-                        if (x0 < n) {
-                            if (all) add(s + x0, x0, 4, false);
-                            else add(s + x0, x0, 4, true);
-                        }
-                } else {
-                    // 32 columns at a time, the last ones perhaps of nobody's
-                    for (int x0 = 0; x0 < columns; x0 += 32) {
-                        float s[32];
-                        tmem_load32(scores + x0, s);
-                        tmem_load_wait();
-                        if (all) add(s, x0, 32, false);
-                        else add(s, x0, 32, true);
-                    }
+                    if (columns == 16) add(s, 0, 16, !all);
+                    else if (all) add(s, x0, 32, false);
+                    else add(s, x0, 32, true);
                 }
                 tmem_fence_before();
-                if (here) add_weight(here, late ? NAN : (sum[0] + sum[1]) + (sum[2] + sum[3]), g0 == 0 && j >= held);
-            };
-            int at = 0;
-            for (int c = c0; c < c1; ++c) {
-                if (c == c0) copy_wait<stages - 1>();
-                else copy_wait<stages - 2>();
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                tmem_fence_before();
-                late = __syncthreads_or(late);
-                tmem_fence_after();
-                if (tid == 0 && !late && c < limits.lost) {
-                    const uint32_t d = tmem + (issued & 1) * kMany, q_low = operand_low(queries, 16);
-                    const uint32_t k_low = operand_low(tiles + at * R::kTile, 16);
-                    const uint32_t idesc = instruction<T>(0, false) | (static_cast<uint32_t>(columns >> 3) << 17);
-#pragma unroll
-                    for (int k = 0; k < kDim / 16; ++k)
-                        mma_smem(d, k_low + ((k >> 2) * R::kPanel + (k & 3) * 32) / 16, q_low + ((k >> 2) * panel + (k & 3) * 32) / 16, idesc, k > 0);
-                    mma_commit(&sh.done[issued & 1]);
+                float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (columns > 128) {
+                    if (half) sh.part[key] = total;
+                    __syncthreads();
+                    if (!half) total += sh.part[key];
                 }
-                ++issued;
-                if (++at == stages) at = 0;
-                if (c > c0) finish(c - 1, issued - 2);
+                if (here >= 0) add_weight(w_head + here * w.weights.page_stride + (j & (a.page_size - 1)), late ? NAN : total, g0 == 0 && j >= held);
             }
-            finish(c1 - 1, issued - 1);
             copy_wait<0>();
         }
         if (tile_last >= pl.end || !next_tile<kRows, kWhole>(a, &r, &head, &request, &tile)) break;

@@ -51,6 +51,8 @@ WEIGHTS = [
     ([500], [70], 6, 2, 128, 8, "bf16", "phd"),              # the last tokens of a prompt
     ([0, 90], [33, 1], 4, 4, 64, 256, "fp16", "phd"),        # a prompt beside a decode
     ([40] * 60, [1] * 60, 8, 4, 64, 16, "bf16", "phd"),
+    ([170], [110], 12, 3, 96, 16, "bf16", "hpd"),            # more rows than are gone through at once
+    ([33, 0], [64, 65], 2, 1, 128, 32, "fp16", "phd"),
 ]
 
 
