@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) kv_summarize_kernel(const Summ
 // What bounds it: 2 * dim + 4 bytes a page and kv head from memory, which many rows
 // read at 2.8 TB/s (64 tokens, 286K pages and heads, 71 MB: 25 us): a CTA's start,
 // the first pages' way and the selection are as long as the pages' way.  One token
-// of 131K positions: 16.5 us.
+// of 131K positions: 14.9 us.
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 static_assert(sizeof(topk::Shared) % 16 == 0, "the queries behind it are read 16 bytes at a time");
@@ -881,7 +881,7 @@ constexpr int kMaxSmem = 224 * 1024;
 // Which kernels take a call, measured with 32 heads on 8 of dim 128, us: as many rows as SMs and up to kRowPages blocks of
 // the table, a CTA of the tensor cores to each (64 tokens of 62 / 243 / 937 blocks 10 / 14 / 38; in threads 11 / 18 / 54).
 // Fewer rows and up to kShort blocks, a CTA of threads to each (16 tokens 5.7 / 6.9, one 5.3 / 6.2; two kernels 6.9 / 8.8
-// and 6.4 / 6.6).  Else two kernels (16 tokens of 937 17, in threads 20; one 8.1, in threads 15).
+// and 6.4 / 6.6).  Else two kernels (16 tokens of 937 16, in threads 20; one 8.1, in threads 15).
 constexpr int kShort = 256;
 
 int query_bytes(const SelectArgs& a) { return ((a.group + 3) & ~3) * 4 + a.group * 2 * a.dim; }
