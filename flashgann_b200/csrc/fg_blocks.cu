@@ -69,6 +69,21 @@ constexpr float k127th = 1.f / 127.f;  // a product, rounded once: what a quotie
 
 __device__ __forceinline__ int clamped(const int32_t* p, int most) { return max(0, min(__ldg(p), most)); }
 
+// The first of n ascending places that is past something, or the last: 32 at a time, by whole warps.
+template <typename Past>
+__device__ __forceinline__ int first_past(int n, Past past) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0;
+    while (n > 1) {
+        const int step = (n + 31) / 32, at = lo + (lane + 1) * step - 1;
+        const uint32_t is = __ballot_sync(0xFFFFFFFFu, at >= lo + n || past(min(at, lo + n - 1)));
+        const int f = is ? __ffs(is) - 1 : 31;
+        n = min(step, n - f * step);
+        lo += f * step;
+    }
+    return lo;
+}
+
 // ---- summary ----
 //
 // Of the keys k_t, 0 <= t < n, of a page and kv head: with hi_d = max_t k_td,
@@ -93,13 +108,8 @@ __global__ void __launch_bounds__(kSumWarps * 32) kv_summarize_kernel(const Summ
     if (item >= items) return;
     // the last request whose numbers begin at or before this one
     const int shift = a.cache.page_shift;
-    int lo = 0, hi = a.req.requests - 1;
     const auto first_item = [&](int b) { return static_cast<int64_t>(clamped(a.req.query_start + b, a.req.tokens) >> shift) + 2 * static_cast<int64_t>(b); };
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (first_item(mid) <= item) lo = mid;
-        else hi = mid - 1;
-    }
+    const int lo = first_past(a.req.requests, [&](int b) { return first_item(b + 1) > item; });
     const int rows = clamped(a.req.query_start + lo + 1, a.req.tokens) - clamped(a.req.query_start + lo, a.req.tokens);
     const int kv_len = max(0, __ldg(a.req.kv_len + lo));
     if (rows <= 0 || kv_len == 0) return;
@@ -217,22 +227,13 @@ struct Row {
     const int32_t* table;    // of the first of them
 };
 // The request of a row is the first that ends after it.  In a decode step that is the row's own number, which is tried
-// first, with all that is read of it under way together; else it is searched for, 32 places at a time.  By whole warps.
+// first, with all that is read of it under way together; else it is searched for.  By whole warps.
 __device__ __forceinline__ Row row_of(const SelectArgs& a, int token) {
     const Requests& q = a.req;
     int lo = min(token, q.requests - 1);
     int start = clamped(q.query_start + lo, q.tokens), end = clamped(q.query_start + lo + 1, q.tokens), len = __ldg(q.kv_len + lo);
     if (token < start || token >= end) {
-        const int lane = threadIdx.x & 31;
-        int n = q.requests;
-        lo = 0;
-        while (n > 1) {
-            const int step = (n + 31) / 32, at = lo + (lane + 1) * step - 1;
-            const uint32_t past = __ballot_sync(0xFFFFFFFFu, at >= lo + n || clamped(q.query_start + min(at, lo + n - 1) + 1, q.tokens) > token);
-            const int f = past ? __ffs(past) - 1 : 31;
-            n = min(step, n - f * step);
-            lo += f * step;
-        }
+        lo = first_past(q.requests, [&](int b) { return clamped(q.query_start + b + 1, q.tokens) > token; });
         start = clamped(q.query_start + lo, q.tokens);
         end = clamped(q.query_start + lo + 1, q.tokens);
         len = __ldg(q.kv_len + lo);
