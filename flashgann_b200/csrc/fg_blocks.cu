@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) kv_summarize_kernel(const Summ
 // to each row.
 //
 // What bounds it: 2 * dim + 4 bytes a page and kv head from memory, which many rows
-// read at 2.8 TB/s (64 tokens, 286K pages and heads, 71 MB: 25 us): a CTA's start,
+// read at 3.0 TB/s (64 tokens, 286K pages and heads, 71 MB: 23.5 us): a CTA's start,
 // the first pages' way and the selection are as long as the pages' way.  One token
 // of 131K positions: 14.9 us.
 constexpr int kThreads = 256;
@@ -632,10 +632,11 @@ __global__ void __launch_bounds__(kPartThreads, 2) score_blocks_kernel(const Sel
 }
 
 // All of a row (a token's kv head) in one CTA: as score_blocks_kernel with the row's pages as items, kPart at a time, and one
-// kv head's queries for all of them; the keys stay in shared memory, and the largest are found where the ring was.
-constexpr int kRowPages = 1024;  // that a row may have
+// kv head's queries for all of them; the keys stay in shared memory, and the largest are found where the pages were.  One
+// place for pages and four CTAs to an SM: what one waits for, the others cover (64 ragged tokens 23.5 us; two places and three
+// CTAs 25.4, three and two 27.7).
+constexpr int kRowPages = 4096;  // that a row may have
 constexpr int kRowGroup = 16;    // and query heads
-constexpr int kRowStages = 2;
 
 struct RowScoring {
     alignas(16) float t[kRowGroup];
@@ -647,11 +648,11 @@ struct RowScoring {
 template <int kDim>
 constexpr int kRowQueries = Tile<kDim>::kPanels * kRowGroup * 128;  // a multiple of 1024
 template <int kDim>
-constexpr int kRowBytes = 1024 + kRowStages * Tile<kDim>::kBytes + kRowQueries<kDim> + kRowPages * 4 + static_cast<int>(sizeof(RowScoring));
-static_assert((kRowBytes<128> + 1024) * 3 <= 228 * 1024, "three CTAs to an SM");
+constexpr int kRowBytes = 1024 + Tile<kDim>::kBytes + kRowQueries<kDim> + static_cast<int>(sizeof(RowScoring));  // and the keys
+static_assert((kRowBytes<128> + kRowPages * 4 + 1024) * 4 <= 228 * 1024, "four CTAs to an SM");
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kPartThreads, 3) select_rows_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(kPartThreads, 4) select_rows_kernel(const SelectArgs a) {
     using namespace attn;
     using Tl = Tile<kDim>;
     extern __shared__ char smem[];
@@ -661,11 +662,11 @@ __global__ void __launch_bounds__(kPartThreads, 3) select_rows_kernel(const Sele
     const uint32_t tiles = (smem_addr(smem) + 1023) & ~1023u;
     char* base = smem + (tiles - smem_addr(smem));
     const int columns = columns_of(a.group);
-    char* q8 = base + kRowStages * Tl::kBytes;  // columns rows of 128 bytes, panel by panel
-    uint32_t* keys = reinterpret_cast<uint32_t*>(q8 + kRowQueries<kDim>);
-    RowScoring& sh = *reinterpret_cast<RowScoring*>(keys + kRowPages);
+    char* q8 = base + Tl::kBytes;  // columns rows of 128 bytes, panel by panel
+    RowScoring& sh = *reinterpret_cast<RowScoring*>(q8 + kRowQueries<kDim>);
+    uint32_t* keys = reinterpret_cast<uint32_t*>(&sh + 1);  // no more than the table has blocks: what is left is L1's
     topk::Shared& s = *reinterpret_cast<topk::Shared*>(base);
-    static_assert(sizeof(topk::Shared) <= kRowStages * Tl::kBytes, "where the ring was");
+    static_assert(sizeof(topk::Shared) <= Tl::kBytes, "where the pages were");
 
     const Queries<T, kDim> queries(a, token, head * a.group, a.group);
     const uint2 query = loads ? queries.load(warp) : make_uint2(0, 0);  // beside what follows
@@ -705,7 +706,7 @@ __global__ void __launch_bounds__(kPartThreads, 3) select_rows_kernel(const Sele
             // a thread has 16 bytes (of each 128) of 8 pages, whose numbers are looked up an item ahead
             const int8_t* from = a.summary.bounds + head * a.summary.bounds_head_stride + (tid & 7) * 16;
             const uint32_t to = tiles + (tid >> 3) * 128 + (((tid & 7) ^ ((tid >> 3) & 7)) << 4);
-            int page[kPart / 16], item = 0, stage = 0;
+            int page[kPart / 16], item = 0;
             const auto look = [&] {
 #pragma unroll
                 for (int x = 0; x < kPart / 16; ++x) page[x] = page_of(a, r, item * kPart + 16 * x + (tid >> 3));
@@ -719,15 +720,13 @@ __global__ void __launch_bounds__(kPartThreads, 3) select_rows_kernel(const Sele
 #pragma unroll
                         for (int b = 0; b < Tl::kPanels; ++b)
                             if (128 * (b + 1) <= 2 * kDim || (tid & 7) < (2 * kDim % 128) / 16)
-                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + stage * Tl::kBytes + b * Tl::kPanel + x * 2048),
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + b * Tl::kPanel + x * 2048),
                                              "l"(src + b * 128), "r"(size)
                                              : "memory");
                     }
-                    if (++stage == kRowStages) stage = 0;
                     ++item;
                     look();
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
             };
             look();
             bring();
@@ -742,13 +741,13 @@ __global__ void __launch_bounds__(kPartThreads, 3) select_rows_kernel(const Sele
                 if (lane == 0) sh.t[row] = t;
             });
             for (int x = 0; x < items; ++x) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kRowStages - 2) : "memory");
+                asm volatile("cp.async.wait_all;" ::: "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 late = __syncthreads_or(late);
-                if (x > 0) wait(x - 1);
-                bring();  // where item x - 1 was
+                wait(x);
+                bring();  // where item x was
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            asm volatile("cp.async.wait_all;" ::: "memory");
         } else {
             const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) << 21);
             const float* scales = a.summary.scale + head * a.summary.scale_head_stride;
@@ -784,7 +783,6 @@ __global__ void __launch_bounds__(kPartThreads, 3) select_rows_kernel(const Sele
                     most = max(most, key);
                 }
             };
-            int stage = 0;
             // all of a warp's lanes walk along, so that addresses stay in uniform registers; one issues
             const bool issues = warp == 0 && elect_one();
             const uint32_t tm = uniform(tmem), pages_low = uniform(operand_low(tiles, 16)), q_low = uniform(operand_low(smem_addr(q8), 16));
@@ -794,22 +792,20 @@ __global__ void __launch_bounds__(kPartThreads, 3) select_rows_kernel(const Sele
                 late = __syncthreads_or(late);
                 tmem_fence_after();
                 if (warp == 0 && !late) {
-                    const uint32_t page_low = uniform(pages_low + stage * (Tl::kBytes / 16)), d = uniform(tm + (x & 1) * kSlice);
+                    const uint32_t d = uniform(tm + (x & 1) * kSlice);
                     if (issues) {
 #pragma unroll
                         for (int k = 0; k < 2 * kDim / 32; ++k)
-                            mma_smem_s8(d, page_low + ((k >> 2) * Tl::kPanel + (k & 3) * 32) / 16, q_low + (k >> 2) * q_panel + (k & 3) * 2, desc, k > 0);
+                            mma_smem_s8(d, pages_low + ((k >> 2) * Tl::kPanel + (k & 3) * 32) / 16, q_low + (k >> 2) * q_panel + (k & 3) * 2, desc, k > 0);
                         mma_commit(&sh.done[x & 1]);
                     }
                     __syncwarp();
                 }
-                if (++stage == kRowStages) stage = 0;
-                if (x > 0) finish(x - 1);
+                finish(x);
             }
-            finish(items - 1);
             tmem_fence_before();
         }
-        // products end before the ring is used for something else and the CTA ends, also after a wait that ran out
+        // products end before their place is used for something else and the CTA ends, also after a wait that ran out
         late = __syncthreads_or(late);
         if (threadIdx.x == 0 && late) {
             mma_commit(&sh.drain);
@@ -880,7 +876,7 @@ __global__ void __launch_bounds__(kRowThreads) choose_blocks_kernel(const Select
 
 constexpr int kMaxSmem = 224 * 1024;
 // Which kernels take a call, measured with 32 heads on 8 of dim 128, us: as many rows as SMs and up to kRowPages blocks of
-// the table, a CTA of the tensor cores to each (64 tokens of 62 / 243 / 937 blocks 10 / 14 / 38; in threads 11 / 18 / 54).
+// the table, a CTA of the tensor cores to each (64 tokens of 62 / 243 / 937 blocks 9 / 12 / 28; in threads 11 / 18 / 54).
 // Fewer rows and up to kShort blocks, a CTA of threads to each (16 tokens 5.7 / 6.9, one 5.3 / 6.2; two kernels 6.9 / 8.8
 // and 6.4 / 6.6).  Else two kernels (16 tokens of 937 16, in threads 20; one 8.1, in threads 15).
 constexpr int kShort = 256;
@@ -913,7 +909,7 @@ cudaError_t launch_select(const SelectArgs& a, cudaStream_t stream) {
         static SmemOnce once;
         const cudaError_t e = once.set(reinterpret_cast<const void*>(select_rows_kernel<T, kDim>), kMaxSmem);
         if (e != cudaSuccess) return e;
-        select_rows_kernel<T, kDim><<<rows, kPartThreads, kRowBytes<kDim>, stream>>>(a);
+        select_rows_kernel<T, kDim><<<rows, kPartThreads, kRowBytes<kDim> + a.req.table_width * 4, stream>>>(a);
         return cudaGetLastError();
     }
     if (!a.scores) {

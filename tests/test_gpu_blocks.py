@@ -130,6 +130,8 @@ SELECTIONS = [
     ([290] * 40, [1] * 40, 12, 4, 96, 1, "fp16"),       # the same, more than 256 pages
     ([2300, 100] * 10, [1] * 20, 128, 8, 128, 8, "bf16"),
     ([280] * 80, [1] * 80, 40, 2, 64, 1, "bf16"),       # many rows of many heads
+    ([4000] + [50] * 18, [1] * 19, 8, 8, 96, 1, "bf16"),  # many rows of as many pages as one CTA takes
+    ([4200] + [10] * 18, [1] * 19, 8, 8, 64, 1, "fp16"),   # and of more
 ]
 
 
