@@ -422,7 +422,9 @@ int fg_select_blocks_workspace_bytes(const fg_kv_summary* summary, const fg_bloc
  * a request is its positions [x * page_size, (x + 1) * page_size), the page
  * block_table[x].  Blocks with a key that window and first tokens do not show
  * (a position >= sinks and <= p - window) are chosen from; those without a page
- * in the cache are not.  The score is in the 8-bit arithmetic of the summary:
+ * in the cache are not.  A block's score is that of all keys that were summed
+ * up, later tokens of the same step among them (the attention reads none of
+ * those).  The score is in the 8-bit arithmetic of the summary:
  * with top the largest |q_d| of a query head, Q_d = q_d * 127 / top rounded to
  * the nearest whole number and t = top times the 32-bit number nearest 1 / 127,
  *   score = max over the kv head's query heads of
