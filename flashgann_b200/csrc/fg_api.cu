@@ -1121,6 +1121,11 @@ extern "C" __attribute__((visibility("default"))) void fg_test_key_weights_lose_
     fg::set_key_weights_waits(first, tries);
 }
 
+// For tests only: the place that the search for a row's request ends at, of n of which those from `first` on are past it.
+extern "C" __attribute__((visibility("default"))) int32_t fg_test_first_past(int32_t n, int32_t first) {
+    return fg::first_past_on_host(n, first);
+}
+
 int fg_paged_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream) {
     g_err.clear();
     return attention(cache, args, kMask, stream);

@@ -69,19 +69,33 @@ constexpr float k127th = 1.f / 127.f;  // a product, rounded once: what a quotie
 
 __device__ __forceinline__ int clamped(const int32_t* p, int most) { return max(0, min(__ldg(p), most)); }
 
+// Places [lo, lo + n), the first of which that is past something is looked for: in 32 runs of them at once.
+struct Span {
+    int lo, n;
+    __host__ __device__ __forceinline__ int run() const { return (n + 31) / 32; }
+    // whether run x ends with a place that is past, or with the last place of all or behind it: of such runs the first has
+    // places, and if none is past, the last place
+    template <typename Past>
+    __host__ __device__ __forceinline__ bool ends(int x, const Past& past) const {
+        const int at = lo + (x + 1) * run() - 1;
+        return at >= lo + n - 1 || past(at);
+    }
+    __host__ __device__ __forceinline__ void take(int x) {
+        const int first = x * run();
+        n = n - first < run() ? n - first : run();
+        lo += first;
+    }
+};
+
 // The first of n ascending places that is past something, or the last: 32 at a time, by whole warps.
 template <typename Past>
-__device__ __forceinline__ int first_past(int n, Past past) {
-    const int lane = threadIdx.x & 31;
-    int lo = 0;
-    while (n > 1) {
-        const int step = (n + 31) / 32, at = lo + (lane + 1) * step - 1;
-        const uint32_t is = __ballot_sync(0xFFFFFFFFu, at >= lo + n || past(min(at, lo + n - 1)));
-        const int f = is ? __ffs(is) - 1 : 31;
-        n = min(step, n - f * step);
-        lo += f * step;
+__device__ __forceinline__ int first_past(int n, const Past& past) {
+    Span s = {0, n};
+    while (s.n > 1) {
+        const uint32_t is = __ballot_sync(0xFFFFFFFFu, s.ends(threadIdx.x & 31, past));  // never 0: run 31 ends behind n - 2
+        s.take(__ffs(is) - 1);
     }
-    return lo;
+    return s.lo;
 }
 
 // ---- summary ----
@@ -957,6 +971,20 @@ cudaError_t summarize_by_dim(const SummarizeArgs& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+int first_past_on_host(int n, int first) {
+    struct Past {
+        int first;
+        __host__ __device__ bool operator()(int x) const { return x >= first; }
+    };
+    Span s = {0, n};
+    while (s.n > 1) {
+        int x = 0;
+        while (!s.ends(x, Past{first})) ++x;
+        s.take(x);
+    }
+    return s.lo;
+}
 
 bool select_counts(int tokens, int kv_heads, int table_width) {
     return static_cast<int64_t>(tokens) * kv_heads <= INT32_MAX && static_cast<int64_t>(tokens) * (table_width / kPart + 1) <= INT32_MAX &&

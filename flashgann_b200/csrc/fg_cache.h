@@ -30,6 +30,9 @@ struct Summary {
     int64_t bounds_page_stride = 0, bounds_head_stride = 0, scale_page_stride = 0, scale_head_stride = 0;
 };
 
+// For tests: the search by which a row's or a page's request is found, where `first` and all after it are past.
+int first_past_on_host(int n, int first);
+
 struct SummarizeArgs {
     PagedRows cache;
     Summary summary;
