@@ -1335,10 +1335,12 @@ int fg_attention_weights_device(const fg_kv_cache* cache, const fg_attention* x,
     if (!x) return fail(FG_ERR_ARG, "null arguments");
     if ((rc = check_counts(cache, x, kMask))) return rc;
     if ((rc = check_weights(cache, d_weights, weights_page_stride, weights_head_stride))) return rc;
-    if (x->tokens == 0 || x->requests == 0) return FG_OK;
-    if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, x->tokens, x->heads, "q"))) return rc;
-    if (!x->lse) return fail(FG_ERR_ARG, "null lse");
-    if ((rc = check_requests(x->block_table, x->table_width, x->table_stride, x->query_start, x->kv_len, x->requests, x->tokens))) return rc;
+    if (x->requests == 0 || (x->tokens == 0 && !d_held)) return FG_OK;  // without tokens, weights past `held` still start at 0
+    if (x->tokens > 0) {
+        if ((rc = check_rows(x->q, x->q_token_stride, x->q_head_stride, x->tokens, x->heads, "q"))) return rc;
+        if (!x->lse) return fail(FG_ERR_ARG, "null lse");
+    }
+    if ((rc = check_requests(x->block_table, x->table_width, x->table_stride, x->query_start, x->kv_len, x->requests, std::max(x->tokens, 1)))) return rc;
     fg::AttentionParams a = params(cache, x);
     fg::WeightsArgs w;
     w.weights = key_weights(d_weights, weights_page_stride, weights_head_stride);

@@ -100,7 +100,8 @@ __device__ __forceinline__ int div_group(const AttentionParams& a, int n) {
 //   kTokens  the group's heads of as many tokens as fit kRows rows
 //   kToken   one token, tile_rows heads of the group (what each head retrieved is its own)
 //   kChosen  the same, of which all rows see the token's chosen pages
-//   kWhole   all rows of the request; the keys that any of them sees, and those that have no weight yet
+//   kWhole   all rows of the request; the keys that any of them sees, and those that have no weight yet (also where there
+//            are no rows)
 enum Layout { kPacked, kTokens, kToken, kChosen, kWhole };
 
 template <int kRows, Layout kLayout>
@@ -112,7 +113,7 @@ struct Tiles {
     }
     __device__ static __forceinline__ int count(const AttentionParams& a, const Request& r) {
         if (kOne) return r.rows * per(a);
-        if (kLayout == kWhole) return r.rows > 0;
+        if (kLayout == kWhole) return r.rows > 0 || (a.held && a.held[r.index] < r.kv_len);
         if (kLayout == kTokens) return (r.rows + per(a) - 1) / per(a);
         return (r.rows * a.group + kRows - 1) / kRows;
     }
@@ -159,9 +160,12 @@ __device__ __forceinline__ TileKeys tile_keys(const AttentionParams& a, const Re
     const int64_t room = min(static_cast<int64_t>(a.table_width) * a.page_size, static_cast<int64_t>(INT32_MAX - 1023));
     k.hi = p1 < 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(p1) + 1, room));
     k.lo = (a.window < 0 || p0 < a.window) ? 0 : min(p0 - a.window + 1, k.hi);
-    if (kLayout == kWhole) k.lo = min(k.lo, a.held ? max(0, a.held[r.index]) : max(0, p0));
+    if (kLayout == kWhole) {
+        const int held = a.held ? max(0, a.held[r.index]) : max(0, p0);
+        k.lo = min(r.rows > 0 ? k.lo : k.hi, held);
+    }
     k.base = k.lo & -a.base_align;
-    k.sink_hi = min(a.sinks, k.base);
+    k.sink_hi = kLayout == kWhole && r.rows == 0 ? 0 : min(a.sinks, k.base);
     k.sink_chunks = (k.sink_hi + kChunk - 1) / kChunk;
     k.near_chunks = (k.hi - k.base + kChunk - 1) / kChunk;
     k.id_chunks = 0;
@@ -337,7 +341,7 @@ __device__ __forceinline__ bool next_tile(const AttentionParams& a, Request* r, 
             if (++*head == a.kv_heads) return false;
         }
         *r = load_request(a, *request);
-    } while (r->rows == 0);
+    } while (kLayout == kWhole ? Tiles<kRows, kLayout>::count(a, *r) == 0 : r->rows == 0);
     return true;
 }
 

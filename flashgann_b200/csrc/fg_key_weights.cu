@@ -21,6 +21,9 @@
 // 256 rows on 8192 keys took 38 us; with 128 rows at a time and a thread to a key
 // 20.)  Blocks are split over the CTAs as in fg_attention.cuh.
 //
+// A request without rows has its keys from `held` on set to 0 by one walk over them,
+// in which no row adds anything (its queries are zeros).
+//
 // Waits for products are bounded: one that runs out ends the CTA's work, with NaN
 // in the keys that are left.
 #include <algorithm>
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
         const T* k_head = static_cast<const T*>(a.k_cache) + head * a.head_stride;
         float* w_head = w.weights.w + head * w.weights.head_stride;
         const auto first_key = [&](int c) { return c < keys.sink_chunks ? c * kBlock : keys.base + (c - keys.sink_chunks) * kBlock; };
-        for (int g0 = 0; c0 < c1 && g0 < rows; g0 += kMany) {
+        for (int g0 = 0; c0 < c1 && g0 < max(rows, 1); g0 += kMany) {
             const int n = min(rows - g0, kMany), columns = n <= 16 ? 16 : (n + 31) & ~31;
             constexpr int panel = kMany * 128;  // of the queries
             const uint32_t queries = tiles + R::kTile, desc = uniform(instruction<T>(0, false) | (static_cast<uint32_t>(columns >> 3) << 17));
@@ -159,14 +162,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_weights_kernel
             __syncthreads();  // the blocks before are done with
             int page = find(c0), next = find(c0 + 1);
             for (int x = tid; x < columns * (kDim / 8); x += kThreads) {
-                const int at = x / (kDim / 8), piece = x % (kDim / 8), i = div_group(a, g0 + min(at, n - 1));
+                const int at = x / (kDim / 8), piece = x % (kDim / 8), i = div_group(a, g0 + max(0, min(at, n - 1)));
                 const T* src = static_cast<const T*>(a.q) + static_cast<int64_t>(r.start + i) * a.q_token_stride +
                                static_cast<int64_t>(head * a.group + g0 + min(at, n - 1) - i * a.group) * a.q_head_stride + piece * 8;
-                copy16(queries + (piece >> 3) * panel + at * 128 + (((piece & 7) ^ (at & 7)) << 4), src, true);
+                copy16(queries + (piece >> 3) * panel + at * 128 + (((piece & 7) ^ (at & 7)) << 4), n > 0 ? src : k_head, n > 0);
             }
             for (int x = tid; x < columns; x += kThreads) {
-                const int i = div_group(a, g0 + min(x, n - 1));
-                const float l = __ldg(w.lse + static_cast<int64_t>(r.start + i) * a.heads + head * a.group + g0 + min(x, n - 1) - i * a.group);
+                const int i = div_group(a, g0 + max(0, min(x, n - 1)));
+                const float l =
+                    n > 0 ? __ldg(w.lse + static_cast<int64_t>(r.start + i) * a.heads + head * a.group + g0 + min(x, n - 1) - i * a.group) : INFINITY;
                 const bool adds = x < n && isfinite(l);
                 sh.lse[x] = adds ? l : INFINITY;
                 sh.p[x] = adds ? p0 + i : -1;
@@ -343,7 +347,7 @@ struct FewShared {
     alignas(16) int p[kStages + 2][kFew];      // and their positions; -1 there
     // of the block that is brought next and the one behind it; in elements
     int64_t row[2][kBlock];     // where a key's row begins; -1: it is not there
-    int64_t query[2][kFew];     // and a query's, where the block is the first of its segment
+    int64_t query[2][kFew];     // and a query's, where the block is the first of its segment; -1: there is none
     int opens[2];
     uint64_t done[2];
     uint64_t drain;
@@ -402,10 +406,12 @@ __global__ void __launch_bounds__(2 * kBlock, kCtasPerSm) attention_weights_few_
             if (tid == 0) sh.opens[told & 1] = at.opens;
             if (at.opens && ++segment == Sh::kStages + 2) segment = 0;
             if (at.opens && tid < kFew) {
-                const int n = at.g0 + min(tid, min(kFew, at.rows - at.g0) - 1), i = div_group(a, n), g = n - i * a.group;  // the last row again past the end
-                const float l = __ldg(w.lse + static_cast<int64_t>(at.r.start + i) * a.heads + at.head * a.group + g);
+                // the last row again past the end
+                const int n = max(0, at.g0 + min(tid, min(kFew, at.rows - at.g0) - 1)), i = div_group(a, n), g = n - i * a.group;
+                const float l = at.rows > 0 ? __ldg(w.lse + static_cast<int64_t>(at.r.start + i) * a.heads + at.head * a.group + g) : INFINITY;
                 const bool adds = at.g0 + tid < at.rows && isfinite(l);
-                sh.query[told & 1][tid] = static_cast<int64_t>(at.r.start + i) * a.q_token_stride + static_cast<int64_t>(at.head * a.group + g) * a.q_head_stride;
+                sh.query[told & 1][tid] =
+                    at.rows > 0 ? static_cast<int64_t>(at.r.start + i) * a.q_token_stride + static_cast<int64_t>(at.head * a.group + g) * a.q_head_stride : -1;
                 sh.lse[segment][tid] = adds ? l : INFINITY;
                 sh.p[segment][tid] = adds ? at.r.kv_len - at.r.rows + i : -1;
             }
@@ -420,8 +426,9 @@ __global__ void __launch_bounds__(2 * kBlock, kCtasPerSm) attention_weights_few_
 #pragma unroll
                     for (int x = tid; x < kFew * (kDim / 8); x += kBlock) {
                         const int row = x / (kDim / 8), piece = x % (kDim / 8);
+                        const int64_t query = sh.query[brought & 1][row];
                         copy16(queries + q_slot * R::kQuery + (piece >> 3) * (kFew * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4),
-                               static_cast<const T*>(a.q) + sh.query[brought & 1][row] + piece * 8, !late);
+                               query >= 0 ? static_cast<const T*>(a.q) + query + piece * 8 : from, query >= 0 && !late);
                     }
                 }
 #pragma unroll

@@ -462,7 +462,8 @@ int fg_block_attention_device(const fg_kv_cache* cache, const fg_attention* args
  * step's attention left it), block_table, query_start, kv_len, window, sinks,
  * scale and the counts; out, ids, workspace and max_new are not looked at.
  * d_held [requests]: tokens whose weights are there already (NULL: those before
- * the new ones); weights from there to kv_len[b] start at 0, whatever was there.
+ * the new ones); weights from there to kv_len[b] start at 0, whatever was there,
+ * also of requests without new tokens, and in a call without any.
  * Rows whose lse is not finite add nothing.  Sums are 32 bits, in the order of
  * the rows: the same bits on every run, but where requests share a page, whose
  * sums are added to it in any order (of shared pages none may be new).  Only the last tokens of a prompt may be
