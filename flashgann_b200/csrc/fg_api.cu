@@ -1121,6 +1121,11 @@ extern "C" __attribute__((visibility("default"))) void fg_test_key_weights_lose_
     fg::set_key_weights_waits(first, tries);
 }
 
+// And of the selection's kernels of the tensor cores: products of a CTA are not issued from item `first` on (-2 in its rows).
+extern "C" __attribute__((visibility("default"))) void fg_test_selection_lose_items(int32_t first, int32_t tries) {
+    fg::set_selection_waits(first, tries);
+}
+
 // For tests only: the place that the search for a row's request ends at, of n of which those from `first` on are past it.
 extern "C" __attribute__((visibility("default"))) int32_t fg_test_first_past(int32_t n, int32_t first) {
     return fg::first_past_on_host(n, first);

@@ -365,6 +365,20 @@ struct Pages {
     }
 };
 
+// A wait for products that runs out leaves its row's pages without scores.  Their keys say so (order_key gives none between
+// kNone and that of -inf), and the whole list is -2 then: a shorter one, or another, would look like a choice.
+constexpr uint32_t kLostKey = 1;
+constexpr int32_t kLostBlock = -2;
+struct Limits {
+    int tries, lost;  // of waits; item from which on no products are issued (none: INT32_MAX)
+};
+
+// The list of a row whose scores are lost, by all threads.
+__device__ __forceinline__ void give_up(const SelectArgs& a, int token, int head) {
+    int32_t* out = a.blocks + token * a.blocks_token_stride + head * a.blocks_head_stride;
+    for (int x = threadIdx.x; x < a.count; x += static_cast<int>(blockDim.x)) out[x] = kLostBlock;
+}
+
 // The largest keys of a row to its place in the result.
 template <int kRowThreads, typename Keys>
 __device__ __forceinline__ void choose(const SelectArgs& a, topk::Shared& s, const Row& r, int token, int head, topk::Threshold thr, const Keys& keys) {
@@ -455,10 +469,9 @@ int scoring_bytes(int group) {
 // its pages.  Pages are lanes of TMEM, the queries its columns: a thread of the first four warps has a page's scores to
 // itself.  The other four bring the items: pages' bounds by cp.async and rounded queries, into the 128-byte swizzled layout
 // and a ring of kStages.  Between two barriers one item's products run, the scores of the one before are read, and its place
-// is filled again.  (One warp after the other for all of it: 700 instructions, 2.2 us to an item.)  A wait for products that
-// runs out leaves the keys of pages that are not there.
+// is filled again.  (One warp after the other for all of it: 700 instructions, 2.2 us to an item.)
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kPartThreads, 2) score_blocks_kernel(const SelectArgs a, int heads_each) {
+__global__ void __launch_bounds__(kPartThreads, 2) score_blocks_kernel(const SelectArgs a, int heads_each, const Limits limits) {
     using namespace attn;
     using Tl = Tile<kDim>;
     extern __shared__ char smem[];
@@ -499,7 +512,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) score_blocks_kernel(const Sel
     const auto wait = [&](int item) {  // for its products
         if (late) return;
         for (int k = 0; !bar_try(&sh.done[item & 1], (item >> 1) & 1); ++k)
-            if (k >= kTries) {
+            if (k >= limits.tries) {
                 late = true;
                 break;
             }
@@ -598,7 +611,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) score_blocks_kernel(const Sel
             tmem_fence_before();
             t_slot = (t_slot + 1) % (kStages + 1);
             if (last) {
-                if (i < n) *out = page < 0 || late ? topk::kNone : topk::order_key(scale == INFINITY ? INFINITY : __fmul_rn(best, scale));
+                if (i < n) *out = late ? kLostKey : page < 0 ? topk::kNone : topk::order_key(scale == INFINITY ? INFINITY : __fmul_rn(best, scale));
                 out += a.req.table_width;
                 best = -INFINITY;
                 scale = next;
@@ -617,7 +630,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) score_blocks_kernel(const Sel
             tmem_fence_before();
             late = __syncthreads_or(late);
             tmem_fence_after();
-            if (warp == 0 && !late) {
+            if (warp == 0 && !late && x < limits.lost) {
                 const uint32_t page_low = uniform(pages_low + stage * (Tl::kBytes / 16)), q_low = uniform(queries_low + stage * q_step);
                 const uint32_t d = uniform(tm + (x & 1) * kSlice);
                 if (issues) {
@@ -666,7 +679,7 @@ constexpr int kRowBytes = 1024 + Tile<kDim>::kBytes + kRowQueries<kDim> + static
 static_assert((kRowBytes<128> + kRowPages * 4 + 1024) * 4 <= 228 * 1024, "four CTAs to an SM");
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(kPartThreads, 4) select_rows_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(kPartThreads, 4) select_rows_kernel(const SelectArgs a, const Limits limits) {
     using namespace attn;
     using Tl = Tile<kDim>;
     extern __shared__ char smem[];
@@ -710,7 +723,7 @@ __global__ void __launch_bounds__(kPartThreads, 4) select_rows_kernel(const Sele
         const auto wait = [&](int item) {  // for its products
             if (late) return;
             for (int k = 0; !bar_try(&sh.done[item & 1], (item >> 1) & 1); ++k)
-                if (k >= kTries) {
+                if (k >= limits.tries) {
                     late = true;
                     break;
                 }
@@ -791,7 +804,7 @@ __global__ void __launch_bounds__(kPartThreads, 4) select_rows_kernel(const Sele
                     }
                 tmem_fence_before();
                 if (i < r.n) {
-                    const uint32_t key = now < 0 || late ? topk::kNone : topk::order_key(by == INFINITY ? INFINITY : __fmul_rn(best, by));
+                    const uint32_t key = now < 0 ? topk::kNone : topk::order_key(by == INFINITY ? INFINITY : __fmul_rn(best, by));
                     keys[i] = key;
                     least = min(least, key);
                     most = max(most, key);
@@ -805,7 +818,7 @@ __global__ void __launch_bounds__(kPartThreads, 4) select_rows_kernel(const Sele
                 tmem_fence_before();
                 late = __syncthreads_or(late);
                 tmem_fence_after();
-                if (warp == 0 && !late) {
+                if (warp == 0 && !late && x < limits.lost) {
                     const uint32_t d = uniform(tm + (x & 1) * kSlice);
                     if (issues) {
 #pragma unroll
@@ -829,6 +842,7 @@ __global__ void __launch_bounds__(kPartThreads, 4) select_rows_kernel(const Sele
         topk::clear<kPartThreads>(s);
         __syncthreads();
         if (threadIdx.x < 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmem) : "memory");
+        if (late) return give_up(a, token, head);
         topk::range(s, least, most);
         __syncthreads();
         thr = topk::threshold<kPartThreads, topk::One>(s, r.n, a.count, topk::read_keys<kPartThreads>([&](int i) { return keys[i]; }));
@@ -851,8 +865,9 @@ __global__ void __launch_bounds__(kRowThreads) choose_blocks_kernel(const Select
     const uint32_t* scores = a.scores + (static_cast<int64_t>(token) * a.kv_heads + head) * a.req.table_width;
     const auto read = [&](int i) { return scored ? __ldcg(scores + i) : page_of(a, r, i) >= 0 ? 1u : topk::kNone; };
     uint32_t least = 0xFFFFFFFFu, most = 0;
+    bool lost = false;
     const auto all = [&](const auto& keys) {
-        __syncthreads();
+        if (__syncthreads_or(lost && scored)) return give_up(a, token, head);
         topk::Threshold thr = {0, 0};
         if (scored) {
             topk::range(s, least, most);
@@ -874,6 +889,7 @@ __global__ void __launch_bounds__(kRowThreads) choose_blocks_kernel(const Select
             if (g.first + 32 * x + static_cast<int>(threadIdx.x & 31) < g.last) {
                 least = min(least, keys.k[x]);
                 most = max(most, keys.k[x]);
+                lost = lost || keys.k[x] == kLostKey;
             }
         all(keys);
     } else {
@@ -883,10 +899,13 @@ __global__ void __launch_bounds__(kRowThreads) choose_blocks_kernel(const Select
             if (i < room) near[i] = key;
             least = min(least, key);
             most = max(most, key);
+            lost = lost || key == kLostKey;
         }
         all(topk::read_keys<kRowThreads>([&](int i) { return i < room ? near[i] : read(i); }));
     }
 }
+
+Limits g_limits = {kTries, INT32_MAX};
 
 constexpr int kMaxSmem = 224 * 1024;
 // Which kernels take a call, measured with 32 heads on 8 of dim 128, us: as many rows as SMs and up to kRowPages blocks of
@@ -923,7 +942,7 @@ cudaError_t launch_select(const SelectArgs& a, cudaStream_t stream) {
         static SmemOnce once;
         const cudaError_t e = once.set(reinterpret_cast<const void*>(select_rows_kernel<T, kDim>), kMaxSmem);
         if (e != cudaSuccess) return e;
-        select_rows_kernel<T, kDim><<<rows, kPartThreads, kRowBytes<kDim> + a.req.table_width * 4, stream>>>(a);
+        select_rows_kernel<T, kDim><<<rows, kPartThreads, kRowBytes<kDim> + a.req.table_width * 4, stream>>>(a, g_limits);
         return cudaGetLastError();
     }
     if (!a.scores) {
@@ -943,7 +962,7 @@ cudaError_t launch_select(const SelectArgs& a, cudaStream_t stream) {
     int each = a.kv_heads;
     while (each > 1 && static_cast<int64_t>(a.req.tokens) * parts * ((a.kv_heads + (each + 1) / 2 - 1) / ((each + 1) / 2)) <= 2 * a.sms) each = (each + 1) / 2;
     const dim3 grid(a.req.tokens * parts, static_cast<unsigned>((a.kv_heads + each - 1) / each));
-    score_blocks_kernel<T, kDim><<<grid, kPartThreads, scoring_bytes<kDim>(a.group), stream>>>(a, each);
+    score_blocks_kernel<T, kDim><<<grid, kPartThreads, scoring_bytes<kDim>(a.group), stream>>>(a, each, g_limits);
     const cudaError_t started = cudaGetLastError();
     if (started != cudaSuccess) return started;
     if (a.req.table_width <= 1024) return launch_choose<256, 4>(a, rows, stream);
@@ -971,6 +990,8 @@ cudaError_t summarize_by_dim(const SummarizeArgs& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+void set_selection_waits(int lost, int tries) { g_limits = {tries < 0 ? kTries : tries, lost < 0 ? INT32_MAX : lost}; }
 
 int first_past_on_host(int n, int first) {
     struct Past {

@@ -52,6 +52,7 @@ struct SelectArgs {
     uint32_t* scores = nullptr;  // workspace
     int sms = 0;
 };
+void set_selection_waits(int lost_item, int tries);  // for tests; below 0: none, and a limit of a second
 bool select_counts(int tokens, int kv_heads, int table_width);  // whether a launch can have so many CTAs
 size_t select_workspace(int tokens, int kv_heads, int table_width);  // 0 where the scores stay in shared memory
 cudaError_t launch_select_blocks(const SelectArgs& a, cudaStream_t stream);

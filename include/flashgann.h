@@ -432,7 +432,9 @@ int fg_select_blocks_workspace_bytes(const fg_kv_summary* summary, const fg_bloc
  * the products after the sum in 32 bits (a bound of q.k, so for attention with a
  * positive scale); a query head with a value that is not finite counts as 0, a
  * page of scale inf has the score inf.  Of equal scores the lowest block comes
- * first.  The same bits on every run.  The last axis of blocks is contiguous.
+ * first.  The same bits on every run.  Waits inside a kernel are bounded: one
+ * that runs out (a second; a sound device has none) leaves -2 in all of its
+ * row's places.  The last axis of blocks is contiguous.
  * Rows past query_start[requests] are not written.  Needs a window >= 0 and
  * heads / summary->heads <= 256. */
 int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selection* args, void* stream);
