@@ -185,15 +185,35 @@ __global__ void __launch_bounds__(kThreads, 2) kv_evict_kernel(const EvictArgs a
     }
 }
 
+// CTAs to a row, by what its table holds at most (a row's length is not known here): one for up to 640 positions, four for up
+// to 2048, then as many as there are SMs for.  us with 8 kv heads of 128 of one request, few rows move / all move.  (Over this,
+// 2 heads of 64, and four requests of 8 heads of 96, four CTAs take 1.06 of one's time at 480 and 520 positions, 1.01 at 640,
+// 0.98 at 670 and 740, 0.93 at 800.)
+//     positions    1             4             8
+//     480          9.9 / 13.2    10.2 / 13.0   11.4 / 14.5
+//     640          11.2 / 15.9   11.2 / 14.8   11.9 / 16.5
+//     800          12.2 / 16.1   11.5 / 13.8   12.3 / 17.2
+//     1100         15.1 / 21.6   12.3 / 16.0   12.2 / 17.5
+//     1800         16.3 / 26.1   13.7 / 19.1   13.2 / 19.4
+//     2200         25.3 / 39.2   18.2 / 23.0   17.8 / 20.1
+//     16000        42.1 / 69.0   23.8 / 33.7   20.1 / 27.6
+// Two CTAs pay for the cluster and gain little: 64 rows, one / two, 800 positions 12.5 / 14.7 (all move 19.3 / 20.5), 1100 15.5
+// / 17.4 (26.9 / 27.5), 2200 25.6 / 27.0 (57 / 48), 4000 34.7 / 34.8 (87 / 70).  More CTAs than SMs: 32 rows of 1100 positions
+// 18.1 with four CTAs, 34.4 with eight.
+constexpr int kOneCta = 640, kFourCtas = 2048;
+int row_ctas(int64_t rows, int64_t most, int sms) {
+    if (most <= kOneCta) return 1;
+    if (most <= kFourCtas) return rows * 4 <= sms ? 4 : 1;
+    int ranks = 1;
+    while (ranks < kMaxCluster && rows * ranks * 2 <= sms) ranks *= 2;
+    return ranks;
+}
+
 template <int kDim>
 cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.requests) * a.cache.heads;
     const int64_t most = std::min<int64_t>(static_cast<int64_t>(a.table_width) << a.cache.page_shift, INT32_MAX);
-    int ranks = 1;
-    // CTAs to a row: one for up to 640 positions, else as many as there are SMs for, with 256 positions each.  us with 8 kv
-    // heads of one request, 1 / 4 or 8: 576 positions 15.4 / 15.0 (few moves 14.3 / 16.4), 1100 27.2 / 20.6, 2200 43 / 25; of
-    // four requests of 1100 27.7 / 20.4 (more CTAs than SMs: 34)
-    while (ranks < kMaxCluster && rows * ranks * 2 <= a.sms && most > 640 && most > 256 * ranks) ranks *= 2;
+    const int ranks = row_ctas(rows, most, a.sms);
     constexpr int kRoom = (kMaxSmem - static_cast<int>(sizeof(topk::Shared))) / 4;
     const int room = static_cast<int>(std::min<int64_t>((most + ranks - 1) / ranks, kRoom));
     static_assert(Ring<128>::kBytes + sizeof(Moves) <= kMaxSmem && (kMaxSmem + 1024) * 2 <= 228 * 1024, "two CTAs to an SM");
