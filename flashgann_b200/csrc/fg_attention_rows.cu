@@ -843,9 +843,16 @@ cudaError_t launch(AttentionParams a, cudaStream_t stream) {
     a.ctas *= kCtasPerSm;
     if (kForm == kChosen && split) {
         // Tiles of chosen pages are much the same length: where there are fewer than CTAs, as many CTAs to each, so that few
-        // have two (32 tokens of 85 chunks 40.7 -> 36.7 us, 30 of 76 24.9 -> 23.0, 8 of 85 18.3 -> 18.9).
+        // have two, unless too many CTAs then have nothing.  us, as many to each / an even share of the work to each of 296:
+        //     one to each (from 178 tiles on): of 85 chunks 152 32.3 / 29.4, 168 31.2 / 30.1, 180 31.2 / 31.2, 192 31.5 / 32.4,
+        //       256 36.7 / 40.6; of 145 156 47.0 / 41.7, 180 48.2 / 45.7, 208 49.4 / 50.6, 264 56 / 61; of 45 and dim 64 152
+        //       14.5 / 16.1, 192 14.9 / 18.1
+        //     more (two from 104 tiles on, three from 70): of 85 64 18.5 / 18.2, 76 20.0 / 20.5, 88 20.7 / 21.7, 100 23.9 /
+        //       22.6, 108 24.1 / 23.6, 120 24.7 / 25.3, 144 26.8 / 27.9; of 145 100 33.3 / 31.9, 108 34.0 / 33.3, 120 35.3 /
+        //       35.2, 132 36.8 / 37.7; of 80 and dim 96 100 23.2 / 22.8, 108 23.5 / 24.2, 132 25.3 / 26.2
         const int64_t tiles = static_cast<int64_t>(a.tokens) * a.kv_heads * ((a.group + a.tile_rows - 1) / a.tile_rows);
-        if (tiles < a.ctas) a.ctas = static_cast<int>(tiles * (a.ctas / tiles));
+        const int64_t each = a.ctas / tiles, used = tiles * each;
+        if (each == 1 ? used * 5 >= a.ctas * 3 : used * 10 >= a.ctas * 7) a.ctas = static_cast<int>(used);
     }
     a.unit_shift = split ? unit_shift(a) : 24;  // a unit: one chunk for each warp (or more, see there), or a tile
     a.tile_units = split ? kTileUnits : 0;
