@@ -175,7 +175,8 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor
     (fg_kv_evict_device): each kv head keeps the first ``sinks`` tokens, the
     last ``recent`` and the heaviest of those between, by weights float32
     [pages, kv_heads, page_size] from ``attention_weights``; keys, values and
-    weights of those move to the first positions, in order.
+    weights of those move to the first positions, in order.  A length past what
+    the table holds counts as that.
 
     Table entries from ceil(budget / page_size) on of such requests are free
     afterwards; kv_len of the result is the next step's ctx_len.  Page

@@ -1375,6 +1375,10 @@ int fg_kv_evict_device(const fg_kv_cache* cache, float* d_weights, int64_t weigh
     if (table_stride < 0) return fail(FG_ERR_ARG, "negative table stride");
     if (static_cast<int64_t>(requests) * cache->heads > INT32_MAX / 8)
         return fail(FG_ERR_UNSUPPORTED, "%d requests of %d heads", requests, cache->heads);
+    // each CTA reads its row's length, and one of a request's writes the new one
+    const auto at = [](const int32_t* p) { return reinterpret_cast<uintptr_t>(p); };
+    if (std::max(at(d_kv_len), at(d_kv_len_out)) - std::min(at(d_kv_len), at(d_kv_len_out)) < static_cast<uint64_t>(requests) * sizeof(int32_t))
+        return fail(FG_ERR_ARG, "kv_len and its output overlap");
     fg::EvictArgs a;
     a.cache = paged_rows(cache);
     a.v = cache->v;

@@ -479,9 +479,11 @@ int fg_attention_weights_device(const fg_kv_cache* cache, const fg_attention* ar
  * of the largest weights stay (of equal weights the lowest position; NaN counts
  * as -inf, positions without a page are lighter still) and move, in ascending
  * order, to positions 0 to budget - 1: rows of K and V and their weights, in
- * place.  d_kv_len_out[requests] = min(kv_len, budget) (not d_kv_len itself);
- * d_kept [requests, heads, budget]: the position that each was at, -1 past the
- * request's length.  Requests within the budget stay as they are.  Pages of
+ * place.  Lengths count as max(0, min(kv_len, table_width * page_size)): the
+ * last positions are those of the table where a length passes it.
+ * d_kv_len_out[requests]: the smaller of that and the budget (it may not overlap
+ * d_kv_len); d_kept [requests, heads, budget]: the position that each was at, -1
+ * past the request's length.  Requests within the budget stay as they are.  Pages of
  * block_table from ceil(budget / page_size) on are free afterwards (where all
  * layers that share the table are done); pages that two requests share must not
  * be evicted from.  sinks + recent <= budget, budget >= 1. */
