@@ -129,11 +129,13 @@ def select_blocks(q: torch.Tensor, bounds: torch.Tensor, scale: torch.Tensor, bl
                   sinks: int = 0, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """For each new token and kv head the ``count`` pages (numbers of blocks of
     page_size positions) whose bound on the token's scores is highest, among
-    those with keys that window and first tokens do not show: int32 [T,
+    those that end past the first tokens and begin before the window: int32 [T,
     kv_heads, count], ascending, then -1 (fg_select_blocks_device).
 
     q [T, heads, dim]; bounds and scale from ``kv_summarize``.  The heads of a
-    group choose together, by the largest of their bounds."""
+    group choose together, by the largest of their bounds.  Queries are rounded
+    to 8 bits for it, so that a bound holds but for that rounding.  A row that is
+    -2 throughout says that the kernel gave up a wait."""
     return _torch_ops.select_blocks(q, bounds, scale, block_table, query_start, kv_len, count, page_size, window, sinks,
                                     out, _handle(stream))
 
@@ -146,7 +148,8 @@ def block_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (fg_block_attention_device): blocks int32 [T, kv_heads, count], as
     ``select_blocks`` returns them or any others (block x: positions x *
     page_size to (x + 1) * page_size - 1; negative, repeated and future ones
-    and positions that are visible already count nothing)."""
+    and positions that are visible already count nothing).  Sums are 32 bits,
+    the weights of the product with V are rounded to the cache's type."""
     out, lse = _torch_ops.attention(q, k_cache, v_cache, block_table, query_start, kv_len, 1, blocks, True, window,
                                     sinks, scale, out, return_lse, _handle(stream))
     return (out, lse) if return_lse else out

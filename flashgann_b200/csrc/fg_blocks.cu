@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kSumWarps * 32) kv_summarize_kernel(const Summ
 // ---- selection ----
 //
 // A query is rounded to 127ths of its largest value like the bounds: Q_d, and
-// t = top / 127.  Its score of a page is an upper bound of q.k over the page's
+// t = top / 127.  Its score of a page is an upper bound of Q.k t over the page's
 // keys, in 8-bit arithmetic,
 //     I = sum_d Q_d * (Q_d < 0 ? lower_d : upper_d),     score = max_h (I_h t_h) * scale
 // over the heads h of the group.  I is a product of (min(Q, 0), max(Q, 0)) with
@@ -958,7 +958,8 @@ cudaError_t launch_select(const SelectArgs& a, cudaStream_t stream) {
     const cudaError_t e = scoring.set(reinterpret_cast<const void*>(score_blocks_kernel<T, kDim>), kMaxSmem);
     if (e != cudaSuccess) return e;
     const unsigned parts = (static_cast<unsigned>(a.req.table_width) + kPart - 1) / kPart;
-    // kv heads to a CTA: all, or fewer as long as all CTAs run at once, two to an SM
+    // kv heads to a CTA: all, or fewer as long as there are places for all CTAs at once, two to an SM (with more than 16 heads of
+    // 128 to a kv head, 123 KB of shared memory, one: they may take two rounds then)
     int each = a.kv_heads;
     while (each > 1 && static_cast<int64_t>(a.req.tokens) * parts * ((a.kv_heads + (each + 1) / 2 - 1) / ((each + 1) / 2)) <= 2 * a.sms) each = (each + 1) / 2;
     const dim3 grid(a.req.tokens * parts, static_cast<unsigned>((a.kv_heads + each - 1) / each));

@@ -375,8 +375,9 @@ int fg_retrieved_attention_device(const fg_kv_cache* cache, const fg_attention* 
  * [page, head, 1, d] are the least and the largest value of the page's keys in
  * element d, rounded down and up to whole multiples (-127 to 127) of
  * scale[page, head], which is the largest magnitude times the 32-bit number
- * nearest 1 / 127.  scale is inf (and the bounds 0) where a key is not finite.  The last two axes are contiguous;
- * bounds and its strides are multiples of 16 bytes. */
+ * nearest 1 / 127.  scale is inf (and the bounds 0) where a key is not finite.
+ * The last two axes are contiguous; bounds and its strides are multiples of 16
+ * bytes. */
 typedef struct fg_kv_summary {
     int8_t* bounds;
     float* scale;
@@ -420,18 +421,22 @@ int fg_select_blocks_workspace_bytes(const fg_kv_summary* summary, const fg_bloc
 /* For the new token at position p (as in fg_paged_attention_device) and each kv
  * head, the `count` blocks of the highest score, ascending, then -1.  Block x of
  * a request is its positions [x * page_size, (x + 1) * page_size), the page
- * block_table[x].  Blocks with a key that window and first tokens do not show
- * (a position >= sinks and <= p - window) are chosen from; those without a page
- * in the cache are not.  A block's score is that of all keys that were summed
- * up, later tokens of the same step among them (the attention reads none of
- * those).  The score is in the 8-bit arithmetic of the summary:
+ * block_table[x].  Blocks that end past the first tokens and begin before the
+ * window (x * page_size <= p - window and (x + 1) * page_size > sinks) are
+ * chosen from: all with a position that neither shows, and, where window and
+ * first tokens meet inside of one block, that block, which adds nothing.  Those
+ * without a page in the cache are not.  A block's score is that of all keys that
+ * were summed up, later tokens of the same step among them (the attention reads
+ * none of those).  The score is in the 8-bit arithmetic of the summary:
  * with top the largest |q_d| of a query head, Q_d = q_d * 127 / top rounded to
  * the nearest whole number and t = top times the 32-bit number nearest 1 / 127,
  *   score = max over the kv head's query heads of
  *           (sum_d Q_d * bounds[Q_d < 0 ? 0 : 1][d]) * t, times scale,
- * the products after the sum in 32 bits (a bound of q.k, so for attention with a
- * positive scale); a query head with a value that is not finite counts as 0, a
- * page of scale inf has the score inf.  Of equal scores the lowest block comes
+ * the products after the sum in 32 bits.  But for their roundings it bounds the
+ * q.k of the page's keys for the query that Q_d * t stands for; that of q itself
+ * may pass it by the query's rounding, top / 254 * sum_d |k_d| at most.  (So it
+ * is for attention with a positive scale.)  A query head with a value that is not
+ * finite counts as 0, a page of scale inf has the score inf.  Of equal scores the lowest block comes
  * first.  The same bits on every run.  Waits inside a kernel are bounded: one
  * that runs out (a second; a sound device has none) leaves -2 in all of its
  * row's places.  The last axis of blocks is contiguous.
@@ -444,8 +449,9 @@ int fg_select_blocks_device(const fg_kv_summary* summary, const fg_block_selecti
  * positions in ids[token, head's kv head, :].  The visible keys are a set:
  * blocks in any order, a block that repeats counts once, as do its positions
  * that window and first tokens show already; negative blocks and those past the
- * context count nothing.  Needs a window >= 0; at most 1024 blocks for each kv
- * head. */
+ * context count nothing.  The weights of the product with V are rounded to the
+ * cache's type, as in fg_paged_attention_device.  Needs a window >= 0; at most
+ * 1024 blocks for each kv head. */
 int fg_block_attention_device(const fg_kv_cache* cache, const fg_attention* args, void* stream);
 
 /* ---- eviction by attention weight ----
