@@ -228,9 +228,9 @@ __global__ void __launch_bounds__(kSumWarps * 32) kv_summarize_kernel(const Summ
 // to each row.
 //
 // What bounds it: 2 * dim + 4 bytes a page and kv head from memory, which many rows
-// read at 3.0 TB/s (64 tokens, 286K pages and heads, 71 MB: 23.5 us): a CTA's start,
+// read at 2.9 TB/s (64 tokens, 286K pages and heads, 71 MB: 24.5 us): a CTA's start,
 // the first pages' way and the selection are as long as the pages' way.  One token
-// of 131K positions: 14.9 us.
+// of 131K positions: 14.2 us.
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 static_assert(sizeof(topk::Shared) % 16 == 0, "the queries behind it are read 16 bytes at a time");
@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(kPartThreads, 2) score_blocks_kernel(const Sel
 
 // All of a row (a token's kv head) in one CTA: as score_blocks_kernel with the row's pages as items, kPart at a time, and one
 // kv head's queries for all of them; the keys stay in shared memory, and the largest are found where the pages were.  One
-// place for pages and four CTAs to an SM: what one waits for, the others cover (64 ragged tokens 23.5 us; two places and three
+// place for pages and four CTAs to an SM: what one waits for, the others cover (64 ragged tokens 24.5 us; two places and three
 // CTAs 25.4, three and two 27.7).
 constexpr int kRowPages = 4096;  // that a row may have
 constexpr int kRowGroup = 16;    // and query heads

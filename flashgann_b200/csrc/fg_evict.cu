@@ -17,8 +17,9 @@
 // thread to a row, which moves the row's weight too.
 //
 // What bounds it: the weights' way and, of the rows that move, there and back.
-// 32 requests of 900 to 8000 positions to 1024, 8 kv heads of 128: 59 us, of
-// which the selection takes about 10, for 258 MB.
+// 32 requests of 900 to 8000 positions to 1024, 8 kv heads of 128, 94 % of the rows
+// move, 258 MB: 74 us from memory, 60 where three sets of inputs take turns in L2,
+// of which the selection takes about 10.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
